@@ -148,6 +148,19 @@ SIGNATURES: dict[str, tuple] = {
     "camelid_hip_rmsnorm_q8_0_gemv": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, vp, vp, C.c_float, vp, vp]),
     "camelid_hip_gate_up_silu": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, vp, vp, vp, vp, C.c_float, vp, vp, vp]),
     "camelid_hip_verify": (C.c_int, [vp, vp, vp, vp, C.c_uint32, C.c_uint32, C.c_float, vp]),
+    "camelid_hip_paged_rope_kv": (C.c_int, [vp, C.c_uint32, C.c_uint32, vp, C.c_uint32, C.c_uint32, C.c_uint32,
+                                            C.c_uint32, C.c_uint32, vp, vp, vp, vp, C.c_float, vp, C.c_uint32, vp, vp,
+                                            C.c_uint32, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp, vp, vp]),
+    "camelid_hip_paged_attention_workspace": (C.c_size_t, [C.c_uint32] * 8),
+    "camelid_hip_paged_attention": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, C.c_uint32,
+                                              C.c_uint32, C.c_uint32, vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, vp,
+                                              C.c_uint32, vp, C.c_float, vp, C.c_uint32, vp, vp, C.c_size_t, vp, vp]),
+    "camelid_hip_paged_evict_workspace": (C.c_size_t, [C.c_uint32] * 5),
+    "camelid_hip_paged_evict": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp,
+                                          C.c_uint32, vp, C.c_uint32, C.c_uint32, vp, vp, vp, C.c_size_t, vp, vp]),
+    "camelid_hip_verify_drafts_workspace": (C.c_size_t, [C.c_uint32] * 3),
+    "camelid_hip_verify_drafts": (C.c_int, [vp, vp, C.c_uint32, vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, vp, vp,
+                                            vp, vp, vp, vp, C.c_size_t, vp]),
     "camelid_hip_inorder_sum_rows": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, vp]),
     "camelid_hip_expf": (C.c_int, [vp, vp, C.c_size_t, vp]),
     "camelid_expf_host": (None, [f32p, f32p, C.c_size_t]),

@@ -32,6 +32,7 @@
 #include <vector>
 
 #include "../../include/camelid_hip.h"
+#include "errors.h"
 #include "kernels_decode.h"
 #include "kernels_prefill.h"
 #include "kernels_kquant.h"
@@ -1804,6 +1805,14 @@ std::string proj_problem(uint8_t quant, uint32_t k) {
 }  // namespace
 
 // ====================================================================== C ABI
+int cm::fail_global(const char* what, const char* why) noexcept {
+  try {
+    return fail(nullptr, std::string(what) + ": " + why);
+  } catch (...) {  // no memory for the message
+    return 1;
+  }
+}
+
 extern "C" {
 
 const char* camelid_hip_last_error(const camelid_hip_engine* e) { return e ? e->err.c_str() : g_last_error.c_str(); }

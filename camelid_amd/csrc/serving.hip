@@ -1,0 +1,226 @@
+// serving.hip -- C entry points of batched serving over a paged cache (include/camelid_hip.h):
+// RoPE + store, attention of new tokens, eviction, and verification of drafts by given random
+// numbers.  Each call checks its arguments on the host, launches on the caller's stream, allocates
+// nothing and waits for nothing, so it may be captured into a graph.
+#include <hip/hip_runtime.h>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/camelid_hip.h"
+#include "errors.h"
+#include "kernels_paged.h"
+#include "kernels_verify.h"
+
+namespace {
+
+using cm::TY_BF16;
+using cm::TY_F16;
+using cm::TY_F32;
+
+int launched(const char* what) {
+  const hipError_t st = hipGetLastError();
+  return st == hipSuccess ? 0 : cm::fail_global(what, hipGetErrorString(st));
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Cache geometry; null: the reason why it is refused in *why.
+bool paged_geometry(cm::Paged* g, uint32_t n_seqs, uint32_t n_kv, uint32_t hd, uint32_t n_pages, uint32_t page_size,
+                    const uint32_t* table, uint32_t stride, const uint32_t* lens, uint32_t* status, const char** why) {
+  *why = nullptr;
+  if (hd != 64 && hd != 128 && hd != 256) *why = "head_dim must be 64, 128 or 256";
+  else if (!n_kv || n_kv > 1024) *why = "n_kv must be in 1..=1024";
+  else if (page_size < 8 || page_size > 4096 || (page_size & (page_size - 1)))
+    *why = "page_size must be a power of two in 8..=4096";
+  else if (!n_pages || !stride) *why = "n_pages and table_stride must be nonzero";
+  else if ((uint64_t)stride * page_size > (1u << 24)) *why = "table_stride * page_size must be at most 2^24 positions";
+  else if ((uint64_t)n_seqs * n_kv > (1u << 20)) *why = "n_seqs * n_kv must be at most 2^20";
+  else if (!aligned4(table) || !aligned4(lens) || !aligned4(status)) *why = "table, lens and status must be 4-byte aligned";
+  if (*why) return false;
+  uint32_t shift = 3;
+  while ((1u << shift) < page_size) ++shift;
+  *g = cm::Paged{table, lens, status, stride, n_pages, shift, n_kv, hd, n_seqs};
+  return true;
+}
+
+bool heads_ok(uint32_t n_heads, uint32_t n_kv) { return n_kv && n_heads && n_heads % n_kv == 0 && n_heads <= 4096; }
+bool type_ok(uint32_t t) { return t == TY_F32 || t == TY_F16 || t == TY_BF16; }
+bool kv_type_ok(uint32_t t) { return t == TY_F16 || t == TY_BF16; }
+
+}  // namespace
+
+extern "C" {
+
+int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new, const uint32_t* new_lens,
+                              uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t rope_dim, uint32_t split_half,
+                              const float* cos_tab, const float* sin_tab, const float* q_norm, const float* k_norm,
+                              float eps, void* q_out, uint32_t q_type, void* kc, void* vc, uint32_t kv_type,
+                              uint32_t n_pages, uint32_t page_size, const uint32_t* table, uint32_t table_stride,
+                              const uint32_t* lens, uint32_t* status, void* stream) {
+  const char* me = "paged_rope_kv";
+  if (!n_seqs || !n_new) return 0;
+  if (!qkv || !q_out || !kc || !vc || !table || !lens) return cm::fail_global(me, "null argument");
+  cm::Paged g;
+  const char* why;
+  if (!paged_geometry(&g, n_seqs, n_kv, hd, n_pages, page_size, table, table_stride, lens, status, &why))
+    return cm::fail_global(me, why);
+  if (!heads_ok(n_heads, n_kv)) return cm::fail_global(me, "n_heads must be a nonzero multiple of n_kv, at most 4096");
+  if (rope_dim > hd || rope_dim % 2) return cm::fail_global(me, "rope_dim must be even and at most head_dim");
+  if (rope_dim && (!cos_tab || !sin_tab)) return cm::fail_global(me, "null argument");
+  if (!type_ok(q_type) || !kv_type_ok(kv_type)) return cm::fail_global(me, "unknown type");
+  if (q_type != TY_F32 && q_type != kv_type)
+    return cm::fail_global(me, "16-bit q rows must have the cache's type");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(kc) || !aligned16(vc) || !aligned4(cos_tab) ||
+      !aligned4(sin_tab) || !aligned4(q_norm) || !aligned4(k_norm) || !aligned4(new_lens))
+    return cm::fail_global(me, "qkv, q_out and the cache must be 16-byte aligned, the rest 4-byte aligned");
+  const uint64_t grid = (uint64_t)n_seqs * n_new * (n_heads + n_kv);
+  if (grid > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  const auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(64), 0, (hipStream_t)stream, g, qkv, n_new, new_lens,
+                       n_heads, rope_dim, split_half, cos_tab, sin_tab, q_norm, k_norm, eps, q_out,
+                       static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc));
+  };
+  if (kv_type == TY_F16) {
+    if (q_type == TY_F32) go(cm::k_paged_rope_kv<TY_F32, TY_F16>);
+    else go(cm::k_paged_rope_kv<TY_F16, TY_F16>);
+  } else {
+    if (q_type == TY_F32) go(cm::k_paged_rope_kv<TY_F32, TY_BF16>);
+    else go(cm::k_paged_rope_kv<TY_BF16, TY_BF16>);
+  }
+  return launched(me);
+}
+
+size_t camelid_hip_paged_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
+                                             uint32_t hd, uint32_t page_size, uint32_t table_stride,
+                                             uint32_t with_weights) {
+  (void)n_new;
+  (void)n_heads;
+  (void)hd;
+  (void)with_weights;
+  return up256((size_t)n_seqs * n_kv * page_size * table_stride * 4);
+}
+
+int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_stride, uint32_t n_seqs, uint32_t n_new,
+                                const uint32_t* new_lens, uint32_t n_heads, uint32_t n_kv, uint32_t hd, const void* kc,
+                                const void* vc, uint32_t kv_type, uint32_t n_pages, uint32_t page_size,
+                                const uint32_t* table, uint32_t table_stride, const uint32_t* lens, float scale,
+                                void* out, uint32_t out_stride, float* weights, void* workspace,
+                                size_t workspace_bytes, uint32_t* status, void* stream) {
+  const char* me = "paged_attention";
+  if (!n_seqs || !n_new) return 0;
+  if (!q || !kc || !vc || !table || !lens || !out || !workspace) return cm::fail_global(me, "null argument");
+  cm::Paged g;
+  const char* why;
+  if (!paged_geometry(&g, n_seqs, n_kv, hd, n_pages, page_size, table, table_stride, lens, status, &why))
+    return cm::fail_global(me, why);
+  if (!heads_ok(n_heads, n_kv)) return cm::fail_global(me, "n_heads must be a nonzero multiple of n_kv, at most 4096");
+  if (n_new > CAMELID_MAX_VERIFY_K) return cm::fail_global(me, "at most 8 new tokens per sequence");
+  if (!type_ok(q_type) || !kv_type_ok(kv_type)) return cm::fail_global(me, "unknown type");
+  if (q_type != TY_F32 && q_type != kv_type)
+    return cm::fail_global(me, "16-bit q rows must have the cache's type");
+  if (!std::isfinite(scale)) return cm::fail_global(me, "attention score scale must be finite");
+  const uint32_t unit = q_type == TY_F32 ? 4 : 8;
+  if (q_stride < (uint64_t)n_heads * hd || out_stride < (uint64_t)n_heads * hd || q_stride % unit || out_stride % unit)
+    return cm::fail_global(me, "q_stride and out_stride must hold n_heads * head_dim elements and be whole 16-byte units");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc) || !aligned16(workspace) ||
+      !aligned4(weights) || !aligned4(new_lens))
+    return cm::fail_global(me, "q, out, the cache and the workspace must be 16-byte aligned, the rest 4-byte aligned");
+  if (workspace_bytes < camelid_hip_paged_attention_workspace(n_seqs, n_new, n_heads, n_kv, hd, page_size,
+                                                              table_stride, weights != nullptr))
+    return cm::fail_global(me, "workspace too small (camelid_hip_paged_attention_workspace)");
+  const auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(n_seqs * n_kv), dim3(256), 0, (hipStream_t)stream, g, q, q_stride, n_new, new_lens,
+                       n_heads, static_cast<const uint16_t*>(kc), static_cast<const uint16_t*>(vc), scale, out,
+                       out_stride, weights, static_cast<float*>(workspace));
+  };
+  if (kv_type == TY_F16) {
+    if (q_type == TY_F32) go(cm::k_paged_attention<TY_F32, TY_F16>);
+    else go(cm::k_paged_attention<TY_F16, TY_F16>);
+  } else {
+    if (q_type == TY_F32) go(cm::k_paged_attention<TY_F32, TY_BF16>);
+    else go(cm::k_paged_attention<TY_BF16, TY_BF16>);
+  }
+  return launched(me);
+}
+
+size_t camelid_hip_paged_evict_workspace(uint32_t n_seqs, uint32_t n_kv, uint32_t page_size, uint32_t table_stride,
+                                         uint32_t keep) {
+  (void)page_size;
+  (void)table_stride;
+  return up256((size_t)n_seqs * 8) + up256((size_t)n_seqs * n_kv * keep * 4);
+}
+
+int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_size, uint32_t n_kv, uint32_t hd,
+                            const uint32_t* table, uint32_t table_stride, const uint32_t* lens, uint32_t n_seqs,
+                            float* weights, uint32_t keep, uint32_t recent, uint32_t* lens_out, uint32_t* kept,
+                            void* workspace, size_t workspace_bytes, uint32_t* status, void* stream) {
+  const char* me = "paged_evict";
+  if (!n_seqs) return 0;
+  if (!kc || !vc || !table || !lens || !weights || !lens_out || !workspace) return cm::fail_global(me, "null argument");
+  cm::Paged g;
+  const char* why;
+  if (!paged_geometry(&g, n_seqs, n_kv, hd, n_pages, page_size, table, table_stride, lens, status, &why))
+    return cm::fail_global(me, why);
+  if (!keep || keep > (1u << 24)) return cm::fail_global(me, "keep must be in 1..=2^24");
+  if (recent > keep) return cm::fail_global(me, "recent must be at most keep");
+  if (!aligned16(kc) || !aligned16(vc) || !aligned16(workspace) || !aligned4(weights) || !aligned4(lens_out) ||
+      !aligned4(kept))
+    return cm::fail_global(me, "the cache and the workspace must be 16-byte aligned, the rest 4-byte aligned");
+  if (workspace_bytes < camelid_hip_paged_evict_workspace(n_seqs, n_kv, page_size, table_stride, keep))
+    return cm::fail_global(me, "workspace too small (camelid_hip_paged_evict_workspace)");
+  uint32_t* old_lens = static_cast<uint32_t*>(workspace);
+  uint32_t* new_lens = old_lens + n_seqs;
+  uint32_t* src = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + up256((size_t)n_seqs * 8));
+  hipLaunchKernelGGL(cm::k_evict_select, dim3(n_seqs * n_kv), dim3(cm::EV_NT), 0, (hipStream_t)stream, g, weights,
+                     keep, recent, src, old_lens, new_lens, kept);
+  const uint32_t slices = hd / 8 + hd / 32;
+  hipLaunchKernelGGL(cm::k_evict_move, dim3(n_seqs * n_kv * slices), dim3(cm::EM_NT), 0, (hipStream_t)stream, g,
+                     static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc), keep, src, old_lens, new_lens, lens_out);
+  return launched(me);
+}
+
+static uint32_t vd_parts(uint32_t vocab) { return (vocab + cm::VD_CHUNK - 1) / cm::VD_CHUNK; }
+
+size_t camelid_hip_verify_drafts_workspace(uint32_t n_seqs, uint32_t n_draft, uint32_t vocab) {
+  return up256((size_t)n_seqs * (2 * (size_t)n_draft + 1) * vd_parts(vocab) * sizeof(cm::VdPart));
+}
+
+int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint32_t logits_type,
+                              const uint32_t* draft_tokens, const uint32_t* draft_lens, uint32_t n_seqs,
+                              uint32_t n_draft, uint32_t vocab, const float* temperature, const float* uniforms,
+                              uint32_t* accepted, uint32_t* tokens_out, float* logprobs_out, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  const char* me = "verify_drafts";
+  if (!n_seqs) return 0;
+  if (!target || !temperature || !uniforms || !accepted || !tokens_out || !workspace || (n_draft && !draft_tokens))
+    return cm::fail_global(me, "null argument");
+  if (n_draft > 31) return cm::fail_global(me, "at most 31 drafts per sequence");
+  if (!vocab || vocab > (1u << 24)) return cm::fail_global(me, "vocab must be in 1..=2^24");
+  if (n_seqs > 65535) return cm::fail_global(me, "at most 65535 sequences");
+  if (!type_ok(logits_type)) return cm::fail_global(me, "unknown type");
+  const uintptr_t unit = logits_type == TY_F32 ? 3 : 1;
+  if (((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft_logits)) & unit) ||
+      !aligned16(workspace) || !aligned4(draft_tokens) || !aligned4(draft_lens) || !aligned4(temperature) ||
+      !aligned4(uniforms) || !aligned4(accepted) || !aligned4(tokens_out) || !aligned4(logprobs_out))
+    return cm::fail_global(me, "the workspace must be 16-byte aligned, the rest aligned to its elements");
+  if (workspace_bytes < camelid_hip_verify_drafts_workspace(n_seqs, n_draft, vocab))
+    return cm::fail_global(me, "workspace too small (camelid_hip_verify_drafts_workspace)");
+  const void* draft = n_draft ? draft_logits : nullptr;
+  const uint32_t rows = draft ? 2 * n_draft + 1 : n_draft + 1, parts = vd_parts(vocab);
+  cm::VdPart* ws = static_cast<cm::VdPart*>(workspace);
+  if ((uint64_t)n_seqs * rows > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  const auto go = [&](auto stats, auto pick) {
+    hipLaunchKernelGGL(stats, dim3(parts, n_seqs * rows), dim3(cm::VD_NT), 0, (hipStream_t)stream, target, draft,
+                       draft_lens, n_draft, vocab, temperature, ws);
+    hipLaunchKernelGGL(pick, dim3(n_seqs), dim3(cm::VP_NT), 0, (hipStream_t)stream, target, draft, draft_tokens,
+                       draft_lens, n_draft, vocab, temperature, uniforms, parts, ws, accepted, tokens_out, logprobs_out);
+  };
+  if (logits_type == TY_F32) go(cm::k_vd_stats<TY_F32>, cm::k_vd_pick<TY_F32>);
+  else if (logits_type == TY_F16) go(cm::k_vd_stats<TY_F16>, cm::k_vd_pick<TY_F16>);
+  else go(cm::k_vd_stats<TY_BF16>, cm::k_vd_pick<TY_BF16>);
+  return launched(me);
+}
+
+}  // extern "C"

@@ -349,6 +349,98 @@ int camelid_hip_expf(const float* x, float* y, size_t n, void* stream);
 /* The same expf restatement evaluated on the host (test hook). */
 void camelid_expf_host(const float* x, float* y, size_t n);
 
+/* ---------------------------------------------------------------------------------------
+ * Batched serving over a paged cache (no reference counterpart: Camelid serves one stream from
+ * one contiguous cache).  The calls stand beside camelid_hip_rope_kv, camelid_hip_attention_decode
+ * and the greedy verify above: many sequences in one call, their K and V in pages of one pool.
+ *
+ * Cache.  kc and vc hold n_pages pages of page_size positions (a power of two, 8..=4096), 16-bit
+ * elements of kv_type (CAMELID_F16 or CAMELID_BF16).  K of one page is [n_kv][hd / 8][page_size][8],
+ * V is [n_kv][page_size / 8][hd][8]: the granules of camelid_hip_rope_kv's cache, with a page in the
+ * place of the position range.  hd is 64, 128 or 256.  Position p of sequence s is at offset
+ * p % page_size of page table[s * table_stride + p / page_size]; table_stride * page_size <= 2^24.
+ * New tokens.  lens[s] counts the positions of sequence s with its new tokens, new_lens[s] (NULL:
+ * n_new for every sequence) the new tokens: token t < new_lens[s] is activation row s * n_new + t and
+ * position lens[s] - new_lens[s] + t.  Rows t >= new_lens[s] are padding: not read, not written.
+ * Pointers are device pointers, table, lens and the like included: they may change between the
+ * replays of a captured graph.  Buffers of 16-bit elements and activations are 16-byte aligned.
+ * Every call is asynchronous on `stream` (of the current device), allocates nothing and waits for
+ * nothing; it may be captured.  A workspace belongs to one call at a time: calls (or graphs) that
+ * can run at the same time need workspaces of their own; what one holds afterwards has no meaning.
+ * Errors that only the device can see set bits of *status (NULL: not told; the caller clears it):
+ * CAMELID_PAGED_BAD_LENGTH, lens[s] beyond the table row or new_lens[s] above n_new or lens[s]: the
+ * call leaves that sequence alone; CAMELID_PAGED_BAD_PAGE, a page id >= n_pages among a sequence's
+ * positions: its positions are neither stored nor attended to, and the sequence is not evicted from.
+ * No memory outside the buffers is touched in either case. */
+enum { CAMELID_F32 = 0, CAMELID_F16 = 1, CAMELID_BF16 = 2 };
+enum { CAMELID_PAGED_BAD_PAGE = 1, CAMELID_PAGED_BAD_LENGTH = 2 };
+
+/* Optional per-head RMSNorm (q_norm, k_norm [hd]; NULL: none), RoPE and cache store of the new
+ * tokens: qkv [n_seqs * n_new][(n_heads + 2 n_kv) * hd] f32, cos_tab / sin_tab [n_seqs * n_new]
+ * [rope_dim / 2] (each row's own position), q_out [n_seqs * n_new][n_heads * hd] of q_type
+ * (CAMELID_F32 or the cache's type).  The arithmetic is camelid_hip_rope_kv's, so f32 q rows and an
+ * f16 cache hold the same bits.  n_new has no limit but the grid's (prompts); two rows must not
+ * share a position of a page. */
+int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new, const uint32_t* new_lens,
+                              uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t rope_dim, uint32_t split_half,
+                              const float* cos_tab, const float* sin_tab, const float* q_norm, const float* k_norm,
+                              float eps, void* q_out, uint32_t q_type, void* kc, void* vc, uint32_t kv_type,
+                              uint32_t n_pages, uint32_t page_size, const uint32_t* table, uint32_t table_stride,
+                              const uint32_t* lens, uint32_t* status, void* stream);
+/* Attention of the new tokens (1..=CAMELID_MAX_VERIFY_K per sequence) over the cache, their own
+ * positions included: out[row][h] = sum_p softmax_p(scale q[row][h].k_p) v_p over p <= the row's
+ * position, query head h reading KV head h / (n_heads / n_kv).  q and out: rows of q_stride and
+ * out_stride elements (multiples of 16 bytes) of q_type (CAMELID_F32 or the cache's type).  Scores,
+ * softmax and sums are f32.  K and V of masked positions, whatever their bits, do not reach a row.
+ * weights (NULL: not kept): f32 [n_seqs][n_kv][table_stride * page_size]; every cached position's
+ * softmax weights, summed over the sequence's new tokens and the KV head's query heads, are added to
+ * it (a new token's own position starts at 0).  n_heads * n_new row sums are taken in a fixed order:
+ * the same call gives the same bits.
+ * _workspace: bytes for calls of at most these sizes (with_weights: weights != NULL). */
+size_t camelid_hip_paged_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
+                                             uint32_t hd, uint32_t page_size, uint32_t table_stride,
+                                             uint32_t with_weights);
+int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_stride, uint32_t n_seqs, uint32_t n_new,
+                                const uint32_t* new_lens, uint32_t n_heads, uint32_t n_kv, uint32_t hd, const void* kc,
+                                const void* vc, uint32_t kv_type, uint32_t n_pages, uint32_t page_size,
+                                const uint32_t* table, uint32_t table_stride, const uint32_t* lens, float scale,
+                                void* out, uint32_t out_stride, float* weights, void* workspace,
+                                size_t workspace_bytes, uint32_t* status, void* stream);
+/* Eviction by accumulated attention weight, in place: a sequence of lens[s] > keep positions keeps,
+ * for each KV head on its own, its last `recent` positions (recent <= keep) and the keep - recent of
+ * highest weights[s][head][p] among the others (of equal weights the lower position; NaN lowest),
+ * in their order, K, V and weights moved to positions [0, keep); lens_out[s] = min(lens[s], keep)
+ * (lens_out may be lens).  kept (NULL: not told) [n_seqs][n_kv][keep]: the positions kept, entries
+ * from lens_out[s] on untouched.  Cache positions and weights from keep on keep their bits.  Pages of
+ * the evicted sequences must belong to one table entry each. */
+size_t camelid_hip_paged_evict_workspace(uint32_t n_seqs, uint32_t n_kv, uint32_t page_size, uint32_t table_stride,
+                                         uint32_t keep);
+int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_size, uint32_t n_kv, uint32_t hd,
+                            const uint32_t* table, uint32_t table_stride, const uint32_t* lens, uint32_t n_seqs,
+                            float* weights, uint32_t keep, uint32_t recent, uint32_t* lens_out, uint32_t* kept,
+                            void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
+/* Verification of drafted tokens by speculative sampling with given uniform numbers (verify_batch's
+ * accept rule, inference.rs:2864-2873, for sampled generation).  target [n_seqs][n_draft + 1][vocab]
+ * and draft_logits [n_seqs][n_draft][vocab] (NULL: each draft was certain, as looked-up or greedy
+ * drafts are) of logits_type (f32, f16 or bf16), draft_tokens [n_seqs][n_draft], draft_lens[n_seqs]
+ * (NULL: n_draft; larger values count as n_draft), temperature [n_seqs], uniforms
+ * [n_seqs][n_draft + 1] in [0, 1).  With p_t = softmax(target row t / T), q_t alike: draft t is
+ * accepted while u_t q_t(x_t) < p_t(x_t); the token behind the accepted ones is the smallest i with
+ * C_i > u_last S, C the prefix sums and S the sum of max(p_t - q_t, 0) at the first rejected draft
+ * (of p_t where nothing is left), of p_n behind the last draft.  T = 0 (or below, or NaN): the
+ * argmax, lowest index of equals, accepts and replaces.  Exponentials and sums are f64.
+ * accepted[s]: drafts accepted; tokens_out [n_seqs][n_draft + 1]: these, the drawn token, then
+ * 0xffffffff; logprobs_out (NULL: not told) [n_seqs][n_draft + 1]: the natural log of p of each of
+ * these tokens (T = 0: of softmax(target)), then 0.  n_draft = 0 samples one token per sequence;
+ * n_draft <= 31.  A draft token >= vocab is rejected.  A row needed whose logits hold NaN or +inf, or
+ * nothing above -inf, ends its sequence: its token is 0xffffffff, its log-probability NaN. */
+size_t camelid_hip_verify_drafts_workspace(uint32_t n_seqs, uint32_t n_draft, uint32_t vocab);
+int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint32_t logits_type,
+                              const uint32_t* draft_tokens, const uint32_t* draft_lens, uint32_t n_seqs,
+                              uint32_t n_draft, uint32_t vocab, const float* temperature, const float* uniforms,
+                              uint32_t* accepted, uint32_t* tokens_out, float* logprobs_out, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
