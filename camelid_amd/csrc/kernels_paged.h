@@ -155,94 +155,6 @@ __global__ __launch_bounds__(64) void k_paged_rope_kv(Paged g, const float* __re
 }
 
 // ---------------------------------------------------------------------------
-// Attention of the new tokens over the cache, one workgroup per (sequence, KV head):
-//   s_p = scale * (q . k_p) for p <= first + t;  w = softmax(s);  o = sum_p w_p v_p
-// and, where weights are kept, weights[s][kv head][p] = (p < first ? weights : 0) + the sum of w_p
-// over the new tokens and the KV head's query heads.  A position of a bad page counts as masked.
-template <int QT, int KT>
-__global__ __launch_bounds__(256) void k_paged_attention(Paged g, const void* __restrict__ q, uint32_t q_stride,
-                                                         uint32_t n_new, const uint32_t* __restrict__ new_lens,
-                                                         uint32_t n_heads, const uint16_t* __restrict__ kc,
-                                                         const uint16_t* __restrict__ vc, float scale,
-                                                         void* __restrict__ out, uint32_t out_stride,
-                                                         float* __restrict__ weights, float* __restrict__ scores) {
-  __shared__ float qs[256];
-  __shared__ float red[256];
-  const uint32_t s = blockIdx.x / g.n_kv, h = blockIdx.x % g.n_kv, tid = threadIdx.x;
-  uint32_t first, len;
-  if (!paged_rows(g, new_lens, n_new, s, &first, &len)) return;
-  const uint32_t grp = n_heads / g.n_kv, cap = g.stride << g.shift, mask = (1u << g.shift) - 1u;
-  const uint32_t* tab = g.table + (size_t)s * g.stride;
-  float* sc = scores + (size_t)blockIdx.x * cap;
-  float* wsum = weights ? weights + (size_t)blockIdx.x * cap : nullptr;
-  if (wsum)
-    for (uint32_t p = first + tid; p < len; p += 256) wsum[p] = 0.0f;
-  for (uint32_t r = 0; r < (len - first) * grp; ++r) {
-    const uint32_t t = r / grp, qh = h * grp + r % grp, n = first + t + 1;
-    const size_t row = (size_t)s * n_new + t;
-    __syncthreads();
-    for (uint32_t d = tid; d < g.hd; d += 256) qs[d] = load_as_f32<QT>(q, row * q_stride + (size_t)qh * g.hd + d);
-    __syncthreads();
-    float m = -INFINITY;
-    for (uint32_t p = tid; p < n; p += 256) {
-      const uint32_t page = tab[p >> g.shift];
-      float v = -INFINITY;
-      if (page < g.n_pages) {
-        const size_t base = paged_base(g, page, h);
-        float dot = 0.0f;
-        for (uint32_t d = 0; d < g.hd; ++d) dot = dot + qs[d] * from_bits16<KT>(kc[base + paged_k(g, p & mask, d)]);
-        v = dot * scale;
-      } else {
-        paged_flag(g, PG_BAD_PAGE);
-      }
-      sc[p] = v;
-      m = (m > v || m != m) ? m : v;  // a NaN score stays the maximum, as a NaN row should
-    }
-    red[tid] = m;
-    __syncthreads();
-    for (uint32_t w = 128; w; w >>= 1) {
-      if (tid < w) {
-        const float a = red[tid], b = red[tid + w];
-        red[tid] = (a > b || a != a) ? a : b;
-      }
-      __syncthreads();
-    }
-    m = red[0];
-    __syncthreads();
-    float sum = 0.0f;
-    for (uint32_t p = tid; p < n; p += 256) {
-      const bool seen = tab[p >> g.shift] < g.n_pages;
-      const float e = seen ? expf(sc[p] - m) : 0.0f;
-      sc[p] = e;
-      sum += e;
-    }
-    red[tid] = sum;
-    __syncthreads();
-    for (uint32_t w = 128; w; w >>= 1) {
-      if (tid < w) red[tid] += red[tid + w];
-      __syncthreads();
-    }
-    const float total = red[0];
-    const bool none = total == 0.0f && m == -INFINITY;  // every position's page is bad
-    __syncthreads();
-    for (uint32_t p = tid; p < n; p += 256) {
-      const float w = none ? 0.0f : sc[p] / total;
-      sc[p] = w;
-      if (wsum) wsum[p] += w;
-    }
-    __syncthreads();
-    for (uint32_t d = tid; d < g.hd; d += 256) {
-      float acc = 0.0f;
-      for (uint32_t p = 0; p < n; ++p) {
-        const uint32_t page = tab[p >> g.shift];
-        if (page < g.n_pages) acc = acc + sc[p] * from_bits16<KT>(vc[paged_base(g, page, h) + paged_v(g, p & mask, d)]);
-      }
-      store_from_f32<QT>(out, row * out_stride + (size_t)qh * g.hd + d, acc);
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------
 // Eviction.  A sequence of more than `keep` positions keeps, for each KV head, its last `recent`
 // positions and the keep - recent of highest accumulated weight among the others (equal weights:
 // the lower position; a NaN counts as the lowest weight), in their order, moved to positions

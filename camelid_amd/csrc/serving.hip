@@ -8,7 +8,7 @@
 
 #include "../../include/camelid_hip.h"
 #include "errors.h"
-#include "kernels_paged.h"
+#include "kernels_paged_attn.h"
 #include "kernels_verify.h"
 
 namespace {
@@ -48,6 +48,50 @@ bool paged_geometry(cm::Paged* g, uint32_t n_seqs, uint32_t n_kv, uint32_t hd, u
 bool heads_ok(uint32_t n_heads, uint32_t n_kv) { return n_kv && n_heads && n_heads % n_kv == 0 && n_heads <= 4096; }
 bool type_ok(uint32_t t) { return t == TY_F32 || t == TY_F16 || t == TY_BF16; }
 bool kv_type_ok(uint32_t t) { return t == TY_F16 || t == TY_BF16; }
+
+// What a call of the attention needs: row blocks of 16 * nr query rows, workgroups, workspace.
+struct PaSizes {
+  uint32_t nr, n_wg;
+  size_t part_o, stats, scores, bytes;  // offsets of the workspace's parts, its size
+};
+
+PaSizes pa_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap,
+                 bool weights) {
+  PaSizes z;
+  const uint64_t rows = n_new * (n_heads / n_kv);
+  z.nr = rows > 16 && hd <= 128 ? 2 : 1;
+  // as many workgroups as the chip holds at once (256 CUs; k_pa_split's launch bounds)
+  z.n_wg = 256 * (hd == 64 ? 3 : hd == 128 ? 2 : 1);
+  const size_t slots = 2 * (size_t)z.n_wg * 16 * z.nr;
+  z.part_o = up256(slots * 8);
+  z.stats = z.part_o + up256(slots * hd * 4);
+  z.scores = z.stats + (weights ? up256(n_seqs * n_kv * rows * 8) : 0);
+  z.bytes = z.scores + (weights ? up256(n_seqs * n_kv * rows * cap * 4) : 0);
+  return z;
+}
+
+template <int HD, int KT, int QT, int NR>
+bool pa_launch(const cm::PaArgs& a, hipStream_t stream) {
+  const auto split = cm::k_pa_split<HD, KT, QT, NR>;
+  constexpr size_t lds = (size_t)4 * 16 * NR * (HD + 4 + 2) * 4;
+  if (lds > 64 * 1024) {
+    const hipError_t st = hipFuncSetAttribute(reinterpret_cast<const void*>(split),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (st != hipSuccess) return cm::fail_global("paged_attention", hipGetErrorString(st)) == 0;
+  }
+  hipLaunchKernelGGL(split, dim3(a.n_wg), dim3(cm::PA_NT), lds, stream, a);
+  const uint32_t rows = a.n_new * (a.n_heads / a.g.n_kv), sh = a.g.n_seqs * a.g.n_kv;
+  const uint32_t spans = a.weights ? ((a.g.stride << a.g.shift) + cm::PJ_SPAN - 1) / cm::PJ_SPAN : 0;
+  hipLaunchKernelGGL((cm::k_pa_join<HD, QT, NR>), dim3(sh * (rows + spans)), dim3(cm::PA_NT), 0, stream, a, rows, spans);
+  return true;
+}
+
+template <int KT, int QT>
+bool pa_launch_hd(const cm::PaArgs& a, uint32_t nr, hipStream_t stream) {
+  if (a.g.hd == 64) return nr == 1 ? pa_launch<64, KT, QT, 1>(a, stream) : pa_launch<64, KT, QT, 2>(a, stream);
+  if (a.g.hd == 128) return nr == 1 ? pa_launch<128, KT, QT, 1>(a, stream) : pa_launch<128, KT, QT, 2>(a, stream);
+  return pa_launch<256, KT, QT, 1>(a, stream);
+}
 
 }  // namespace
 
@@ -95,11 +139,9 @@ int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new,
 size_t camelid_hip_paged_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
                                              uint32_t hd, uint32_t page_size, uint32_t table_stride,
                                              uint32_t with_weights) {
-  (void)n_new;
-  (void)n_heads;
-  (void)hd;
-  (void)with_weights;
-  return up256((size_t)n_seqs * n_kv * page_size * table_stride * 4);
+  if (!n_kv) return 0;
+  const PaSizes z = pa_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride, with_weights != 0);
+  return z.bytes;
 }
 
 int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_stride, uint32_t n_seqs, uint32_t n_new,
@@ -121,6 +163,8 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   if (q_type != TY_F32 && q_type != kv_type)
     return cm::fail_global(me, "16-bit q rows must have the cache's type");
   if (!std::isfinite(scale)) return cm::fail_global(me, "attention score scale must be finite");
+  const uint64_t groups = (uint64_t)n_seqs * n_kv * (n_new * (n_heads / n_kv) + (weights ? 1 + ((uint64_t)table_stride * page_size >> 10) : 0));
+  if (groups > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
   const uint32_t unit = q_type == TY_F32 ? 4 : 8;
   if (q_stride < (uint64_t)n_heads * hd || out_stride < (uint64_t)n_heads * hd || q_stride % unit || out_stride % unit)
     return cm::fail_global(me, "q_stride and out_stride must hold n_heads * head_dim elements and be whole 16-byte units");
@@ -130,19 +174,32 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   if (workspace_bytes < camelid_hip_paged_attention_workspace(n_seqs, n_new, n_heads, n_kv, hd, page_size,
                                                               table_stride, weights != nullptr))
     return cm::fail_global(me, "workspace too small (camelid_hip_paged_attention_workspace)");
-  const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(n_seqs * n_kv), dim3(256), 0, (hipStream_t)stream, g, q, q_stride, n_new, new_lens,
-                       n_heads, static_cast<const uint16_t*>(kc), static_cast<const uint16_t*>(vc), scale, out,
-                       out_stride, weights, static_cast<float*>(workspace));
-  };
-  if (kv_type == TY_F16) {
-    if (q_type == TY_F32) go(cm::k_paged_attention<TY_F32, TY_F16>);
-    else go(cm::k_paged_attention<TY_F16, TY_F16>);
-  } else {
-    if (q_type == TY_F32) go(cm::k_paged_attention<TY_F32, TY_BF16>);
-    else go(cm::k_paged_attention<TY_BF16, TY_BF16>);
-  }
-  return launched(me);
+  const PaSizes z = pa_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride, weights != nullptr);
+  char* ws = static_cast<char*>(workspace);
+  cm::PaArgs a{};
+  a.g = g;
+  a.q = q;
+  a.new_lens = new_lens;
+  a.kc = static_cast<const uint16_t*>(kc);
+  a.vc = static_cast<const uint16_t*>(vc);
+  a.out = out;
+  a.part_ml = reinterpret_cast<float*>(ws);
+  a.part_o = reinterpret_cast<float*>(ws + z.part_o);
+  a.stats = reinterpret_cast<float*>(ws + z.stats);
+  a.scores = weights ? reinterpret_cast<float*>(ws + z.scores) : nullptr;
+  a.weights = weights;
+  a.scale = scale;
+  a.p_bits = kv_type == TY_F16 ? 14.0f : 0.0f;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.n_new = n_new;
+  a.n_heads = n_heads;
+  a.n_wg = z.n_wg;
+  const bool ok = kv_type == TY_F16 ? (q_type == TY_F32 ? pa_launch_hd<TY_F16, TY_F32>(a, z.nr, (hipStream_t)stream)
+                                                        : pa_launch_hd<TY_F16, TY_F16>(a, z.nr, (hipStream_t)stream))
+                                    : (q_type == TY_F32 ? pa_launch_hd<TY_BF16, TY_F32>(a, z.nr, (hipStream_t)stream)
+                                                        : pa_launch_hd<TY_BF16, TY_BF16>(a, z.nr, (hipStream_t)stream));
+  return ok ? launched(me) : 1;
 }
 
 size_t camelid_hip_paged_evict_workspace(uint32_t n_seqs, uint32_t n_kv, uint32_t page_size, uint32_t table_stride,
