@@ -6,13 +6,12 @@
 // so the kernel's work is to keep HBM busy whatever the batch looks like.
 //
 // Split.  A segment is (sequence, KV head, block of 16 NR query rows); its tiles are 32 positions.
-// All segments' tiles form one list, dealt out in equal runs to the workgroups (planned on the
-// device from lens, so a captured graph follows growing caches): a workgroup's run may cover part of
-// a long segment or several short ones.  The query rows of a segment are the new tokens times the KV
-// head's query heads, so K and V are read once for all of them.  A segment that lies inside one run is
-// finished there; of the others each run writes its part (running maximum, sum, unnormalised rows)
-// to one of its two slots, since only its first and its last segment can be cut, and k_pa_join joins
-// them.
+// The query rows are the new tokens times the KV head's query heads, so K and V are read once for
+// all of them.  A segment is cut into pieces of about equal size, none above `target` tiles, which
+// comes from the batch's tiles altogether; a workgroup does one piece.  Every wave of every workgroup
+// works the plan out from lens (a captured graph follows growing caches).  A segment of one piece is
+// finished there; of the others each piece writes its part (maximum, sum, unnormalised rows), and
+// k_pa_join joins them.
 //
 // Inside a workgroup the 4 waves take a segment's tiles in turn, each with a softmax state of its own,
 // joined through LDS at the segment's end.  A wave reads its K and V granules (16 bytes: 8 dims of a
@@ -28,6 +27,7 @@
 // two 16-bit numbers (three bf16 for f32 outputs), so they keep 16 bits at least where the output
 // has 8 or 11.  f16 weights carry a factor 2^14: small ones next to the row's maximum stay normal.
 #pragma once
+#include <type_traits>
 #include "kernels_paged.h"
 
 namespace cm {
@@ -49,13 +49,17 @@ struct PaArgs {
   const uint16_t* vc;
   void* out;
   float* scores;   // [seq][kv head][row][cap], log2 domain; null: no weights kept
-  float* stats;    // [seq][kv head][row][2]: maximum and sum of segments finished in one run
-  float* part_ml;  // [slot][16 NR][2]
-  float* part_o;   // [slot][16 NR][hd]
+  float* stats;    // [seq][kv head][row][2]: maximum and sum of the rows of uncut segments
+  uint2* cuts;     // [seq][kv head][block]: a segment's first slot and its pieces
+  float* part_ml;  // [slot][row of the block][2]
+  float* part_o;   // [slot][row of the block][hd]
   float* weights;
   float scale;
   float p_bits;    // weights are held times 2^p_bits
-  uint32_t q_stride, out_stride, n_new, n_heads, n_wg;
+  uint32_t q_stride, out_stride, n_new, n_heads;
+  uint32_t at_once;   // pieces that run at the same time
+  uint32_t blocks;    // row blocks of a sequence with n_new new tokens
+  uint32_t part_rows; // rows of a slot
 };
 
 // 16-bit operand vectors
@@ -92,7 +96,36 @@ __device__ __forceinline__ float pa_sum4(float x) {
   return u2f(b[0]) + u2f(b[1]);
 }
 
-// ---- the plan: tiles of all segments as one list
+// Lanes' values by data-parallel moves (a few clocks each; a shuffle goes through LDS).
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t pa_dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+// Inclusive prefix sum over the wave.
+__device__ __forceinline__ uint32_t pa_scan(uint32_t x) {
+  x += pa_dpp<0x111>(x);  // from 1, 2, 4, 8 lanes below in the row of 16
+  x += pa_dpp<0x112>(x);
+  x += pa_dpp<0x114>(x);
+  x += pa_dpp<0x118>(x);
+  x += pa_dpp<0x142, 0xa>(x);  // rows 1 and 3: the end of the row below
+  x += pa_dpp<0x143, 0xc>(x);  // rows 2 and 3: the end of row 1
+  return x;
+}
+// Maximum of |.| (bits of a nonnegative float) over aligned groups of N = 8, 16 or 32 lanes.
+template <int N>
+__device__ __forceinline__ uint32_t pa_group_max(uint32_t x) {
+  x = max(x, pa_dpp<0xb1>(x));   // lane ^ 1
+  x = max(x, pa_dpp<0x4e>(x));   // lane ^ 2
+  x = max(x, pa_dpp<0x141>(x));  // mirrored in 8
+  if (N > 8) x = max(x, pa_dpp<0x140>(x));  // mirrored in 16
+  if (N > 16) {
+    auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max((uint32_t)b[0], (uint32_t)b[1]);
+  }
+  return x;
+}
+
+// ---- the plan
 struct PaSeq {
   uint32_t len, first, rows, tiles, blocks;  // blocks: row blocks of the sequence
 };
@@ -109,78 +142,68 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, uint32_t s, bool flag) 
   q.blocks = (q.rows + 16 * NR - 1) / (16 * NR);
   return q;
 }
-__device__ __forceinline__ uint64_t pa_count(const PaArgs& a, const PaSeq& q) {
-  return (uint64_t)q.tiles * q.blocks * a.g.n_kv;
+
+// Tiles of a piece at most, for `total` of the batch.  Small batches: one tile per wave, or as many as
+// bring the pieces below what the chip holds at once (a second round of workgroups costs its
+// whole latency again).  Large ones: 16, so that workgroups ending early make room for others, and
+// more once that makes over 2048 pieces.
+__device__ __forceinline__ uint32_t pa_target(const PaArgs& a, uint32_t total) {
+  const uint32_t one = (total + a.at_once - 1) / a.at_once;
+  return one <= 16 ? max(4u, one) : max(16u, (total + 2047) / 2048);
 }
 
-struct PaPlan {
-  uint64_t total;     // tiles
-  uint64_t segments;
-  uint64_t before;    // tiles before sequence `at`
-  uint32_t at;
+struct PaPiece {
+  uint32_t s, h, rb, t0, t1, n, slot;  // n: the segment's pieces; slot: this piece's (n > 1)
+  PaSeq q;
+  bool any;
 };
 
-// Workgroups that get a run: one tile for each wave at least, or one segment.
-__device__ __forceinline__ uint32_t pa_runs(const PaArgs& a, uint64_t total, uint64_t segments) {
-  uint64_t n = (total + 3) / 4;
-  if (segments > n) n = segments;
-  return (uint32_t)(n < a.n_wg ? n : a.n_wg);
-}
-__device__ __forceinline__ uint64_t pa_begin(uint64_t total, uint32_t runs, uint32_t i) {
-  return total * i / runs;  // (below 2^40 tiles and 2^12 runs)
-}
-// The run that holds tile x.
-__device__ __forceinline__ uint32_t pa_run_of(uint64_t total, uint32_t runs, uint64_t x) {
-  return (uint32_t)(((x + 1) * runs - 1) / total);
-}
-
-// Totals, and for want < total the sequence that holds tile `want` (i < n_seqs: tiles before
-// sequence i as `want`).  Every thread of the workgroup calls it; sh: 3 x 4 + 3 words.
-template <int NR, typename F>
-__device__ __forceinline__ PaPlan pa_plan(const PaArgs& a, uint64_t* sh, bool flag, F want_of) {
-  const uint32_t tid = threadIdx.x, n = a.g.n_seqs, per = (n + PA_NT - 1) / PA_NT;
-  const uint32_t s0 = min(n, tid * per), s1 = min(n, s0 + per);
-  uint64_t tiles = 0, segs = 0;
+// Piece `index` of the batch (pieces in the order sequence, KV head, block, tiles).  Each wave works
+// it out by itself: a lane for every 64th part of the sequences.
+template <int NR>
+__device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, bool flag) {
+  const uint32_t lane = threadIdx.x & 63u, n = a.g.n_seqs, per = (n + 63) / 64;
+  const uint32_t s0 = min(n, lane * per), s1 = min(n, s0 + per);
+  uint32_t total = 0;
+  PaSeq q{};
   for (uint32_t s = s0; s < s1; ++s) {
-    const PaSeq q = pa_seq<NR>(a, s, flag);
-    tiles += pa_count(a, q);
-    segs += (uint64_t)q.blocks * a.g.n_kv;
+    q = pa_seq<NR>(a, s, flag);
+    total += q.tiles * q.blocks * a.g.n_kv;
   }
-  uint64_t x = tiles, y = segs;
-  const uint32_t lane = tid & 63u, w = tid >> 6;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t u = __shfl_up(x, o), v = __shfl_up(y, o);
-    if (lane >= (uint32_t)o) {
-      x += u;
-      y += v;
-    }
+  total = __builtin_amdgcn_readlane(pa_scan(total), 63);
+  const uint32_t target = pa_target(a, total);
+  const auto count = [&](const PaSeq& z) { return (z.tiles + target - 1) / target; };
+  uint32_t mine = 0, cut = 0;
+  for (uint32_t s = s0; s < s1; ++s) {
+    if (per > 1) q = pa_seq<NR>(a, s, false);
+    const uint32_t c = count(q), k = c * q.blocks * a.g.n_kv;
+    mine += k;
+    if (c > 1) cut += k;
   }
-  if (lane == 63) {
-    sh[w] = x;
-    sh[4 + w] = y;
+  const uint32_t x = pa_scan(mine), y = pa_scan(cut);
+  PaPiece p;
+  const uint64_t here = __ballot(index < x);
+  p.any = here != 0;
+  if (!p.any) return p;
+  const int owner = __builtin_ctzll(here);
+  uint32_t before = __builtin_amdgcn_readlane(x - mine, owner), slots = __builtin_amdgcn_readlane(y - cut, owner);
+  uint32_t s = owner * per;
+  for (;; ++s) {
+    q = pa_seq<NR>(a, s, false);
+    const uint32_t c = count(q), k = c * q.blocks * a.g.n_kv;
+    if (index - before < k) break;
+    before += k;
+    if (c > 1) slots += k;
   }
-  __syncthreads();
-  PaPlan p;
-  p.total = sh[0] + sh[1] + sh[2] + sh[3];
-  p.segments = sh[4] + sh[5] + sh[6] + sh[7];
-  for (uint32_t i = 0; i < w; ++i) x += sh[i];
-  const uint64_t want = want_of(p.total, p.segments);
-  uint64_t c = x - tiles;
-  if (want >= c && want < x) {
-    for (uint32_t s = s0; s < s1; ++s) {
-      const uint64_t k = pa_count(a, pa_seq<NR>(a, s, false));
-      if (want < c + k) {
-        sh[8] = c;
-        sh[9] = s;
-        break;
-      }
-      c += k;
-    }
-  }
-  __syncthreads();
-  p.before = sh[8];
-  p.at = (uint32_t)sh[9];
-  __syncthreads();
+  p.s = s;
+  p.q = q;
+  p.n = count(q);
+  const uint32_t at = index - before, seg = at / p.n, piece = at - seg * p.n;
+  p.h = seg / q.blocks;
+  p.rb = seg - p.h * q.blocks;
+  p.t0 = (uint32_t)((uint64_t)q.tiles * piece / p.n);
+  p.t1 = (uint32_t)((uint64_t)q.tiles * (piece + 1) / p.n);
+  p.slot = slots + seg * p.n + piece;
   return p;
 }
 
@@ -189,100 +212,34 @@ __device__ __forceinline__ uint32_t pa_page(const PaArgs& a, const uint32_t* tab
   return pos < len ? tab[pos >> a.g.shift] : 0u;
 }
 
-// One run of tiles per workgroup.
+// Workgroups of a CU, by registers and LDS.
+constexpr int pa_per_cu(int hd, int nr) { return hd == 64 ? 5 - nr : hd == 128 ? 4 - nr : 2; }
+
+// One piece per workgroup.
 template <int HD, int KT, int QT, int NR>
-__global__ __launch_bounds__(PA_NT, HD == 64 ? 3 : (HD == 128 && !(NR == 2 && KT == TY_BF16 && QT == TY_F32)) ? 2 : 1)
-void k_pa_split(PaArgs a) {
+__global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a) {
   typedef typename Op16<KT>::v8 v8;
   typedef typename Op16<KT>::e e16;
   constexpr int NQ = QT != TY_F32 ? 1 : KT == TY_F16 ? 2 : 3;  // 16-bit terms of a query
   constexpr int NP = QT == TY_F32 && KT == TY_BF16 ? 3 : 2;    // ... of a weight
   constexpr int KS = HD / 32, DS = HD / 16;
   constexpr int ROWS = 16 * NR, PITCH = HD + 4;
-  extern __shared__ float smem[];  // [4][ROWS][PITCH] rows, [4][ROWS][2] states
+  extern __shared__ float smem[];  // [4][ROWS][PITCH] rows, [4][ROWS][2] states, [ROWS]
   float* s_ml = smem + 4 * ROWS * PITCH;
-  uint64_t* s_plan = reinterpret_cast<uint64_t*>(smem);
+  float* s_c = s_ml + 4 * ROWS * 2;  // [ROWS] scale log2(e) / the row's power of two
+  float* s_q = smem;                 // [NR][NQ][KS][64] operands of 16 bytes
   const uint32_t tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t col = lane & 15u, grp = lane >> 4;
   const Paged& g = a.g;
   const uint32_t group = a.n_heads / g.n_kv, cap = g.stride << g.shift;
 
-  const PaPlan plan = pa_plan<NR>(a, s_plan, blockIdx.x == 0, [&](uint64_t total, uint64_t segs) {
-    const uint32_t runs = pa_runs(a, total, segs);
-    return blockIdx.x < runs ? pa_begin(total, runs, blockIdx.x) : total;
-  });
-  if (!plan.total) return;
-  const uint32_t runs = pa_runs(a, plan.total, plan.segments);
-  if (blockIdx.x >= runs) return;
-  const uint64_t x0 = pa_begin(plan.total, runs, blockIdx.x), x1 = pa_begin(plan.total, runs, blockIdx.x + 1);
-  uint64_t x = x0, rem = x0 - plan.before;
-  uint32_t s = plan.at;
-  PaSeq sq = pa_seq<NR>(a, s, false);
-  uint64_t in_seq = pa_count(a, sq);
-
-  while (x < x1) {
-    while (rem >= in_seq) {  // (sequences without tiles are passed over)
-      rem -= in_seq;
-      sq = pa_seq<NR>(a, ++s, false);
-      in_seq = pa_count(a, sq);
-    }
-    const uint32_t seg = (uint32_t)(rem / sq.tiles), t0 = (uint32_t)(rem - (uint64_t)seg * sq.tiles);
-    const uint32_t t1 = (uint32_t)min((uint64_t)sq.tiles, t0 + (x1 - x));
-    const uint32_t h = seg / sq.blocks, rb = seg - h * sq.blocks;
+  const PaPiece pc = pa_piece<NR>(a, blockIdx.x, blockIdx.x == 0);
+  if (!pc.any) return;
+  const PaSeq& sq = pc.q;
+  const uint32_t s = pc.s, h = pc.h, rb = pc.rb, t0 = pc.t0, t1 = pc.t1;
+  {
     const uint32_t* tab = g.table + (size_t)s * g.stride;
     const uint32_t len = sq.len, first = sq.first;
-
-    // ---- this lane's query rows (one per 16-row block) as operands
-    v8 qf[NR][NQ][KS];
-    float c[NR];
-    uint32_t limit[NR];
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      const uint32_t row = rb * ROWS + r * 16 + col;
-      const bool real = row < sq.rows;
-      const uint32_t t = real ? row / group : 0u, qh = h * group + (real ? row - t * group : 0u);
-      limit[r] = first + t;
-      const size_t src = ((size_t)s * a.n_new + t) * a.q_stride + (size_t)qh * HD + 8 * grp;
-      c[r] = a.scale * PA_LOG2E;
-      if constexpr (QT != TY_F32) {
-        const e16* p = static_cast<const e16*>(a.q) + src;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) qf[r][0][j] = *reinterpret_cast<const v8*>(p + 32 * j);
-      } else {
-        const float* p = static_cast<const float*>(a.q) + src;
-        float f[KS][8], top = 0.0f;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          const f32x4 u = *reinterpret_cast<const f32x4*>(p + 32 * j), v = *reinterpret_cast<const f32x4*>(p + 32 * j + 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[j][i] = u[i];
-            f[j][4 + i] = v[i];
-            top = fmaxf(top, fmaxf(fabsf(u[i]), fabsf(v[i])));
-          }
-        }
-        int up = 0;
-        if (KT == TY_F16) {  // the row's largest element to [2^13, 2^14)
-          top = pa_max4(top);
-          const int ex = (int)((f2u(top) >> 23) & 255u) - 127;
-          up = ex == 128 ? 0 : max(-100, min(100, 13 - ex));
-          c[r] = ldexpf(c[r], -up);
-        }
-#pragma unroll
-        for (int j = 0; j < KS; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float v = KT == TY_F16 ? ldexpf(f[j][i], up) : f[j][i];
-            const bool fin = fabsf(v) < INFINITY;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-              const e16 b = (e16)v;
-              qf[r][n][j][i] = b;
-              v = fin ? v - (float)b : 0.0f;
-            }
-          }
-      }
-    }
 
     f32x4 o[NR][DS];
     float m[NR], l[NR];
@@ -294,8 +251,9 @@ void k_pa_split(PaArgs a) {
       for (int d = 0; d < DS; ++d) o[r][d] = f32x4{0, 0, 0, 0};
     }
 
-    // ---- tiles t0 + w', t0 + w' + 4, ...: consecutive tiles of the run go to consecutive waves
-    const uint32_t ta = t0 + ((w - (uint32_t)(x - x0)) & 3u);
+    // ---- tiles t0 + w, t0 + w + 4, ...: the first one's pages, then its K and V, are on their way before
+    // the query rows are made ready
+    const uint32_t ta = t0 + w;
     const uint32_t kpos = 8 * (col >> 2), ko = kpos + (col & 3u);  // this lane's K row in a tile
     const size_t head_elems = (size_t)HD << g.shift;
     const uint32_t pmask = (1u << g.shift) - 1u;
@@ -319,12 +277,78 @@ void k_pa_split(PaArgs a) {
 #pragma unroll
       for (int d = 0; d < DS; ++d) vf[d] = *reinterpret_cast<const v8*>(p + d * 128);
     };
+    uint32_t pk = 0, pv = 0, pkn = 0, pvn = 0;
     if (ta < t1) {
-      uint32_t pk = pa_page(a, tab, ta * PA_TILE + kpos, len), pv = pa_page(a, tab, ta * PA_TILE + 8 * grp, len);
-      uint32_t pkn = pa_page(a, tab, (ta + 4) * PA_TILE + kpos, len),
-               pvn = pa_page(a, tab, (ta + 4) * PA_TILE + 8 * grp, len);
+      pk = pa_page(a, tab, ta * PA_TILE + kpos, len);
+      pv = pa_page(a, tab, ta * PA_TILE + 8 * grp, len);
+      pkn = pa_page(a, tab, (ta + 4) * PA_TILE + kpos, len);
+      pvn = pa_page(a, tab, (ta + 4) * PA_TILE + 8 * grp, len);
+    }
+    // the query rows as operands in LDS: unit (row, 8 dims) of every thread, a row in HD / 8 lanes
+    constexpr int LPR = HD / 8, UNITS = ROWS * LPR, PASSES = (UNITS + PA_NT - 1) / PA_NT;
+    typedef typename std::conditional<QT == TY_F32, float, e16>::type QE;
+    typedef QE q8v __attribute__((ext_vector_type(8)));
+    q8v raw[PASSES];
+#pragma unroll
+    for (int k = 0; k < PASSES; ++k) {
+      const uint32_t u = tid + k * PA_NT, row = rb * ROWS + u / LPR;
+      const uint32_t t = row / group, qh = h * group + (row - t * group);
+      raw[k] = q8v{};
+      if (u < UNITS && row < sq.rows)
+        raw[k] = *reinterpret_cast<const q8v*>(static_cast<const QE*>(a.q) + ((size_t)s * a.n_new + t) * a.q_stride +
+                                               (size_t)qh * HD + 8 * (u % LPR));
+    }
+    if (ta < t1) {
       load_k(ta * PA_TILE, pk);
       load_v(ta * PA_TILE, pv);
+    }
+#pragma unroll
+    for (int k = 0; k < PASSES; ++k) {
+      const uint32_t u = tid + k * PA_NT, row = u / LPR, d8 = u % LPR;
+      float factor = a.scale * PA_LOG2E;
+      int up = 0;
+      if constexpr (QT == TY_F32 && KT == TY_F16) {  // the row's largest element to [2^13, 2^14)
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, f2u(raw[k][i]) & 0x7fffffffu);
+        const int ex = (int)(pa_group_max<LPR>(top) >> 23) - 127;
+        up = ex == 128 ? 0 : max(-100, min(100, 13 - ex));
+        factor = ldexpf(factor, -up);
+      }
+      v8 term[NQ];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (QT != TY_F32) {
+          term[0][i] = raw[k][i];
+        } else {
+          float v = KT == TY_F16 ? ldexpf(raw[k][i], up) : raw[k][i];
+          const bool fin = fabsf(v) < INFINITY;
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            const e16 b = (e16)v;
+            term[n][i] = b;
+            v = fin ? v - (float)b : 0.0f;
+          }
+        }
+      }
+      if (UNITS >= PA_NT || u < UNITS) {
+        // lane 16 (d8 % 4) + row % 16 of 32-dim step d8 / 4
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+          *reinterpret_cast<v8*>(&s_q[((((row >> 4) * NQ + n) * KS + (d8 >> 2)) * 64 + (d8 & 3u) * 16 + (row & 15u)) * 4]) = term[n];
+        if (d8 == 0) s_c[row] = factor;
+      }
+    }
+    __syncthreads();
+    float c[NR];
+    uint32_t limit[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const uint32_t row = rb * ROWS + r * 16 + col;
+      c[r] = s_c[r * 16 + col];
+      limit[r] = first + (row < sq.rows ? row / group : 0u);
+    }
+    if (ta < t1) {
       for (uint32_t t = ta; t < t1; t += 4) {
         const uint32_t pos0 = t * PA_TILE;
         const bool next = t + 4 < t1;
@@ -334,11 +358,18 @@ void k_pa_split(PaArgs a) {
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             sc[r][b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int n = NQ - 1; n >= 0; --n)  // the small terms first
-#pragma unroll
-              for (int j = 0; j < KS; ++j) sc[r][b] = Op16<KT>::mfma(kf[b][j], qf[r][n][j], sc[r][b]);
           }
+        asm volatile("" ::: "memory");  // (the query operands stay in LDS: registers)
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int n = NQ - 1; n >= 0; --n)  // the small terms first
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              const v8 qf = *reinterpret_cast<const v8*>(&s_q[(((r * NQ + n) * KS + j) * 64 + lane) * 4]);
+              sc[r][0] = Op16<KT>::mfma(kf[0][j], qf, sc[r][0]);
+              sc[r][1] = Op16<KT>::mfma(kf[1][j], qf, sc[r][1]);
+            }
         uint32_t pv2 = 0;
         const bool page_ok = pv < g.n_pages;
         if (next) {
@@ -472,7 +503,7 @@ void k_pa_split(PaArgs a) {
     }
 
     // ---- the waves' states joined; rows finished, or a part written
-    __syncthreads();
+    __syncthreads();  // (the query operands lie where the states go)
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       const float sum = pa_sum4(l[r]);
@@ -485,8 +516,8 @@ void k_pa_split(PaArgs a) {
         *reinterpret_cast<f32x4*>(&smem[(w * ROWS + r * 16 + col) * PITCH + 16 * d + 4 * grp]) = o[r][d];
     }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == sq.tiles;
-    const uint32_t slot = 2 * blockIdx.x + (x == x0 ? 0u : 1u);
+    const bool whole = pc.n == 1;
+    if (t0 == 0 && tid == 0) a.cuts[((size_t)s * g.n_kv + h) * a.blocks + rb] = make_uint2(pc.slot, pc.n);
     const uint32_t here = min((uint32_t)ROWS, sq.rows - rb * ROWS);
     for (uint32_t i = tid; i < here * (HD / 4); i += PA_NT) {
       const uint32_t row = i / (HD / 4), d = (i % (HD / 4)) * 4;
@@ -522,108 +553,59 @@ void k_pa_split(PaArgs a) {
           st[1] = L;
         }
       } else {
-        *reinterpret_cast<f32x4*>(&a.part_o[((size_t)slot * ROWS + row) * HD + d]) = y;
+        *reinterpret_cast<f32x4*>(&a.part_o[((size_t)pc.slot * a.part_rows + row) * HD + d]) = y;
         if (d == 0) {
-          a.part_ml[((size_t)slot * ROWS + row) * 2] = M;
-          a.part_ml[((size_t)slot * ROWS + row) * 2 + 1] = L;
+          a.part_ml[((size_t)pc.slot * a.part_rows + row) * 2] = M;
+          a.part_ml[((size_t)pc.slot * a.part_rows + row) * 2 + 1] = L;
         }
       }
     }
-    __syncthreads();
-    x += t1 - t0;
-    rem += t1 - t0;
   }
 }
 
-// The slots of a segment that starts at tile x (of `tiles`): runs i0 .. i1, run i0's first or second
-// slot, the later runs' first.
-struct PaCut {
-  uint32_t i0, i1, slot0;
-};
-__device__ __forceinline__ PaCut pa_cut(const PaPlan& p, uint32_t runs, uint64_t x, uint32_t tiles) {
-  PaCut c;
-  c.i0 = pa_run_of(p.total, runs, x);
-  c.i1 = pa_run_of(p.total, runs, x + tiles - 1);
-  c.slot0 = 2 * c.i0 + (pa_begin(p.total, runs, c.i0) == x ? 0u : 1u);
-  return c;
-}
-__device__ __forceinline__ uint32_t pa_slot(const PaCut& c, uint32_t i) { return i == c.i0 ? c.slot0 : 2 * i; }
-
 // Joins the cut segments: workgroup (sequence, KV head, row) for rows below `n_rows`; then, where
-// weights are kept, workgroup (sequence, KV head, 1024 positions).
-constexpr uint32_t PJ_SPAN = 1024, PJ_ROWS = 64;
+// weights are kept, workgroup (sequence, KV head, 256 positions).
+constexpr uint32_t PJ_SPAN = 256, PJ_ROWS = 64;
 template <int HD, int QT, int NR>
 __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, uint32_t spans) {
   constexpr int ROWS = 16 * NR, PARTS = PA_NT / (HD / 4);
-  __shared__ uint64_t s_plan[16];
   __shared__ f32x4 s_o[PARTS][HD / 4];
-  __shared__ float s_l[PARTS];
+  __shared__ float s_ml[PARTS][2];
   __shared__ float s_stat[PJ_ROWS][2];
   const Paged& g = a.g;
   const uint32_t tid = threadIdx.x, group = a.n_heads / g.n_kv, n_out = g.n_seqs * g.n_kv * n_rows;
   const bool is_out = blockIdx.x < n_out;
   const uint32_t sh = is_out ? blockIdx.x / n_rows : (blockIdx.x - n_out) / spans, s = sh / g.n_kv, h = sh % g.n_kv;
-  const uint32_t row = blockIdx.x % n_rows, span = (blockIdx.x - n_out) % spans;  // (one of the two has a meaning)
-  const PaSeq sq = pa_seq<NR>(a, s, false);
-  if (is_out ? row >= sq.rows : !sq.rows || span * PJ_SPAN >= sq.len) return;
-  // tiles before this sequence: every sequence's own count, as the runs were dealt out
-  uint64_t before = 0;
-  const PaPlan p = [&] {
-    const uint32_t n = g.n_seqs;
-    uint64_t tiles = 0, segs = 0, pre = 0;
-    for (uint32_t i = tid; i < n; i += PA_NT) {
-      const PaSeq q = pa_seq<NR>(a, i, false);
-      const uint64_t k = pa_count(a, q);
-      tiles += k;
-      segs += (uint64_t)q.blocks * g.n_kv;
-      if (i < s) pre += k;
-    }
-    for (int o = 32; o; o >>= 1) {
-      tiles += __shfl_xor(tiles, o);
-      segs += __shfl_xor(segs, o);
-      pre += __shfl_xor(pre, o);
-    }
-    if ((tid & 63u) == 0) {
-      s_plan[tid >> 6] = tiles;
-      s_plan[4 + (tid >> 6)] = segs;
-      s_plan[8 + (tid >> 6)] = pre;
-    }
-    __syncthreads();
-    PaPlan q;
-    q.total = s_plan[0] + s_plan[1] + s_plan[2] + s_plan[3];
-    q.segments = s_plan[4] + s_plan[5] + s_plan[6] + s_plan[7];
-    before = s_plan[8] + s_plan[9] + s_plan[10] + s_plan[11];
-    q.before = before;
-    q.at = s;
-    return q;
-  }();
-  const uint32_t runs = pa_runs(a, p.total, p.segments);
+  const uint2* cuts = a.cuts + (size_t)sh * a.blocks;
   if (is_out) {
-    const uint32_t rb = row / ROWS, r = row % ROWS;
-    const PaCut c = pa_cut(p, runs, before + ((uint64_t)h * sq.blocks + rb) * sq.tiles, sq.tiles);
-    if (c.i0 == c.i1) return;  // finished in its run
+    const uint32_t row = blockIdx.x - sh * n_rows, rb = row / ROWS, r = row % ROWS;
+    const uint2 cut = cuts[rb];
+    const PaSeq sq = pa_seq<NR>(a, s, false);
+    if (row >= sq.rows || cut.y == 1) return;  // (finished by its one piece)
     const uint32_t d = tid % (HD / 4), part = tid / (HD / 4);
-    float M = -INFINITY;
-    for (uint32_t i = c.i0 + (tid & 63u); i <= c.i1; i += 64)
-      M = fmaxf(M, a.part_ml[((size_t)pa_slot(c, i) * ROWS + r) * 2]);
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
+    float M = -INFINITY, L = 0.0f;
     f32x4 y = f32x4{0, 0, 0, 0};
-    for (uint32_t i = c.i0 + part; i <= c.i1; i += PARTS) {
-      const size_t at = (size_t)pa_slot(c, i) * ROWS + r;
-      const float f = __builtin_amdgcn_exp2f(a.part_ml[at * 2] - ref);
-      L += f * a.part_ml[at * 2 + 1];
-      y += f * *reinterpret_cast<const f32x4*>(&a.part_o[at * HD + 4 * d]);
+    const auto add = [&](float m2, float l2, f32x4 y2) {
+      const float top = fmaxf(M, m2), ref = top == -INFINITY ? 0.0f : top;
+      const float f = __builtin_amdgcn_exp2f(M - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+      L = L * f + l2 * f2;
+      y = y * f + y2 * f2;
+      M = top;
+    };
+#pragma unroll 4
+    for (uint32_t i = part; i < cut.y; i += PARTS) {
+      const size_t at = (size_t)(cut.x + i) * a.part_rows + r;
+      const float2 ml = *reinterpret_cast<const float2*>(&a.part_ml[at * 2]);
+      add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(&a.part_o[at * HD + 4 * d]));
     }
     s_o[part][d] = y;
-    if (d == 0) s_l[part] = L;
+    if (d == 0) {
+      s_ml[part][0] = M;
+      s_ml[part][1] = L;
+    }
     __syncthreads();
     if (part == 0) {
-      for (int i = 1; i < PARTS; ++i) {
-        L += s_l[i];
-        y += s_o[i][d];
-      }
+      for (int i = 1; i < PARTS; ++i) add(s_ml[i][0], s_ml[i][1], s_o[i][d]);
       const f32x4 z = M == -INFINITY ? f32x4{0, 0, 0, 0} : y / L;
       const size_t dst = ((size_t)s * a.n_new + row / group) * a.out_stride + (size_t)(h * group + row % group) * HD + 4 * d;
       if constexpr (QT == TY_F32) {
@@ -639,51 +621,54 @@ __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, ui
     }
     return;
   }
-  // weights of positions [span * 1024, ...): the scores against each row's maximum and sum
+  // weights of 256 positions: the scores against each row's maximum and sum
+  const uint32_t pos = (blockIdx.x - n_out - sh * spans) * PJ_SPAN + tid;
+  const PaSeq sq = pa_seq<NR>(a, s, false);
+  if (!sq.rows || pos - tid >= sq.len) return;
   const uint32_t cap = g.stride << g.shift;
   const size_t all = (size_t)a.n_new * group, base = (size_t)sh * all;
   float* wp = a.weights + (size_t)sh * cap;
-  float acc[PJ_SPAN / PA_NT];
-#pragma unroll
-  for (uint32_t k = 0; k < PJ_SPAN / PA_NT; ++k) {
-    const uint32_t pos = span * PJ_SPAN + k * PA_NT + tid;
-    acc[k] = pos < sq.first ? wp[pos] : 0.0f;
-  }
+  float acc = pos < sq.first ? wp[pos] : 0.0f;
   for (uint32_t r0 = 0; r0 < sq.rows; r0 += PJ_ROWS) {
+    const uint32_t n = min(PJ_ROWS, sq.rows - r0);
     __syncthreads();
-    if (tid < PJ_ROWS && r0 + tid < sq.rows) {
-      const uint32_t full = r0 + tid, rb = full / ROWS, r = full % ROWS;
-      const PaCut c = pa_cut(p, runs, before + ((uint64_t)h * sq.blocks + rb) * sq.tiles, sq.tiles);
+    // a quarter wave per row: 16 lanes over its parts
+    for (uint32_t k = tid >> 4; k < n; k += PA_NT / 16) {
+      const uint32_t full = r0 + k, rb = full / ROWS, r = full % ROWS, lane = tid & 15u;
+      const uint2 cut = cuts[rb];
       float M = -INFINITY, L = 0.0f;
-      if (c.i0 == c.i1) {
+      if (cut.y == 1) {
         M = a.stats[(base + full) * 2];
         L = a.stats[(base + full) * 2 + 1];
       } else {
-        for (uint32_t i = c.i0; i <= c.i1; ++i) M = fmaxf(M, a.part_ml[((size_t)pa_slot(c, i) * ROWS + r) * 2]);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        for (uint32_t i = c.i0; i <= c.i1; ++i) {
-          const size_t at = (size_t)pa_slot(c, i) * ROWS + r;
-          L += __builtin_amdgcn_exp2f(a.part_ml[at * 2] - ref) * a.part_ml[at * 2 + 1];
+        for (uint32_t i = lane; i < cut.y; i += 16) {
+          const float2 ml = *reinterpret_cast<const float2*>(&a.part_ml[((size_t)(cut.x + i) * a.part_rows + r) * 2]);
+          const float top = fmaxf(M, ml.x), ref = top == -INFINITY ? 0.0f : top;
+          L = L * __builtin_amdgcn_exp2f(M - ref) + ml.y * __builtin_amdgcn_exp2f(ml.x - ref);
+          M = top;
+        }
+        for (int o = 8; o; o >>= 1) {
+          const float m2 = __shfl_xor(M, o), l2 = __shfl_xor(L, o);
+          const float top = fmaxf(M, m2), ref = top == -INFINITY ? 0.0f : top;
+          // (both orders give the same bits: the two lanes agree)
+          const float p = L * __builtin_amdgcn_exp2f(M - ref), q = l2 * __builtin_amdgcn_exp2f(m2 - ref);
+          L = p + q;
+          M = top;
         }
       }
-      s_stat[tid][0] = M == -INFINITY ? 0.0f : M - a.p_bits;
-      s_stat[tid][1] = M == -INFINITY ? 0.0f : 1.0f / L;
+      if (lane == 0) {
+        s_stat[k][0] = M == -INFINITY ? 0.0f : M - a.p_bits;
+        s_stat[k][1] = M == -INFINITY ? 0.0f : 1.0f / L;
+      }
     }
     __syncthreads();
-    const uint32_t n = min(PJ_ROWS, sq.rows - r0);
-#pragma unroll
-    for (uint32_t k = 0; k < PJ_SPAN / PA_NT; ++k) {
-      const uint32_t pos = span * PJ_SPAN + k * PA_NT + tid;
-      if (pos < sq.len)
-        for (uint32_t r = 0; r < n; ++r)
-          acc[k] += __builtin_amdgcn_exp2f(a.scores[(base + r0 + r) * cap + pos] - s_stat[r][0]) * s_stat[r][1];
+    if (pos < sq.len) {
+#pragma unroll 4
+      for (uint32_t r = 0; r < n; ++r)
+        acc += __builtin_amdgcn_exp2f(a.scores[(base + r0 + r) * cap + pos] - s_stat[r][0]) * s_stat[r][1];
     }
   }
-#pragma unroll
-  for (uint32_t k = 0; k < PJ_SPAN / PA_NT; ++k) {
-    const uint32_t pos = span * PJ_SPAN + k * PA_NT + tid;
-    if (pos < sq.len) wp[pos] = acc[k];
-  }
+  if (pos < sq.len) wp[pos] = acc;
 }
 
 }  // namespace cm

@@ -3,6 +3,7 @@
 // numbers.  Each call checks its arguments on the host, launches on the caller's stream, allocates
 // nothing and waits for nothing, so it may be captured into a graph.
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -51,35 +52,48 @@ bool kv_type_ok(uint32_t t) { return t == TY_F16 || t == TY_BF16; }
 
 // What a call of the attention needs: row blocks of 16 * nr query rows, workgroups, workspace.
 struct PaSizes {
-  uint32_t nr, n_wg;
-  size_t part_o, stats, scores, bytes;  // offsets of the workspace's parts, its size
+  uint32_t nr, blocks, part_rows, at_once, grid;
+  bool join;                                  // some segment may be cut, or weights are kept
+  bool fits;                                  // the plan's 32-bit counts hold
+  size_t part_o, cuts, stats, scores, bytes;  // offsets of the workspace's parts, its size
 };
 
 PaSizes pa_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap,
                  bool weights) {
   PaSizes z;
-  const uint64_t rows = n_new * (n_heads / n_kv);
+  const uint64_t rows = n_new * (n_heads / n_kv), cap_tiles = (cap + cm::PA_TILE - 1) / cm::PA_TILE;
   z.nr = rows > 16 && hd <= 128 ? 2 : 1;
-  // as many workgroups as the chip holds at once (256 CUs; k_pa_split's launch bounds)
-  z.n_wg = 256 * (hd == 64 ? 3 : hd == 128 ? 2 : 1);
-  const size_t slots = 2 * (size_t)z.n_wg * 16 * z.nr;
-  z.part_o = up256(slots * 8);
-  z.stats = z.part_o + up256(slots * hd * 4);
+  z.blocks = (uint32_t)((rows + 16 * z.nr - 1) / (16 * z.nr));
+  z.part_rows = (uint32_t)std::min<uint64_t>(rows, 16 * z.nr);
+  // 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
+  z.at_once = 256 * cm::pa_per_cu((int)hd, (int)z.nr) * 7 / 8;
+  const uint64_t segments = n_seqs * n_kv * z.blocks, most = 2048;
+  z.fits = segments * cap_tiles < (1ull << 31);
+  // a segment has at most ceil(its tiles / 4) pieces, all of them together at most 2048 and one each
+  const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + 3) / 4));
+  z.grid = (uint32_t)std::min<uint64_t>(pieces, 0x7fffffffu);
+  z.join = cap_tiles > 4 || weights;
+  // cut segments have more tiles than the target: at most 2048 of them, twice as many pieces
+  const size_t slots = cap_tiles > 4 ? (size_t)std::min(2 * most, pieces) : 0;
+  z.part_o = up256(slots * z.part_rows * 8);
+  z.cuts = z.part_o + up256(slots * z.part_rows * hd * 4);
+  z.stats = z.cuts + up256(segments * 8);
   z.scores = z.stats + (weights ? up256(n_seqs * n_kv * rows * 8) : 0);
   z.bytes = z.scores + (weights ? up256(n_seqs * n_kv * rows * cap * 4) : 0);
   return z;
 }
 
 template <int HD, int KT, int QT, int NR>
-bool pa_launch(const cm::PaArgs& a, hipStream_t stream) {
+bool pa_launch(const cm::PaArgs& a, const PaSizes& z, hipStream_t stream) {
   const auto split = cm::k_pa_split<HD, KT, QT, NR>;
-  constexpr size_t lds = (size_t)4 * 16 * NR * (HD + 4 + 2) * 4;
+  constexpr size_t lds = (size_t)16 * NR * (4 * (HD + 4 + 2) + 1) * 4;
   if (lds > 64 * 1024) {
     const hipError_t st = hipFuncSetAttribute(reinterpret_cast<const void*>(split),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (st != hipSuccess) return cm::fail_global("paged_attention", hipGetErrorString(st)) == 0;
   }
-  hipLaunchKernelGGL(split, dim3(a.n_wg), dim3(cm::PA_NT), lds, stream, a);
+  hipLaunchKernelGGL(split, dim3(z.grid), dim3(cm::PA_NT), lds, stream, a);
+  if (!z.join) return true;
   const uint32_t rows = a.n_new * (a.n_heads / a.g.n_kv), sh = a.g.n_seqs * a.g.n_kv;
   const uint32_t spans = a.weights ? ((a.g.stride << a.g.shift) + cm::PJ_SPAN - 1) / cm::PJ_SPAN : 0;
   hipLaunchKernelGGL((cm::k_pa_join<HD, QT, NR>), dim3(sh * (rows + spans)), dim3(cm::PA_NT), 0, stream, a, rows, spans);
@@ -87,10 +101,10 @@ bool pa_launch(const cm::PaArgs& a, hipStream_t stream) {
 }
 
 template <int KT, int QT>
-bool pa_launch_hd(const cm::PaArgs& a, uint32_t nr, hipStream_t stream) {
-  if (a.g.hd == 64) return nr == 1 ? pa_launch<64, KT, QT, 1>(a, stream) : pa_launch<64, KT, QT, 2>(a, stream);
-  if (a.g.hd == 128) return nr == 1 ? pa_launch<128, KT, QT, 1>(a, stream) : pa_launch<128, KT, QT, 2>(a, stream);
-  return pa_launch<256, KT, QT, 1>(a, stream);
+bool pa_launch_hd(const cm::PaArgs& a, const PaSizes& z, hipStream_t stream) {
+  if (a.g.hd == 64) return z.nr == 1 ? pa_launch<64, KT, QT, 1>(a, z, stream) : pa_launch<64, KT, QT, 2>(a, z, stream);
+  if (a.g.hd == 128) return z.nr == 1 ? pa_launch<128, KT, QT, 1>(a, z, stream) : pa_launch<128, KT, QT, 2>(a, z, stream);
+  return pa_launch<256, KT, QT, 1>(a, z, stream);
 }
 
 }  // namespace
@@ -163,7 +177,7 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   if (q_type != TY_F32 && q_type != kv_type)
     return cm::fail_global(me, "16-bit q rows must have the cache's type");
   if (!std::isfinite(scale)) return cm::fail_global(me, "attention score scale must be finite");
-  const uint64_t groups = (uint64_t)n_seqs * n_kv * (n_new * (n_heads / n_kv) + (weights ? 1 + ((uint64_t)table_stride * page_size >> 10) : 0));
+  const uint64_t groups = (uint64_t)n_seqs * n_kv * (n_new * (n_heads / n_kv) + (weights ? 1 + ((uint64_t)table_stride * page_size >> 8) : 0));
   if (groups > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
   const uint32_t unit = q_type == TY_F32 ? 4 : 8;
   if (q_stride < (uint64_t)n_heads * hd || out_stride < (uint64_t)n_heads * hd || q_stride % unit || out_stride % unit)
@@ -175,6 +189,7 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
                                                               table_stride, weights != nullptr))
     return cm::fail_global(me, "workspace too small (camelid_hip_paged_attention_workspace)");
   const PaSizes z = pa_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride, weights != nullptr);
+  if (!z.fits) return cm::fail_global(me, "n_seqs * n_kv * table_stride * page_size too large for one call");
   char* ws = static_cast<char*>(workspace);
   cm::PaArgs a{};
   a.g = g;
@@ -185,6 +200,7 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   a.out = out;
   a.part_ml = reinterpret_cast<float*>(ws);
   a.part_o = reinterpret_cast<float*>(ws + z.part_o);
+  a.cuts = reinterpret_cast<uint2*>(ws + z.cuts);
   a.stats = reinterpret_cast<float*>(ws + z.stats);
   a.scores = weights ? reinterpret_cast<float*>(ws + z.scores) : nullptr;
   a.weights = weights;
@@ -194,11 +210,13 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   a.out_stride = out_stride;
   a.n_new = n_new;
   a.n_heads = n_heads;
-  a.n_wg = z.n_wg;
-  const bool ok = kv_type == TY_F16 ? (q_type == TY_F32 ? pa_launch_hd<TY_F16, TY_F32>(a, z.nr, (hipStream_t)stream)
-                                                        : pa_launch_hd<TY_F16, TY_F16>(a, z.nr, (hipStream_t)stream))
-                                    : (q_type == TY_F32 ? pa_launch_hd<TY_BF16, TY_F32>(a, z.nr, (hipStream_t)stream)
-                                                        : pa_launch_hd<TY_BF16, TY_BF16>(a, z.nr, (hipStream_t)stream));
+  a.at_once = z.at_once;
+  a.blocks = z.blocks;
+  a.part_rows = z.part_rows;
+  const bool ok = kv_type == TY_F16 ? (q_type == TY_F32 ? pa_launch_hd<TY_F16, TY_F32>(a, z, (hipStream_t)stream)
+                                                        : pa_launch_hd<TY_F16, TY_F16>(a, z, (hipStream_t)stream))
+                                    : (q_type == TY_F32 ? pa_launch_hd<TY_BF16, TY_F32>(a, z, (hipStream_t)stream)
+                                                        : pa_launch_hd<TY_BF16, TY_BF16>(a, z, (hipStream_t)stream));
   return ok ? launched(me) : 1;
 }
 
