@@ -156,6 +156,7 @@ struct PaPiece {
   uint32_t s, h, rb, t0, t1, n, slot;  // n: the segment's pieces; slot: this piece's (n > 1)
   PaSeq q;
   bool any;
+  bool stream;  // the batch's K and V are beyond what the memory-side cache holds
 };
 
 // Piece `index` of the batch (pieces in the order sequence, KV head, block, tiles).  Each wave works
@@ -201,8 +202,13 @@ __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, boo
   const uint32_t at = index - before, seg = at / p.n, piece = at - seg * p.n;
   p.h = seg / q.blocks;
   p.rb = seg - p.h * q.blocks;
-  p.t0 = (uint32_t)((uint64_t)q.tiles * piece / p.n);
-  p.t1 = (uint32_t)((uint64_t)q.tiles * (piece + 1) / p.n);
+  const uint32_t even = q.tiles / p.n, more = q.tiles - even * p.n;  // the first `more` pieces take one tile more
+  p.t0 = piece * even + min(piece, more);
+  p.t1 = p.t0 + even + (piece < more ? 1u : 0u);
+  // 256 MiB.  One new token, 32 query heads, hd 128, f16: plain loads 45.6 us and loads that leave the
+  // caches alone 47.9 for 269 MB read again and again, 54.9 and 49.7 for 4 such caches in turn, 101.8 and
+  // 91.7 for 538 MB; 28.9 and 31.6 for 134 MB.  (Several row blocks read K and V several times.)
+  p.stream = a.blocks == 1 && total > (1u << 28) / (PA_TILE * 4 * a.g.hd);
   p.slot = slots + seg * p.n + piece;
   return p;
 }
@@ -210,6 +216,21 @@ __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, boo
 // A granule's page of the tile at pos0: the table entry of position pos0 + 8 gran.
 __device__ __forceinline__ uint32_t pa_page(const PaArgs& a, const uint32_t* tab, uint32_t pos, uint32_t len) {
   return pos < len ? tab[pos >> a.g.shift] : 0u;
+}
+
+// N granules, `step` apart; stream: without keeping them in the caches.  (The empty asm statements keep
+// the compiler from making one plain load of the two.)
+template <int N, typename V>
+__device__ __forceinline__ void pa_load(bool stream, const V* p, size_t step, V* to) {
+  if (stream) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = __builtin_nontemporal_load(p + i * step);
+    asm volatile("" ::: "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = p[i * step];
+  }
 }
 
 // Workgroups of a CU, by registers and LDS.
@@ -263,19 +284,15 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
       if (page >= g.n_pages) page = 0;
       const uint16_t* p = a.kc + ((size_t)page * g.n_kv + h) * head_elems +
                           (((size_t)grp << g.shift) + ((pos0 + ko) & pmask)) * 8;
-#pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        const uint16_t* pj = p + ((size_t)(4 * j) << (g.shift + 3));
-        kf[0][j] = *reinterpret_cast<const v8*>(pj);
-        kf[1][j] = *reinterpret_cast<const v8*>(pj + 32);
-      }
+      const size_t step = (size_t)4 << g.shift;  // granules of 32 dims
+      pa_load<KS>(pc.stream, reinterpret_cast<const v8*>(p), step, kf[0]);
+      pa_load<KS>(pc.stream, reinterpret_cast<const v8*>(p) + 4, step, kf[1]);
     };
     const auto load_v = [&](uint32_t pos0, uint32_t page) {
       if (page >= g.n_pages) page = 0;
       const uint16_t* p = a.vc + ((size_t)page * g.n_kv + h) * head_elems +
                           ((size_t)(((pos0 + 8 * grp) & pmask) >> 3) * HD + col) * 8;
-#pragma unroll
-      for (int d = 0; d < DS; ++d) vf[d] = *reinterpret_cast<const v8*>(p + d * 128);
+      pa_load<DS>(pc.stream, reinterpret_cast<const v8*>(p), 16, vf);
     };
     uint32_t pk = 0, pv = 0, pkn = 0, pvn = 0;
     if (ta < t1) {
