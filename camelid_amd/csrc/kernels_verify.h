@@ -10,42 +10,66 @@
 // T = 0 (or below, or NaN): the argmax, first of equals, accepts and replaces.
 // Exponentials and sums are f64: the token depends on which side of one of ~1e5 prefix sums u S
 // lies, and f32 sums would move the borders by more than their distances.
+//
+// Bound: every row's logits read once (k_vd_stats: a wave per 2048 of them, its maximum and its sum of
+// exponentials; no barriers behind the loads), where 12 f64 operations a logit take about 0.6 of the
+// time that f32 logits take to arrive from HBM.  Only sequences that rejected a draft of a draft
+// model read two rows again for max(p - q, 0) (k_vd_rest, spread over the chip like the first pass);
+// otherwise the shares' sums are known.  k_vd_pick then needs one share's logits.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <type_traits>
 #include "device_math.h"
 #include "kernels_paged.h"
 
 namespace cm {
 
 constexpr int VD_NT = 256;
-constexpr uint32_t VD_CHUNK = 4096;  // logits of one workgroup's share of a row
+constexpr uint32_t VD_SHARE = 2048;  // logits of one wave's share of a row
+constexpr uint32_t VD_MAX_ROWS = 63;
 
-// One share of one row: the largest logit, its first index, and the sum of exp((l - max) / T).
+// One share of one row: the sum of exp((l - m) / T), the largest logit m and its first index.
 struct VdPart {
   double z;
   float m;
   uint32_t i;
 };
 
-// exp((l - m) / T) for l <= m, m finite
-__device__ __forceinline__ double vd_exp(float l, float m, double inv_t) {
-  return l == -INFINITY ? 0.0 : exp(((double)l - (double)m) * inv_t);
+// ---- 2^(x / 64) for whole x: a table of 64 powers in LDS
+__device__ __forceinline__ void vd_table(double* tab) {
+  if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+}
+// exp(y / T) for y <= 0, by = 64 log2(e) / T: y by = k + r, |r| <= 1/2; 2^(k / 64) from the table, e^(r ln 2 / 64)
+// by its series to the fifth power (the next term is below 4e-17).
+__device__ __forceinline__ double vd_exp(double y, double by, const double* tab) {
+  constexpr double A = 0x1.62e42fefa39efp-1 / 64.0;  // ln 2 / 64
+  const double k = fmax(rint(y * by), -131072.0);  // (2^-2048 and below, y = -inf: 0)
+  const double r = fmax(fma(y, by, -k), -1.0);
+  const int n = (int)k;
+  double p = fma(r, A * A * A * A * A / 120.0, A * A * A * A / 24.0);
+  p = fma(r, p, A * A * A / 6.0);
+  p = fma(r, p, A * A / 2.0);
+  p = fma(r, p, A);
+  p = fma(r, p, 1.0);
+  return ldexp(p * tab[n & 63], n >> 6);
 }
 
 __device__ __forceinline__ bool vd_greedy(float t) { return !(t > 0.0f); }
-// 1 / T; a greedy sequence's log-probabilities are those of T = 1
-__device__ __forceinline__ double vd_inv(float t) { return vd_greedy(t) ? 1.0 : 1.0 / (double)t; }
+// 64 log2(e) / T; a greedy sequence's log-probabilities are those of T = 1
+__device__ __forceinline__ double vd_by(float t) {
+  return 64.0 * 0x1.71547652b82fep+0 / (vd_greedy(t) ? 1.0 : (double)t);
+}
 
 // A row without a distribution: a NaN or +inf logit, or none above -inf.
 __device__ __forceinline__ bool vd_bad(float m) { return !(m > -INFINITY && m < INFINITY); }
 
-// (m, i) of the larger logit; a NaN is larger than all; the lower index of equals.
-__device__ __forceinline__ void vd_max(float& m, uint32_t& i, float m2, uint32_t i2) {
-  const bool take = (m2 != m2) ? (m == m || i2 < i) : (m == m && (m2 > m || (m2 == m && i2 < i)));
-  if (take) {
-    m = m2;
-    i = i2;
-  }
+// Bits that order as the logits do, -0 as +0, NaN above all.
+__device__ __forceinline__ uint32_t vd_key(float l) {
+  const uint32_t u = f2u(l + 0.0f);
+  return l != l ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float vd_unkey(uint32_t k) {
+  return k == 0xffffffffu ? NAN : u2f((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
 __device__ __forceinline__ double vd_wave_sum(double v) {
@@ -53,195 +77,371 @@ __device__ __forceinline__ double vd_wave_sum(double v) {
   return v;
 }
 
-// Row r of a sequence: rows [0, n_draft] target, [n_draft + 1, 2 n_draft] draft t = r - n_draft - 1.
+// This lane's logits of the share that begins at v0: vectors of 16 bytes (rows may begin at any element),
+// vector j of lane i at v0 + (64 j + i) V; -inf behind the row's end.
 template <int LT>
-__global__ __launch_bounds__(VD_NT) void k_vd_stats(const void* __restrict__ target, const void* __restrict__ draft,
-                                                    const uint32_t* __restrict__ draft_lens, uint32_t n_draft,
-                                                    uint32_t vocab, const float* __restrict__ temperature,
-                                                    VdPart* __restrict__ parts) {
-  __shared__ float sm[VD_NT / 64];
-  __shared__ uint32_t si[VD_NT / 64];
-  __shared__ double sz[VD_NT / 64];
-  const uint32_t rows = draft ? 2 * n_draft + 1 : n_draft + 1;
-  const uint32_t s = blockIdx.y / rows, r = blockIdx.y % rows;
-  const uint32_t n = draft_lens ? min(draft_lens[s], n_draft) : n_draft;
-  const bool is_target = r <= n_draft;
-  const uint32_t t = is_target ? r : r - n_draft - 1;
+struct VdLogits {
+  static constexpr int V = LT == TY_F32 ? 4 : 8, N = 32 / V;
+  typedef typename std::conditional<LT == TY_F32, float, uint16_t>::type E;
+  typedef E vec __attribute__((ext_vector_type(V), aligned(sizeof(E))));
+  vec x[N];
+  __device__ __forceinline__ void load(const void* row, uint32_t v0, uint32_t vocab) {
+    const E* p = static_cast<const E*>(row);
+    const uint32_t lane = threadIdx.x & 63u;
+    if (v0 + VD_SHARE <= vocab) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = *reinterpret_cast<const vec*>(p + v0 + (64 * j + lane) * V);
+      return;
+    }
+    constexpr E low = LT == TY_F32 ? (E)-INFINITY : LT == TY_F16 ? (E)0xfc00u : (E)0xff80u;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const uint32_t v = v0 + (64 * j + lane) * V + e;
+        x[j][e] = v < vocab ? p[v] : low;
+      }
+  }
+  __device__ __forceinline__ float at(int j, int e) const {
+    if constexpr (LT == TY_F32) return x[j][e];
+    else return from_bits16<LT>(x[j][e]);
+  }
+  static __device__ __forceinline__ uint32_t index(uint32_t v0, int j, int e) {
+    return v0 + (64 * j + (threadIdx.x & 63u)) * V + e;
+  }
+};
+
+struct VdArgs {
+  const void* target;
+  const void* draft;  // null: drafts are certain
+  const uint32_t* tokens;
+  const uint32_t* draft_lens;
+  const float* temperature;
+  const float* uniforms;
+  VdPart* parts;      // [seq][row][share]: target rows 0 .. n_draft, then draft rows
+  double* rest;       // [seq][share]: sums of max(p - q, 0) of a sequence that rejected a draft
+  uint32_t* accepted;
+  uint32_t* out;
+  float* logprobs;
+  uint32_t n_draft, vocab, shares;
+};
+
+__device__ __forceinline__ uint32_t vd_rows(const VdArgs& a) { return a.draft ? 2 * a.n_draft + 1 : a.n_draft + 1; }
+__device__ __forceinline__ uint32_t vd_drafts(const VdArgs& a, uint32_t s) {
+  return a.draft_lens ? min(a.draft_lens[s], a.n_draft) : a.n_draft;
+}
+template <int LT>
+__device__ __forceinline__ const void* vd_target(const VdArgs& a, uint32_t s, uint32_t t) {
+  return static_cast<const char*>(a.target) + ((size_t)s * (a.n_draft + 1) + t) * a.vocab * (LT == TY_F32 ? 4 : 2);
+}
+template <int LT>
+__device__ __forceinline__ const void* vd_draft(const VdArgs& a, uint32_t s, uint32_t t) {
+  return static_cast<const char*>(a.draft) + ((size_t)s * a.n_draft + t) * a.vocab * (LT == TY_F32 ? 4 : 2);
+}
+
+// Each wave a share of a row: grid (4 shares, row) flattened.
+template <int LT>
+__global__ __launch_bounds__(VD_NT) void k_vd_stats(VdArgs a) {
+  __shared__ double tab[64];
+  const uint32_t groups = (a.shares + 3) / 4, row = blockIdx.x / groups;
+  const uint32_t share = (blockIdx.x - row * groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t rows = vd_rows(a), s = row / rows, r = row - s * rows;
+  const uint32_t n = vd_drafts(a, s);
+  const bool is_target = r <= a.n_draft;
+  const uint32_t t = is_target ? r : r - a.n_draft - 1;
   if (is_target ? t > n : t >= n) return;
-  const void* src = is_target ? target : draft;
-  const size_t base = ((size_t)s * (is_target ? n_draft + 1 : n_draft) + t) * vocab;
-  const uint32_t v0 = blockIdx.x * VD_CHUNK, v1 = min(vocab, v0 + VD_CHUNK);
-  float m = -INFINITY;
-  uint32_t at = v0;
-  for (uint32_t v = v0 + threadIdx.x; v < v1; v += VD_NT) vd_max(m, at, load_as_f32<LT>(src, base + v), v);
-  for (int o = 32; o; o >>= 1) {
-    const float m2 = __shfl_xor(m, o);
-    const uint32_t i2 = __shfl_xor(at, o);
-    vd_max(m, at, m2, i2);
-  }
-  const uint32_t w = threadIdx.x >> 6;
-  if ((threadIdx.x & 63u) == 0) {
-    sm[w] = m;
-    si[w] = at;
-  }
+  const bool live = share < a.shares;
+  VdLogits<LT> x;
+  const uint32_t v0 = share * VD_SHARE;
+  const float temp = a.temperature[s];
+  if (live) x.load(is_target ? vd_target<LT>(a, s, t) : vd_draft<LT>(a, s, t), v0, a.vocab);
+  vd_table(tab);
   __syncthreads();
-  m = sm[0];
-  at = si[0];
-  for (int i = 1; i < VD_NT / 64; ++i) vd_max(m, at, sm[i], si[i]);
+  if (!live) return;
+  uint32_t top = 0, at = 0xffffffffu;
+#pragma unroll
+  for (int j = 0; j < x.N; ++j)
+#pragma unroll
+    for (int e = 0; e < x.V; ++e) top = max(top, vd_key(x.at(j, e)));
+  for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor(top, o));
+#pragma unroll
+  for (int j = x.N - 1; j >= 0; --j)
+#pragma unroll
+    for (int e = x.V - 1; e >= 0; --e)
+      if (vd_key(x.at(j, e)) == top) at = x.index(v0, j, e);
+  for (int o = 32; o; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o));
+  const float m = vd_unkey(top);
   double z = 0.0;
   if (!vd_bad(m)) {
-    const double inv_t = vd_inv(temperature[s]);
-    for (uint32_t v = v0 + threadIdx.x; v < v1; v += VD_NT) z += vd_exp(load_as_f32<LT>(src, base + v), m, inv_t);
+    const double by = vd_by(temp), md = (double)m;
+#pragma unroll
+    for (int j = 0; j < x.N; ++j)
+#pragma unroll
+      for (int e = 0; e < x.V; ++e) z += vd_exp((double)x.at(j, e) - md, by, tab);
+    z = vd_wave_sum(z);
   }
-  z = vd_wave_sum(z);
-  if ((threadIdx.x & 63u) == 0) sz[w] = z;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < VD_NT / 64; ++i) z += sz[i];
-    parts[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = VdPart{z, m, at};
-  }
+  if ((threadIdx.x & 63u) == 0) a.parts[(size_t)row * a.shares + share] = VdPart{z, m, at};
 }
 
-// A row's statistics from its shares.
-__device__ __forceinline__ VdPart vd_row(const VdPart* p, uint32_t n, double inv_t) {
-  float m = p[0].m;
-  uint32_t at = p[0].i;
-  for (uint32_t i = 1; i < n; ++i) vd_max(m, at, p[i].m, p[i].i);
-  double z = 0.0;
-  if (!vd_bad(m))
-    for (uint32_t i = 0; i < n; ++i) z += p[i].z * vd_exp(p[i].m, m, inv_t);
-  return VdPart{z, m, at};
-}
+// ---- acceptance: every workgroup of k_vd_rest and k_vd_pick works out its sequence's
+enum { VD_DRAW = 0, VD_GREEDY = 1, VD_NONE = 2 };
+struct VdShared {
+  double tab[64];
+  VdPart row[VD_MAX_ROWS + 1];  // a row's largest logit, its index, the sum over the row
+  uint32_t took, state;
+};
 
-// One workgroup per sequence: acceptance, then the token drawn at the row where it ends.
-constexpr int VP_NT = 1024;
 template <int LT>
-__global__ __launch_bounds__(VP_NT) void k_vd_pick(const void* __restrict__ target, const void* __restrict__ draft,
-                                                   const uint32_t* __restrict__ tokens,
-                                                   const uint32_t* __restrict__ draft_lens, uint32_t n_draft,
-                                                   uint32_t vocab, const float* __restrict__ temperature,
-                                                   const float* __restrict__ uniforms, uint32_t n_parts,
-                                                   const VdPart* __restrict__ parts, uint32_t* __restrict__ accepted,
-                                                   uint32_t* __restrict__ out, float* __restrict__ logprobs) {
-  __shared__ VdPart s_row[64];
-  __shared__ uint32_t s_took, s_state;  // state 0: draw, 1: greedy, 2: no distribution
-  __shared__ double s_sum[VP_NT];
-  __shared__ uint32_t s_pick;
-  const uint32_t s = blockIdx.x, tid = threadIdx.x;
-  const uint32_t rows = draft ? 2 * n_draft + 1 : n_draft + 1;
-  const uint32_t n = draft_lens ? min(draft_lens[s], n_draft) : n_draft;
-  const float temp = temperature[s];
+__device__ __forceinline__ void vd_accept(const VdArgs& a, uint32_t s, VdShared& sh) {
+  const uint32_t tid = threadIdx.x, rows = vd_rows(a), n = vd_drafts(a, s);
+  const float temp = a.temperature[s];
   const bool greedy = vd_greedy(temp);
-  const double inv_t = vd_inv(temp);
-  if (tid < rows) {
-    const uint32_t t = tid <= n_draft ? tid : tid - n_draft - 1;
-    if (tid <= n_draft ? t <= n : t < n) s_row[tid] = vd_row(parts + ((size_t)s * rows + tid) * n_parts, n_parts, inv_t);
-  }
+  const double by = vd_by(temp);
+  vd_table(sh.tab);
   __syncthreads();
-  const uint32_t* tok = tokens + (size_t)s * n_draft;
-  const float* u = uniforms + (size_t)s * (n_draft + 1);
-  if (tid == 0) {
-    uint32_t t = 0, state = greedy ? 1 : 0;
-    for (;; ++t) {
-      const VdPart& P = s_row[t];
-      if (vd_bad(P.m)) state = 2;
-      if (t < n && draft && !greedy && vd_bad(s_row[n_draft + 1 + t].m)) state = 2;
-      if (t == n || state == 2) break;
-      const uint32_t x = tok[t];
-      if (greedy) {
-        if (x != P.i) break;
-        continue;
+  for (uint32_t r = tid >> 4; r < rows; r += VD_NT / 16) {  // 16 lanes a row
+    const uint32_t t = r <= a.n_draft ? r : r - a.n_draft - 1, lane = tid & 15u;
+    if (r <= a.n_draft ? t > n : t >= n) continue;
+    const VdPart* p = a.parts + ((size_t)s * rows + r) * a.shares;
+    uint32_t top = 0, at = 0xffffffffu;
+    for (uint32_t i = lane; i < a.shares; i += 16) {
+      const uint32_t k = vd_key(p[i].m);
+      if (k > top) {
+        top = k;
+        at = p[i].i;
       }
-      if (x >= vocab) break;
-      const double px = vd_exp(load_as_f32<LT>(target, ((size_t)s * (n_draft + 1) + t) * vocab + x), P.m, inv_t) / P.z;
-      double qx = 1.0;
-      if (draft) {
-        const VdPart& Q = s_row[n_draft + 1 + t];
-        qx = vd_exp(load_as_f32<LT>(draft, ((size_t)s * n_draft + t) * vocab + x), Q.m, inv_t) / Q.z;
-      }
-      if (!((double)u[t] * qx < px)) break;
     }
-    s_took = t;
-    s_state = state;
+    for (int o = 8; o; o >>= 1) {
+      const uint32_t k2 = __shfl_xor(top, o), i2 = __shfl_xor(at, o);
+      if (k2 > top || (k2 == top && i2 < at)) {
+        top = k2;
+        at = i2;
+      }
+    }
+    const float m = vd_unkey(top);
+    double z = 0.0;
+    if (!vd_bad(m))
+      for (uint32_t i = lane; i < a.shares; i += 16) z += p[i].z * vd_exp((double)p[i].m - (double)m, by, sh.tab);
+    for (int o = 8; o; o >>= 1) z += __shfl_xor(z, o);
+    if (lane == 0) sh.row[r] = VdPart{z, m, at};
   }
   __syncthreads();
-  const uint32_t took = s_took;
-  const VdPart P = s_row[took];
-  const size_t pb = ((size_t)s * (n_draft + 1) + took) * vocab;
-  uint32_t pick = 0xffffffffu;
-  if (s_state == 1) {
-    pick = P.i;
-  } else if (s_state == 0) {
-    const bool rejected = took < n;
-    const VdPart Q = rejected && draft ? s_row[n_draft + 1 + took] : VdPart{1.0, 0.0f, 0};
-    const size_t qb = ((size_t)s * n_draft + took) * vocab;
-    const uint32_t x = rejected ? tok[took] : 0xffffffffu;
-    auto mass = [&](uint32_t v, bool whole) {
-      const double p = vd_exp(load_as_f32<LT>(target, pb + v), P.m, inv_t) / P.z;
-      if (!rejected || whole) return p;
-      const double q = draft ? vd_exp(load_as_f32<LT>(draft, qb + v), Q.m, inv_t) / Q.z : (v == x ? 1.0 : 0.0);
-      return fmax(p - q, 0.0);
-    };
-    const uint32_t per = (vocab + VP_NT - 1) / VP_NT, a = tid * per, b = min(vocab, a + per);
-    bool whole = false;
-    double total = 0.0;
-    for (int round = 0; round < 2; ++round) {  // (nothing left of p - q: p itself)
-      double z = 0.0;
-      for (uint32_t v = a; v < b; ++v) z += mass(v, whole);
-      s_sum[tid] = z;
-      __syncthreads();
-      total = 0.0;
-      if (tid == 0) {
-        for (int i = 0; i < VP_NT; ++i) {
-          const double y = s_sum[i];
-          s_sum[i] = total;
-          total += y;
+  if (tid < 64) {  // a lane per draft
+    const uint32_t t = tid;
+    bool go = false, none = false;
+    if (t <= n) {
+      const VdPart P = sh.row[t];
+      none = vd_bad(P.m) || (t < n && a.draft && !greedy && vd_bad(sh.row[a.n_draft + 1 + t].m));
+      if (t < n && !none) {
+        const uint32_t x = a.tokens[(size_t)s * a.n_draft + t];
+        if (greedy) {
+          go = x == P.i;
+        } else if (x < a.vocab) {
+          const double px = vd_exp((double)load_as_f32<LT>(vd_target<LT>(a, s, t), x) - (double)P.m, by, sh.tab) / P.z;
+          double qx = 1.0;
+          if (a.draft) {
+            const VdPart Q = sh.row[a.n_draft + 1 + t];
+            qx = vd_exp((double)load_as_f32<LT>(vd_draft<LT>(a, s, t), x) - (double)Q.m, by, sh.tab) / Q.z;
+          }
+          go = (double)a.uniforms[(size_t)s * (a.n_draft + 1) + t] * qx < px;
         }
-        s_sum[0] = total;  // (the first share begins at 0)
-        s_pick = 0xffffffffu;
       }
+    }
+    const uint32_t took = __builtin_ctzll(~__ballot(go));  // (lane n does not go on)
+    if (t == took) {
+      sh.took = took;
+      sh.state = none ? VD_NONE : greedy ? VD_GREEDY : VD_DRAW;
+    }
+  }
+  __syncthreads();
+}
+
+// max(p - q, 0) of this lane's logits of a share, in its order
+template <int LT, typename F>
+__device__ __forceinline__ void vd_rest_of(const VdLogits<LT>& x, const VdLogits<LT>& y, VdPart P, VdPart Q, double by,
+                                           const double* tab, F take) {
+  const double ip = 1.0 / P.z, iq = 1.0 / Q.z, mp = (double)P.m, mq = (double)Q.m;
+#pragma unroll
+  for (int j = 0; j < x.N; ++j)
+#pragma unroll
+    for (int e = 0; e < x.V; ++e)
+      take(j, e, fmax(vd_exp((double)x.at(j, e) - mp, by, tab) * ip - vd_exp((double)y.at(j, e) - mq, by, tab) * iq, 0.0));
+}
+
+// Draft distributions only: the sums of max(p - q, 0) over the shares, a wave each.
+template <int LT>
+__global__ __launch_bounds__(VD_NT) void k_vd_rest(VdArgs a) {
+  __shared__ VdShared sh;
+  const uint32_t groups = (a.shares + 3) / 4, s = blockIdx.x / groups;
+  const uint32_t share = (blockIdx.x - s * groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  vd_accept<LT>(a, s, sh);
+  const uint32_t took = sh.took;
+  if (sh.state != VD_DRAW || took >= vd_drafts(a, s) || share >= a.shares) return;
+  VdLogits<LT> x, y;
+  x.load(vd_target<LT>(a, s, took), share * VD_SHARE, a.vocab);
+  y.load(vd_draft<LT>(a, s, took), share * VD_SHARE, a.vocab);
+  double sum = 0.0;
+  vd_rest_of<LT>(x, y, sh.row[took], sh.row[a.n_draft + 1 + took], vd_by(a.temperature[s]), sh.tab,
+                 [&](int, int, double v) { sum += v; });
+  sum = vd_wave_sum(sum);
+  if ((threadIdx.x & 63u) == 0) a.rest[(size_t)s * a.shares + share] = sum;
+}
+
+// Inclusive prefix sum over the workgroup; *total the whole.
+__device__ __forceinline__ double vd_scan(double v, double* wave_sums, double* total) {
+  const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(v, o);
+    if (lane >= (uint32_t)o) v += y;
+  }
+  if (lane == 63) wave_sums[w] = v;
+  __syncthreads();
+  double all = 0.0;
+  for (uint32_t i = 0; i < VD_NT / 64; ++i) {
+    if (i == w) v += all;
+    all += wave_sums[i];
+  }
+  __syncthreads();
+  *total = all;
+  return v;
+}
+
+// One workgroup per sequence: acceptance, the share that the number falls into, the token in it.
+template <int LT>
+__global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
+  __shared__ VdShared sh;
+  __shared__ double wave_sums[VD_NT / 64];
+  __shared__ double s_x;
+  __shared__ uint32_t s_first, s_last, s_share;
+  __shared__ double s_before;
+  const uint32_t s = blockIdx.x, tid = threadIdx.x, n = vd_drafts(a, s);
+  vd_accept<LT>(a, s, sh);
+  const uint32_t took = sh.took, state = sh.state;
+  const double by = vd_by(a.temperature[s]);
+  const uint32_t* tok = a.tokens + (size_t)s * a.n_draft;
+  uint32_t pick = 0xffffffffu;
+  if (state == VD_GREEDY) {
+    pick = sh.row[took].i;
+  } else if (state == VD_DRAW) {
+    const VdPart P = sh.row[took];
+    const bool rejected = took < n, apart = rejected && a.draft;  // apart: max(p - q, 0), in units of p
+    const VdPart Q = apart ? sh.row[a.n_draft + 1 + took] : P;
+    const uint32_t x_tok = rejected && !a.draft ? tok[took] : 0xffffffffu;  // its whole mass is taken away
+    const void* prow = vd_target<LT>(a, s, took);
+    const void* qrow = apart ? vd_draft<LT>(a, s, took) : prow;
+    const VdPart* parts = a.parts + ((size_t)s * vd_rows(a) + took) * a.shares;
+    // this thread's 8 logits of a share: their masses (without a draft distribution in units of
+    // exp((l - max) / T))
+    const auto masses = [&](uint32_t share, bool whole, double (&m)[8]) {
+      const uint32_t v0 = share * VD_SHARE + tid * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t v = v0 + i;
+        double y = 0.0;
+        if (v < a.vocab && (whole || v != x_tok)) {
+          y = vd_exp((double)load_as_f32<LT>(prow, v) - (double)P.m, by, sh.tab);
+          if (apart && !whole)
+            y = fmax(y * (1.0 / P.z) - vd_exp((double)load_as_f32<LT>(qrow, v) - (double)Q.m, by, sh.tab) * (1.0 / Q.z), 0.0);
+        }
+        m[i] = y;
+      }
+    };
+    double m[8];
+    if (x_tok < a.vocab) {  // the share of a certain draft, without it
+      masses(x_tok / VD_SHARE, false, m);
+      double sum = 0.0, total;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += m[i];
+      vd_scan(sum, wave_sums, &total);
+      if (tid == 0) s_x = total;
       __syncthreads();
-      total = s_sum[0];
+    }
+    const uint32_t per = (a.shares + VD_NT - 1) / VD_NT, i0 = min(a.shares, tid * per), i1 = min(a.shares, i0 + per);
+    bool whole = false;
+    double total = 0.0, before = 0.0;
+    const auto share_sum = [&](uint32_t i) {
+      if (apart && !whole) return a.rest[(size_t)s * a.shares + i];
+      if (!whole && i == x_tok / VD_SHARE && x_tok < a.vocab) return s_x;
+      return parts[i].z * vd_exp((double)parts[i].m - (double)P.m, by, sh.tab);
+    };
+    for (int round = 0; round < 2; ++round) {  // (nothing left: p itself)
+      double sum = 0.0;
+      for (uint32_t i = i0; i < i1; ++i) sum += share_sum(i);
+      const double incl = vd_scan(sum, wave_sums, &total);
+      before = incl - sum;
       if (total > 0.0) break;
-      __syncthreads();
       whole = true;
     }
-    const double want = (double)u[n_draft] * total;
-    double c = tid == 0 ? 0.0 : s_sum[tid];
-    uint32_t last = 0xffffffffu;
-    for (uint32_t v = a; v < b; ++v) {
-      const double y = mass(v, whole);
-      c += y;
-      if (y > 0.0) last = v;
-      if (c > want) {
-        atomicMin(&s_pick, v);
-        break;
+    const double want = (double)a.uniforms[(size_t)s * (a.n_draft + 1) + a.n_draft] * total;
+    if (tid == 0) {
+      s_first = s_share = 0xffffffffu;
+      s_last = 0;
+    }
+    __syncthreads();
+    {
+      double c = before;
+      uint32_t last = 0xffffffffu, found = 0xffffffffu;
+      for (uint32_t i = i0; i < i1; ++i) {
+        const double y = share_sum(i);
+        c += y;
+        if (y > 0.0) last = i;
+        if (c > want && y > 0.0) {
+          found = i;
+          break;
+        }
       }
+      if (found != 0xffffffffu) atomicMin(&s_share, found);
+      if (last != 0xffffffffu) atomicMax(&s_last, last);
     }
     __syncthreads();
-    pick = s_pick;
-    __syncthreads();
-    if (pick == 0xffffffffu) {  // u S rounded up to S: the last token with any mass
-      if (tid == 0) s_pick = 0;
-      __syncthreads();
-      if (last != 0xffffffffu) atomicMax(&s_pick, last);
-      __syncthreads();
-      pick = s_pick;
+    const uint32_t share = s_share != 0xffffffffu ? s_share : s_last;  // (u S rounded up to S: the last with any mass)
+    if (share >= i0 && share < i1) {
+      double c = before;
+      for (uint32_t i = i0; i < share; ++i) c += share_sum(i);
+      s_before = c;
     }
+    __syncthreads();
+    masses(share, whole, m);
+    double sum = 0.0, unused;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += m[i];
+    const double incl = vd_scan(sum, wave_sums, &unused);
+    if (tid == 0) s_last = 0;
+    __syncthreads();
+    {
+      double c = s_before + (incl - sum);
+      uint32_t last = 0xffffffffu, found = 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t v = share * VD_SHARE + tid * 8 + i;
+        c += m[i];
+        if (m[i] > 0.0) {
+          last = v;
+          if (c > want && found == 0xffffffffu) found = v;
+        }
+      }
+      if (found != 0xffffffffu) atomicMin(&s_first, found);
+      if (last != 0xffffffffu) atomicMax(&s_last, last);
+    }
+    __syncthreads();
+    pick = s_first != 0xffffffffu ? s_first : s_last;
   }
-  if (tid == 0) accepted[s] = took;
-  if (tid <= n_draft) {
+  if (tid == 0) a.accepted[s] = took;
+  if (tid <= a.n_draft) {
     const uint32_t x = tid < took ? tok[tid] : tid == took ? pick : 0xffffffffu;
-    out[(size_t)s * (n_draft + 1) + tid] = x;
-    if (logprobs) {
+    a.out[(size_t)s * (a.n_draft + 1) + tid] = x;
+    if (a.logprobs) {
       float lp = 0.0f;
       if (tid <= took) {
-        const VdPart& R = s_row[tid];
-        lp = x < vocab ? (float)(((double)load_as_f32<LT>(target, ((size_t)s * (n_draft + 1) + tid) * vocab + x) -
-                                  (double)R.m) * inv_t - log(R.z))
-                       : NAN;
+        lp = NAN;
+        if (x < a.vocab) {
+          const VdPart R = sh.row[tid];
+          const float temp = a.temperature[s];
+          const double y = (double)load_as_f32<LT>(vd_target<LT>(a, s, tid), x) - (double)R.m;
+          lp = (float)(y / (vd_greedy(temp) ? 1.0 : (double)temp) - log(R.z));
+        }
       }
-      logprobs[(size_t)s * (n_draft + 1) + tid] = lp;
+      a.logprobs[(size_t)s * (a.n_draft + 1) + tid] = lp;
     }
   }
 }

@@ -256,10 +256,13 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
   return launched(me);
 }
 
-static uint32_t vd_parts(uint32_t vocab) { return (vocab + cm::VD_CHUNK - 1) / cm::VD_CHUNK; }
+static uint32_t vd_shares(uint32_t vocab) { return (vocab + cm::VD_SHARE - 1) / cm::VD_SHARE; }
+static size_t vd_parts_bytes(uint64_t n_seqs, uint64_t n_draft, uint32_t vocab) {
+  return up256(n_seqs * (2 * n_draft + 1) * vd_shares(vocab) * sizeof(cm::VdPart));
+}
 
 size_t camelid_hip_verify_drafts_workspace(uint32_t n_seqs, uint32_t n_draft, uint32_t vocab) {
-  return up256((size_t)n_seqs * (2 * (size_t)n_draft + 1) * vd_parts(vocab) * sizeof(cm::VdPart));
+  return vd_parts_bytes(n_seqs, n_draft, vocab) + up256((size_t)n_seqs * vd_shares(vocab) * 8);
 }
 
 int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint32_t logits_type,
@@ -282,19 +285,32 @@ int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint
     return cm::fail_global(me, "the workspace must be 16-byte aligned, the rest aligned to its elements");
   if (workspace_bytes < camelid_hip_verify_drafts_workspace(n_seqs, n_draft, vocab))
     return cm::fail_global(me, "workspace too small (camelid_hip_verify_drafts_workspace)");
-  const void* draft = n_draft ? draft_logits : nullptr;
-  const uint32_t rows = draft ? 2 * n_draft + 1 : n_draft + 1, parts = vd_parts(vocab);
-  cm::VdPart* ws = static_cast<cm::VdPart*>(workspace);
-  if ((uint64_t)n_seqs * rows > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
-  const auto go = [&](auto stats, auto pick) {
-    hipLaunchKernelGGL(stats, dim3(parts, n_seqs * rows), dim3(cm::VD_NT), 0, (hipStream_t)stream, target, draft,
-                       draft_lens, n_draft, vocab, temperature, ws);
-    hipLaunchKernelGGL(pick, dim3(n_seqs), dim3(cm::VP_NT), 0, (hipStream_t)stream, target, draft, draft_tokens,
-                       draft_lens, n_draft, vocab, temperature, uniforms, parts, ws, accepted, tokens_out, logprobs_out);
+  cm::VdArgs a{};
+  a.target = target;
+  a.draft = n_draft ? draft_logits : nullptr;
+  a.tokens = draft_tokens;
+  a.draft_lens = draft_lens;
+  a.temperature = temperature;
+  a.uniforms = uniforms;
+  a.parts = static_cast<cm::VdPart*>(workspace);
+  a.rest = reinterpret_cast<double*>(static_cast<char*>(workspace) + vd_parts_bytes(n_seqs, n_draft, vocab));
+  a.accepted = accepted;
+  a.out = tokens_out;
+  a.logprobs = logprobs_out;
+  a.n_draft = n_draft;
+  a.vocab = vocab;
+  a.shares = vd_shares(vocab);
+  const uint64_t rows = a.draft ? 2 * n_draft + 1 : n_draft + 1, groups = (a.shares + 3) / 4;
+  if (n_seqs * rows * groups > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  const auto go = [&](auto stats, auto rest, auto pick) {
+    hipLaunchKernelGGL(stats, dim3((uint32_t)(n_seqs * rows * groups)), dim3(cm::VD_NT), 0, (hipStream_t)stream, a);
+    if (a.draft)
+      hipLaunchKernelGGL(rest, dim3((uint32_t)(n_seqs * groups)), dim3(cm::VD_NT), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(pick, dim3(n_seqs), dim3(cm::VD_NT), 0, (hipStream_t)stream, a);
   };
-  if (logits_type == TY_F32) go(cm::k_vd_stats<TY_F32>, cm::k_vd_pick<TY_F32>);
-  else if (logits_type == TY_F16) go(cm::k_vd_stats<TY_F16>, cm::k_vd_pick<TY_F16>);
-  else go(cm::k_vd_stats<TY_BF16>, cm::k_vd_pick<TY_BF16>);
+  if (logits_type == TY_F32) go(cm::k_vd_stats<TY_F32>, cm::k_vd_rest<TY_F32>, cm::k_vd_pick<TY_F32>);
+  else if (logits_type == TY_F16) go(cm::k_vd_stats<TY_F16>, cm::k_vd_rest<TY_F16>, cm::k_vd_pick<TY_F16>);
+  else go(cm::k_vd_stats<TY_BF16>, cm::k_vd_rest<TY_BF16>, cm::k_vd_pick<TY_BF16>);
   return launched(me);
 }
 
