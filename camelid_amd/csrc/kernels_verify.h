@@ -35,29 +35,44 @@ struct VdPart {
   uint32_t i;
 };
 
-// ---- 2^(x / 64) for whole x: a table of 64 powers in LDS
-__device__ __forceinline__ void vd_table(double* tab) {
-  if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+// ---- exp(y / T) for y <= 0, by = 32 log2(e) / T: y by = k + r, |r| <= 1/2; 2^(k / 32) from a table in
+// LDS, e^(r ln 2 / 32) by its series to the fifth power (the next term is below 2.3e-15).  32 entries of 8
+// bytes: every one in banks of its own, lanes that read the same one share it.
+// (kExp2Tab: the bits of 2^(i / 32) less i << 47, so that adding k << 47 makes 2^(k / 32).)
+__device__ __forceinline__ void vd_table(uint64_t* tab) {
+  if (threadIdx.x < 32) tab[threadIdx.x] = kExp2Tab[threadIdx.x];
 }
-// exp(y / T) for y <= 0, by = 64 log2(e) / T: y by = k + r, |r| <= 1/2; 2^(k / 64) from the table, e^(r ln 2 / 64)
-// by its series to the fifth power (the next term is below 4e-17).
-__device__ __forceinline__ double vd_exp(double y, double by, const double* tab) {
-  constexpr double A = 0x1.62e42fefa39efp-1 / 64.0;  // ln 2 / 64
-  const double k = fmax(rint(y * by), -131072.0);  // (2^-2048 and below, y = -inf: 0)
-  const double r = fmax(fma(y, by, -k), -1.0);
-  const int n = (int)k;
+__device__ __forceinline__ double vd_series(double r) {
+  constexpr double A = 0x1.62e42fefa39efp-1 / 32.0;  // ln 2 / 32
   double p = fma(r, A * A * A * A * A / 120.0, A * A * A * A / 24.0);
   p = fma(r, p, A * A * A / 6.0);
   p = fma(r, p, A * A / 2.0);
   p = fma(r, p, A);
-  p = fma(r, p, 1.0);
-  return ldexp(p * tab[n & 63], n >> 6);
+  return fma(r, p, 1.0);
+}
+// Any y <= 0, -inf included; 0 below the exponent range.
+__device__ __forceinline__ double vd_exp(double y, double by, const uint64_t* tab) {
+  const double k = fmax(rint(y * by), -65536.0);
+  const double r = fmax(fma(y, by, -k), -1.0);
+  const int n = (int)k;
+  // 2^(n % 32 / 32) from the table, the rest of n by ldexp (which rounds into the subnormals)
+  return ldexp(vd_series(r) * u2d(tab[n & 31] + ((uint64_t)(n & 31) << 47)), n >> 5);
+}
+// y / T >= -704, so that 2^(k / 32) has a normal exponent: no conversions, the exponent added as bits.
+__device__ __forceinline__ double vd_exp_near(double y, double by, const uint64_t* tab) {
+  const double kd = fma(y, by, 0x1.8p52);  // k in the low bits
+  const uint32_t n = (uint32_t)d2u(kd);
+  const double r = fma(y, by, 0x1.8p52 - kd);
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  u32x2 t = __builtin_bit_cast(u32x2, tab[n & 31u]);  // + n << 47
+  t.y += n << 15;
+  return vd_series(r) * __builtin_bit_cast(double, t);
 }
 
 __device__ __forceinline__ bool vd_greedy(float t) { return !(t > 0.0f); }
-// 64 log2(e) / T; a greedy sequence's log-probabilities are those of T = 1
+// 32 log2(e) / T; a greedy sequence's log-probabilities are those of T = 1
 __device__ __forceinline__ double vd_by(float t) {
-  return 64.0 * 0x1.71547652b82fep+0 / (vd_greedy(t) ? 1.0 : (double)t);
+  return 32.0 * 0x1.71547652b82fep+0 / (vd_greedy(t) ? 1.0 : (double)t);
 }
 
 // A row without a distribution: a NaN or +inf logit, or none above -inf.
@@ -72,10 +87,37 @@ __device__ __forceinline__ float vd_unkey(uint32_t k) {
   return k == 0xffffffffu ? NAN : u2f((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-__device__ __forceinline__ double vd_wave_sum(double v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// A lane's value moved by data-parallel moves; 0 where there is none to move.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double vd_dpp(double x) {
+  const uint64_t u = d2u(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return u2d(((uint64_t)hi << 32) | lo);
 }
+// Inclusive prefix sum over the wave.
+__device__ __forceinline__ double vd_wave_scan(double x) {
+  x += vd_dpp<0x111>(x);
+  x += vd_dpp<0x112>(x);
+  x += vd_dpp<0x114>(x);
+  x += vd_dpp<0x118>(x);
+  x += vd_dpp<0x142, 0xa>(x);
+  x += vd_dpp<0x143, 0xc>(x);
+  return x;
+}
+// The wave's maximum, NaN passed over, in every lane.
+__device__ __forceinline__ float vd_wave_max(float x) {
+  x = fmaxf(x, u2f((uint32_t)__builtin_amdgcn_update_dpp((int)f2u(x), (int)f2u(x), 0xb1, 0xf, 0xf, false)));
+  x = fmaxf(x, u2f((uint32_t)__builtin_amdgcn_update_dpp((int)f2u(x), (int)f2u(x), 0x4e, 0xf, 0xf, false)));
+  x = fmaxf(x, u2f((uint32_t)__builtin_amdgcn_update_dpp((int)f2u(x), (int)f2u(x), 0x141, 0xf, 0xf, false)));
+  x = fmaxf(x, u2f((uint32_t)__builtin_amdgcn_update_dpp((int)f2u(x), (int)f2u(x), 0x140, 0xf, 0xf, false)));
+  const auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+  x = fmaxf(u2f(a[0]), u2f(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+  return fmaxf(u2f(b[0]), u2f(b[1]));
+}
+// The wave's sum, in its last lane.
+__device__ __forceinline__ double vd_wave_sum(double x) { return vd_wave_scan(x); }
 
 // This lane's logits of the share that begins at v0: vectors of 16 bytes (rows may begin at any element),
 // vector j of lane i at v0 + (64 j + i) V; -inf behind the row's end.
@@ -139,54 +181,84 @@ __device__ __forceinline__ const void* vd_draft(const VdArgs& a, uint32_t s, uin
   return static_cast<const char*>(a.draft) + ((size_t)s * a.n_draft + t) * a.vocab * (LT == TY_F32 ? 4 : 2);
 }
 
-// Each wave a share of a row: grid (4 shares, row) flattened.
+// The logits' exponentials of a share, one after the other: by vd_exp_near, and 0 below e^-704 (EXACT;
+// else some e^-704 there: nothing beside the 1 of the maximum), unless the temperature is so high that
+// this bound is beyond f32.
+template <int LT, bool EXACT, typename F>
+__device__ __forceinline__ void vd_each(const VdLogits<LT>& x, float m, float temp, const uint64_t* tab, F take) {
+  const double by = vd_by(temp), md = (double)m;
+  const float low = m - 704.0f * (vd_greedy(temp) ? 1.0f : temp);
+  if (low > -1e38f) {
+#pragma unroll
+    for (int j = 0; j < x.N; ++j)
+#pragma unroll
+      for (int e = 0; e < x.V; ++e) {
+        const float l = x.at(j, e);
+        const double y = vd_exp_near((double)fmaxf(l, low) - md, by, tab);
+        take(j, e, !EXACT || l > low ? y : 0.0);
+      }
+  } else {
+#pragma unroll
+    for (int j = 0; j < x.N; ++j)
+#pragma unroll
+      for (int e = 0; e < x.V; ++e) take(j, e, vd_exp((double)x.at(j, e) - md, by, tab));
+  }
+}
+
+// Each wave `per` shares of a row.
 template <int LT>
-__global__ __launch_bounds__(VD_NT) void k_vd_stats(VdArgs a) {
-  __shared__ double tab[64];
-  const uint32_t groups = (a.shares + 3) / 4, row = blockIdx.x / groups;
-  const uint32_t share = (blockIdx.x - row * groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(VD_NT) void k_vd_stats(VdArgs a, uint32_t per) {
+  __shared__ uint64_t tab[32];
+  const uint32_t groups = (a.shares + 4 * per - 1) / (4 * per), row = blockIdx.x / groups;
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t first = ((blockIdx.x - row * groups) * 4 + w) * per, end = min(a.shares, first + per);
   const uint32_t rows = vd_rows(a), s = row / rows, r = row - s * rows;
   const uint32_t n = vd_drafts(a, s);
   const bool is_target = r <= a.n_draft;
   const uint32_t t = is_target ? r : r - a.n_draft - 1;
   if (is_target ? t > n : t >= n) return;
-  const bool live = share < a.shares;
-  VdLogits<LT> x;
-  const uint32_t v0 = share * VD_SHARE;
+  const void* src = is_target ? vd_target<LT>(a, s, t) : vd_draft<LT>(a, s, t);
   const float temp = a.temperature[s];
-  if (live) x.load(is_target ? vd_target<LT>(a, s, t) : vd_draft<LT>(a, s, t), v0, a.vocab);
+  const bool greedy = vd_greedy(temp);
+  VdLogits<LT> x;
+  if (first < end) x.load(src, first * VD_SHARE, a.vocab);
   vd_table(tab);
   __syncthreads();
-  if (!live) return;
-  uint32_t top = 0, at = 0xffffffffu;
-#pragma unroll
-  for (int j = 0; j < x.N; ++j)
-#pragma unroll
-    for (int e = 0; e < x.V; ++e) top = max(top, vd_key(x.at(j, e)));
-  for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor(top, o));
-#pragma unroll
-  for (int j = x.N - 1; j >= 0; --j)
-#pragma unroll
-    for (int e = x.V - 1; e >= 0; --e)
-      if (vd_key(x.at(j, e)) == top) at = x.index(v0, j, e);
-  for (int o = 32; o; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o));
-  const float m = vd_unkey(top);
-  double z = 0.0;
-  if (!vd_bad(m)) {
-    const double by = vd_by(temp), md = (double)m;
+  for (uint32_t share = first; share < end; ++share) {
+    // the maximum passes NaN over; the sum of the logits does not
+    float m = -INFINITY, any = 0.0f;
 #pragma unroll
     for (int j = 0; j < x.N; ++j)
 #pragma unroll
-      for (int e = 0; e < x.V; ++e) z += vd_exp((double)x.at(j, e) - md, by, tab);
-    z = vd_wave_sum(z);
+      for (int e = 0; e < x.V; ++e) {
+        m = fmaxf(m, x.at(j, e));
+        any += x.at(j, e);
+      }
+    m = vd_wave_max(m);
+    if (__ballot(any != any && m < INFINITY)) m = NAN;
+    uint32_t at = 0xffffffffu;
+    double z = 0.0;
+    if (greedy) {  // nobody else asks for the index
+#pragma unroll
+      for (int j = x.N - 1; j >= 0; --j)
+#pragma unroll
+        for (int e = x.V - 1; e >= 0; --e)
+          if (x.at(j, e) == m) at = x.index(share * VD_SHARE, j, e);
+      for (int o = 32; o; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o));
+    }
+    if (!vd_bad(m) && (!greedy || a.logprobs)) {
+      vd_each<LT, false>(x, m, temp, tab, [&](int, int, double e) { z += e; });
+      z = vd_wave_sum(z);
+    }
+    if ((threadIdx.x & 63u) == 63) a.parts[(size_t)row * a.shares + share] = VdPart{z, m, at};
+    if (share + 1 < end) x.load(src, (share + 1) * VD_SHARE, a.vocab);
   }
-  if ((threadIdx.x & 63u) == 0) a.parts[(size_t)row * a.shares + share] = VdPart{z, m, at};
 }
 
 // ---- acceptance: every workgroup of k_vd_rest and k_vd_pick works out its sequence's
 enum { VD_DRAW = 0, VD_GREEDY = 1, VD_NONE = 2 };
 struct VdShared {
-  double tab[64];
+  uint64_t tab[32];
   VdPart row[VD_MAX_ROWS + 1];  // a row's largest logit, its index, the sum over the row
   uint32_t took, state;
 };
@@ -197,53 +269,73 @@ __device__ __forceinline__ void vd_accept(const VdArgs& a, uint32_t s, VdShared&
   const float temp = a.temperature[s];
   const bool greedy = vd_greedy(temp);
   const double by = vd_by(temp);
+  // what draft t is judged by: lane t of the last wave fetches it while the others sum up the rows
+  const uint32_t t = tid - (VD_NT - 64);
+  uint32_t x_t = 0xffffffffu;
+  float u_t = 0.0f, lp_t = 0.0f, lq_t = 0.0f;
+  if (tid >= VD_NT - 64 && t < n) {
+    x_t = a.tokens[(size_t)s * a.n_draft + t];
+    u_t = a.uniforms[(size_t)s * (a.n_draft + 1) + t];
+    if (x_t < a.vocab) {
+      lp_t = load_as_f32<LT>(vd_target<LT>(a, s, t), x_t);
+      if (a.draft) lq_t = load_as_f32<LT>(vd_draft<LT>(a, s, t), x_t);
+    }
+  }
   vd_table(sh.tab);
   __syncthreads();
-  for (uint32_t r = tid >> 4; r < rows; r += VD_NT / 16) {  // 16 lanes a row
+  for (uint32_t r = tid >> 4; r < rows; r += VD_NT / 16) {  // 16 lanes a row, 8 shares a lane at a time
     const uint32_t t = r <= a.n_draft ? r : r - a.n_draft - 1, lane = tid & 15u;
     if (r <= a.n_draft ? t > n : t >= n) continue;
     const VdPart* p = a.parts + ((size_t)s * rows + r) * a.shares;
     uint32_t top = 0, at = 0xffffffffu;
-    for (uint32_t i = lane; i < a.shares; i += 16) {
-      const uint32_t k = vd_key(p[i].m);
-      if (k > top) {
-        top = k;
-        at = p[i].i;
+    double z = 0.0;
+    for (uint32_t b = lane; b < a.shares; b += 128) {
+      VdPart q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = b + 16 * i < a.shares ? p[b + 16 * i] : VdPart{0.0, -INFINITY, 0xffffffffu};
+      const uint32_t was = top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t k = vd_key(q[i].m);
+        at = k > top ? q[i].i : at;
+        top = max(top, k);
+      }
+      const float m = vd_unkey(top);
+      if (!vd_bad(m)) {
+        if (was) z *= vd_exp((double)vd_unkey(was) - (double)m, by, sh.tab);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z += q[i].z * vd_exp((double)q[i].m - (double)m, by, sh.tab);
       }
     }
+    // the 16 lanes' sums against the row's maximum (a lane without a finite one holds z = 0)
+    const uint32_t mine = top;
     for (int o = 8; o; o >>= 1) {
       const uint32_t k2 = __shfl_xor(top, o), i2 = __shfl_xor(at, o);
-      if (k2 > top || (k2 == top && i2 < at)) {
-        top = k2;
-        at = i2;
-      }
+      at = k2 > top || (k2 == top && i2 < at) ? i2 : at;
+      top = max(top, k2);
     }
     const float m = vd_unkey(top);
-    double z = 0.0;
-    if (!vd_bad(m))
-      for (uint32_t i = lane; i < a.shares; i += 16) z += p[i].z * vd_exp((double)p[i].m - (double)m, by, sh.tab);
+    if (!vd_bad(m)) z *= vd_exp((double)vd_unkey(mine) - (double)m, by, sh.tab);
     for (int o = 8; o; o >>= 1) z += __shfl_xor(z, o);
     if (lane == 0) sh.row[r] = VdPart{z, m, at};
   }
   __syncthreads();
-  if (tid < 64) {  // a lane per draft
-    const uint32_t t = tid;
+  if (tid >= VD_NT - 64) {  // a lane per draft
     bool go = false, none = false;
     if (t <= n) {
       const VdPart P = sh.row[t];
       none = vd_bad(P.m) || (t < n && a.draft && !greedy && vd_bad(sh.row[a.n_draft + 1 + t].m));
       if (t < n && !none) {
-        const uint32_t x = a.tokens[(size_t)s * a.n_draft + t];
         if (greedy) {
-          go = x == P.i;
-        } else if (x < a.vocab) {
-          const double px = vd_exp((double)load_as_f32<LT>(vd_target<LT>(a, s, t), x) - (double)P.m, by, sh.tab) / P.z;
+          go = x_t == P.i;
+        } else if (x_t < a.vocab) {
+          const double px = vd_exp((double)lp_t - (double)P.m, by, sh.tab) / P.z;
           double qx = 1.0;
           if (a.draft) {
             const VdPart Q = sh.row[a.n_draft + 1 + t];
-            qx = vd_exp((double)load_as_f32<LT>(vd_draft<LT>(a, s, t), x) - (double)Q.m, by, sh.tab) / Q.z;
+            qx = vd_exp((double)lq_t - (double)Q.m, by, sh.tab) / Q.z;
           }
-          go = (double)a.uniforms[(size_t)s * (a.n_draft + 1) + t] * qx < px;
+          go = (double)u_t * qx < px;
         }
       }
     }
@@ -254,18 +346,6 @@ __device__ __forceinline__ void vd_accept(const VdArgs& a, uint32_t s, VdShared&
     }
   }
   __syncthreads();
-}
-
-// max(p - q, 0) of this lane's logits of a share, in its order
-template <int LT, typename F>
-__device__ __forceinline__ void vd_rest_of(const VdLogits<LT>& x, const VdLogits<LT>& y, VdPart P, VdPart Q, double by,
-                                           const double* tab, F take) {
-  const double ip = 1.0 / P.z, iq = 1.0 / Q.z, mp = (double)P.m, mq = (double)Q.m;
-#pragma unroll
-  for (int j = 0; j < x.N; ++j)
-#pragma unroll
-    for (int e = 0; e < x.V; ++e)
-      take(j, e, fmax(vd_exp((double)x.at(j, e) - mp, by, tab) * ip - vd_exp((double)y.at(j, e) - mq, by, tab) * iq, 0.0));
 }
 
 // Draft distributions only: the sums of max(p - q, 0) over the shares, a wave each.
@@ -280,20 +360,20 @@ __global__ __launch_bounds__(VD_NT) void k_vd_rest(VdArgs a) {
   VdLogits<LT> x, y;
   x.load(vd_target<LT>(a, s, took), share * VD_SHARE, a.vocab);
   y.load(vd_draft<LT>(a, s, took), share * VD_SHARE, a.vocab);
-  double sum = 0.0;
-  vd_rest_of<LT>(x, y, sh.row[took], sh.row[a.n_draft + 1 + took], vd_by(a.temperature[s]), sh.tab,
-                 [&](int, int, double v) { sum += v; });
+  const VdPart P = sh.row[took], Q = sh.row[a.n_draft + 1 + took];
+  const double ip = 1.0 / P.z, iq = 1.0 / Q.z;
+  const float temp = a.temperature[s];
+  double p[32], sum = 0.0;
+  vd_each<LT, true>(x, P.m, temp, sh.tab, [&](int j, int e, double v) { p[j * x.V + e] = v * ip; });
+  vd_each<LT, true>(y, Q.m, temp, sh.tab, [&](int j, int e, double v) { sum += fmax(p[j * x.V + e] - v * iq, 0.0); });
   sum = vd_wave_sum(sum);
-  if ((threadIdx.x & 63u) == 0) a.rest[(size_t)s * a.shares + share] = sum;
+  if ((threadIdx.x & 63u) == 63) a.rest[(size_t)s * a.shares + share] = sum;
 }
 
 // Inclusive prefix sum over the workgroup; *total the whole.
 __device__ __forceinline__ double vd_scan(double v, double* wave_sums, double* total) {
   const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(v, o);
-    if (lane >= (uint32_t)o) v += y;
-  }
+  v = vd_wave_scan(v);
   if (lane == 63) wave_sums[w] = v;
   __syncthreads();
   double all = 0.0;
@@ -306,13 +386,31 @@ __device__ __forceinline__ double vd_scan(double v, double* wave_sums, double* t
   return v;
 }
 
+// The first thread's `found`, or the last thread's `last` where nobody found anything (threads hold
+// ascending indexes; ~0: none; 0 where there is neither).
+__device__ __forceinline__ uint32_t vd_first_or_last(uint32_t found, uint32_t last, uint2* waves) {
+  const uint64_t f = __ballot(found != 0xffffffffu), l = __ballot(last != 0xffffffffu);
+  const uint32_t a = f ? __builtin_amdgcn_readlane(found, __builtin_ctzll(f)) : 0xffffffffu;
+  const uint32_t b = l ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(l)) : 0xffffffffu;
+  if ((threadIdx.x & 63u) == 0) waves[threadIdx.x >> 6] = make_uint2(a, b);
+  __syncthreads();
+  uint32_t first = 0xffffffffu, end = 0;
+  for (uint32_t i = 0; i < VD_NT / 64; ++i) {
+    const uint2 x = waves[i];
+    first = min(first, x.x);
+    end = x.y != 0xffffffffu ? x.y : end;
+  }
+  __syncthreads();
+  return first != 0xffffffffu ? first : end;
+}
+
 // One workgroup per sequence: acceptance, the share that the number falls into, the token in it.
 template <int LT>
 __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
   __shared__ VdShared sh;
   __shared__ double wave_sums[VD_NT / 64];
   __shared__ double s_x;
-  __shared__ uint32_t s_first, s_last, s_share;
+  __shared__ uint2 waves[VD_NT / 64];
   __shared__ double s_before;
   const uint32_t s = blockIdx.x, tid = threadIdx.x, n = vd_drafts(a, s);
   vd_accept<LT>(a, s, sh);
@@ -332,18 +430,21 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
     const VdPart* parts = a.parts + ((size_t)s * vd_rows(a) + took) * a.shares;
     // this thread's 8 logits of a share: their masses (without a draft distribution in units of
     // exp((l - max) / T))
+    const double ip = 1.0 / P.z, iq = 1.0 / Q.z;
     const auto masses = [&](uint32_t share, bool whole, double (&m)[8]) {
       const uint32_t v0 = share * VD_SHARE + tid * 8;
+      float lp[8], lq[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // (every load on its way before the first is used)
+        const uint32_t v = min(v0 + i, a.vocab - 1);
+        lp[i] = load_as_f32<LT>(prow, v);
+        lq[i] = load_as_f32<LT>(qrow, v);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t v = v0 + i;
-        double y = 0.0;
-        if (v < a.vocab && (whole || v != x_tok)) {
-          y = vd_exp((double)load_as_f32<LT>(prow, v) - (double)P.m, by, sh.tab);
-          if (apart && !whole)
-            y = fmax(y * (1.0 / P.z) - vd_exp((double)load_as_f32<LT>(qrow, v) - (double)Q.m, by, sh.tab) * (1.0 / Q.z), 0.0);
-        }
-        m[i] = y;
+        double y = vd_exp((double)lp[i] - (double)P.m, by, sh.tab);
+        if (apart && !whole) y = fmax(y * ip - vd_exp((double)lq[i] - (double)Q.m, by, sh.tab) * iq, 0.0);
+        m[i] = v0 + i < a.vocab && (whole || v0 + i != x_tok) ? y : 0.0;
       }
     };
     double m[8];
@@ -358,7 +459,7 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
     }
     const uint32_t per = (a.shares + VD_NT - 1) / VD_NT, i0 = min(a.shares, tid * per), i1 = min(a.shares, i0 + per);
     bool whole = false;
-    double total = 0.0, before = 0.0;
+    double total = 0.0, before = 0.0, first_sum = 0.0;
     const auto share_sum = [&](uint32_t i) {
       if (apart && !whole) return a.rest[(size_t)s * a.shares + i];
       if (!whole && i == x_tok / VD_SHARE && x_tok < a.vocab) return s_x;
@@ -366,23 +467,20 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
     };
     for (int round = 0; round < 2; ++round) {  // (nothing left: p itself)
       double sum = 0.0;
-      for (uint32_t i = i0; i < i1; ++i) sum += share_sum(i);
+      first_sum = i0 < i1 ? share_sum(i0) : 0.0;
+      for (uint32_t i = i0; i < i1; ++i) sum += i == i0 ? first_sum : share_sum(i);
       const double incl = vd_scan(sum, wave_sums, &total);
       before = incl - sum;
       if (total > 0.0) break;
       whole = true;
     }
     const double want = (double)a.uniforms[(size_t)s * (a.n_draft + 1) + a.n_draft] * total;
-    if (tid == 0) {
-      s_first = s_share = 0xffffffffu;
-      s_last = 0;
-    }
-    __syncthreads();
+    uint32_t share;  // (u S rounded up to S: the last with any mass)
     {
       double c = before;
       uint32_t last = 0xffffffffu, found = 0xffffffffu;
       for (uint32_t i = i0; i < i1; ++i) {
-        const double y = share_sum(i);
+        const double y = i == i0 ? first_sum : share_sum(i);
         c += y;
         if (y > 0.0) last = i;
         if (c > want && y > 0.0) {
@@ -390,14 +488,11 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
           break;
         }
       }
-      if (found != 0xffffffffu) atomicMin(&s_share, found);
-      if (last != 0xffffffffu) atomicMax(&s_last, last);
+      share = vd_first_or_last(found, last, waves);
     }
-    __syncthreads();
-    const uint32_t share = s_share != 0xffffffffu ? s_share : s_last;  // (u S rounded up to S: the last with any mass)
     if (share >= i0 && share < i1) {
       double c = before;
-      for (uint32_t i = i0; i < share; ++i) c += share_sum(i);
+      for (uint32_t i = i0; i < share; ++i) c += i == i0 ? first_sum : share_sum(i);
       s_before = c;
     }
     __syncthreads();
@@ -406,8 +501,6 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += m[i];
     const double incl = vd_scan(sum, wave_sums, &unused);
-    if (tid == 0) s_last = 0;
-    __syncthreads();
     {
       double c = s_before + (incl - sum);
       uint32_t last = 0xffffffffu, found = 0xffffffffu;
@@ -420,11 +513,8 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
           if (c > want && found == 0xffffffffu) found = v;
         }
       }
-      if (found != 0xffffffffu) atomicMin(&s_first, found);
-      if (last != 0xffffffffu) atomicMax(&s_last, last);
+      pick = vd_first_or_last(found, last, waves);
     }
-    __syncthreads();
-    pick = s_first != 0xffffffffu ? s_first : s_last;
   }
   if (tid == 0) a.accepted[s] = took;
   if (tid <= a.n_draft) {

@@ -302,8 +302,11 @@ int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint
   a.shares = vd_shares(vocab);
   const uint64_t rows = a.draft ? 2 * n_draft + 1 : n_draft + 1, groups = (a.shares + 3) / 4;
   if (n_seqs * rows * groups > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  // shares of a wave: one while the chip holds all waves at once (about 4096), up to 4
+  const uint32_t per = (uint32_t)std::min<uint64_t>(4, std::max<uint64_t>(1, n_seqs * rows * a.shares / 4096));
   const auto go = [&](auto stats, auto rest, auto pick) {
-    hipLaunchKernelGGL(stats, dim3((uint32_t)(n_seqs * rows * groups)), dim3(cm::VD_NT), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(stats, dim3((uint32_t)(n_seqs * rows * ((a.shares + 4 * per - 1) / (4 * per)))), dim3(cm::VD_NT),
+                       0, (hipStream_t)stream, a, per);
     if (a.draft)
       hipLaunchKernelGGL(rest, dim3((uint32_t)(n_seqs * groups)), dim3(cm::VD_NT), 0, (hipStream_t)stream, a);
     hipLaunchKernelGGL(pick, dim3(n_seqs), dim3(cm::VD_NT), 0, (hipStream_t)stream, a);
