@@ -167,49 +167,72 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int EV_NT = 1024;
+constexpr uint32_t EV_NT = 1024;
 
-// Exclusive prefix sum of v over the workgroup's threads; *total the whole sum.
-__device__ __forceinline__ uint32_t evict_scan(uint32_t v, uint32_t* wave_sums, uint32_t* total) {
-  const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
-  uint32_t x = v;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t y = __shfl_up(x, o);
-    if (lane >= (uint32_t)o) x += y;
-  }
-  if (lane == 63) wave_sums[w] = x;
-  __syncthreads();
-  uint32_t before = 0, all = 0;
-  for (uint32_t i = 0; i < EV_NT / 64; ++i) {
-    const uint32_t y = wave_sums[i];
-    if (i < w) before += y;
-    all += y;
-  }
-  __syncthreads();
-  *total = all;
-  return before + x - v;
+// Inclusive prefix sum over the wave by data-parallel moves.
+__device__ __forceinline__ uint32_t ev_wave_scan(uint32_t x) {
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);  // 1, 2, 4, 8 lanes below
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);  // the row below's end
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);  // the lower half's end
+  return x;
 }
 
-// One workgroup per (sequence, KV head): src[keep] = the kept positions in order (also to `kept`),
-// the weights compacted, old_lens[s] = the length before where rows have to move, else 0.
+// One workgroup per (sequence, KV head): src[keep] = the slots (page * page_size + offset) of the kept
+// positions in order, `kept` the positions themselves, the weights compacted, old_lens[s] = the length
+// before where rows have to move, else 0.
+//
+// The smallest kept weight by its digits of 8 bits from the top: a histogram (one for every 4 waves:
+// weights crowd in few exponents) and a suffix sum of its 256 counts.  A thread holds K weights in
+// registers, runs of V at a time, so up to K * 1024 positions are read once; longer rows go through
+// the same code in pieces that are read again.  Then prefix sums of two counts in a word (weights
+// above the smallest, weights equal to it) give every kept position its place.
+// Bound: latency; 16 x 8 rows of 1088 weights 43 -> 11 us against LDS atomics on one histogram searched
+// by one thread.
+template <int K>
 __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restrict__ weights, uint32_t keep,
                                                         uint32_t recent, uint32_t* __restrict__ src,
                                                         uint32_t* __restrict__ old_lens,
                                                         uint32_t* __restrict__ new_lens,
                                                         uint32_t* __restrict__ kept) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t wave_sums[EV_NT / 64];
+  constexpr uint32_t COPIES = EV_NT / 256, PIECE = EV_NT * K;
+  constexpr int V = K < 4 ? K : 4, N = K / V;  // N runs of V positions, EV_NT * V apart
+  typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
+  __shared__ uint32_t hist[COPIES][256];
+  __shared__ uint32_t wave_sums[N][EV_NT / 64];
   __shared__ uint32_t s_digit, s_rank, s_bad;
-  const uint32_t s = blockIdx.x / g.n_kv, h = blockIdx.x % g.n_kv, tid = threadIdx.x;
-  const uint32_t L = g.lens[s], cap = g.stride << g.shift;
+  const uint32_t s = blockIdx.x / g.n_kv, h = blockIdx.x - s * g.n_kv, tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t L = g.lens[s], cap = g.stride << g.shift, mask = (1u << g.shift) - 1u;
+  const uint32_t* tab = g.table + (size_t)s * g.stride;
+  float* w = weights + (size_t)blockIdx.x * cap;
+  const bool too_long = (uint64_t)L > ((uint64_t)g.stride << g.shift);
+  // the first piece's weights, on their way while the pages are looked through
+  float x[N][V];
+  const auto at = [&](uint32_t p0, int i, int e) { return p0 + (i * EV_NT + tid) * V + e; };
+  const auto read = [&](uint32_t p0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (at(p0, i, V) <= L) {
+        const vec y = *reinterpret_cast<const vec*>(w + at(p0, i, 0));
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[i][e] = y[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[i][e] = at(p0, i, e) < L ? w[at(p0, i, e)] : 0.0f;
+      }
+    }
+  };
   if (tid == 0) s_bad = 0;
   __syncthreads();
-  const bool too_long = (uint64_t)L > ((uint64_t)g.stride << g.shift);
   if (too_long) {
     if (tid == 0) paged_flag(g, PG_BAD_LENGTH);
   } else {
-    for (uint32_t i = tid; i < (L + (1u << g.shift) - 1u) >> g.shift; i += EV_NT)
-      if (g.table[(size_t)s * g.stride + i] >= g.n_pages) s_bad = 1;
+    if (L > keep) read(0);
+    bool bad = false;
+    for (uint32_t i = tid; i < (L + mask) >> g.shift; i += EV_NT) bad |= tab[i] >= g.n_pages;
+    if (bad) s_bad = 1;
   }
   __syncthreads();
   if (s_bad && tid == 0) paged_flag(g, PG_BAD_PAGE);
@@ -224,50 +247,93 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
       for (uint32_t j = tid; j < min(L, keep); j += EV_NT) kp[j] = j;
     return;
   }
-  float* w = weights + (size_t)blockIdx.x * cap;
   uint32_t* sp = src + (size_t)blockIdx.x * keep;
   const uint32_t cut = L - recent;
+  const bool one = L <= PIECE;  // the weights stay in registers
   uint32_t rank = keep - recent;  // positions still to be found among the keys equal in the digits so far
+  const bool any = rank != 0;
   uint32_t prefix = 0;
-  for (int b = 24; b >= 0 && rank; b -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  for (int b = 24; b >= 0 && any; b -= 8) {
+    for (uint32_t i = tid; i < COPIES * 256; i += EV_NT) hist[0][i] = 0;
     __syncthreads();
-    for (uint32_t p = tid; p < cut; p += EV_NT) {
-      const uint32_t k = evict_key(w[p]);
-      if (b == 24 || (k >> (b + 8)) == (prefix >> (b + 8))) atomicAdd(&hist[(k >> b) & 255u], 1u);
+    for (uint32_t p0 = 0; p0 < cut; p0 += PIECE) {
+      if (!one) read(p0);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const uint32_t k = evict_key(x[i][e]);
+          if (at(p0, i, e) < cut && (b == 24 || (k >> ((b + 8) & 31)) == (prefix >> ((b + 8) & 31))))
+            atomicAdd(&hist[tid >> 8][(k >> b) & 255u], 1u);
+        }
     }
     __syncthreads();
-    if (tid == 0) {
-      uint32_t left = rank;
-      int d = 255;
-      while (hist[d] < left) left -= hist[d--];
-      s_digit = (uint32_t)d;
-      s_rank = left;
+    if (tid < 64) {  // lane l: digits 255 - 4 l .. 252 - 4 l
+      uint32_t c[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = 0;
+        for (uint32_t v = 0; v < COPIES; ++v) c[i] += hist[v][255 - 4 * lane - i];
+        sum += c[i];
+      }
+      uint32_t above = ev_wave_scan(sum) - sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (above < rank && above + c[i] >= rank) {
+          s_digit = 255 - 4 * lane - i;
+          s_rank = rank - above;
+        }
+        above += c[i];
+      }
     }
     __syncthreads();
     prefix |= s_digit << b;
     rank = s_rank;
-    __syncthreads();
   }
   // kept: every key above `prefix`, the first `rank` keys equal to it, and the recent positions
-  const bool any = keep > recent;
-  uint32_t eq_before = 0, out = 0;
-  for (uint32_t p0 = 0; p0 < L; p0 += EV_NT) {
-    const uint32_t p = p0 + tid;
-    const float x = p < L ? w[p] : 0.0f;
-    const uint32_t k = evict_key(x);
-    const bool other = p < cut && any;
-    const bool eq = other && k == prefix;
-    uint32_t total;
-    const uint32_t eq_rank = eq_before + evict_scan(eq ? 1u : 0u, wave_sums, &total);
-    eq_before += total;
-    const bool take = p < L && (p >= cut || (other && (k > prefix || (eq && eq_rank < rank))));
-    const uint32_t j = out + evict_scan(take ? 1u : 0u, wave_sums, &total);
-    out += total;
-    if (take) {  // j <= p: every later position is still in place
-      sp[j] = p;
-      w[j] = x;
-      if (kp) kp[j] = p;
+  uint32_t eq0 = 0, gt0 = 0;  // of the pieces before
+  for (uint32_t p0 = 0; p0 < L; p0 += PIECE) {
+    if (!one) read(p0);
+    // a position above or equal to the smallest kept weight
+    const auto is_gt = [&](int i, int e) {
+      const uint32_t p = at(p0, i, e);
+      return p < L && (p >= cut || (any && evict_key(x[i][e]) > prefix));
+    };
+    const auto is_eq = [&](int i, int e) { return at(p0, i, e) < cut && any && evict_key(x[i][e]) == prefix; };
+    uint32_t before[N];  // counts in a word: gt, eq << 16 (at most 4096 each in a run of the workgroup)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t count = 0;
+#pragma unroll
+      for (int e = 0; e < V; ++e) count += (is_gt(i, e) ? 1u : 0u) + (is_eq(i, e) ? 0x10000u : 0u);
+      const uint32_t incl = ev_wave_scan(count);
+      before[i] = incl - count;
+      if (lane == 63) wave_sums[i][tid >> 6] = incl;
+    }
+    __syncthreads();  // (every weight of the piece has been read, too)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t all = 0;
+      for (uint32_t v = 0; v < EV_NT / 64; ++v) {
+        const uint32_t y = wave_sums[i][v];
+        if (v < tid >> 6) before[i] += y;
+        all += y;
+      }
+      uint32_t gt = gt0 + (before[i] & 0xffffu), eq = eq0 + (before[i] >> 16);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const bool g1 = is_gt(i, e), e1 = is_eq(i, e);
+        if (g1 || (e1 && eq < rank)) {
+          const uint32_t p = at(p0, i, e), j = gt + min(eq, rank);  // j <= p: no weight still to be read
+          sp[j] = (tab[p >> g.shift] << g.shift) + (p & mask);
+          w[j] = x[i][e];
+          if (kp) kp[j] = p;
+        }
+        gt += g1 ? 1u : 0u;
+        eq += e1 ? 1u : 0u;
+      }
+      gt0 += all & 0xffffu;
+      eq0 += all >> 16;
     }
     __syncthreads();
   }
@@ -275,54 +341,75 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
 
 // The move, in place: output positions in chunks, a chunk's sources read before any of it is
 // written.  A source is never below its output position, so no later chunk misses a row.  One
-// workgroup per (sequence, KV head, 8 dims of K) and per (sequence, KV head, 32 dims of V).
-constexpr uint32_t EM_NT = 256;
-__global__ __launch_bounds__(EM_NT) void k_evict_move(Paged g, uint16_t* __restrict__ kc, uint16_t* __restrict__ vc,
+// workgroup per (sequence, KV head, 8 dims of K) and per (sequence, KV head, 32 dims of V): these
+// never touch each other's bytes.  Chunks as large as the registers allow (2048 rows of K, 1024 of V), since
+// each costs a memory latency.  K moves whole granules; a granule of V gathers 8 positions.
+// Bound: HBM; rows far apart share their 128-byte lines with rows that are left behind.
+constexpr uint32_t EM_NT = 512;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__global__ __launch_bounds__(EM_NT, 6) void k_evict_move(Paged g, uint16_t* __restrict__ kc, uint16_t* __restrict__ vc,
                                                       uint32_t keep, const uint32_t* __restrict__ src,
                                                       const uint32_t* __restrict__ old_lens,
                                                       const uint32_t* __restrict__ new_lens,
                                                       uint32_t* __restrict__ lens_out) {
   const uint32_t slices = g.hd / 8 + g.hd / 32, tid = threadIdx.x;
-  const uint32_t sl = blockIdx.x % slices, sh = blockIdx.x / slices, s = sh / g.n_kv, h = sh % g.n_kv;
+  const uint32_t sh = blockIdx.x / slices, sl = blockIdx.x - sh * slices, s = sh / g.n_kv, h = sh - s * g.n_kv;
   if (sl == 0 && h == 0 && tid == 0) lens_out[s] = new_lens[s];
   if (!old_lens[s]) return;
   const uint32_t* tab = g.table + (size_t)s * g.stride;
   const uint32_t* sp = src + (size_t)sh * keep;
   const uint32_t mask = (1u << g.shift) - 1u;
-  if (sl < g.hd / 8) {
-    for (uint32_t j0 = 0; j0 < keep; j0 += EM_NT) {
-      const uint32_t j = j0 + tid;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (j < keep) {
-        const uint32_t p = sp[j];
-        x = *reinterpret_cast<const uint4*>(kc + paged_base(g, tab[p >> g.shift], h) + paged_k(g, p & mask, sl * 8));
+  if (sl >= g.hd / 32) {
+    constexpr uint32_t R = 4;
+    const uint32_t d = (sl - g.hd / 32) * 8;
+    for (uint32_t j0 = 0; j0 < keep; j0 += R * EM_NT) {
+      u32x4 x[R];
+      uint32_t to[R], slot[R];
+#pragma unroll
+      for (uint32_t r = 0; r < R; ++r) {
+        const uint32_t j = min(j0 + r * EM_NT + tid, keep - 1);
+        slot[r] = sp[j];
+        to[r] = (tab[j >> g.shift] << g.shift) + (j & mask);
       }
+#pragma unroll
+      for (uint32_t r = 0; r < R; ++r)
+        x[r] = *reinterpret_cast<const u32x4*>(kc + paged_base(g, slot[r] >> g.shift, h) + paged_k(g, slot[r] & mask, d));
       __syncthreads();
-      if (j < keep)
-        *reinterpret_cast<uint4*>(kc + paged_base(g, tab[j >> g.shift], h) + paged_k(g, j & mask, sl * 8)) = x;
-      __syncthreads();
+#pragma unroll
+      for (uint32_t r = 0; r < R; ++r)
+        if (j0 + r * EM_NT + tid < keep && slot[r] != to[r])
+          *reinterpret_cast<u32x4*>(kc + paged_base(g, to[r] >> g.shift, h) + paged_k(g, to[r] & mask, d)) = x[r];
     }
     return;
   }
-  const uint32_t d = (sl - g.hd / 8) * 32 + (tid & 31u), step = EM_NT / 32 * 8;
-  for (uint32_t j0 = 0; j0 < keep; j0 += step) {
-    const uint32_t j = j0 + (tid >> 5) * 8;
-    union { uint16_t e[8]; uint4 v; } x;
-    for (uint32_t i = 0; i < 8; ++i) {
-      if (j + i >= keep) continue;
-      const uint32_t p = sp[j + i];
-      x.e[i] = vc[paged_base(g, tab[p >> g.shift], h) + paged_v(g, p & mask, d)];
-    }
-    __syncthreads();
-    if (j < keep) {
-      uint16_t* dst = vc + paged_base(g, tab[j >> g.shift], h) + paged_v(g, j & mask, d);
-      if (j + 8 <= keep) {
-        *reinterpret_cast<uint4*>(dst) = x.v;
-      } else {
-        for (uint32_t i = 0; j + i < keep; ++i) dst[i] = x.e[i];
+  constexpr uint32_t R = 4;  // granules of a thread
+  const uint32_t d = sl * 32 + (tid & 31u);
+  for (uint32_t j0 = 0; j0 < keep; j0 += R * EM_NT / 4) {
+    uint32_t x[R][4];
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+      const uint32_t j = j0 + (r * (EM_NT / 32) + (tid >> 5)) * 8;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i += 2) {
+        const uint32_t a = sp[min(j + i, keep - 1)], b = sp[min(j + i + 1, keep - 1)];
+        x[r][i / 2] = vc[paged_base(g, a >> g.shift, h) + paged_v(g, a & mask, d)] |
+                      (uint32_t)vc[paged_base(g, b >> g.shift, h) + paged_v(g, b & mask, d)] << 16;
       }
     }
     __syncthreads();
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+      const uint32_t j = j0 + (r * (EM_NT / 32) + (tid >> 5)) * 8;
+      if (j >= keep) continue;
+      uint16_t* dst = vc + paged_base(g, tab[j >> g.shift], h) + paged_v(g, j & mask, d);
+      if (j + 8 <= keep) {
+        *reinterpret_cast<u32x4*>(dst) = u32x4{x[r][0], x[r][1], x[r][2], x[r][3]};
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (j + i < keep) dst[i] = (uint16_t)(x[r][i / 2] >> (16 * (i & 1)));
+      }
+    }
   }
 }
 

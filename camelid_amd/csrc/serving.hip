@@ -240,6 +240,8 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
     return cm::fail_global(me, why);
   if (!keep || keep > (1u << 24)) return cm::fail_global(me, "keep must be in 1..=2^24");
   if (recent > keep) return cm::fail_global(me, "recent must be at most keep");
+  if ((uint64_t)n_pages * page_size > 0xffffffffull)
+    return cm::fail_global(me, "n_pages * page_size must be below 2^32");
   if (!aligned16(kc) || !aligned16(vc) || !aligned16(workspace) || !aligned4(weights) || !aligned4(lens_out) ||
       !aligned4(kept))
     return cm::fail_global(me, "the cache and the workspace must be 16-byte aligned, the rest 4-byte aligned");
@@ -248,8 +250,11 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
   uint32_t* old_lens = static_cast<uint32_t*>(workspace);
   uint32_t* new_lens = old_lens + n_seqs;
   uint32_t* src = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + up256((size_t)n_seqs * 8));
-  hipLaunchKernelGGL(cm::k_evict_select, dim3(n_seqs * n_kv), dim3(cm::EV_NT), 0, (hipStream_t)stream, g, weights,
-                     keep, recent, src, old_lens, new_lens, kept);
+  // rows of at most 2048, 8192 and 16384 positions have their weights read once
+  const uint32_t cap = page_size * table_stride;
+  const auto select = cap <= 2048 ? cm::k_evict_select<2> : cap <= 8192 ? cm::k_evict_select<8> : cm::k_evict_select<16>;
+  hipLaunchKernelGGL(select, dim3(n_seqs * n_kv), dim3(cm::EV_NT), 0, (hipStream_t)stream, g, weights, keep, recent, src,
+                     old_lens, new_lens, kept);
   const uint32_t slices = hd / 8 + hd / 32;
   hipLaunchKernelGGL(cm::k_evict_move, dim3(n_seqs * n_kv * slices), dim3(cm::EM_NT), 0, (hipStream_t)stream, g,
                      static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc), keep, src, old_lens, new_lens, lens_out);
