@@ -180,9 +180,17 @@ __device__ __forceinline__ uint32_t ev_wave_scan(uint32_t x) {
   return x;
 }
 
-// One workgroup per (sequence, KV head): src[keep] = the slots (page * page_size + offset) of the kept
-// positions in order, `kept` the positions themselves, the weights compacted, old_lens[s] = the length
-// before where rows have to move, else 0.
+// What the selection leaves for the move, for each (sequence, KV head).
+struct EvictPlan {
+  uint32_t* slot;     // [keep] the slots (page * page_size + offset) of the kept positions, in order
+  uint32_t* from;     // [keep] where row j comes from: 8 * (index of its granule of 8 positions) + position % 8
+  uint32_t* granule;  // [keep] the distinct granules in order: slot / 8
+  uint32_t* old_lens; // [n_seqs] the length before where rows have to move, else 0
+  uint32_t* new_lens; // [n_seqs]
+};
+
+// One workgroup per (sequence, KV head): the plan, `kept` (the positions themselves), the weights
+// compacted.
 //
 // The smallest kept weight by its digits of 8 bits from the top: a histogram (one for every 4 waves:
 // weights crowd in few exponents) and a suffix sum of its 256 counts.  A thread holds K weights in
@@ -193,15 +201,12 @@ __device__ __forceinline__ uint32_t ev_wave_scan(uint32_t x) {
 // by one thread.
 template <int K>
 __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restrict__ weights, uint32_t keep,
-                                                        uint32_t recent, uint32_t* __restrict__ src,
-                                                        uint32_t* __restrict__ old_lens,
-                                                        uint32_t* __restrict__ new_lens,
-                                                        uint32_t* __restrict__ kept) {
+                                                        uint32_t recent, EvictPlan plan, uint32_t* __restrict__ kept) {
   constexpr uint32_t COPIES = EV_NT / 256, PIECE = EV_NT * K;
   constexpr int V = K < 4 ? K : 4, N = K / V;  // N runs of V positions, EV_NT * V apart
   typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
   __shared__ uint32_t hist[COPIES][256];
-  __shared__ uint32_t wave_sums[N][EV_NT / 64];
+  __shared__ uint32_t wave_sums[N][EV_NT / 64], wave_touched[N][EV_NT / 64];
   __shared__ uint32_t s_digit, s_rank, s_bad;
   const uint32_t s = blockIdx.x / g.n_kv, h = blockIdx.x - s * g.n_kv, tid = threadIdx.x, lane = tid & 63u;
   const uint32_t L = g.lens[s], cap = g.stride << g.shift, mask = (1u << g.shift) - 1u;
@@ -238,8 +243,8 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
   if (s_bad && tid == 0) paged_flag(g, PG_BAD_PAGE);
   const bool moves = !too_long && !s_bad && L > keep;
   if (h == 0 && tid == 0) {
-    old_lens[s] = moves ? L : 0u;
-    new_lens[s] = moves ? keep : L;
+    plan.old_lens[s] = moves ? L : 0u;
+    plan.new_lens[s] = moves ? keep : L;
   }
   uint32_t* kp = kept ? kept + (size_t)blockIdx.x * keep : nullptr;
   if (!moves) {
@@ -247,9 +252,17 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
       for (uint32_t j = tid; j < min(L, keep); j += EV_NT) kp[j] = j;
     return;
   }
-  uint32_t* sp = src + (size_t)blockIdx.x * keep;
+  const size_t row0 = (size_t)blockIdx.x * keep;
   const uint32_t cut = L - recent;
   const bool one = L <= PIECE;  // the weights stay in registers
+  uint32_t key[N][V];
+  const auto make_keys = [&] {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) key[i][e] = evict_key(x[i][e]);
+  };
+  make_keys();
   uint32_t rank = keep - recent;  // positions still to be found among the keys equal in the digits so far
   const bool any = rank != 0;
   uint32_t prefix = 0;
@@ -257,12 +270,15 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
     for (uint32_t i = tid; i < COPIES * 256; i += EV_NT) hist[0][i] = 0;
     __syncthreads();
     for (uint32_t p0 = 0; p0 < cut; p0 += PIECE) {
-      if (!one) read(p0);
+      if (!one) {
+        read(p0);
+        make_keys();
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const uint32_t k = evict_key(x[i][e]);
+          const uint32_t k = key[i][e];
           if (at(p0, i, e) < cut && (b == 24 || (k >> ((b + 8) & 31)) == (prefix >> ((b + 8) & 31))))
             atomicAdd(&hist[tid >> 8][(k >> b) & 255u], 1u);
         }
@@ -291,26 +307,29 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
     rank = s_rank;
   }
   // kept: every key above `prefix`, the first `rank` keys equal to it, and the recent positions
-  uint32_t eq0 = 0, gt0 = 0;  // of the pieces before
+  uint32_t eq0 = 0, gt0 = 0, touched0 = 0;  // of the pieces before
   for (uint32_t p0 = 0; p0 < L; p0 += PIECE) {
-    if (!one) read(p0);
-    // a position above or equal to the smallest kept weight
-    const auto is_gt = [&](int i, int e) {
-      const uint32_t p = at(p0, i, e);
-      return p < L && (p >= cut || (any && evict_key(x[i][e]) > prefix));
-    };
-    const auto is_eq = [&](int i, int e) { return at(p0, i, e) < cut && any && evict_key(x[i][e]) == prefix; };
-    uint32_t before[N];  // counts in a word: gt, eq << 16 (at most 4096 each in a run of the workgroup)
+    if (!one) {
+      read(p0);
+      make_keys();
+    }
+    uint32_t gts[N], eqs[N], before[N], page[N];  // before: counts in a word: gt, eq << 16 (at most 4096 each)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      uint32_t count = 0;
+      page[i] = at(p0, i, 0) < L ? tab[at(p0, i, 0) >> g.shift] : 0u;  // (a run lies in one page)
+      gts[i] = eqs[i] = 0;
 #pragma unroll
-      for (int e = 0; e < V; ++e) count += (is_gt(i, e) ? 1u : 0u) + (is_eq(i, e) ? 0x10000u : 0u);
-      const uint32_t incl = ev_wave_scan(count);
+      for (int e = 0; e < V; ++e) {
+        const uint32_t p = at(p0, i, e), k = key[i][e];
+        gts[i] |= (uint32_t)(p < L && (p >= cut || (any && k > prefix))) << e;
+        eqs[i] |= (uint32_t)(p < cut && any && k == prefix) << e;
+      }
+      const uint32_t count = __popc(gts[i]) + (__popc(eqs[i]) << 16), incl = ev_wave_scan(count);
       before[i] = incl - count;
       if (lane == 63) wave_sums[i][tid >> 6] = incl;
     }
     __syncthreads();  // (every weight of the piece has been read, too)
+    uint32_t first[N], takes[N], seen[N];  // first: the run's first output position
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       uint32_t all = 0;
@@ -319,97 +338,150 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
         if (v < tid >> 6) before[i] += y;
         all += y;
       }
-      uint32_t gt = gt0 + (before[i] & 0xffffu), eq = eq0 + (before[i] >> 16);
+      const uint32_t gt = gt0 + (before[i] & 0xffffu);
+      uint32_t eq = eq0 + (before[i] >> 16);
+      first[i] = gt + min(eq, rank);
+      takes[i] = gts[i];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const bool g1 = is_gt(i, e), e1 = is_eq(i, e);
-        if (g1 || (e1 && eq < rank)) {
-          const uint32_t p = at(p0, i, e), j = gt + min(eq, rank);  // j <= p: no weight still to be read
-          sp[j] = (tab[p >> g.shift] << g.shift) + (p & mask);
-          w[j] = x[i][e];
-          if (kp) kp[j] = p;
+      for (int e = 0; e < V; ++e)
+        if ((eqs[i] >> e) & 1u) {
+          if (eq < rank) takes[i] |= 1u << e;
+          ++eq;
         }
-        gt += g1 ? 1u : 0u;
-        eq += e1 ? 1u : 0u;
-      }
       gt0 += all & 0xffffu;
       eq0 += all >> 16;
+      // a granule is 8 / V runs: its first lane counts it where any of them is taken from
+      uint32_t some = takes[i];
+      some |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)some, 0xb1, 0xf, 0xf, false);
+      if (V < 4) some |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)some, 0x4e, 0xf, 0xf, false);
+      const uint32_t incl = ev_wave_scan(some && (lane & (8 / V - 1)) == 0 ? 1u : 0u);
+      seen[i] = incl;
+      if (lane == 63) wave_touched[i][tid >> 6] = incl;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t t = touched0 + seen[i] - 1;
+      for (uint32_t v = 0; v < EV_NT / 64; ++v) {
+        const uint32_t y = wave_touched[i][v];
+        if (v < tid >> 6) t += y;
+        touched0 += y;
+      }
+      uint32_t j = first[i];
+      const uint32_t slot0 = (page[i] << g.shift) + (at(p0, i, 0) & mask);
+      if (takes[i]) plan.granule[row0 + t] = slot0 >> 3;  // (the granule's runs write the same)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if ((takes[i] >> e) & 1u) {  // j <= p: no weight still to be read
+          plan.slot[row0 + j] = slot0 + e;
+          plan.from[row0 + j] = 8 * t + ((slot0 + e) & 7u);
+          w[j] = x[i][e];
+          if (kp) kp[j] = at(p0, i, e);
+          ++j;
+        }
     }
     __syncthreads();
   }
 }
 
 // The move, in place: output positions in chunks, a chunk's sources read before any of it is
-// written.  A source is never below its output position, so no later chunk misses a row.  One
-// workgroup per (sequence, KV head, 8 dims of K) and per (sequence, KV head, 32 dims of V): these
-// never touch each other's bytes.  Chunks as large as the registers allow (2048 rows of K, 1024 of V), since
-// each costs a memory latency.  K moves whole granules; a granule of V gathers 8 positions.
-// Bound: HBM; rows far apart share their 128-byte lines with rows that are left behind.
-constexpr uint32_t EM_NT = 512;
+// written.  A source is never below its output position, so no later chunk misses a row.  Bound:
+// HBM; rows far apart share their 128-byte lines with rows that are left behind.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-__global__ __launch_bounds__(EM_NT, 6) void k_evict_move(Paged g, uint16_t* __restrict__ kc, uint16_t* __restrict__ vc,
-                                                      uint32_t keep, const uint32_t* __restrict__ src,
-                                                      const uint32_t* __restrict__ old_lens,
-                                                      const uint32_t* __restrict__ new_lens,
-                                                      uint32_t* __restrict__ lens_out) {
-  const uint32_t slices = g.hd / 8 + g.hd / 32, tid = threadIdx.x;
-  const uint32_t sh = blockIdx.x / slices, sl = blockIdx.x - sh * slices, s = sh / g.n_kv, h = sh - s * g.n_kv;
-  if (sl == 0 && h == 0 && tid == 0) lens_out[s] = new_lens[s];
-  if (!old_lens[s]) return;
+
+// K: one workgroup per (sequence, KV head, 8 dims), whole granules, chunks of R * EK_NT rows in registers.
+constexpr uint32_t EK_NT = 256;
+__global__ __launch_bounds__(EK_NT, 8) void k_evict_move_k(Paged g, uint16_t* __restrict__ kc, uint32_t keep,
+                                                           EvictPlan plan) {
+  constexpr uint32_t R = 4;
+  const uint32_t slices = g.hd / 8, tid = threadIdx.x;
+  const uint32_t sh = blockIdx.x / slices, d = (blockIdx.x - sh * slices) * 8, s = sh / g.n_kv, h = sh - s * g.n_kv;
+  if (!plan.old_lens[s]) return;
   const uint32_t* tab = g.table + (size_t)s * g.stride;
-  const uint32_t* sp = src + (size_t)sh * keep;
+  const uint32_t* sp = plan.slot + (size_t)sh * keep;
   const uint32_t mask = (1u << g.shift) - 1u;
-  if (sl >= g.hd / 32) {
-    constexpr uint32_t R = 4;
-    const uint32_t d = (sl - g.hd / 32) * 8;
-    for (uint32_t j0 = 0; j0 < keep; j0 += R * EM_NT) {
-      u32x4 x[R];
-      uint32_t to[R], slot[R];
-#pragma unroll
-      for (uint32_t r = 0; r < R; ++r) {
-        const uint32_t j = min(j0 + r * EM_NT + tid, keep - 1);
-        slot[r] = sp[j];
-        to[r] = (tab[j >> g.shift] << g.shift) + (j & mask);
-      }
-#pragma unroll
-      for (uint32_t r = 0; r < R; ++r)
-        x[r] = *reinterpret_cast<const u32x4*>(kc + paged_base(g, slot[r] >> g.shift, h) + paged_k(g, slot[r] & mask, d));
-      __syncthreads();
-#pragma unroll
-      for (uint32_t r = 0; r < R; ++r)
-        if (j0 + r * EM_NT + tid < keep && slot[r] != to[r])
-          *reinterpret_cast<u32x4*>(kc + paged_base(g, to[r] >> g.shift, h) + paged_k(g, to[r] & mask, d)) = x[r];
-    }
-    return;
-  }
-  constexpr uint32_t R = 4;  // granules of a thread
-  const uint32_t d = sl * 32 + (tid & 31u);
-  for (uint32_t j0 = 0; j0 < keep; j0 += R * EM_NT / 4) {
-    uint32_t x[R][4];
+  for (uint32_t j0 = 0; j0 < keep; j0 += R * EK_NT) {
+    u32x4 x[R];
+    uint32_t to[R], slot[R];
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
-      const uint32_t j = j0 + (r * (EM_NT / 32) + (tid >> 5)) * 8;
-#pragma unroll
-      for (uint32_t i = 0; i < 8; i += 2) {
-        const uint32_t a = sp[min(j + i, keep - 1)], b = sp[min(j + i + 1, keep - 1)];
-        x[r][i / 2] = vc[paged_base(g, a >> g.shift, h) + paged_v(g, a & mask, d)] |
-                      (uint32_t)vc[paged_base(g, b >> g.shift, h) + paged_v(g, b & mask, d)] << 16;
-      }
+      const uint32_t j = min(j0 + r * EK_NT + tid, keep - 1);
+      slot[r] = sp[j];
+      to[r] = (tab[j >> g.shift] << g.shift) + (j & mask);
     }
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r)
+      x[r] = *reinterpret_cast<const u32x4*>(kc + paged_base(g, slot[r] >> g.shift, h) + paged_k(g, slot[r] & mask, d));
     __syncthreads();
 #pragma unroll
-    for (uint32_t r = 0; r < R; ++r) {
-      const uint32_t j = j0 + (r * (EM_NT / 32) + (tid >> 5)) * 8;
-      if (j >= keep) continue;
+    for (uint32_t r = 0; r < R; ++r)
+      if (j0 + r * EK_NT + tid < keep && slot[r] != to[r])
+        *reinterpret_cast<u32x4*>(kc + paged_base(g, to[r] >> g.shift, h) + paged_k(g, to[r] & mask, d)) = x[r];
+  }
+}
+
+// V: one workgroup per (sequence, KV head, 16 dims).  A granule holds 8 positions, an output granule
+// gathers from up to 8 of them, so a chunk is as many rows as EM_G distinct granules feed; these go to LDS
+// whole (2-byte loads from memory, 16 bytes apart between lanes, took the L1 47 accesses each: 24 us of
+// the 37 us that the move of 16x1088 -> 1024 rows took) and the output granules are put together from there.
+constexpr uint32_t EM_NT = 512, EM_G = 256, EM_D = 16;
+__global__ __launch_bounds__(EM_NT, 4) void k_evict_move_v(Paged g, uint16_t* __restrict__ vc, uint32_t keep,
+                                                           EvictPlan plan, uint32_t* __restrict__ lens_out) {
+  __shared__ u32x4 s_g[EM_G * EM_D];  // [granule][dim], 8 positions each
+  __shared__ uint32_t s_end[EM_NT / 64];
+  const uint32_t slices = g.hd / EM_D, tid = threadIdx.x;
+  const uint32_t sh = blockIdx.x / slices, sl = blockIdx.x - sh * slices, s = sh / g.n_kv, h = sh - s * g.n_kv;
+  if (sl == 0 && h == 0 && tid == 0) lens_out[s] = plan.new_lens[s];
+  if (!plan.old_lens[s]) return;
+  const uint32_t* tab = g.table + (size_t)s * g.stride;
+  const uint32_t* fp = plan.from + (size_t)sh * keep;
+  const uint32_t* gp = plan.granule + (size_t)sh * keep;
+  const uint32_t mask = (1u << g.shift) - 1u, d = sl * EM_D + (tid % EM_D);
+  const uint16_t* elems = reinterpret_cast<const uint16_t*>(s_g);
+  for (uint32_t j0 = 0, j1; j0 < keep; j0 = j1) {
+    // the chunk's rows [j0, j1): whole output granules (but for the last) whose sources are granules t0 .. t0 + EM_G - 1
+    const uint32_t t0 = fp[j0] >> 3;
+    static_assert(EM_G * 8 <= EM_NT * 8, "every end a chunk can have is looked at");
+    const uint32_t end = min(keep, j0 + 8 * (tid + 1));
+    const uint32_t t_end = fp[end - 1] >> 3;
+    constexpr uint32_t U = EM_G * EM_D / EM_NT;  // granules of a thread
+    // granules up to the last that any chunk from here can have: more than this chunk's are not loaded
+    uint32_t slot[U];
+#pragma unroll
+    for (uint32_t k = 0; k < U; ++k) slot[k] = gp[min(t0 + (k * EM_NT + tid) / EM_D, keep - 1)] << 3;
+    const uint64_t fit = __ballot(j0 + 8 * tid < keep && t_end < t0 + EM_G);
+    if ((tid & 63u) == 0) s_end[tid >> 6] = __popcll(fit);
+    __syncthreads();
+    uint32_t n8 = 0;
+    for (uint32_t i = 0; i < EM_NT / 64; ++i) n8 += s_end[i];
+    j1 = min(keep, j0 + 8 * n8);
+    const uint32_t n_u = ((fp[j1 - 1] >> 3) - t0 + 1) * EM_D;
+    u32x4 x[U];
+#pragma unroll
+    for (uint32_t k = 0; k < U; ++k)
+      if (k * EM_NT + tid < n_u)
+        x[k] = *reinterpret_cast<const u32x4*>(vc + paged_base(g, slot[k] >> g.shift, h) + paged_v(g, slot[k] & mask, d));
+#pragma unroll
+    for (uint32_t k = 0; k < U; ++k)
+      if (k * EM_NT + tid < n_u) s_g[k * EM_NT + tid] = x[k];
+    __syncthreads();
+    for (uint32_t j = j0 + tid / EM_D * 8; j < j1; j += EM_NT / EM_D * 8) {
+      uint32_t v[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t f = fp[min(j + i, keep - 1)];
+        v[i] = elems[(((f >> 3) - t0) * EM_D + tid % EM_D) * 8 + (f & 7u)];
+      }
       uint16_t* dst = vc + paged_base(g, tab[j >> g.shift], h) + paged_v(g, j & mask, d);
       if (j + 8 <= keep) {
-        *reinterpret_cast<u32x4*>(dst) = u32x4{x[r][0], x[r][1], x[r][2], x[r][3]};
+        *reinterpret_cast<u32x4*>(dst) = u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
       } else {
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i)
-          if (j + i < keep) dst[i] = (uint16_t)(x[r][i / 2] >> (16 * (i & 1)));
+          if (j + i < keep) dst[i] = (uint16_t)v[i];
       }
     }
+    __syncthreads();
   }
 }
 

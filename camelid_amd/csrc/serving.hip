@@ -224,7 +224,7 @@ size_t camelid_hip_paged_evict_workspace(uint32_t n_seqs, uint32_t n_kv, uint32_
                                          uint32_t keep) {
   (void)page_size;
   (void)table_stride;
-  return up256((size_t)n_seqs * 8) + up256((size_t)n_seqs * n_kv * keep * 4);
+  return up256((size_t)n_seqs * 8) + 3 * up256((size_t)n_seqs * n_kv * keep * 4);
 }
 
 int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_size, uint32_t n_kv, uint32_t hd,
@@ -247,17 +247,24 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
     return cm::fail_global(me, "the cache and the workspace must be 16-byte aligned, the rest 4-byte aligned");
   if (workspace_bytes < camelid_hip_paged_evict_workspace(n_seqs, n_kv, page_size, table_stride, keep))
     return cm::fail_global(me, "workspace too small (camelid_hip_paged_evict_workspace)");
-  uint32_t* old_lens = static_cast<uint32_t*>(workspace);
-  uint32_t* new_lens = old_lens + n_seqs;
-  uint32_t* src = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + up256((size_t)n_seqs * 8));
+  cm::EvictPlan plan;
+  char* ws = static_cast<char*>(workspace);
+  plan.old_lens = reinterpret_cast<uint32_t*>(ws);
+  plan.new_lens = plan.old_lens + n_seqs;
+  ws += up256((size_t)n_seqs * 8);
+  const size_t rows = up256((size_t)n_seqs * n_kv * keep * 4);
+  plan.slot = reinterpret_cast<uint32_t*>(ws);
+  plan.from = reinterpret_cast<uint32_t*>(ws + rows);
+  plan.granule = reinterpret_cast<uint32_t*>(ws + 2 * rows);
   // rows of at most 2048, 8192 and 16384 positions have their weights read once
   const uint32_t cap = page_size * table_stride;
   const auto select = cap <= 2048 ? cm::k_evict_select<2> : cap <= 8192 ? cm::k_evict_select<8> : cm::k_evict_select<16>;
-  hipLaunchKernelGGL(select, dim3(n_seqs * n_kv), dim3(cm::EV_NT), 0, (hipStream_t)stream, g, weights, keep, recent, src,
-                     old_lens, new_lens, kept);
-  const uint32_t slices = hd / 8 + hd / 32;
-  hipLaunchKernelGGL(cm::k_evict_move, dim3(n_seqs * n_kv * slices), dim3(cm::EM_NT), 0, (hipStream_t)stream, g,
-                     static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc), keep, src, old_lens, new_lens, lens_out);
+  hipLaunchKernelGGL(select, dim3(n_seqs * n_kv), dim3(cm::EV_NT), 0, (hipStream_t)stream, g, weights, keep, recent, plan,
+                     kept);
+  hipLaunchKernelGGL(cm::k_evict_move_k, dim3(n_seqs * n_kv * (hd / 8)), dim3(cm::EK_NT), 0, (hipStream_t)stream, g,
+                     static_cast<uint16_t*>(kc), keep, plan);
+  hipLaunchKernelGGL(cm::k_evict_move_v, dim3(n_seqs * n_kv * (hd / cm::EM_D)), dim3(cm::EM_NT), 0, (hipStream_t)stream,
+                     g, static_cast<uint16_t*>(vc), keep, plan, lens_out);
   return launched(me);
 }
 
