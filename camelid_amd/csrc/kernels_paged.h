@@ -192,8 +192,9 @@ struct EvictPlan {
 // One workgroup per (sequence, KV head): the plan, `kept` (the positions themselves), the weights
 // compacted.
 //
-// The smallest kept weight by its digits of 8 bits from the top: a histogram (one for every 4 waves:
-// weights crowd in few exponents) and a suffix sum of its 256 counts.  A thread holds K weights in
+// The smallest kept weight by its digits from the top, 11, 11 and 10 bits: a histogram (8 bits less of it
+// had the weights crowd in a few counters: 5.2 us for the first of 16383 weights) in two copies and a
+// suffix sum of its counts.  A thread holds K weights in
 // registers, runs of V at a time, so up to K * 1024 positions are read once; longer rows go through
 // the same code in pieces that are read again.  Then prefix sums of two counts in a word (weights
 // above the smallest, weights equal to it) give every kept position its place.
@@ -202,10 +203,10 @@ struct EvictPlan {
 template <int K>
 __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restrict__ weights, uint32_t keep,
                                                         uint32_t recent, EvictPlan plan, uint32_t* __restrict__ kept) {
-  constexpr uint32_t COPIES = EV_NT / 256, PIECE = EV_NT * K;
+  constexpr uint32_t COPIES = 2, BINS = 2048, PIECE = EV_NT * K;
   constexpr int V = K < 4 ? K : 4, N = K / V;  // N runs of V positions, EV_NT * V apart
   typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
-  __shared__ uint32_t hist[COPIES][256];
+  __shared__ uint32_t hist[COPIES][BINS];
   __shared__ uint32_t wave_sums[N][EV_NT / 64], wave_touched[N][EV_NT / 64];
   __shared__ uint32_t s_digit, s_rank, s_bad;
   const uint32_t s = blockIdx.x / g.n_kv, h = blockIdx.x - s * g.n_kv, tid = threadIdx.x, lane = tid & 63u;
@@ -266,8 +267,10 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
   uint32_t rank = keep - recent;  // positions still to be found among the keys equal in the digits so far
   const bool any = rank != 0;
   uint32_t prefix = 0;
-  for (int b = 24; b >= 0 && any; b -= 8) {
-    for (uint32_t i = tid; i < COPIES * 256; i += EV_NT) hist[0][i] = 0;
+  for (int b = 21; b >= 0 && any; b -= b > 10 ? 11 : 10) {
+    const uint32_t bins = b ? BINS : 1024u;  // digits of key >> b below those found, in `prefix` >> above
+    const int above_bits = b + (b ? 11 : 10);
+    for (uint32_t i = tid; i < COPIES * BINS; i += EV_NT) hist[0][i] = 0;
     __syncthreads();
     for (uint32_t p0 = 0; p0 < cut; p0 += PIECE) {
       if (!one) {
@@ -279,28 +282,22 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const uint32_t k = key[i][e];
-          if (at(p0, i, e) < cut && (b == 24 || (k >> ((b + 8) & 31)) == (prefix >> ((b + 8) & 31))))
-            atomicAdd(&hist[tid >> 8][(k >> b) & 255u], 1u);
+          if (at(p0, i, e) < cut && (b == 21 || k >> (above_bits & 31) == prefix >> (above_bits & 31)))
+            atomicAdd(&hist[(tid >> 6) % COPIES][(k >> b) & (bins - 1)], 1u);
         }
     }
     __syncthreads();
-    if (tid < 64) {  // lane l: digits 255 - 4 l .. 252 - 4 l
-      uint32_t c[4], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] = 0;
-        for (uint32_t v = 0; v < COPIES; ++v) c[i] += hist[v][255 - 4 * lane - i];
-        sum += c[i];
-      }
-      uint32_t above = ev_wave_scan(sum) - sum;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (above < rank && above + c[i] >= rank) {
-          s_digit = 255 - 4 * lane - i;
-          s_rank = rank - above;
-        }
-        above += c[i];
-      }
+    // thread t: digits 2047 - 2 t and 2046 - 2 t
+    const uint32_t hi = BINS - 1 - 2 * tid, c0 = hist[0][hi] + hist[1][hi], c1 = hist[0][hi - 1] + hist[1][hi - 1];
+    const uint32_t incl = ev_wave_scan(c0 + c1);
+    if (lane == 63) wave_sums[0][tid >> 6] = incl;
+    __syncthreads();
+    uint32_t above = incl - c0 - c1;
+    for (uint32_t v = 0; v < EV_NT / 64; ++v) above += v < tid >> 6 ? wave_sums[0][v] : 0u;
+    if (above < rank && above + c0 + c1 >= rank) {
+      const bool first = above + c0 >= rank;
+      s_digit = first ? hi : hi - 1;
+      s_rank = rank - above - (first ? 0u : c0);
     }
     __syncthreads();
     prefix |= s_digit << b;
@@ -389,23 +386,21 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
 // HBM; rows far apart share their 128-byte lines with rows that are left behind.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// K: one workgroup per (sequence, KV head, 8 dims), whole granules, chunks of R * EK_NT rows in registers.
-constexpr uint32_t EK_NT = 256;
-__global__ __launch_bounds__(EK_NT, 8) void k_evict_move_k(Paged g, uint16_t* __restrict__ kc, uint32_t keep,
-                                                           EvictPlan plan) {
+// K: one workgroup per (sequence, KV head, 8 dims), whole granules, chunks of R * EM_NT rows in registers.
+constexpr uint32_t EM_NT = 512;
+__device__ __forceinline__ void evict_move_k(const Paged& g, uint16_t* __restrict__ kc, uint32_t keep,
+                                             const EvictPlan& plan, uint32_t sh, uint32_t d) {
   constexpr uint32_t R = 4;
-  const uint32_t slices = g.hd / 8, tid = threadIdx.x;
-  const uint32_t sh = blockIdx.x / slices, d = (blockIdx.x - sh * slices) * 8, s = sh / g.n_kv, h = sh - s * g.n_kv;
-  if (!plan.old_lens[s]) return;
+  const uint32_t tid = threadIdx.x, s = sh / g.n_kv, h = sh - s * g.n_kv;
   const uint32_t* tab = g.table + (size_t)s * g.stride;
   const uint32_t* sp = plan.slot + (size_t)sh * keep;
   const uint32_t mask = (1u << g.shift) - 1u;
-  for (uint32_t j0 = 0; j0 < keep; j0 += R * EK_NT) {
+  for (uint32_t j0 = 0; j0 < keep; j0 += R * EM_NT) {
     u32x4 x[R];
     uint32_t to[R], slot[R];
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
-      const uint32_t j = min(j0 + r * EK_NT + tid, keep - 1);
+      const uint32_t j = min(j0 + r * EM_NT + tid, keep - 1);
       slot[r] = sp[j];
       to[r] = (tab[j >> g.shift] << g.shift) + (j & mask);
     }
@@ -415,7 +410,7 @@ __global__ __launch_bounds__(EK_NT, 8) void k_evict_move_k(Paged g, uint16_t* __
     __syncthreads();
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r)
-      if (j0 + r * EK_NT + tid < keep && slot[r] != to[r])
+      if (j0 + r * EM_NT + tid < keep && slot[r] != to[r])
         *reinterpret_cast<u32x4*>(kc + paged_base(g, to[r] >> g.shift, h) + paged_k(g, to[r] & mask, d)) = x[r];
   }
 }
@@ -424,15 +419,10 @@ __global__ __launch_bounds__(EK_NT, 8) void k_evict_move_k(Paged g, uint16_t* __
 // gathers from up to 8 of them, so a chunk is as many rows as EM_G distinct granules feed; these go to LDS
 // whole (2-byte loads from memory, 16 bytes apart between lanes, took the L1 47 accesses each: 24 us of
 // the 37 us that the move of 16x1088 -> 1024 rows took) and the output granules are put together from there.
-constexpr uint32_t EM_NT = 512, EM_G = 256, EM_D = 16;
-__global__ __launch_bounds__(EM_NT, 4) void k_evict_move_v(Paged g, uint16_t* __restrict__ vc, uint32_t keep,
-                                                           EvictPlan plan, uint32_t* __restrict__ lens_out) {
-  __shared__ u32x4 s_g[EM_G * EM_D];  // [granule][dim], 8 positions each
-  __shared__ uint32_t s_end[EM_NT / 64];
-  const uint32_t slices = g.hd / EM_D, tid = threadIdx.x;
-  const uint32_t sh = blockIdx.x / slices, sl = blockIdx.x - sh * slices, s = sh / g.n_kv, h = sh - s * g.n_kv;
-  if (sl == 0 && h == 0 && tid == 0) lens_out[s] = plan.new_lens[s];
-  if (!plan.old_lens[s]) return;
+constexpr uint32_t EM_G = 128, EM_D = 16;
+__device__ __forceinline__ void evict_move_v(const Paged& g, uint16_t* __restrict__ vc, uint32_t keep,
+                                             const EvictPlan& plan, uint32_t sh, uint32_t sl, u32x4* s_g, uint32_t* s_end) {
+  const uint32_t tid = threadIdx.x, s = sh / g.n_kv, h = sh - s * g.n_kv;
   const uint32_t* tab = g.table + (size_t)s * g.stride;
   const uint32_t* fp = plan.from + (size_t)sh * keep;
   const uint32_t* gp = plan.granule + (size_t)sh * keep;
@@ -483,6 +473,21 @@ __global__ __launch_bounds__(EM_NT, 4) void k_evict_move_v(Paged g, uint16_t* __
     }
     __syncthreads();
   }
+}
+
+// V's workgroups first: they take longer.
+__global__ __launch_bounds__(EM_NT, 8) void k_evict_move(Paged g, uint16_t* __restrict__ kc, uint16_t* __restrict__ vc,
+                                                         uint32_t keep, EvictPlan plan, uint32_t* __restrict__ lens_out) {
+  __shared__ u32x4 s_g[EM_G * EM_D];  // [granule][dim], 8 positions each
+  __shared__ uint32_t s_end[EM_NT / 64];
+  const uint32_t v_slices = g.hd / EM_D, n_v = g.n_seqs * g.n_kv * v_slices;
+  const bool is_v = blockIdx.x < n_v;
+  const uint32_t b = is_v ? blockIdx.x : blockIdx.x - n_v, slices = is_v ? v_slices : g.hd / 8;
+  const uint32_t sh = b / slices, sl = b - sh * slices, s = sh / g.n_kv;
+  if (is_v && sl == 0 && sh == s * g.n_kv && threadIdx.x == 0) lens_out[s] = plan.new_lens[s];
+  if (!plan.old_lens[s]) return;
+  if (is_v) evict_move_v(g, vc, keep, plan, sh, sl, s_g, s_end);
+  else evict_move_k(g, kc, keep, plan, sh, sl * 8);
 }
 
 }  // namespace cm

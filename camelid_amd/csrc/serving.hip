@@ -261,10 +261,8 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
   const auto select = cap <= 2048 ? cm::k_evict_select<2> : cap <= 8192 ? cm::k_evict_select<8> : cm::k_evict_select<16>;
   hipLaunchKernelGGL(select, dim3(n_seqs * n_kv), dim3(cm::EV_NT), 0, (hipStream_t)stream, g, weights, keep, recent, plan,
                      kept);
-  hipLaunchKernelGGL(cm::k_evict_move_k, dim3(n_seqs * n_kv * (hd / 8)), dim3(cm::EK_NT), 0, (hipStream_t)stream, g,
-                     static_cast<uint16_t*>(kc), keep, plan);
-  hipLaunchKernelGGL(cm::k_evict_move_v, dim3(n_seqs * n_kv * (hd / cm::EM_D)), dim3(cm::EM_NT), 0, (hipStream_t)stream,
-                     g, static_cast<uint16_t*>(vc), keep, plan, lens_out);
+  hipLaunchKernelGGL(cm::k_evict_move, dim3(n_seqs * n_kv * (hd / cm::EM_D + hd / 8)), dim3(cm::EM_NT), 0,
+                     (hipStream_t)stream, g, static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc), keep, plan, lens_out);
   return launched(me);
 }
 
