@@ -154,6 +154,192 @@ __global__ __launch_bounds__(64) void k_paged_rope_kv(Paged g, const float* __re
   }
 }
 
+// The same for rope_dim = head_dim, one workgroup per (granule of 8 positions, role): q heads, K
+// heads or V heads, so that the up to 8 new tokens of a granule are stored together: V as whole granules
+// (a granule holds 8 positions of a dim), K as 8 granules side by side.
+//   q, K: HD / 16 lanes per (token, head), each 8 dims of either half, which hold the pairs of both
+//         pairings; the norm's sum in order by one lane per (token, head) from LDS.
+//   V:    a lane per dim.
+// Bound: HBM.  207 MB (4 prompts of up to 2047 tokens, 24 + 8 + 8 heads of 128): 115 us with one wave per
+// (token, head) and 2-byte stores.
+constexpr uint32_t RK_NT = 256;
+constexpr uint32_t rk_heads(uint32_t hd) { return RK_NT / (hd / 16) / 8; }  // q or K heads of a workgroup
+constexpr uint32_t rk_v_heads(uint32_t hd) { return RK_NT / hd; }
+__host__ __device__ constexpr uint32_t rk_roles(uint32_t hd, uint32_t n_heads, uint32_t n_kv) {
+  return (n_heads + rk_heads(hd) - 1) / rk_heads(hd) + (n_kv + rk_heads(hd) - 1) / rk_heads(hd) +
+         (n_kv + rk_v_heads(hd) - 1) / rk_v_heads(hd);
+}
+// Granules that n_new consecutive positions can reach into.
+constexpr uint32_t rk_granules(uint32_t n_new) { return (n_new + 6) / 8 + 1; }
+
+typedef float f32x4v __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void rk_load8(const float* p, float (&x)[8]) {
+  const f32x4v a = *reinterpret_cast<const f32x4v*>(p), b = *reinterpret_cast<const f32x4v*>(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = a[i];
+    x[4 + i] = b[i];
+  }
+}
+typedef uint32_t rk_u32x4 __attribute__((ext_vector_type(4)));
+template <int T>
+__device__ __forceinline__ rk_u32x4 rk_pack8(const float (&x)[8]) {
+  rk_u32x4 u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = to_bits16<T>(x[2 * i]) | (uint32_t)to_bits16<T>(x[2 * i + 1]) << 16;
+  return u;
+}
+
+template <int HD, int QT, int KT>
+__global__ __launch_bounds__(RK_NT) void k_paged_rope_kv8(Paged g, const float* __restrict__ qkv, uint32_t n_new,
+                                                          const uint32_t* __restrict__ new_lens, uint32_t n_heads,
+                                                          uint32_t split_half, const float* __restrict__ cosv,
+                                                          const float* __restrict__ sinv,
+                                                          const float* __restrict__ q_norm,
+                                                          const float* __restrict__ k_norm, float eps,
+                                                          void* __restrict__ q_out, uint16_t* __restrict__ kc,
+                                                          uint16_t* __restrict__ vc, uint32_t roles,
+                                                          uint32_t granules) {
+  constexpr uint32_t LPR = HD / 16, PAIRS = RK_NT / LPR, HEADS = rk_heads(HD), V_HEADS = rk_v_heads(HD), HALF = HD / 2;
+  __shared__ float s_x[PAIRS][HD + 4];
+  __shared__ float s_scale[PAIRS];
+  const uint32_t tid = threadIdx.x, role = blockIdx.x % roles, sg = blockIdx.x / roles;
+  const uint32_t s = sg / granules, gi = sg - s * granules;
+  uint32_t first, len;
+  if (!paged_rows(g, new_lens, n_new, s, &first, &len)) return;
+  const uint32_t p0 = (first & ~7u) + 8 * gi;  // the granule's first position
+  if (p0 >= len) return;
+  const size_t width = (size_t)(n_heads + 2 * g.n_kv) * HD;
+  const uint32_t q_roles = (n_heads + HEADS - 1) / HEADS, k_roles = (g.n_kv + HEADS - 1) / HEADS;
+  const uint32_t mask = (1u << g.shift) - 1u;
+  const bool isq = role < q_roles;
+  uint32_t page = 0;
+  if (!isq) {
+    page = g.table[(size_t)s * g.stride + (p0 >> g.shift)];
+    if (page >= g.n_pages) {
+      if (tid == 0) paged_flag(g, PG_BAD_PAGE);
+      return;
+    }
+  }
+  if (role >= q_roles + k_roles) {
+    const uint32_t h = (role - q_roles - k_roles) * V_HEADS + tid / HD, d = tid % HD;
+    if (h >= g.n_kv) return;
+    const float* src = qkv + ((size_t)s * n_new) * width + (size_t)(n_heads + g.n_kv + h) * HD + d;
+    float x[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t p = p0 + i;
+      x[i] = p >= first && p < len ? src[(size_t)(p - first) * width] : 0.0f;
+    }
+    uint16_t* dst = vc + paged_base(g, page, h) + paged_v(g, p0 & mask, d);
+    const rk_u32x4 u = rk_pack8<KT>(x);
+    if (p0 >= first && p0 + 8 <= len) {
+      *reinterpret_cast<rk_u32x4*>(dst) = u;
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i)
+        if (p0 + i >= first && p0 + i < len) dst[i] = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
+    }
+    return;
+  }
+  const uint32_t j = tid % LPR, pair = tid / LPR, i8 = pair % 8;
+  const uint32_t h = (isq ? role : role - q_roles) * HEADS + pair / 8;
+  const uint32_t p = p0 + i8;
+  const bool live = p >= first && p < len && h < (isq ? n_heads : g.n_kv);
+  const size_t row = (size_t)s * n_new + (p - first);
+  float a[8], b[8];  // dims 8 j .. and HALF + 8 j ..
+  float ca[8], sa[8];
+  if (live) {
+    const float* src = qkv + row * width + (size_t)(isq ? h : n_heads + h) * HD;
+    rk_load8(src + 8 * j, a);
+    rk_load8(src + HALF + 8 * j, b);
+    const float *c = cosv + row * HALF, *sn = sinv + row * HALF;
+    if (split_half) {  // pairs 8 j .. 8 j + 7: (a, b)
+      rk_load8(c + 8 * j, ca);
+      rk_load8(sn + 8 * j, sa);
+    } else {  // pairs 4 j .. inside a, HALF / 2 + 4 j .. inside b
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const f32x4v x = *reinterpret_cast<const f32x4v*>(c + k * (HALF / 2) + 4 * j);
+        const f32x4v y = *reinterpret_cast<const f32x4v*>(sn + k * (HALF / 2) + 4 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ca[4 * k + i] = x[i];
+          sa[4 * k + i] = y[i];
+        }
+      }
+    }
+  }
+  const float* nw = isq ? q_norm : k_norm;
+  if (nw) {
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s_x[pair][8 * j + i] = a[i];
+        s_x[pair][HALF + 8 * j + i] = b[i];
+      }
+    }
+    __syncthreads();
+    if (tid < PAIRS) {  // (padding rows sum what lies there)
+      float acc = 0.0f;
+#pragma unroll 8
+      for (uint32_t d = 0; d < HD; ++d) {
+        const float x = s_x[tid][d];
+        acc = acc + x * x;
+      }
+      s_scale[tid] = 1.0f / sqrtf(acc / (float)HD + eps);
+    }
+    __syncthreads();
+    if (live) {
+      const float sc = s_scale[pair];
+      float wa[8], wb[8];
+      rk_load8(nw + 8 * j, wa);
+      rk_load8(nw + HALF + 8 * j, wb);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] = (a[i] * sc) * wa[i];
+        b[i] = (b[i] * sc) * wb[i];
+      }
+    }
+  }
+  if (!live) return;
+  if (split_half) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x0 = a[i], x1 = b[i];
+      a[i] = (x0 * ca[i]) - (x1 * sa[i]);
+      b[i] = (x0 * sa[i]) + (x1 * ca[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x0 = a[2 * i], x1 = a[2 * i + 1], y0 = b[2 * i], y1 = b[2 * i + 1];
+      a[2 * i] = (x0 * ca[i]) - (x1 * sa[i]);
+      a[2 * i + 1] = (x0 * sa[i]) + (x1 * ca[i]);
+      b[2 * i] = (y0 * ca[4 + i]) - (y1 * sa[4 + i]);
+      b[2 * i + 1] = (y0 * sa[4 + i]) + (y1 * ca[4 + i]);
+    }
+  }
+  if (!isq) {
+    uint16_t* dst = kc + paged_base(g, page, h);
+    *reinterpret_cast<rk_u32x4*>(dst + paged_k(g, p & mask, 8 * j)) = rk_pack8<KT>(a);
+    *reinterpret_cast<rk_u32x4*>(dst + paged_k(g, p & mask, HALF + 8 * j)) = rk_pack8<KT>(b);
+    return;
+  }
+  const size_t at = (row * n_heads + h) * HD + 8 * j;
+  if constexpr (QT == TY_F32) {
+    f32x4v* dst = reinterpret_cast<f32x4v*>(static_cast<float*>(q_out) + at);
+    dst[0] = f32x4v{a[0], a[1], a[2], a[3]};
+    dst[1] = f32x4v{a[4], a[5], a[6], a[7]};
+    dst[HALF / 4] = f32x4v{b[0], b[1], b[2], b[3]};
+    dst[HALF / 4 + 1] = f32x4v{b[4], b[5], b[6], b[7]};
+  } else {
+    uint16_t* dst = static_cast<uint16_t*>(q_out) + at;
+    *reinterpret_cast<rk_u32x4*>(dst) = rk_pack8<QT>(a);
+    *reinterpret_cast<rk_u32x4*>(dst + HALF) = rk_pack8<QT>(b);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Eviction.  A sequence of more than `keep` positions keeps, for each KV head, its last `recent`
 // positions and the keep - recent of highest accumulated weight among the others (equal weights:

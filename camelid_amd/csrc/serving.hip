@@ -133,10 +133,40 @@ int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new,
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(kc) || !aligned16(vc) || !aligned4(cos_tab) ||
       !aligned4(sin_tab) || !aligned4(q_norm) || !aligned4(k_norm) || !aligned4(new_lens))
     return cm::fail_global(me, "qkv, q_out and the cache must be 16-byte aligned, the rest 4-byte aligned");
-  const uint64_t grid = (uint64_t)n_seqs * n_new * (n_heads + n_kv);
-  if (grid > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  const uint64_t rows = (uint64_t)n_seqs * n_new * (n_heads + n_kv);
+  if (rows > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  if (rope_dim == hd) {
+    const uint32_t roles = cm::rk_roles(hd, n_heads, n_kv), granules = cm::rk_granules(n_new);
+    const uint64_t grid = (uint64_t)n_seqs * granules * roles;  // (below 2 * rows)
+    if (grid > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+    const auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(cm::RK_NT), 0, (hipStream_t)stream, g, qkv, n_new, new_lens,
+                         n_heads, split_half, cos_tab, sin_tab, q_norm, k_norm, eps, q_out, static_cast<uint16_t*>(kc),
+                         static_cast<uint16_t*>(vc), roles, granules);
+    };
+    const auto typed = [&](auto f32_f16, auto f16, auto f32_bf16, auto bf16) {
+      if (kv_type == TY_F16) {
+        if (q_type == TY_F32) go(f32_f16);
+        else go(f16);
+      } else {
+        if (q_type == TY_F32) go(f32_bf16);
+        else go(bf16);
+      }
+    };
+    if (hd == 64)
+      typed(cm::k_paged_rope_kv8<64, TY_F32, TY_F16>, cm::k_paged_rope_kv8<64, TY_F16, TY_F16>,
+            cm::k_paged_rope_kv8<64, TY_F32, TY_BF16>, cm::k_paged_rope_kv8<64, TY_BF16, TY_BF16>);
+    else if (hd == 128)
+      typed(cm::k_paged_rope_kv8<128, TY_F32, TY_F16>, cm::k_paged_rope_kv8<128, TY_F16, TY_F16>,
+            cm::k_paged_rope_kv8<128, TY_F32, TY_BF16>, cm::k_paged_rope_kv8<128, TY_BF16, TY_BF16>);
+    else
+      typed(cm::k_paged_rope_kv8<256, TY_F32, TY_F16>, cm::k_paged_rope_kv8<256, TY_F16, TY_F16>,
+            cm::k_paged_rope_kv8<256, TY_F32, TY_BF16>, cm::k_paged_rope_kv8<256, TY_BF16, TY_BF16>);
+    return launched(me);
+  }
+  // part of a head rotated: pairs fall anywhere
   const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(64), 0, (hipStream_t)stream, g, qkv, n_new, new_lens,
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)rows), dim3(64), 0, (hipStream_t)stream, g, qkv, n_new, new_lens,
                        n_heads, rope_dim, split_half, cos_tab, sin_tab, q_norm, k_norm, eps, q_out,
                        static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc));
   };
