@@ -156,7 +156,6 @@ struct PaPiece {
   uint32_t s, h, rb, t0, t1, n, slot;  // n: the segment's pieces; slot: this piece's (n > 1)
   PaSeq q;
   bool any;
-  bool stream;  // the batch's K and V are beyond what the memory-side cache holds
 };
 
 // Piece `index` of the batch (pieces in the order sequence, KV head, block, tiles).  Each wave works
@@ -205,10 +204,6 @@ __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, boo
   const uint32_t even = q.tiles / p.n, more = q.tiles - even * p.n;  // the first `more` pieces take one tile more
   p.t0 = piece * even + min(piece, more);
   p.t1 = p.t0 + even + (piece < more ? 1u : 0u);
-  // 256 MiB.  One new token, 32 query heads, hd 128, f16: plain loads 45.6 us and loads that leave the
-  // caches alone 47.9 for 269 MB read again and again, 54.9 and 49.7 for 4 such caches in turn, 101.8 and
-  // 91.7 for 538 MB; 28.9 and 31.6 for 134 MB.  (Several row blocks read K and V several times.)
-  p.stream = a.blocks == 1 && total > (1u << 28) / (PA_TILE * 4 * a.g.hd);
   p.slot = slots + seg * p.n + piece;
   return p;
 }
@@ -218,26 +213,19 @@ __device__ __forceinline__ uint32_t pa_page(const PaArgs& a, const uint32_t* tab
   return pos < len ? tab[pos >> a.g.shift] : 0u;
 }
 
-// N granules, `step` apart; stream: without keeping them in the caches.  (The empty asm statements keep
-// the compiler from making one plain load of the two.)
-template <int N, typename V>
-__device__ __forceinline__ void pa_load(bool stream, const V* p, size_t step, V* to) {
-  if (stream) {
-    asm volatile("" ::: "memory");
+// N granules, `step` apart; STREAM: without keeping them in the caches.
+template <bool STREAM, int N, typename V>
+__device__ __forceinline__ void pa_load(const V* p, size_t step, V* to) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) to[i] = __builtin_nontemporal_load(p + i * step);
-    asm volatile("" ::: "memory");
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) to[i] = p[i * step];
-  }
+  for (int i = 0; i < N; ++i) to[i] = STREAM ? __builtin_nontemporal_load(p + i * step) : p[i * step];
 }
 
 // Workgroups of a CU, by registers and LDS.
 constexpr int pa_per_cu(int hd, int nr) { return hd == 64 ? 5 - nr : hd == 128 ? 4 - nr : 2; }
 
-// One piece per workgroup.
-template <int HD, int KT, int QT, int NR>
+// One piece per workgroup.  STREAM: the batch's K and V are beyond what the memory-side cache holds and
+// pass the caches by.
+template <int HD, int KT, int QT, int NR, bool STREAM>
 __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a) {
   typedef typename Op16<KT>::v8 v8;
   typedef typename Op16<KT>::e e16;
@@ -285,14 +273,14 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
       const uint16_t* p = a.kc + ((size_t)page * g.n_kv + h) * head_elems +
                           (((size_t)grp << g.shift) + ((pos0 + ko) & pmask)) * 8;
       const size_t step = (size_t)4 << g.shift;  // granules of 32 dims
-      pa_load<KS>(pc.stream, reinterpret_cast<const v8*>(p), step, kf[0]);
-      pa_load<KS>(pc.stream, reinterpret_cast<const v8*>(p) + 4, step, kf[1]);
+      pa_load<STREAM, KS>(reinterpret_cast<const v8*>(p), step, kf[0]);
+      pa_load<STREAM, KS>(reinterpret_cast<const v8*>(p) + 4, step, kf[1]);
     };
     const auto load_v = [&](uint32_t pos0, uint32_t page) {
       if (page >= g.n_pages) page = 0;
       const uint16_t* p = a.vc + ((size_t)page * g.n_kv + h) * head_elems +
                           ((size_t)(((pos0 + 8 * grp) & pmask) >> 3) * HD + col) * 8;
-      pa_load<DS>(pc.stream, reinterpret_cast<const v8*>(p), 16, vf);
+      pa_load<STREAM, DS>(reinterpret_cast<const v8*>(p), 16, vf);
     };
     uint32_t pk = 0, pv = 0, pkn = 0, pvn = 0;
     if (ta < t1) {

@@ -85,7 +85,12 @@ PaSizes pa_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_k
 
 template <int HD, int KT, int QT, int NR>
 bool pa_launch(const cm::PaArgs& a, const PaSizes& z, hipStream_t stream) {
-  const auto split = cm::k_pa_split<HD, KT, QT, NR>;
+  // K and V that the batch's tables can hold, against the 256 MB of the memory-side cache (several row
+  // blocks read them several times).  One new token, 32 query heads, hd 128, f16: plain loads 28.9 us and
+  // streaming loads 31.6 for 134 MB read again and again, 33.9 and 32.2 for 8 such caches in turn; 45.6 and
+  // 47.9 for 269 MB, 54.9 and 49.7 for 4 of them; 101.8 and 91.7 for 538 MB
+  const bool passing = z.blocks == 1 && ((uint64_t)a.g.n_seqs * a.g.n_kv * HD * 4 * a.g.stride << a.g.shift) > (256u << 20);
+  const auto split = passing ? cm::k_pa_split<HD, KT, QT, NR, true> : cm::k_pa_split<HD, KT, QT, NR, false>;
   constexpr size_t lds = (size_t)16 * NR * (4 * (HD + 4 + 2) + 1) * 4;
   if (lds > 64 * 1024) {
     const hipError_t st = hipFuncSetAttribute(reinterpret_cast<const void*>(split),
