@@ -255,6 +255,42 @@ __global__ __launch_bounds__(VD_NT) void k_vd_stats(VdArgs a, uint32_t per) {
   }
 }
 
+// Logits v0 .. v0 + 7 of a row (-inf behind its end), every load on its way before the first is used.
+template <int LT>
+__device__ __forceinline__ void vd_load8(const void* row, uint32_t v0, uint32_t vocab, float (&l)[8]) {
+  typedef typename VdLogits<LT>::vec vec;
+  constexpr int V = VdLogits<LT>::V;
+  if (v0 + 8 <= vocab) {
+    vec x[8 / V];
+#pragma unroll
+    for (int k = 0; k < 8 / V; ++k)
+      x[k] = *reinterpret_cast<const vec*>(static_cast<const typename VdLogits<LT>::E*>(row) + v0 + k * V);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (LT == TY_F32) l[i] = x[i / V][i % V];
+      else l[i] = from_bits16<LT>(x[i / V][i % V]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l[i] = v0 + i < vocab ? load_as_f32<LT>(row, v0 + i) : -INFINITY;
+  }
+}
+// exp((l - m) / T) of 8 logits, as vd_each's.
+__device__ __forceinline__ void vd_exp8(const float (&l)[8], float m, float temp, const uint64_t* tab, double (&y)[8]) {
+  const double by = vd_by(temp), md = (double)m;
+  const float low = m - 704.0f * (vd_greedy(temp) ? 1.0f : temp);
+  if (low > -1e38f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double e = vd_exp_near((double)fmaxf(l[i], low) - md, by, tab);
+      y[i] = l[i] > low ? e : 0.0;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = vd_exp((double)l[i] - md, by, tab);
+  }
+}
+
 // ---- acceptance: every workgroup of k_vd_rest and k_vd_pick works out its sequence's
 enum { VD_DRAW = 0, VD_GREEDY = 1, VD_NONE = 2 };
 struct VdShared {
@@ -303,8 +339,13 @@ __device__ __forceinline__ void vd_accept(const VdArgs& a, uint32_t s, VdShared&
       const float m = vd_unkey(top);
       if (!vd_bad(m)) {
         if (was) z *= vd_exp((double)vd_unkey(was) - (double)m, by, sh.tab);
+        float l[8];
+        double e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z += q[i].z * vd_exp((double)q[i].m - (double)m, by, sh.tab);
+        for (int i = 0; i < 8; ++i) l[i] = q[i].m;
+        vd_exp8(l, m, temp, sh.tab, e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z += q[i].z * e[i];
       }
     }
     // the 16 lanes' sums against the row's maximum (a lane without a finite one holds z = 0)
@@ -415,7 +456,8 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
   const uint32_t s = blockIdx.x, tid = threadIdx.x, n = vd_drafts(a, s);
   vd_accept<LT>(a, s, sh);
   const uint32_t took = sh.took, state = sh.state;
-  const double by = vd_by(a.temperature[s]);
+  const float temp = a.temperature[s];
+  const double by = vd_by(temp);
   const uint32_t* tok = a.tokens + (size_t)s * a.n_draft;
   uint32_t pick = 0xffffffffu;
   if (state == VD_GREEDY) {
@@ -434,18 +476,17 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
     const auto masses = [&](uint32_t share, bool whole, double (&m)[8]) {
       const uint32_t v0 = share * VD_SHARE + tid * 8;
       float lp[8], lq[8];
+      vd_load8<LT>(prow, v0, a.vocab, lp);
+      if (apart && !whole) vd_load8<LT>(qrow, v0, a.vocab, lq);
+      vd_exp8(lp, P.m, temp, sh.tab, m);
+      if (apart && !whole) {
+        double q[8];
+        vd_exp8(lq, Q.m, temp, sh.tab, q);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {  // (every load on its way before the first is used)
-        const uint32_t v = min(v0 + i, a.vocab - 1);
-        lp[i] = load_as_f32<LT>(prow, v);
-        lq[i] = load_as_f32<LT>(qrow, v);
+        for (int i = 0; i < 8; ++i) m[i] = fmax(m[i] * ip - q[i] * iq, 0.0);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        double y = vd_exp((double)lp[i] - (double)P.m, by, sh.tab);
-        if (apart && !whole) y = fmax(y * ip - vd_exp((double)lq[i] - (double)Q.m, by, sh.tab) * iq, 0.0);
-        m[i] = v0 + i < a.vocab && (whole || v0 + i != x_tok) ? y : 0.0;
-      }
+      for (int i = 0; i < 8; ++i) m[i] = v0 + i < a.vocab && (whole || v0 + i != x_tok) ? m[i] : 0.0;
     };
     double m[8];
     if (x_tok < a.vocab) {  // the share of a certain draft, without it
@@ -526,7 +567,6 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
         lp = NAN;
         if (x < a.vocab) {
           const VdPart R = sh.row[tid];
-          const float temp = a.temperature[s];
           const double y = (double)load_as_f32<LT>(vd_target<LT>(a, s, tid), x) - (double)R.m;
           lp = (float)(y / (vd_greedy(temp) ? 1.0 : (double)temp) - log(R.z));
         }
