@@ -161,6 +161,8 @@ SIGNATURES: dict[str, tuple] = {
     "camelid_hip_verify_drafts_workspace": (C.c_size_t, [C.c_uint32] * 3),
     "camelid_hip_verify_drafts": (C.c_int, [vp, vp, C.c_uint32, vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, vp, vp,
                                             vp, vp, vp, vp, C.c_size_t, vp]),
+    "camelid_hip_verify_sampled": (C.c_int, [vp, f32p, f32p, f32p, C.c_uint32, C.c_uint32, C.c_float, u32p, f32p,
+                                             C.c_float, f32p, u32p, u32p, f32p]),
     "camelid_hip_inorder_sum_rows": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, vp]),
     "camelid_hip_expf": (C.c_int, [vp, vp, C.c_size_t, vp]),
     "camelid_expf_host": (None, [f32p, f32p, C.c_size_t]),

@@ -190,6 +190,12 @@ struct camelid_hip_engine {
   // their logits and greedy tokens
   float *v_embs = nullptr, *v_cos = nullptr, *v_sin = nullptr, *v_logits = nullptr, *v_pv = nullptr;
   uint32_t *v_tok = nullptr, *v_pi = nullptr;
+  // sampled verify: its small inputs and outputs, the drafts' logits and the workspace (on first use)
+  uint32_t* vs_in = nullptr;   // tokens [K], then as f32: temperature [1], uniforms [K]
+  uint32_t* vs_out = nullptr;  // accepted [1], tokens [K], then as f32: log-probabilities [K]
+  float* vs_draft = nullptr;   // [K][vocab]
+  char* vs_ws = nullptr;
+  size_t vs_ws_bytes = 0;
   uint32_t filled = 0;
   uint32_t cur_pos = 0;  // host copy of the position being computed (profiling byte counts)
   bool capture = false;
@@ -2249,11 +2255,13 @@ int camelid_hip_prefill(camelid_hip_engine* e, const float* embs, const float* c
   return 0;
 }
 
-int camelid_hip_verify(camelid_hip_engine* e, const float* embs, const float* cos_all, const float* sin_all,
-                       uint32_t base_position, uint32_t k, float scale, uint32_t* tokens_out) {
+// The argument checks and the forward of the verify calls: the k tokens' K/V stored, their logits in
+// e->v_logits [k][vocab] and, with `greedy`, the argmax of each row in e->v_tok; launched, not waited for.
+static int verify_forward(camelid_hip_engine* e, const float* embs, const float* cos_all, const float* sin_all,
+                          uint32_t base_position, uint32_t k, float scale, bool greedy) {
   if (!e) return fail(nullptr, "null engine");
   if (!ready(e)) return fail(e, "weights not ready");
-  if (!embs || !cos_all || !sin_all || !tokens_out) return fail(e, "null argument");
+  if (!embs || !cos_all || !sin_all) return fail(e, "null argument");
   const camelid_hip_dims& d = e->d;
   if (k == 0 || k > CAMELID_MAX_VERIFY_K) return fail(e, "verify: k out of 1..=8");
   if ((size_t)base_position + k > d.max_pos) return fail(e, "verify beyond max_pos");
@@ -2284,9 +2292,11 @@ int camelid_hip_verify(camelid_hip_engine* e, const float* embs, const float* co
       launch_kgemm(e->out_k, k, e->pf_kd, e->pf_kq, e->v_logits, d.vocab, nullptr, e->stream, e->pf_kqt);
     else
       launch_gemm(e->out, k, e->pf_xq, e->pf_xs, e->v_logits, nullptr, e->stream);
-    CM_LAUNCH(cm::k_argmax_rows_part, dim3(cm::AMR_PARTS, k), dim3(256), 0, e->stream, e->v_logits, (int)d.vocab,
-              e->v_pv, e->v_pi);
-    CM_LAUNCH(cm::k_argmax_rows_finish, dim3(k), dim3(64), 0, e->stream, e->v_pv, e->v_pi, e->v_tok);
+    if (greedy) {
+      CM_LAUNCH(cm::k_argmax_rows_part, dim3(cm::AMR_PARTS, k), dim3(256), 0, e->stream, e->v_logits, (int)d.vocab,
+                e->v_pv, e->v_pi);
+      CM_LAUNCH(cm::k_argmax_rows_finish, dim3(k), dim3(64), 0, e->stream, e->v_pv, e->v_pi, e->v_tok);
+    }
   } else {
     // k single-token steps; the head writes each greedy token to v_tok[step]
     *e->p_st = cm::StepState{base_position, 0u, 0u, 0u};
@@ -2298,6 +2308,9 @@ int camelid_hip_verify(camelid_hip_engine* e, const float* embs, const float* co
       e->cur_pos = base_position + t;
       run_stack(e, e->v_cos + (size_t)t * half, e->v_sin + (size_t)t * half, 0, scale);
       run_head(e, e->v_tok, k);
+      if (!greedy)
+        HIP_TRY(e, hipMemcpyAsync(e->v_logits + (size_t)t * d.vocab, e->logits, (size_t)d.vocab * 4,
+                                  hipMemcpyDeviceToDevice, e->stream));
     }
     if (nf_end(e)) return 1;
   }
@@ -2305,13 +2318,73 @@ int camelid_hip_verify(camelid_hip_engine* e, const float* embs, const float* co
     e->filled = 0;
     return 1;
   }
+  return 0;
+}
+
+// Waits for the verify calls' work.
+static int verify_wait(camelid_hip_engine* e) {
   hipError_t st = hipStreamSynchronize(e->stream);
   if (st != hipSuccess) {
     e->filled = 0;
     return fail(e, std::string("verify: ") + hipGetErrorString(st));
   }
-  if (nf_failed(e)) return 1;
+  return nf_failed(e);
+}
+
+int camelid_hip_verify(camelid_hip_engine* e, const float* embs, const float* cos_all, const float* sin_all,
+                       uint32_t base_position, uint32_t k, float scale, uint32_t* tokens_out) {
+  if (e && ready(e) && !tokens_out) return fail(e, "null argument");
+  if (verify_forward(e, embs, cos_all, sin_all, base_position, k, scale, true) || verify_wait(e)) return 1;
   HIP_TRY(e, hipMemcpy(tokens_out, e->v_tok, (size_t)k * 4, hipMemcpyDeviceToHost));
+  return 0;
+}
+
+int camelid_hip_verify_sampled(camelid_hip_engine* e, const float* embs, const float* cos_all, const float* sin_all,
+                               uint32_t base_position, uint32_t k, float scale, const uint32_t* draft_tokens,
+                               const float* draft_logits, float temperature, const float* uniforms,
+                               uint32_t* accepted_out, uint32_t* tokens_out, float* logprobs_out) {
+  if (!e) return fail(nullptr, "null engine");
+  if (!uniforms || !accepted_out || !tokens_out || (k > 1 && !draft_tokens)) return fail(e, "null argument");
+  if (!(temperature >= 0.0f) || !std::isfinite(temperature)) return fail(e, "temperature must be finite and not negative");
+  for (uint32_t t = 0; t < k && t < CAMELID_MAX_VERIFY_K; ++t) {
+    if (!(uniforms[t] >= 0.0f && uniforms[t] < 1.0f)) return fail(e, "uniforms must be in [0, 1)");
+    if (t + 1 < k && draft_tokens[t] >= e->d.vocab) return fail(e, "draft token out of range");
+  }
+  if (k == 0 || k > CAMELID_MAX_VERIFY_K) return fail(e, "verify: k out of 1..=8");
+  HIP_TRY(e, hipSetDevice(e->device));
+  const uint32_t vocab = e->d.vocab, drafts = k - 1;
+  constexpr size_t K = CAMELID_MAX_VERIFY_K;
+  const bool with_draft = draft_logits && drafts;
+  if (!e->vs_in && dev_alloc(e, &e->vs_in, 2 * K + 1)) return 1;
+  if (!e->vs_out && dev_alloc(e, &e->vs_out, 2 * K + 1)) return 1;
+  if (with_draft && !e->vs_draft && dev_alloc(e, &e->vs_draft, (K - 1) * (size_t)vocab)) return 1;
+  if (!e->vs_ws) {
+    e->vs_ws_bytes = camelid_hip_verify_drafts_workspace(1, K - 1, vocab);
+    if (dev_alloc(e, &e->vs_ws, e->vs_ws_bytes)) return 1;
+  }
+  uint32_t in[2 * K + 1] = {}, out[2 * K + 1];
+  if (drafts) std::memcpy(in, draft_tokens, drafts * 4);
+  std::memcpy(in + K, &temperature, 4);
+  std::memcpy(in + K + 1, uniforms, (size_t)k * 4);
+  HIP_TRY(e, hipMemcpy(e->vs_in, in, sizeof in, hipMemcpyHostToDevice));
+  if (with_draft) HIP_TRY(e, hipMemcpy(e->vs_draft, draft_logits, (size_t)drafts * vocab * 4, hipMemcpyHostToDevice));
+  if (verify_forward(e, embs, cos_all, sin_all, base_position, k, scale, false)) return 1;
+  const float* fin = reinterpret_cast<const float*>(e->vs_in + K);
+  if (camelid_hip_verify_drafts(e->v_logits, with_draft ? e->vs_draft : nullptr, CAMELID_F32, e->vs_in, nullptr, 1,
+                                drafts, vocab, fin, fin + 1, e->vs_out, e->vs_out + 1,
+                                reinterpret_cast<float*>(e->vs_out + 1 + K), e->vs_ws, e->vs_ws_bytes, e->stream)) {
+    e->filled = 0;
+    return fail(e, g_last_error);
+  }
+  if (verify_wait(e)) return 1;
+  HIP_TRY(e, hipMemcpy(out, e->vs_out, sizeof out, hipMemcpyDeviceToHost));
+  if (out[0] >= k || out[1 + out[0]] == 0xffffffffu) {
+    e->filled = 0;
+    return fail(e, "verify: logits without a distribution (NaN or infinite)");
+  }
+  *accepted_out = out[0];
+  std::memcpy(tokens_out, out + 1, (size_t)k * 4);
+  if (logprobs_out) std::memcpy(logprobs_out, out + 1 + K, (size_t)k * 4);
   return 0;
 }
 

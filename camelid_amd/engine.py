@@ -212,6 +212,26 @@ class HipResidentDecode:
                                                base_position, k, scale, N.ptr(out, C.c_uint32)))
         return out
 
+    def verify_sampled(self, embeddings, cos_all, sin_all, base_position: int, scale: float, draft_tokens, uniforms,
+                       temperature: float, draft_logits=None):
+        """The k tokens of embeddings at [base_position, base_position + k), the last k - 1 of them drafts, in
+        one batched forward; each draft accepted or replaced by sampling (camelid_hip_verify_sampled).
+        Returns (tokens, log-probabilities): the accepted drafts and the token drawn behind them.
+        filled is left to the caller (base_position + len(tokens))."""
+        d = self.dims
+        k = self._rows_checked(embeddings, cos_all, sin_all)
+        e, c, s = _f32(embeddings), _f32(cos_all), _f32(sin_all)
+        drafts = _sized(np.ascontiguousarray(draft_tokens, dtype=np.uint32).reshape(-1), k - 1, "draft_tokens")
+        u = _sized(_f32(uniforms).reshape(-1), k, "uniforms")
+        dl = _sized(_f32(draft_logits), (k - 1) * d.vocab, "draft_logits") if draft_logits is not None else None
+        acc = C.c_uint32(0)
+        toks, lps = np.empty(k, np.uint32), np.empty(k, np.float32)
+        self._chk(self._lib.camelid_hip_verify_sampled(
+            self._h, N.ptr(e, C.c_float), N.ptr(c, C.c_float), N.ptr(s, C.c_float), base_position, k, scale,
+            N.ptr(drafts, C.c_uint32) if k > 1 else None, N.ptr(dl, C.c_float) if dl is not None and k > 1 else None,
+            temperature, N.ptr(u, C.c_float), C.byref(acc), N.ptr(toks, C.c_uint32), N.ptr(lps, C.c_float)))
+        return toks[:acc.value + 1], lps[:acc.value + 1]
+
     def generate(self, token: int, position: int, n_steps: int, scale: float) -> np.ndarray:
         """Device-side greedy loop (forward_token_device, cuda_resident.rs:7529)."""
         out = np.empty(n_steps, np.uint32)

@@ -377,8 +377,39 @@ class ResidentSession:
             pos += 1
         return out
 
+    def generate_sampled(self, prompt, n_new: int, temperature: float, rng: np.random.Generator,
+                         max_draft: int = 0) -> list[int]:
+        """n_new tokens sampled at `temperature` (0: greedy).  max_draft > 0: up to that many tokens
+        looked up in the text so far are verified with each step (HipResidentDecode.verify_sampled),
+        which leaves the distribution as it is and saves steps where the text repeats itself."""
+        text = [int(t) for t in prompt]
+        self.engine.set_filled(0)
+        self.prefill(text[:-1])
+        out: list[int] = []
+        while len(out) < n_new:
+            pos = len(text) - 1
+            room = min(max_draft, HipResidentDecode.MAX_VERIFY_K - 1, n_new - len(out) - 1,
+                       self.engine.max_pos() - pos - 1)
+            step = [text[-1]] + (lookup_draft(text, room) if room > 0 else [])
+            cos, sin = self.model.rope_tables(pos, len(step))
+            u = rng.random(len(step), dtype=np.float32)
+            toks, _ = self.engine.verify_sampled(self.model.embed(step), cos, sin, pos, self.cfg.scale(), step[1:], u,
+                                                 temperature)
+            text += [int(t) for t in toks]
+            out += [int(t) for t in toks]
+            self.engine.set_filled(pos + len(toks))
+        return out
+
     def close(self) -> None:
         self.engine.close()
+
+
+def lookup_draft(text, n: int) -> list[int]:
+    """Up to n tokens that followed the latest earlier occurrence of the text's last two."""
+    for i in range(len(text) - 3, -1, -1):
+        if text[i:i + 2] == text[-2:]:
+            return [int(t) for t in text[i + 2:i + 2 + n]]
+    return []
 
 
 def tiny_config(**kw) -> ModelConfig:

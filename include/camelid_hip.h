@@ -121,6 +121,19 @@ int camelid_hip_prefill(camelid_hip_engine* e, const float* embs, const float* c
 int camelid_hip_verify(camelid_hip_engine* e, const float* embs, const float* cos_all, const float* sin_all,
                        uint32_t base_position, uint32_t k, float scale, uint32_t* tokens_out);
 
+/* verify_batch for sampled generation (no reference counterpart; the accept rule of
+ * camelid_hip_verify_drafts below): the k tokens of embs at positions [base_position, base_position +
+ * k) in one batched forward, as camelid_hip_verify; the token of row t + 1 is draft_tokens[t] (k - 1 of
+ * them), accepted or replaced by sampling at `temperature` (0: the argmax) with uniforms [k] in
+ * [0, 1).  draft_logits (host, [k - 1][vocab]; NULL: each draft was certain): the drafts' own
+ * distributions.  *accepted_out drafts are accepted; tokens_out [k] receives them, the token drawn
+ * behind them, then 0xffffffff; logprobs_out (NULL: not told) [k] their log-probabilities.  k = 1
+ * samples the next token.  filled is not changed: the caller sets it to base_position + 1 + accepted. */
+int camelid_hip_verify_sampled(camelid_hip_engine* e, const float* embs, const float* cos_all, const float* sin_all,
+                               uint32_t base_position, uint32_t k, float scale, const uint32_t* draft_tokens,
+                               const float* draft_logits, float temperature, const float* uniforms,
+                               uint32_t* accepted_out, uint32_t* tokens_out, float* logprobs_out);
+
 /* Device-side token loop (forward_token_device, cuda_resident.rs:7529; embed_gather_q8_0
  * :2995; rope_select :3012).  set_embedding uploads token_embd (Q8_0); set_rope_table
  * uploads cos/sin for positions [0, n_pos).  generate runs n_steps greedy steps starting

@@ -950,3 +950,81 @@ def test_calls_replay_in_a_graph_and_run_on_other_streams(native):
         _hip(native, "hipStreamSynchronize", st)
         _same(b.results(), wants[seed], seed)
         _hip(native, "hipStreamDestroy", st)
+
+
+# ------------------------------------------------------------------------------- the engine's own path
+@pytest.mark.parametrize("prefill", ["batched", "token"])
+def test_verify_sampled_draws_from_the_engine_logits(native, monkeypatch, prefill):
+    """Drafts verified by sampling on the engine: exactly what the definition gives on the logits that
+    single-token steps return (the forward is bit-identical to them)."""
+    from camelid_amd.model import ResidentSession, SyntheticModel, prompt_tokens, rope_tables, tiny_config
+    monkeypatch.setenv("CAMELID_HIP_PREFILL", prefill)
+    cfg = tiny_config(prompt_len=20)
+    model = SyntheticModel.generate(cfg)
+    prompt = prompt_tokens(cfg)
+    rng = np.random.default_rng(51)
+    sess = ResidentSession(model, 40)
+    eng, base = sess.engine, len(prompt) - 1
+    sess.prefill(prompt[:-1])
+    for k in (1, 2, 5, 8):
+        for temp in (0.0, 0.7, 1.3):
+            for with_draft in (False, True):
+                eng.set_filled(base)
+                drafts = [int(t) for t in rng.integers(0, cfg.vocab, k - 1)]
+                rows, step = [], [int(prompt[-1])] + drafts
+                for i in range(k):
+                    greedy = sess.step(step[i], base + i, logits=True)
+                    rows.append(eng.last_logits.astype(np.float64))
+                    if i < k - 1 and rng.random() < 0.6:  # some drafts right
+                        step[i + 1] = int(greedy)
+                drafts = step[1:]
+                target = np.array(rows)[None]
+                dl = (target[:, :k - 1] + rng.normal(0, 0.5, (1, k - 1, cfg.vocab))).astype(np.float32) \
+                    if with_draft and k > 1 else None
+                u = rng.random(k, dtype=np.float32)
+                eng.set_filled(base)
+                cos, sin = rope_tables(cfg, base, k)
+                toks, lps = eng.verify_sampled(model.embed(step), cos, sin, base, cfg.scale(), drafts, u, temp,
+                                               None if dl is None else dl[0])
+                want = verify_reference(target, None if dl is None else dl.astype(np.float64), np.array([drafts], np.int64)
+                                        .reshape(1, k - 1), [k - 1], [temp], u[None])
+                n = int(want[0][0]) + 1
+                assert [int(t) for t in toks] == want[1][0, :n].tolist(), (k, temp, with_draft)
+                assert (np.abs(lps - want[2][0, :n]) <= 2 * U * np.abs(want[2][0, :n]) + 1e-12).all()
+    # the session's sampled generation: greedy at 0 with and without looked-up drafts; runs at 1
+    sess.engine.set_filled(0)
+    greedy = sess.generate(prompt, 12)
+    assert sess.generate_sampled(prompt, 12, 0.0, np.random.default_rng(1)) == greedy
+    text = list(prompt[:8]) * 2 + list(prompt[:3])
+    want = sess.generate(text, 12)
+    assert sess.generate_sampled(text, 12, 0.0, np.random.default_rng(1), max_draft=5) == want
+    assert len(sess.generate_sampled(text, 12, 1.0, np.random.default_rng(2), max_draft=5)) == 12
+    sess.close()
+
+
+def test_verify_sampled_refusals(native):
+    from camelid_amd._native import HipError
+    from camelid_amd.model import ResidentSession, SyntheticModel, prompt_tokens, rope_tables, tiny_config
+    cfg = tiny_config(prompt_len=8)
+    model = SyntheticModel.generate(cfg)
+    sess = ResidentSession(model, 16)
+    prompt = prompt_tokens(cfg)
+    sess.prefill(prompt[:-1])
+    base = len(prompt) - 1
+
+    def call(k=2, drafts=(3,), u=(0.5, 0.5), temp=1.0, pos=base):
+        cos, sin = rope_tables(cfg, pos, k)
+        return sess.engine.verify_sampled(model.embed([1] * k), cos, sin, pos, cfg.scale(), list(drafts), list(u), temp)
+
+    for change, match in ((dict(u=(0.5, 1.0)), "uniforms"), (dict(u=(float("nan"), 0.1)), "uniforms"),
+                          (dict(temp=-1.0), "temperature"), (dict(temp=float("inf")), "temperature"),
+                          (dict(drafts=(cfg.vocab,)), "draft token"), (dict(pos=base + 1), "base_position"),
+                          (dict(k=9, drafts=[1] * 8, u=[0.1] * 9), "k out of")):
+        with pytest.raises(HipError, match=match):
+            call(**change)
+    with pytest.raises(ValueError, match="draft_tokens"):
+        call(drafts=(1, 2))
+    with pytest.raises(ValueError, match="uniforms"):
+        call(u=(0.5,))
+    assert len(call()[0]) in (1, 2)  # nothing above has hurt the engine
+    sess.close()
