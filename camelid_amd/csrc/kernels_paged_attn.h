@@ -60,6 +60,8 @@ struct PaArgs {
   uint32_t at_once;   // pieces that run at the same time
   uint32_t blocks;    // row blocks of a sequence with n_new new tokens
   uint32_t part_rows; // rows of a slot
+  uint32_t group;       // query heads of a KV head
+  uint32_t group_magic; // ceil(2^32 / group), 0 for group = 1: row / group for row * group < 2^32
 };
 
 // 16-bit operand vectors
@@ -125,6 +127,10 @@ __device__ __forceinline__ uint32_t pa_group_max(uint32_t x) {
   return x;
 }
 
+__device__ __forceinline__ uint32_t pa_token(const PaArgs& a, uint32_t row) {
+  return a.group_magic ? __umulhi(row, a.group_magic) : row;
+}
+
 // ---- the plan
 struct PaSeq {
   uint32_t len, first, rows, tiles, blocks;  // blocks: row blocks of the sequence
@@ -137,7 +143,7 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, uint32_t s, bool flag) 
   if (!ok && flag) paged_flag(a.g, PG_BAD_LENGTH);
   q.len = L;
   q.first = L - m;
-  q.rows = ok ? m * (a.n_heads / a.g.n_kv) : 0u;
+  q.rows = ok ? m * a.group : 0u;
   q.tiles = q.rows ? (L + PA_TILE - 1) / PA_TILE : 0u;
   q.blocks = (q.rows + 16 * NR - 1) / (16 * NR);
   return q;
@@ -199,7 +205,7 @@ __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, boo
   p.q = q;
   p.n = count(q);
   const uint32_t at = index - before, seg = at / p.n, piece = at - seg * p.n;
-  p.h = seg / q.blocks;
+  p.h = q.blocks == 1 ? seg : seg / q.blocks;
   p.rb = seg - p.h * q.blocks;
   const uint32_t even = q.tiles / p.n, more = q.tiles - even * p.n;  // the first `more` pieces take one tile more
   p.t0 = piece * even + min(piece, more);
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
   const uint32_t tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t col = lane & 15u, grp = lane >> 4;
   const Paged& g = a.g;
-  const uint32_t group = a.n_heads / g.n_kv, cap = g.stride << g.shift;
+  const uint32_t group = a.group, cap = g.stride << g.shift;
 
   const PaPiece pc = pa_piece<NR>(a, blockIdx.x, blockIdx.x == 0);
   if (!pc.any) return;
@@ -297,7 +303,7 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
 #pragma unroll
     for (int k = 0; k < PASSES; ++k) {
       const uint32_t u = tid + k * PA_NT, row = rb * ROWS + u / LPR;
-      const uint32_t t = row / group, qh = h * group + (row - t * group);
+      const uint32_t t = pa_token(a, row), qh = h * group + (row - t * group);
       raw[k] = q8v{};
       if (u < UNITS && row < sq.rows)
         raw[k] = *reinterpret_cast<const q8v*>(static_cast<const QE*>(a.q) + ((size_t)s * a.n_new + t) * a.q_stride +
@@ -351,7 +357,7 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
     for (int r = 0; r < NR; ++r) {
       const uint32_t row = rb * ROWS + r * 16 + col;
       c[r] = s_c[r * 16 + col];
-      limit[r] = first + (row < sq.rows ? row / group : 0u);
+      limit[r] = first + (row < sq.rows ? pa_token(a, row) : 0u);
     }
     if (ta < t1) {
       for (uint32_t t = ta; t < t1; t += 4) {
@@ -541,7 +547,8 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
       if (whole) {
         // no position left (bad pages): zeros
         const f32x4 z = M == -INFINITY ? f32x4{0, 0, 0, 0} : y / L;
-        const size_t dst = ((size_t)s * a.n_new + full / group) * a.out_stride + (size_t)(h * group + full % group) * HD + d;
+        const uint32_t t = pa_token(a, full);
+        const size_t dst = ((size_t)s * a.n_new + t) * a.out_stride + (size_t)(h * group + (full - t * group)) * HD + d;
         if constexpr (QT == TY_F32) {
           *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + dst) = z;
         } else {
@@ -568,26 +575,28 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
   }
 }
 
-// Joins the cut segments: workgroup (sequence, KV head, row) for rows below `n_rows`; then, where
-// weights are kept, workgroup (sequence, KV head, 256 positions).
-constexpr uint32_t PJ_SPAN = 256, PJ_ROWS = 64;
-template <int HD, int QT, int NR>
-__global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, uint32_t spans) {
-  constexpr int ROWS = 16 * NR, PARTS = PA_NT / (HD / 4);
+// Joins the cut segments: workgroups of PER rows of a (sequence, KV head), a row's parts dealt out to
+// PARTS / PER groups of HD / 4 lanes; then, where weights are kept, workgroups of 256 positions.
+constexpr uint32_t PJ_SPAN = 256, PJ_ROWS = 64, PJ_AHEAD = 16;
+constexpr uint32_t pj_parts(uint32_t hd) { return PA_NT / (hd / 4); }
+template <int HD, int QT, int NR, uint32_t PER>
+__global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, uint32_t row_groups,
+                                                   uint32_t spans) {
+  constexpr uint32_t ROWS = 16 * NR, PARTS = pj_parts(HD), STEP = PARTS / PER;
   __shared__ f32x4 s_o[PARTS][HD / 4];
   __shared__ float s_ml[PARTS][2];
   __shared__ float s_stat[PJ_ROWS][2];
   const Paged& g = a.g;
-  const uint32_t tid = threadIdx.x, group = a.n_heads / g.n_kv, n_out = g.n_seqs * g.n_kv * n_rows;
+  const uint32_t tid = threadIdx.x, n_out = g.n_seqs * g.n_kv * row_groups;
   const bool is_out = blockIdx.x < n_out;
-  const uint32_t sh = is_out ? blockIdx.x / n_rows : (blockIdx.x - n_out) / spans, s = sh / g.n_kv, h = sh % g.n_kv;
+  const uint32_t sh = is_out ? blockIdx.x / row_groups : (blockIdx.x - n_out) / spans, s = sh / g.n_kv, h = sh - s * g.n_kv;
   const uint2* cuts = a.cuts + (size_t)sh * a.blocks;
   if (is_out) {
-    const uint32_t row = blockIdx.x - sh * n_rows, rb = row / ROWS, r = row % ROWS;
-    const uint2 cut = cuts[rb];
+    const uint32_t d = tid % (HD / 4), unit = tid / (HD / 4), part = unit / PER;
+    const uint32_t row = (blockIdx.x - sh * row_groups) * PER + unit % PER, rb = row / ROWS, r = row % ROWS;
+    const uint2 cut = row < n_rows ? cuts[rb] : make_uint2(0, 1);
     const PaSeq sq = pa_seq<NR>(a, s, false);
-    if (row >= sq.rows || cut.y == 1) return;  // (finished by its one piece)
-    const uint32_t d = tid % (HD / 4), part = tid / (HD / 4);
+    const bool live = row < sq.rows && cut.y > 1;  // (else finished by its one piece)
     float M = -INFINITY, L = 0.0f;
     f32x4 y = f32x4{0, 0, 0, 0};
     const auto add = [&](float m2, float l2, f32x4 y2) {
@@ -597,22 +606,25 @@ __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, ui
       y = y * f + y2 * f2;
       M = top;
     };
+    if (live) {
 #pragma unroll 4
-    for (uint32_t i = part; i < cut.y; i += PARTS) {
-      const size_t at = (size_t)(cut.x + i) * a.part_rows + r;
-      const float2 ml = *reinterpret_cast<const float2*>(&a.part_ml[at * 2]);
-      add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(&a.part_o[at * HD + 4 * d]));
+      for (uint32_t i = part; i < cut.y; i += STEP) {
+        const size_t at = (size_t)(cut.x + i) * a.part_rows + r;
+        const float2 ml = *reinterpret_cast<const float2*>(&a.part_ml[at * 2]);
+        add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(&a.part_o[at * HD + 4 * d]));
+      }
     }
-    s_o[part][d] = y;
+    s_o[unit][d] = y;
     if (d == 0) {
-      s_ml[part][0] = M;
-      s_ml[part][1] = L;
+      s_ml[unit][0] = M;
+      s_ml[unit][1] = L;
     }
     __syncthreads();
-    if (part == 0) {
-      for (int i = 1; i < PARTS; ++i) add(s_ml[i][0], s_ml[i][1], s_o[i][d]);
+    if (part == 0 && live) {
+      for (uint32_t i = unit + PER; i < PARTS; i += PER) add(s_ml[i][0], s_ml[i][1], s_o[i][d]);
       const f32x4 z = M == -INFINITY ? f32x4{0, 0, 0, 0} : y / L;
-      const size_t dst = ((size_t)s * a.n_new + row / group) * a.out_stride + (size_t)(h * group + row % group) * HD + 4 * d;
+      const uint32_t t = pa_token(a, row);
+      const size_t dst = ((size_t)s * a.n_new + t) * a.out_stride + (size_t)(h * a.group + (row - t * a.group)) * HD + 4 * d;
       if constexpr (QT == TY_F32) {
         *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + dst) = z;
       } else {
@@ -626,16 +638,24 @@ __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, ui
     }
     return;
   }
-  // weights of 256 positions: the scores against each row's maximum and sum
+  // weights of 256 positions: the scores, PJ_AHEAD rows' on their way at a time, against each row's
+  // maximum and sum
   const uint32_t pos = (blockIdx.x - n_out - sh * spans) * PJ_SPAN + tid;
   const PaSeq sq = pa_seq<NR>(a, s, false);
   if (!sq.rows || pos - tid >= sq.len) return;
   const uint32_t cap = g.stride << g.shift;
-  const size_t all = (size_t)a.n_new * group, base = (size_t)sh * all;
+  const size_t all = (size_t)a.n_new * a.group, base = (size_t)sh * all;
+  const uint32_t at_pos = min(pos, sq.len - 1);
   float* wp = a.weights + (size_t)sh * cap;
-  float acc = pos < sq.first ? wp[pos] : 0.0f;
+  float acc = at_pos < sq.first ? wp[at_pos] : 0.0f;
   for (uint32_t r0 = 0; r0 < sq.rows; r0 += PJ_ROWS) {
     const uint32_t n = min(PJ_ROWS, sq.rows - r0);
+    float sc[PJ_AHEAD];
+    const auto fetch = [&](uint32_t k) {
+#pragma unroll
+      for (uint32_t i = 0; i < PJ_AHEAD; ++i) sc[i] = a.scores[(base + min(r0 + k + i, sq.rows - 1)) * cap + at_pos];
+    };
+    fetch(0);
     __syncthreads();
     // a quarter wave per row: 16 lanes over its parts
     for (uint32_t k = tid >> 4; k < n; k += PA_NT / 16) {
@@ -667,10 +687,11 @@ __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, ui
       }
     }
     __syncthreads();
-    if (pos < sq.len) {
-#pragma unroll 4
-      for (uint32_t r = 0; r < n; ++r)
-        acc += __builtin_amdgcn_exp2f(a.scores[(base + r0 + r) * cap + pos] - s_stat[r][0]) * s_stat[r][1];
+    for (uint32_t k = 0; k < n; k += PJ_AHEAD) {
+      if (k) fetch(k);
+#pragma unroll
+      for (uint32_t i = 0; i < PJ_AHEAD; ++i)
+        if (k + i < n) acc += __builtin_amdgcn_exp2f(sc[i] - s_stat[k + i][0]) * s_stat[k + i][1];
     }
   }
   if (pos < sq.len) wp[pos] = acc;

@@ -99,9 +99,18 @@ bool pa_launch(const cm::PaArgs& a, const PaSizes& z, hipStream_t stream) {
   }
   hipLaunchKernelGGL(split, dim3(z.grid), dim3(cm::PA_NT), lds, stream, a);
   if (!z.join) return true;
-  const uint32_t rows = a.n_new * (a.n_heads / a.g.n_kv), sh = a.g.n_seqs * a.g.n_kv;
+  // segments of up to 16 pieces: a row to one group of lanes (16x1100 with 5 drafts: 6.6 us against 7.6
+  // with a workgroup a row); longer ones: a workgroup a row (1x8199: 4.1 us against 6.6)
+  const uint32_t rows = a.n_new * a.group, sh = a.g.n_seqs * a.g.n_kv;
   const uint32_t spans = a.weights ? ((a.g.stride << a.g.shift) + cm::PJ_SPAN - 1) / cm::PJ_SPAN : 0;
-  hipLaunchKernelGGL((cm::k_pa_join<HD, QT, NR>), dim3(sh * (rows + spans)), dim3(cm::PA_NT), 0, stream, a, rows, spans);
+  const auto join = [&](auto per, auto kernel) {
+    const uint32_t row_groups = (rows + per.value - 1) / per.value;
+    hipLaunchKernelGGL(kernel, dim3(sh * (row_groups + spans)), dim3(cm::PA_NT), 0, stream, a, rows, row_groups, spans);
+  };
+  if ((a.g.stride << a.g.shift) <= 16 * 4 * cm::PA_TILE)
+    join(std::integral_constant<uint32_t, cm::pj_parts(HD)>{}, cm::k_pa_join<HD, QT, NR, cm::pj_parts(HD)>);
+  else
+    join(std::integral_constant<uint32_t, 1>{}, cm::k_pa_join<HD, QT, NR, 1>);
   return true;
 }
 
@@ -245,6 +254,8 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   a.out_stride = out_stride;
   a.n_new = n_new;
   a.n_heads = n_heads;
+  a.group = n_heads / n_kv;
+  a.group_magic = a.group == 1 ? 0 : (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
   a.at_once = z.at_once;
   a.blocks = z.blocks;
   a.part_rows = z.part_rows;
