@@ -181,14 +181,22 @@ __device__ __forceinline__ const void* vd_draft(const VdArgs& a, uint32_t s, uin
   return static_cast<const char*>(a.draft) + ((size_t)s * a.n_draft + t) * a.vocab * (LT == TY_F32 ? 4 : 2);
 }
 
+// The logit below which exp((l - m) / T) is under e^-704, and whether vd_exp_near may go by it: m - 704 T has
+// to be an f32 well below m (tiny temperatures) and above the lowest (huge ones).
+__device__ __forceinline__ float vd_low(float m, float temp, bool* near) {
+  const float span = 704.0f * (vd_greedy(temp) ? 1.0f : temp), low = m - span;
+  *near = low > -1e38f && span > fabsf(m) * 0x1p-16f;
+  return low;
+}
+
 // The logits' exponentials of a share, one after the other: by vd_exp_near, and 0 below e^-704 (EXACT;
-// else some e^-704 there: nothing beside the 1 of the maximum), unless the temperature is so high that
-// this bound is beyond f32.
+// else some e^-704 there: nothing beside the 1 of the maximum) where vd_low has it so.
 template <int LT, bool EXACT, typename F>
 __device__ __forceinline__ void vd_each(const VdLogits<LT>& x, float m, float temp, const uint64_t* tab, F take) {
   const double by = vd_by(temp), md = (double)m;
-  const float low = m - 704.0f * (vd_greedy(temp) ? 1.0f : temp);
-  if (low > -1e38f) {
+  bool near;
+  const float low = vd_low(m, temp, &near);
+  if (near) {
 #pragma unroll
     for (int j = 0; j < x.N; ++j)
 #pragma unroll
@@ -278,8 +286,9 @@ __device__ __forceinline__ void vd_load8(const void* row, uint32_t v0, uint32_t 
 // exp((l - m) / T) of 8 logits, as vd_each's.
 __device__ __forceinline__ void vd_exp8(const float (&l)[8], float m, float temp, const uint64_t* tab, double (&y)[8]) {
   const double by = vd_by(temp), md = (double)m;
-  const float low = m - 704.0f * (vd_greedy(temp) ? 1.0f : temp);
-  if (low > -1e38f) {
+  bool near;
+  const float low = vd_low(m, temp, &near);
+  if (near) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const double e = vd_exp_near((double)fmaxf(l[i], low) - md, by, tab);

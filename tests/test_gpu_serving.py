@@ -763,6 +763,25 @@ def test_verify_masked_and_missing_distributions(native):
     assert want[1][1, 0] == NONE and want[1][2, 1] == NONE and want[1][3, 2] == NONE
 
 
+@pytest.mark.parametrize("has_draft", [False, True])
+def test_verify_extreme_temperatures(native, has_draft):
+    """From temperatures so low that only the largest logit is left (and its equals), past the f32 step of
+    the logits, to ones so high that every token that is not masked is as likely as any other."""
+    rng = np.random.default_rng(35)
+    temps = np.array([1e-40, 1e-30, 1e-12, 1e-7, 1e-5, 1e-3, 50.0, 1e6, 1e34, 1e36, 3e38, np.inf], np.float32)
+    n, k, vocab = len(temps), 2, 3000
+    target = rng.normal(0, 4, (n, k + 1, vocab)) + 1000.0 * rng.choice([-1, 0, 1], (n, 1, 1))
+    target[:, :, 5::7] = -np.inf
+    target[:, 1, 100:103] = target[:, 1].max(-1, keepdims=True) + 1.0    # three equal best ones
+    target = value(typed(target, F32), F32)
+    draft = value(typed(target[:, :k] + rng.normal(0, 1, (n, k, vocab)), F32), F32) if has_draft else None
+    tokens = target[:, :k].argmax(-1)
+    u = rng.random((n, k + 1)).astype(np.float32)
+    with np.errstate(all="ignore"):
+        want = verify_reference(target, draft, tokens, [k] * n, temps, u)
+    check_verify(run_verify(native, target, draft, tokens, [k] * n, temps, u, F32), want)
+
+
 def test_verify_frequencies(native):
     """What comes out of one draft and its correction is distributed as the target: 20000 sequences of
     one small vocabulary, each token's count within 6 standard deviations."""
@@ -1028,3 +1047,41 @@ def test_verify_sampled_refusals(native):
         call(u=(0.5,))
     assert len(call()[0]) in (1, 2)  # nothing above has hurt the engine
     sess.close()
+
+
+@pytest.mark.parametrize("nh,n_kv,hd,new", [(32, 8, 128, 5), (16, 4, 256, 2), (64, 2, 64, 8)])
+def test_attention_with_large_workgroups_replays_in_a_graph(native, nh, n_kv, hd, new):
+    """Kernels that need more LDS than 64 KB, captured as their first call and replayed over a cache that
+    grows between the replays, against eager calls."""
+    rng = np.random.default_rng(61)
+    n, ps, cap = 3, 16, 1024
+    pg = Pages(rng, [cap] * n, ps, n_kv, hd, F16, extra_stride=0)
+    pg.upload()
+    q = _dev(rng.normal(0, 1, (n * new, nh * hd)).astype(np.float32))
+    size = native.camelid_hip_paged_attention_workspace(n, new, nh, n_kv, hd, ps, pg.stride, 0)
+    ws, out = _buf(size), _dev(np.zeros((n * new, nh * hd), np.float32))
+
+    def call(stream):
+        _ok(native.camelid_hip_paged_attention(q.ptr, F32, nh * hd, n, new, None, nh, n_kv, hd, pg.dk.ptr, pg.dv.ptr, F16,
+                                               pg.n_pages, ps, pg.dt.ptr, pg.stride, pg.dl.ptr, 0.1, out.ptr, nh * hd,
+                                               None, ws.ptr, size, pg.dstat.ptr, stream))
+
+    stream, graph, run = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    _hip(native, "hipStreamCreate", C.byref(stream))
+    _hip(native, "hipStreamBeginCapture", stream, 1)
+    call(stream)
+    _hip(native, "hipStreamEndCapture", stream, C.byref(graph))
+    _hip(native, "hipGraphInstantiate", C.byref(run), graph, None, None, C.c_size_t(0))
+    for lens in ([new] * n, [8, 300, 33], [cap, 9, 513], [1000, 1001, 1002]):
+        pg.dl.upload(np.array(lens, np.uint32))
+        _ok(native.camelid_hip_synchronize())
+        call(None)
+        want = out.download(np.uint32, n * new * nh * hd)
+        out.upload(np.zeros((n * new, nh * hd), np.float32))
+        _hip(native, "hipGraphLaunch", run, stream)
+        _hip(native, "hipStreamSynchronize", stream)
+        assert (out.download(np.uint32, n * new * nh * hd) == want).all(), lens
+    assert pg.status() == 0
+    _hip(native, "hipGraphExecDestroy", run)
+    _hip(native, "hipGraphDestroy", graph)
+    _hip(native, "hipStreamDestroy", stream)
