@@ -233,14 +233,14 @@ __global__ __launch_bounds__(VD_NT) void k_vd_stats(VdArgs a, uint32_t per) {
   vd_table(tab);
   __syncthreads();
   for (uint32_t share = first; share < end; ++share) {
-    // the maximum passes NaN over; the sum of the logits does not
+    // the maximum passes NaN over; the sum of the logits does not (/ 64, so that it stays finite)
     float m = -INFINITY, any = 0.0f;
 #pragma unroll
     for (int j = 0; j < x.N; ++j)
 #pragma unroll
       for (int e = 0; e < x.V; ++e) {
         m = fmaxf(m, x.at(j, e));
-        any += x.at(j, e);
+        any = fmaf(x.at(j, e), 0x1p-6f, any);
       }
     m = vd_wave_max(m);
     if (__ballot(any != any && m < INFINITY)) m = NAN;
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
       if (!whole && i == x_tok / VD_SHARE && x_tok < a.vocab) return s_x;
       return parts[i].z * vd_exp((double)parts[i].m - (double)P.m, by, sh.tab);
     };
-    for (int round = 0; round < 2; ++round) {  // (nothing left: p itself)
+    for (int again = 0; again < 2; ++again) {  // (nothing left: p itself)
       double sum = 0.0;
       first_sum = i0 < i1 ? share_sum(i0) : 0.0;
       for (uint32_t i = i0; i < i1; ++i) sum += i == i0 ? first_sum : share_sum(i);

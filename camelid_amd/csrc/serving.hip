@@ -25,6 +25,8 @@ int launched(const char* what) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+// A launch holds at most 2^32 - 1 threads.
+bool grid_ok(uint64_t groups, uint32_t threads) { return groups * threads <= 0xffffffffull; }
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Cache geometry; null: the reason why it is refused in *why.
@@ -68,10 +70,10 @@ PaSizes pa_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_k
   // 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
   z.at_once = 256 * cm::pa_per_cu((int)hd, (int)z.nr) * 7 / 8;
   const uint64_t segments = n_seqs * n_kv * z.blocks, most = 2048;
-  z.fits = segments * cap_tiles < (1ull << 31);
   // a segment has at most ceil(its tiles / 4) pieces, all of them together at most 2048 and one each
   const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + 3) / 4));
-  z.grid = (uint32_t)std::min<uint64_t>(pieces, 0x7fffffffu);
+  z.fits = segments * cap_tiles < (1ull << 31) && grid_ok(pieces, cm::PA_NT);
+  z.grid = (uint32_t)pieces;
   z.join = cap_tiles > 4 || weights;
   // cut segments have more tiles than the target: at most 2048 of them, twice as many pieces
   const size_t slots = cap_tiles > 4 ? (size_t)std::min(2 * most, pieces) : 0;
@@ -148,11 +150,11 @@ int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new,
       !aligned4(sin_tab) || !aligned4(q_norm) || !aligned4(k_norm) || !aligned4(new_lens))
     return cm::fail_global(me, "qkv, q_out and the cache must be 16-byte aligned, the rest 4-byte aligned");
   const uint64_t rows = (uint64_t)n_seqs * n_new * (n_heads + n_kv);
-  if (rows > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  if (!grid_ok(rows, 64)) return cm::fail_global(me, "too many rows in one call");
   if (rope_dim == hd) {
     const uint32_t roles = cm::rk_roles(hd, n_heads, n_kv), granules = cm::rk_granules(n_new);
-    const uint64_t grid = (uint64_t)n_seqs * granules * roles;  // (below 2 * rows)
-    if (grid > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+    const uint64_t grid = (uint64_t)n_seqs * granules * roles;
+    if (!grid_ok(grid, cm::RK_NT)) return cm::fail_global(me, "too many rows in one call");
     const auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(cm::RK_NT), 0, (hipStream_t)stream, g, qkv, n_new, new_lens,
                          n_heads, split_half, cos_tab, sin_tab, q_norm, k_norm, eps, q_out, static_cast<uint16_t*>(kc),
@@ -222,7 +224,7 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
     return cm::fail_global(me, "16-bit q rows must have the cache's type");
   if (!std::isfinite(scale)) return cm::fail_global(me, "attention score scale must be finite");
   const uint64_t groups = (uint64_t)n_seqs * n_kv * (n_new * (n_heads / n_kv) + (weights ? 1 + ((uint64_t)table_stride * page_size >> 8) : 0));
-  if (groups > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  if (!grid_ok(groups, cm::PA_NT)) return cm::fail_global(me, "too many rows in one call");
   const uint32_t unit = q_type == TY_F32 ? 4 : 8;
   if (q_stride < (uint64_t)n_heads * hd || out_stride < (uint64_t)n_heads * hd || q_stride % unit || out_stride % unit)
     return cm::fail_global(me, "q_stride and out_stride must hold n_heads * head_dim elements and be whole 16-byte units");
@@ -286,6 +288,8 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
     return cm::fail_global(me, why);
   if (!keep || keep > (1u << 24)) return cm::fail_global(me, "keep must be in 1..=2^24");
   if (recent > keep) return cm::fail_global(me, "recent must be at most keep");
+  const uint64_t movers = (uint64_t)n_seqs * n_kv * (hd / cm::EM_D + hd / 8);
+  if (!grid_ok(movers, cm::EM_NT)) return cm::fail_global(me, "n_seqs * n_kv * head_dim too large for one call");
   if ((uint64_t)n_pages * page_size > 0xffffffffull)
     return cm::fail_global(me, "n_pages * page_size must be below 2^32");
   if (!aligned16(kc) || !aligned16(vc) || !aligned16(workspace) || !aligned4(weights) || !aligned4(lens_out) ||
@@ -307,7 +311,7 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
   const auto select = cap <= 2048 ? cm::k_evict_select<2> : cap <= 8192 ? cm::k_evict_select<8> : cm::k_evict_select<16>;
   hipLaunchKernelGGL(select, dim3(n_seqs * n_kv), dim3(cm::EV_NT), 0, (hipStream_t)stream, g, weights, keep, recent, plan,
                      kept);
-  hipLaunchKernelGGL(cm::k_evict_move, dim3(n_seqs * n_kv * (hd / cm::EM_D + hd / 8)), dim3(cm::EM_NT), 0,
+  hipLaunchKernelGGL(cm::k_evict_move, dim3((uint32_t)movers), dim3(cm::EM_NT), 0,
                      (hipStream_t)stream, g, static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc), keep, plan, lens_out);
   return launched(me);
 }
@@ -357,7 +361,7 @@ int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint
   a.vocab = vocab;
   a.shares = vd_shares(vocab);
   const uint64_t rows = a.draft ? 2 * n_draft + 1 : n_draft + 1, groups = (a.shares + 3) / 4;
-  if (n_seqs * rows * groups > 0x7fffffffull) return cm::fail_global(me, "too many rows in one call");
+  if (!grid_ok(n_seqs * rows * groups, cm::VD_NT)) return cm::fail_global(me, "too many rows in one call");
   // shares of a wave: one while the chip holds all waves at once (about 4096), up to 4
   const uint32_t per = (uint32_t)std::min<uint64_t>(4, std::max<uint64_t>(1, n_seqs * rows * a.shares / 4096));
   const auto go = [&](auto stats, auto rest, auto pick) {

@@ -377,6 +377,8 @@ void camelid_expf_host(const float* x, float* y, size_t n);
  * position lens[s] - new_lens[s] + t.  Rows t >= new_lens[s] are padding: not read, not written.
  * Pointers are device pointers, table, lens and the like included: they may change between the
  * replays of a captured graph.  Buffers of 16-bit elements and activations are 16-byte aligned.
+ * The buffers of a call do not overlap unless its comment says so.  Sizes that one launch cannot hold
+ * (2^32 threads) are refused.
  * Every call is asynchronous on `stream` (of the current device), allocates nothing and waits for
  * nothing; it may be captured.  A workspace belongs to one call at a time: calls (or graphs) that
  * can run at the same time need workspaces of their own; what one holds afterwards has no meaning.
@@ -392,8 +394,8 @@ enum { CAMELID_PAGED_BAD_PAGE = 1, CAMELID_PAGED_BAD_LENGTH = 2 };
  * tokens: qkv [n_seqs * n_new][(n_heads + 2 n_kv) * hd] f32, cos_tab / sin_tab [n_seqs * n_new]
  * [rope_dim / 2] (each row's own position), q_out [n_seqs * n_new][n_heads * hd] of q_type
  * (CAMELID_F32 or the cache's type).  The arithmetic is camelid_hip_rope_kv's, so f32 q rows and an
- * f16 cache hold the same bits.  n_new has no limit but the grid's (prompts); two rows must not
- * share a position of a page. */
+ * f16 cache hold the same bits.  n_new has no limit but the grid's (prompts); no two of a call's rows
+ * may have the same place in the cache. */
 int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new, const uint32_t* new_lens,
                               uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t rope_dim, uint32_t split_half,
                               const float* cos_tab, const float* sin_tab, const float* q_norm, const float* k_norm,
@@ -409,7 +411,9 @@ int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new,
  * softmax weights, summed over the sequence's new tokens and the KV head's query heads, are added to
  * it (a new token's own position starts at 0).  n_heads * n_new row sums are taken in a fixed order:
  * the same call gives the same bits.
- * _workspace: bytes for calls of at most these sizes (with_weights: weights != NULL). */
+ * An infinity or NaN in K or V that a row does see makes that row's outputs infinite or NaN.
+ * _workspace: bytes for calls with this n_heads, n_kv and hd and at most the other sizes (with_weights:
+ * weights != NULL). */
 size_t camelid_hip_paged_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
                                              uint32_t hd, uint32_t page_size, uint32_t table_stride,
                                              uint32_t with_weights);
@@ -425,7 +429,8 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
  * in their order, K, V and weights moved to positions [0, keep); lens_out[s] = min(lens[s], keep)
  * (lens_out may be lens).  kept (NULL: not told) [n_seqs][n_kv][keep]: the positions kept, entries
  * from lens_out[s] on untouched.  Cache positions and weights from keep on keep their bits.  Pages of
- * the evicted sequences must belong to one table entry each. */
+ * the evicted sequences must belong to one table entry each.  _workspace: bytes for calls of at most
+ * these sizes (keep counts, page_size and table_stride do not). */
 size_t camelid_hip_paged_evict_workspace(uint32_t n_seqs, uint32_t n_kv, uint32_t page_size, uint32_t table_stride,
                                          uint32_t keep);
 int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_size, uint32_t n_kv, uint32_t hd,
@@ -446,7 +451,8 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
  * 0xffffffff; logprobs_out (NULL: not told) [n_seqs][n_draft + 1]: the natural log of p of each of
  * these tokens (T = 0: of softmax(target)), then 0.  n_draft = 0 samples one token per sequence;
  * n_draft <= 31.  A draft token >= vocab is rejected.  A row needed whose logits hold NaN or +inf, or
- * nothing above -inf, ends its sequence: its token is 0xffffffff, its log-probability NaN. */
+ * nothing above -inf, ends its sequence: its token is 0xffffffff, its log-probability NaN.
+ * _workspace: bytes for calls of at most these sizes. */
 size_t camelid_hip_verify_drafts_workspace(uint32_t n_seqs, uint32_t n_draft, uint32_t vocab);
 int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint32_t logits_type,
                               const uint32_t* draft_tokens, const uint32_t* draft_lens, uint32_t n_seqs,

@@ -350,6 +350,7 @@ ATT_CASES = [
     (40, 8, 128, [4100], [1], 16, BF16, BF16, False),
     (32, 8, 128, [5003], [1], 4096, F32, F16, False),
     (71, 1, 64, [333, 12], [2, 8], 32, F32, F16, True),
+    (4, 2, 64, [i * 37 % 400 for i in range(150)], [min(i * 37 % 400, i % 4) for i in range(150)], 16, F32, F16, True),
 ]
 
 
@@ -687,7 +688,7 @@ VERIFY_CASES = [
     # seqs, drafts, vocab, draft logits, type
     (1, 4, 32000, False, F32), (5, 3, 1000, True, F32), (7, 0, 4097, False, F16), (3, 7, 151936, True, BF16),
     (2, 1, 1, True, F32), (4, 5, 63, False, BF16), (9, 2, 8191, True, F16), (2, 31, 500, True, F32),
-    (3, 4, 128256, False, F32),
+    (3, 4, 128256, False, F32), (2, 1, 700001, True, F16), (1, 2, 600000, False, BF16),
 ]
 
 
@@ -780,6 +781,22 @@ def test_verify_extreme_temperatures(native, has_draft):
     with np.errstate(all="ignore"):
         want = verify_reference(target, draft, tokens, [k] * n, temps, u)
     check_verify(run_verify(native, target, draft, tokens, [k] * n, temps, u, F32), want)
+
+
+def test_verify_logits_near_the_largest(native):
+    """Sums of a row's logits are beyond f32 (and beside -inf nearly NaN); every row has a distribution."""
+    rng = np.random.default_rng(36)
+    n, k, vocab = 4, 1, 5000
+    target = np.full((n, k + 1, vocab), -np.inf)
+    target[:, :, :600] = 3e38
+    target[1:, :, 300:900] = rng.uniform(1e38, 3.4e38, (n - 1, k + 1, 600))
+    target[2, :, 1000:] = -3.4e38
+    target = value(typed(target, F32), F32)
+    temps = np.array([1.0, 3e37, 1e38, 0.0], np.float32)
+    u = rng.random((n, k + 1)).astype(np.float32)
+    tokens = target[:, :k].argmax(-1)
+    want = verify_reference(target, None, tokens, [k] * n, temps, u)
+    check_verify(run_verify(native, target, None, tokens, [k] * n, temps, u, F32), want)
 
 
 def test_verify_frequencies(native):
@@ -1085,3 +1102,100 @@ def test_attention_with_large_workgroups_replays_in_a_graph(native, nh, n_kv, hd
     _hip(native, "hipGraphExecDestroy", run)
     _hip(native, "hipGraphDestroy", graph)
     _hip(native, "hipStreamDestroy", stream)
+
+
+def test_a_cache_past_two_to_the_32_elements(native):
+    """The same calls over a small pool and over the far end of one whose offsets pass 32 bits (in elements
+    and in bytes): the same bits everywhere."""
+    rng = np.random.default_rng(62)
+    n, n_kv, nh, hd, ps, new = 2, 8, 16, 128, 4096, 100
+    page = n_kv * hd * ps
+    far = (1 << 32) // page + 1
+    table = np.array([[3, 0], [1, 2]], np.uint32)
+    prompts = rng.normal(0, 1, (n * new, (nh + 2 * n_kv) * hd)).astype(np.float32)
+    angle = rng.uniform(0, 7, (n * new, hd // 2))
+    dq, dc, dn = _dev(prompts), _dev(np.cos(angle).astype(np.float32)), _dev(np.sin(angle).astype(np.float32))
+    drafts = _dev(rng.normal(0, 1, (n * 2, nh * hd)).astype(np.float32))
+    results = []
+    for offset in (0, far):
+        pages = offset + 4
+        kc, vc = _buf(pages * page * 2), _buf(pages * page * 2)
+        dt, dl, stat = _dev(table + np.uint32(offset)), _dev(np.full(n, new, np.uint32)), _dev(np.zeros(1, np.uint32))
+        q_out, out = _buf(n * new * nh * hd * 4), _dev(np.zeros((n * 2, nh * hd), np.float32))
+        weights = _dev(np.zeros((n, n_kv, 2 * ps), np.float32))
+        # a prompt over the end of each first page, in three calls; half of them by the path for part of a head
+        at = ps - 130
+        for rope_dim in (hd, hd - 32, hd):
+            at += new
+            dl.upload(np.full(n, at, np.uint32))
+            _ok(native.camelid_hip_paged_rope_kv(dq.ptr, n, new, None, nh, n_kv, hd, rope_dim, 1, dc.ptr, dn.ptr, None, None,
+                                                 1e-5, q_out.ptr, F32, kc.ptr, vc.ptr, F16, pages, ps, dt.ptr, 2, dl.ptr,
+                                                 stat.ptr, None))
+            _ok(native.camelid_hip_synchronize())
+        # the positions before them: none; their pages hold whatever the allocation held, so only the newest
+        # tokens' own pages count: a second table whose sequences begin at the second page
+        dt2 = _dev((table[:, 1:] + np.uint32(offset)).astype(np.uint32))
+        held = at - ps
+        dl.upload(np.full(n, held, np.uint32))
+        size = native.camelid_hip_paged_attention_workspace(n, 2, nh, n_kv, hd, ps, 1, 1)
+        ws = _buf(size)
+        evict = native.camelid_hip_paged_evict_workspace(n, n_kv, ps, 1, 64)
+        ws2, kept = _buf(evict), _dev(np.zeros((n, n_kv, 64), np.uint32))
+        got = []
+        for turn in range(2):
+            _ok(native.camelid_hip_paged_attention(drafts.ptr, F32, nh * hd, n, 2, None, nh, n_kv, hd, kc.ptr, vc.ptr, F16,
+                                                   pages, ps, dt2.ptr, 1, dl.ptr, 0.09, out.ptr, nh * hd, weights.ptr,
+                                                   ws.ptr, size, stat.ptr, None))
+            got.append(out.download(np.uint32, n * 2 * nh * hd))
+            if turn == 0:
+                _ok(native.camelid_hip_paged_evict(kc.ptr, vc.ptr, pages, ps, n_kv, hd, dt2.ptr, 1, dl.ptr, n, weights.ptr,
+                                                   64, 16, dl.ptr, kept.ptr, ws2.ptr, evict, stat.ptr, None))
+                _ok(native.camelid_hip_synchronize())
+                assert dl.download(np.uint32, n).tolist() == [64, 64]
+                got.append(kept.download(np.uint32, n * n_kv * 64))
+        assert stat.download(np.uint32, 1)[0] == 0
+        assert np.isfinite(got[0].view(np.float32)).all() and got[0].view(np.float32).std() > 0.01
+        results.append(got)
+        for b in (kc, vc):
+            b.free()
+    for near, off in zip(*results):
+        assert (near == off).all()
+
+
+def test_attention_on_two_streams_at_once(native):
+    """Two batches in flight on two streams, each with a workspace of its own, as one after the other."""
+    rng = np.random.default_rng(63)
+    jobs = []
+    for nh, n_kv, lens, new in ((32, 8, [1500] * 12, 5), (32, 2, [6000, 1, 40], 1)):
+        pg = Pages(rng, lens, 32, n_kv, 128, F16)
+        pg.upload()
+        n = len(lens)
+        size = native.camelid_hip_paged_attention_workspace(n, new, nh, n_kv, 128, 32, pg.stride, 0)
+        q = _dev(rng.normal(0, 1, (n * new, nh * 128)).astype(np.float32))
+        pg.dl.upload(np.maximum(pg.lens, new).astype(np.uint32))
+        stream = C.c_void_p()
+        _hip(native, "hipStreamCreate", C.byref(stream))
+        jobs.append((pg, q, n, new, nh, n_kv, _buf(size), size, _buf(n * new * nh * 128 * 4), stream))
+
+    def call(job, stream):
+        pg, q, n, new, nh, n_kv, ws, size, out, _ = job
+        _ok(native.camelid_hip_paged_attention(q.ptr, F32, nh * 128, n, new, None, nh, n_kv, 128, pg.dk.ptr, pg.dv.ptr, F16,
+                                               pg.n_pages, 32, pg.dt.ptr, pg.stride, pg.dl.ptr, 0.1, out.ptr, nh * 128,
+                                               None, ws.ptr, size, pg.dstat.ptr, stream))
+
+    def read(job):
+        return job[8].download(np.uint32, job[2] * job[3] * job[4] * 128)
+
+    want = []
+    for job in jobs:
+        call(job, None)
+        _ok(native.camelid_hip_synchronize())
+        want.append(read(job))
+    for _ in range(8):
+        for job in jobs:
+            call(job, job[9])
+    for job, w in zip(jobs, want):
+        _hip(native, "hipStreamSynchronize", job[9])
+        assert (read(job) == w).all()
+    for job in jobs:
+        _hip(native, "hipStreamDestroy", job[9])

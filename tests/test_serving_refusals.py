@@ -32,7 +32,8 @@ GEOMETRY = [(dict(hd=96), "head_dim"), (dict(n_kv=0), "n_kv"), (dict(page_size=2
     (dict(n_heads=7), "multiple of n_kv"), (dict(n_heads=0), "multiple of n_kv"), (dict(rope_dim=66), "rope_dim"),
     (dict(rope_dim=63), "rope_dim"), (dict(cos=None), "null"), (dict(qkv=None), "null"), (dict(q_type=3), "type"),
     (dict(kv_type=0), "type"), (dict(q_type=2), "cache's type"), (dict(qkv=P + 4), "aligned"),
-    (dict(q_out=P + 8), "aligned"), (dict(n_new=1 << 30), "too many rows")])
+    (dict(q_out=P + 8), "aligned"), (dict(n_new=1 << 30), "too many rows"),
+    (dict(n_new=1 << 23), "too many rows"), (dict(n_new=1 << 23, rope_dim=32), "too many rows")])
 def test_rope_kv_refuses(native, change, match):
     from camelid_amd._native import HipError
     with pytest.raises(HipError, match="paged_rope_kv: .*" + match):
@@ -44,7 +45,9 @@ def test_rope_kv_refuses(native, change, match):
     (dict(kv_type=0), "type"), (dict(q_type=2), "cache's type"), (dict(scale=float("nan")), "finite"),
     (dict(scale=float("inf")), "finite"), (dict(q_stride=508), "q_stride"), (dict(out_stride=514), "q_stride"),
     (dict(q=P + 4), "aligned"), (dict(ws=None), "null"), (dict(ws=P + 4), "aligned"), (dict(out=None), "null"),
-    (dict(ws_bytes=0), "workspace too small"), (dict(weights=P + 1), "aligned")])
+    (dict(ws_bytes=0), "workspace too small"), (dict(weights=P + 1), "aligned"),
+    (dict(n_seqs=1 << 19, n_new=8), "too many rows"), (dict(n_seqs=1 << 18, stride=1 << 19, weights=P), "too many rows"),
+    (dict(n_seqs=1 << 18, stride=1 << 20, ws_bytes=1 << 60), "too large for one call")])
 def test_attention_refuses(native, change, match):
     from camelid_amd._native import HipError
     with pytest.raises(HipError, match="paged_attention: .*" + match):
@@ -53,7 +56,8 @@ def test_attention_refuses(native, change, match):
 
 @pytest.mark.parametrize("change,match", GEOMETRY + [
     (dict(keep=0), "keep"), (dict(recent=17), "recent"), (dict(weights=None), "null"), (dict(lens_out=None), "null"),
-    (dict(ws_bytes=0), "workspace too small"), (dict(ws=P + 4), "aligned"), (dict(kept=P + 2), "aligned")])
+    (dict(ws_bytes=0), "workspace too small"), (dict(ws=P + 4), "aligned"), (dict(kept=P + 2), "aligned"),
+    (dict(n_seqs=1 << 19, ws_bytes=1 << 60), "too large for one call")])
 def test_evict_refuses(native, change, match):
     from camelid_amd._native import HipError
     with pytest.raises(HipError, match="paged_evict: .*" + match):
