@@ -90,7 +90,8 @@ __device__ __forceinline__ void store_from_f32(void* p, size_t i, float v) {
 // Per-head RMSNorm (optional) + RoPE of the new tokens' q and k rows, K and V into the pages.
 //   norm: x_d = (x_d * (1 / sqrt(sum x^2 / hd + eps))) * w_d, the sum over d in order
 //   pair: (a, b) -> (a c - b s, a s + b c), each product and sum rounded in f32
-// the arithmetic of k_rope_kv, so an f16 cache holds the same bits.  One wave per (row, head).
+// the arithmetic of k_rope_kv, so an f16 cache holds the same bits.  One wave per (row, head), for
+// rope_dim < head_dim: pairs fall anywhere in the head.
 template <int QT, int KT>
 __global__ __launch_bounds__(64) void k_paged_rope_kv(Paged g, const float* __restrict__ qkv, uint32_t n_new,
                                                       const uint32_t* __restrict__ new_lens, uint32_t n_heads,
@@ -160,8 +161,9 @@ __global__ __launch_bounds__(64) void k_paged_rope_kv(Paged g, const float* __re
 //   q, K: HD / 16 lanes per (token, head), each 8 dims of either half, which hold the pairs of both
 //         pairings; the norm's sum in order by one lane per (token, head) from LDS.
 //   V:    a lane per dim.
-// Bound: HBM.  207 MB (4 prompts of up to 2047 tokens, 24 + 8 + 8 heads of 128): 115 us with one wave per
-// (token, head) and 2-byte stores.
+// Bound: HBM.  207 MB (4 prompts of up to 2047 tokens, 24 + 8 + 8 heads of 128): 37 us, 5.6 TB/s (84 us
+// with one wave per (token, head) and 2-byte stores); launch and latency for decode steps: 3 us for one
+// token of 32 + 4 + 4 heads of 64, 6 us for 24 sequences of up to 5 tokens of 32 + 8 + 8 heads of 128.
 constexpr uint32_t RK_NT = 256;
 constexpr uint32_t rk_heads(uint32_t hd) { return RK_NT / (hd / 16) / 8; }  // q or K heads of a workgroup
 constexpr uint32_t rk_v_heads(uint32_t hd) { return RK_NT / hd; }
@@ -378,14 +380,14 @@ struct EvictPlan {
 // One workgroup per (sequence, KV head): the plan, `kept` (the positions themselves), the weights
 // compacted.
 //
-// The smallest kept weight by its digits from the top, 11, 11 and 10 bits: a histogram (8 bits less of it
-// had the weights crowd in a few counters: 5.2 us for the first of 16383 weights) in two copies and a
-// suffix sum of its counts.  A thread holds K weights in
-// registers, runs of V at a time, so up to K * 1024 positions are read once; longer rows go through
-// the same code in pieces that are read again.  Then prefix sums of two counts in a word (weights
-// above the smallest, weights equal to it) give every kept position its place.
-// Bound: latency; 16 x 8 rows of 1088 weights 43 -> 11 us against LDS atomics on one histogram searched
-// by one thread.
+// The smallest kept weight by its digits from the top, 11, 11 and 10 bits: for each a histogram in two
+// copies and a suffix sum of its counts (digits of 8 bits had the weights crowd in few bins:
+// 5.2 us for the first digit of 16383).  A thread holds K weights in registers, runs of V
+// at a time, so up to K * 1024 positions are read once; longer rows go through the same code in pieces that
+// are read again.  Then prefix sums of two counts in a word (weights above the smallest, weights equal
+// to it) give every kept position its place.
+// Bound: latency (barriers between the digits): 16 x 8 rows of 1088 weights 7.6 us (43 with 8-bit digits in
+// one histogram searched by one thread), 4 x 8 rows of up to 16383 weights 16.6 us.
 template <int K>
 __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restrict__ weights, uint32_t keep,
                                                         uint32_t recent, EvictPlan plan, uint32_t* __restrict__ kept) {
@@ -569,7 +571,9 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
 
 // The move, in place: output positions in chunks, a chunk's sources read before any of it is
 // written.  A source is never below its output position, so no later chunk misses a row.  Bound:
-// HBM; rows far apart share their 128-byte lines with rows that are left behind.
+// HBM: 16 x 8 x 1024 of 1088 rows of 128 dims, 134 MB, 24 us, 5.6 TB/s; 4 x 8 x 2048 of up to 16383
+// rows 19 us, where rows far apart share their 128-byte lines with rows that are left behind (about 160
+// MB of lines for 67 MB).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // K: one workgroup per (sequence, KV head, 8 dims), whole granules, chunks of R * EM_NT rows in registers.

@@ -12,10 +12,13 @@
 // lies, and f32 sums would move the borders by more than their distances.
 //
 // Bound: every row's logits read once (k_vd_stats: a wave per 2048 of them, its maximum and its sum of
-// exponentials; no barriers behind the loads), where 12 f64 operations a logit take about 0.6 of the
-// time that f32 logits take to arrive from HBM.  Only sequences that rejected a draft of a draft
-// model read two rows again for max(p - q, 0) (k_vd_rest, spread over the chip like the first pass);
-// otherwise the shares' sums are known.  k_vd_pick then needs one share's logits.
+// exponentials; no barriers behind the loads).  139 MB of f32 logits (32 sequences with up to 5 drafts of a
+// draft model, 151936 tokens) take 31 us, 4.4 TB/s; 15 instructions a logit, 9 of them f64, are about half
+// of that.  Only sequences that rejected a draft of a draft model read two rows again for max(p - q, 0)
+// (k_vd_rest, spread over the chip like the first pass: 15 us there); otherwise the shares' sums are known.
+// k_vd_pick then needs one share's logits: latency (9 us there, 7 us for one sequence without a draft model).
+// Rest and pick as one launch, the draw by the sequence's last workgroup, took 47 us: its fences write back
+// and invalidate the L2.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <type_traits>
@@ -36,18 +39,17 @@ struct VdPart {
 };
 
 // ---- exp(y / T) for y <= 0, by = 32 log2(e) / T: y by = k + r, |r| <= 1/2; 2^(k / 32) from a table in
-// LDS, e^(r ln 2 / 32) by its series to the fifth power (the next term is below 2.3e-15).  32 entries of 8
-// bytes: every one in banks of its own, lanes that read the same one share it.
+// LDS, e^(r ln 2 / 32) as 1 + r times the cubic that meets (e^(r ln 2 / 32) - 1) / r in the four Chebyshev
+// points of [-1/2, 1/2]: relative error below 1.6e-13.  32 entries of 8 bytes: every one in banks of its
+// own, lanes that read the same one share it.
 // (kExp2Tab: the bits of 2^(i / 32) less i << 47, so that adding k << 47 makes 2^(k / 32).)
 __device__ __forceinline__ void vd_table(uint64_t* tab) {
   if (threadIdx.x < 32) tab[threadIdx.x] = kExp2Tab[threadIdx.x];
 }
 __device__ __forceinline__ double vd_series(double r) {
-  constexpr double A = 0x1.62e42fefa39efp-1 / 32.0;  // ln 2 / 32
-  double p = fma(r, A * A * A * A * A / 120.0, A * A * A * A / 24.0);
-  p = fma(r, p, A * A * A / 6.0);
-  p = fma(r, p, A * A / 2.0);
-  p = fma(r, p, A);
+  double p = fma(r, 0x1.3b2b07bdf576cp-27, 0x1.c6b13c3469da5p-20);
+  p = fma(r, p, 0x1.ebfbdff82240ap-13);
+  p = fma(r, p, 0x1.62e42fef8dc67p-6);
   return fma(r, p, 1.0);
 }
 // Any y <= 0, -inf included; 0 below the exponent range.
@@ -58,17 +60,6 @@ __device__ __forceinline__ double vd_exp(double y, double by, const uint64_t* ta
   // 2^(n % 32 / 32) from the table, the rest of n by ldexp (which rounds into the subnormals)
   return ldexp(vd_series(r) * u2d(tab[n & 31] + ((uint64_t)(n & 31) << 47)), n >> 5);
 }
-// y / T >= -704, so that 2^(k / 32) has a normal exponent: no conversions, the exponent added as bits.
-__device__ __forceinline__ double vd_exp_near(double y, double by, const uint64_t* tab) {
-  const double kd = fma(y, by, 0x1.8p52);  // k in the low bits
-  const uint32_t n = (uint32_t)d2u(kd);
-  const double r = fma(y, by, 0x1.8p52 - kd);
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-  u32x2 t = __builtin_bit_cast(u32x2, tab[n & 31u]);  // + n << 47
-  t.y += n << 15;
-  return vd_series(r) * __builtin_bit_cast(double, t);
-}
-
 __device__ __forceinline__ bool vd_greedy(float t) { return !(t > 0.0f); }
 // 32 log2(e) / T; a greedy sequence's log-probabilities are those of T = 1
 __device__ __forceinline__ double vd_by(float t) {
@@ -181,35 +172,57 @@ __device__ __forceinline__ const void* vd_draft(const VdArgs& a, uint32_t s, uin
   return static_cast<const char*>(a.draft) + ((size_t)s * a.n_draft + t) * a.vocab * (LT == TY_F32 ? 4 : 2);
 }
 
-// The logit below which exp((l - m) / T) is under e^-704, and whether vd_exp_near may go by it: m - 704 T has
-// to be an f32 well below m (tiny temperatures) and above the lowest (huge ones).
-__device__ __forceinline__ float vd_low(float m, float temp, bool* near) {
-  const float span = 704.0f * (vd_greedy(temp) ? 1.0f : temp), low = m - span;
-  *near = low > -1e38f && span > fabsf(m) * 0x1p-16f;
-  return low;
+// What a row's exponentials exp((l - m) / T) are taken against.  near: down to `low` = m - 704 T, an f32 well
+// below m (not at tiny temperatures) and above the lowest (not at huge ones), 2^(k / 32) has a normal exponent,
+// which is added as bits, and l by needs no subtraction: with m by = K + f, K whole, exp((l - m) / T) is
+// 2^(-f / 32) (`factor`, once a sum) times 2^((l by - K) / 32).
+struct VdRef {
+  double by, md, shift, factor;
+  float low;
+  bool near;
+};
+__device__ __forceinline__ VdRef vd_ref(float m, float temp) {
+  VdRef f;
+  f.by = vd_by(temp);
+  f.md = (double)m;
+  const float span = 704.0f * (vd_greedy(temp) ? 1.0f : temp);
+  f.low = m - span;
+  f.near = f.low > -1e38f && span > fabsf(m) * 0x1p-16f;
+  const double whole = f.near ? rint(f.md * f.by) : 0.0;
+  f.shift = 0x1.8p52 - whole;
+  f.factor = f.near ? vd_series(-fma(f.md, f.by, -whole)) : 1.0;
+  return f;
+}
+// l >= low; the exponential is *a * *b * factor.
+__device__ __forceinline__ void vd_exp_near(float l, const VdRef& f, const uint64_t* tab, double* a, double* b) {
+  const double x = (double)l, kd = fma(x, f.by, f.shift);  // k in the low bits
+  const uint32_t n = (uint32_t)d2u(kd);
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  u32x2 t = __builtin_bit_cast(u32x2, tab[n & 31u]);  // + n << 47
+  t.y += n << 15;
+  *a = vd_series(fma(x, f.by, f.shift - kd));
+  *b = __builtin_bit_cast(double, t);
 }
 
-// The logits' exponentials of a share, one after the other: by vd_exp_near, and 0 below e^-704 (EXACT;
-// else some e^-704 there: nothing beside the 1 of the maximum) where vd_low has it so.
+// The logits' exponentials of a share, one after the other, as two terms of a product that f.factor belongs
+// to: 0 below e^-704 (EXACT; else some e^-704 there: nothing beside the 1 of the maximum) where f.near.
 template <int LT, bool EXACT, typename F>
-__device__ __forceinline__ void vd_each(const VdLogits<LT>& x, float m, float temp, const uint64_t* tab, F take) {
-  const double by = vd_by(temp), md = (double)m;
-  bool near;
-  const float low = vd_low(m, temp, &near);
-  if (near) {
+__device__ __forceinline__ void vd_each(const VdLogits<LT>& x, const VdRef& f, const uint64_t* tab, F take) {
+  if (f.near) {
 #pragma unroll
     for (int j = 0; j < x.N; ++j)
 #pragma unroll
       for (int e = 0; e < x.V; ++e) {
         const float l = x.at(j, e);
-        const double y = vd_exp_near((double)fmaxf(l, low) - md, by, tab);
-        take(j, e, !EXACT || l > low ? y : 0.0);
+        double a, b;
+        vd_exp_near(fmaxf(l, f.low), f, tab, &a, &b);
+        take(j, e, !EXACT || l > f.low ? a : 0.0, b);
       }
   } else {
 #pragma unroll
     for (int j = 0; j < x.N; ++j)
 #pragma unroll
-      for (int e = 0; e < x.V; ++e) take(j, e, vd_exp((double)x.at(j, e) - md, by, tab));
+      for (int e = 0; e < x.V; ++e) take(j, e, vd_exp((double)x.at(j, e) - f.md, f.by, tab), 1.0);
   }
 }
 
@@ -233,17 +246,12 @@ __global__ __launch_bounds__(VD_NT) void k_vd_stats(VdArgs a, uint32_t per) {
   vd_table(tab);
   __syncthreads();
   for (uint32_t share = first; share < end; ++share) {
-    // the maximum passes NaN over; the sum of the logits does not (/ 64, so that it stays finite)
-    float m = -INFINITY, any = 0.0f;
+    float m = -INFINITY;  // or NaN, where there is one
 #pragma unroll
     for (int j = 0; j < x.N; ++j)
 #pragma unroll
-      for (int e = 0; e < x.V; ++e) {
-        m = fmaxf(m, x.at(j, e));
-        any = fmaf(x.at(j, e), 0x1p-6f, any);
-      }
-    m = vd_wave_max(m);
-    if (__ballot(any != any && m < INFINITY)) m = NAN;
+      for (int e = 0; e < x.V; ++e) m = __builtin_elementwise_maximum(m, x.at(j, e));
+    m = __ballot(m != m) ? NAN : vd_wave_max(m);
     uint32_t at = 0xffffffffu;
     double z = 0.0;
     if (greedy) {  // nobody else asks for the index
@@ -255,8 +263,9 @@ __global__ __launch_bounds__(VD_NT) void k_vd_stats(VdArgs a, uint32_t per) {
       for (int o = 32; o; o >>= 1) at = min(at, (uint32_t)__shfl_xor(at, o));
     }
     if (!vd_bad(m) && (!greedy || a.logprobs)) {
-      vd_each<LT, false>(x, m, temp, tab, [&](int, int, double e) { z += e; });
-      z = vd_wave_sum(z);
+      const VdRef f = vd_ref(m, temp);
+      vd_each<LT, false>(x, f, tab, [&](int, int, double p, double q) { z = fma(p, q, z); });
+      z = vd_wave_sum(z) * f.factor;
     }
     if ((threadIdx.x & 63u) == 63) a.parts[(size_t)row * a.shares + share] = VdPart{z, m, at};
     if (share + 1 < end) x.load(src, (share + 1) * VD_SHARE, a.vocab);
@@ -285,18 +294,17 @@ __device__ __forceinline__ void vd_load8(const void* row, uint32_t v0, uint32_t 
 }
 // exp((l - m) / T) of 8 logits, as vd_each's.
 __device__ __forceinline__ void vd_exp8(const float (&l)[8], float m, float temp, const uint64_t* tab, double (&y)[8]) {
-  const double by = vd_by(temp), md = (double)m;
-  bool near;
-  const float low = vd_low(m, temp, &near);
-  if (near) {
+  const VdRef f = vd_ref(m, temp);
+  if (f.near) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const double e = vd_exp_near((double)fmaxf(l[i], low) - md, by, tab);
-      y[i] = l[i] > low ? e : 0.0;
+      double a, b;
+      vd_exp_near(fmaxf(l[i], f.low), f, tab, &a, &b);
+      y[i] = l[i] > f.low ? a * b * f.factor : 0.0;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = vd_exp((double)l[i] - md, by, tab);
+    for (int i = 0; i < 8; ++i) y[i] = vd_exp((double)l[i] - f.md, f.by, tab);
   }
 }
 
@@ -411,11 +419,12 @@ __global__ __launch_bounds__(VD_NT) void k_vd_rest(VdArgs a) {
   x.load(vd_target<LT>(a, s, took), share * VD_SHARE, a.vocab);
   y.load(vd_draft<LT>(a, s, took), share * VD_SHARE, a.vocab);
   const VdPart P = sh.row[took], Q = sh.row[a.n_draft + 1 + took];
-  const double ip = 1.0 / P.z, iq = 1.0 / Q.z;
   const float temp = a.temperature[s];
+  const VdRef fp = vd_ref(P.m, temp), fq = vd_ref(Q.m, temp);
+  const double ip = fp.factor / P.z, iq = fq.factor / Q.z;
   double p[32], sum = 0.0;
-  vd_each<LT, true>(x, P.m, temp, sh.tab, [&](int j, int e, double v) { p[j * x.V + e] = v * ip; });
-  vd_each<LT, true>(y, Q.m, temp, sh.tab, [&](int j, int e, double v) { sum += fmax(p[j * x.V + e] - v * iq, 0.0); });
+  vd_each<LT, true>(x, fp, sh.tab, [&](int j, int e, double u, double v) { p[j * x.V + e] = u * v * ip; });
+  vd_each<LT, true>(y, fq, sh.tab, [&](int j, int e, double u, double v) { sum += fmax(p[j * x.V + e] - u * v * iq, 0.0); });
   sum = vd_wave_sum(sum);
   if ((threadIdx.x & 63u) == 63) a.rest[(size_t)s * a.shares + share] = sum;
 }
