@@ -3,7 +3,12 @@
 //   s_p = scale (q . k_p) for p <= the row's position;  w = softmax(s);  o = sum_p w_p v_p
 //
 // Bound: the cache's bytes (4 hd per position and KV head, against 4 hd flop per position and row),
-// so the kernel's work is to keep HBM busy whatever the batch looks like.
+// so the kernel's work is to keep HBM busy whatever the batch looks like.  Heads of 128:
+//   4 sequences of 65536, 32 + 8 heads: 166 + 5 us (split + join), 6.3 TB/s
+//   64 of up to 4001, 24 + 8 heads: 90 + 5 us, 5.7 TB/s
+//   1 of 8199, 32 + 8 heads: 9.6 + 4.4 us for 34 MB: latency (launch 1, plan 1.2, pages 0.6, K and V and
+//     the query operands 2, products and softmax 1.4, states joined and written 1.3, then the join's launch)
+//   16 of up to 1100, up to 5 new tokens, weights kept: 17.4 + 6.4 us for 39 MB: the same, two tiles a wave
 //
 // Split.  A segment is (sequence, KV head, block of 16 NR query rows); its tiles are 32 positions.
 // The query rows are the new tokens times the KV head's query heads, so K and V are read once for
@@ -576,7 +581,9 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
 }
 
 // Joins the cut segments: workgroups of PER rows of a (sequence, KV head), a row's parts dealt out to
-// PARTS / PER groups of HD / 4 lanes; then, where weights are kept, workgroups of 256 positions.
+// PARTS / PER groups of HD / 4 lanes; then, where weights are kept, workgroups of 256 positions.  Bound:
+// latency (4.4 us for 8 segments of 65 pieces), with weights the scores' bytes too.  A launch of its own:
+// joins by the last workgroup of a segment would need device-wide fences, which write back the L2.
 constexpr uint32_t PJ_SPAN = 256, PJ_ROWS = 64, PJ_AHEAD = 16;
 constexpr uint32_t pj_parts(uint32_t hd) { return PA_NT / (hd / 4); }
 template <int HD, int QT, int NR, uint32_t PER>

@@ -16,7 +16,7 @@
 // draft model, 151936 tokens) take 31 us, 4.4 TB/s; 15 instructions a logit, 9 of them f64, are about half
 // of that.  Only sequences that rejected a draft of a draft model read two rows again for max(p - q, 0)
 // (k_vd_rest, spread over the chip like the first pass: 15 us there); otherwise the shares' sums are known.
-// k_vd_pick then needs one share's logits: latency (9 us there, 7 us for one sequence without a draft model).
+// k_vd_pick then needs one share's logits: latency (7 us there and for one sequence without a draft model).
 // Rest and pick as one launch, the draw by the sequence's last workgroup, took 47 us: its fences write back
 // and invalidate the L2.
 #pragma once
@@ -153,6 +153,7 @@ struct VdArgs {
   const float* uniforms;
   VdPart* parts;      // [seq][row][share]: target rows 0 .. n_draft, then draft rows
   double* rest;       // [seq][share]: sums of max(p - q, 0) of a sequence that rejected a draft
+  VdPart* judged;     // [seq][64]: what k_vd_rest's vd_accept found, the last entry's i took | state << 8
   uint32_t* accepted;
   uint32_t* out;
   float* logprobs;
@@ -308,7 +309,7 @@ __device__ __forceinline__ void vd_exp8(const float (&l)[8], float m, float temp
   }
 }
 
-// ---- acceptance: every workgroup of k_vd_rest and k_vd_pick works out its sequence's
+// ---- acceptance: every workgroup of k_vd_rest, else of k_vd_pick, works out its sequence's
 enum { VD_DRAW = 0, VD_GREEDY = 1, VD_NONE = 2 };
 struct VdShared {
   uint64_t tab[32];
@@ -414,6 +415,9 @@ __global__ __launch_bounds__(VD_NT) void k_vd_rest(VdArgs a) {
   const uint32_t share = (blockIdx.x - s * groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   vd_accept<LT>(a, s, sh);
   const uint32_t took = sh.took;
+  if (share < 4 && threadIdx.x <= VD_MAX_ROWS)  // the sequence's first workgroup
+    a.judged[(size_t)s * (VD_MAX_ROWS + 1) + threadIdx.x] =
+        threadIdx.x < VD_MAX_ROWS ? sh.row[threadIdx.x] : VdPart{0.0, 0.0f, took | sh.state << 8};
   if (sh.state != VD_DRAW || took >= vd_drafts(a, s) || share >= a.shares) return;
   VdLogits<LT> x, y;
   x.load(vd_target<LT>(a, s, took), share * VD_SHARE, a.vocab);
@@ -472,7 +476,20 @@ __global__ __launch_bounds__(VD_NT) void k_vd_pick(VdArgs a) {
   __shared__ uint2 waves[VD_NT / 64];
   __shared__ double s_before;
   const uint32_t s = blockIdx.x, tid = threadIdx.x, n = vd_drafts(a, s);
-  vd_accept<LT>(a, s, sh);
+  if (a.draft) {  // k_vd_rest has worked it out (32 sequences: 6.9 us, 9.4 with working it out again)
+    vd_table(sh.tab);
+    if (tid <= VD_MAX_ROWS) {
+      const VdPart x = a.judged[(size_t)s * (VD_MAX_ROWS + 1) + tid];
+      sh.row[tid] = x;
+      if (tid == VD_MAX_ROWS) {
+        sh.took = x.i & 0xffu;
+        sh.state = x.i >> 8;
+      }
+    }
+    __syncthreads();
+  } else {
+    vd_accept<LT>(a, s, sh);
+  }
   const uint32_t took = sh.took, state = sh.state;
   const float temp = a.temperature[s];
   const double by = vd_by(temp);

@@ -322,7 +322,8 @@ static size_t vd_parts_bytes(uint64_t n_seqs, uint64_t n_draft, uint32_t vocab) 
 }
 
 size_t camelid_hip_verify_drafts_workspace(uint32_t n_seqs, uint32_t n_draft, uint32_t vocab) {
-  return vd_parts_bytes(n_seqs, n_draft, vocab) + up256((size_t)n_seqs * vd_shares(vocab) * 8);
+  return vd_parts_bytes(n_seqs, n_draft, vocab) + up256((size_t)n_seqs * vd_shares(vocab) * 8) +
+         (size_t)n_seqs * (cm::VD_MAX_ROWS + 1) * sizeof(cm::VdPart);
 }
 
 int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint32_t logits_type,
@@ -354,6 +355,7 @@ int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint
   a.uniforms = uniforms;
   a.parts = static_cast<cm::VdPart*>(workspace);
   a.rest = reinterpret_cast<double*>(static_cast<char*>(workspace) + vd_parts_bytes(n_seqs, n_draft, vocab));
+  a.judged = reinterpret_cast<cm::VdPart*>(reinterpret_cast<char*>(a.rest) + up256((size_t)n_seqs * vd_shares(vocab) * 8));
   a.accepted = accepted;
   a.out = tokens_out;
   a.logprobs = logprobs_out;
