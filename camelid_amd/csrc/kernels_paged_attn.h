@@ -8,7 +8,7 @@
 //   64 of up to 4001, 24 + 8 heads: 90 + 5 us, 5.7 TB/s
 //   1 of 8199, 32 + 8 heads: 9.6 + 4.4 us for 34 MB: latency (launch 1, plan 1.2, pages 0.6, K and V and
 //     the query operands 2, products and softmax 1.4, states joined and written 1.3, then the join's launch)
-//   16 of up to 1100, up to 5 new tokens, weights kept: 17.4 + 6.4 us for 39 MB: the same, two tiles a wave
+//   16 of up to 1100, up to 5 new tokens, weights kept: 17.5 + 6.2 us for 39 MB: the same, two tiles a wave
 //
 // Split.  A segment is (sequence, KV head, block of 16 NR query rows); its tiles are 32 positions.
 // The query rows are the new tokens times the KV head's query heads, so K and V are read once for
@@ -156,11 +156,12 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, uint32_t s, bool flag) 
 
 // Tiles of a piece at most, for `total` of the batch.  Small batches: one tile per wave, or as many as
 // bring the pieces below what the chip holds at once (a second round of workgroups costs its
-// whole latency again).  Large ones: 16, so that workgroups ending early make room for others, and
+// whole latency again), the same for every wave (16x1100 with 5 drafts: 22.9 us at 8 tiles, 24.0 at 5).
+// Large ones: 16, so that workgroups ending early make room for others, and
 // more once that makes over 2048 pieces.
 __device__ __forceinline__ uint32_t pa_target(const PaArgs& a, uint32_t total) {
   const uint32_t one = (total + a.at_once - 1) / a.at_once;
-  return one <= 16 ? max(4u, one) : max(16u, (total + 2047) / 2048);
+  return one <= 16 ? max(4u, (one + 3) & ~3u) : max(16u, (total + 2047) / 2048);
 }
 
 struct PaPiece {
