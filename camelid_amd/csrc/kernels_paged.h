@@ -355,8 +355,6 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr uint32_t EV_NT = 1024;
-
 // Inclusive prefix sum over the wave by data-parallel moves.
 __device__ __forceinline__ uint32_t ev_wave_scan(uint32_t x) {
   x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);  // 1, 2, 4, 8 lanes below
@@ -380,22 +378,24 @@ struct EvictPlan {
 // One workgroup per (sequence, KV head): the plan, `kept` (the positions themselves), the weights
 // compacted.
 //
-// The smallest kept weight by its digits from the top, 11, 11 and 10 bits: for each a histogram in two
-// copies and a suffix sum of its counts (digits of 8 bits had the weights crowd in few bins:
-// 5.2 us for the first digit of 16383).  A thread holds K weights in registers, runs of V
-// at a time, so up to K * 1024 positions are read once; longer rows go through the same code in pieces that
-// are read again.  Then prefix sums of two counts in a word (weights above the smallest, weights equal
-// to it) give every kept position its place.
-// Bound: latency (barriers between the digits): 16 x 8 rows of 1088 weights 7.6 us (43 with 8-bit digits in
-// one histogram searched by one thread), 4 x 8 rows of up to 16383 weights 16.6 us.
-template <int K>
-__global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restrict__ weights, uint32_t keep,
+// The smallest kept weight by its digits from the top: for each a histogram in two copies and a suffix sum of
+// its counts.  A thread holds K weights in registers, runs of V at a time, so up to K * NT positions are read
+// once; longer rows go through the same code in pieces that are read again.  Then prefix sums of two counts
+// in a word (weights above the smallest, weights equal to it) give every kept position its place.
+// Rows of up to 512 positions: 256 threads, four digits of 8 bits (95 x 8 rows of up to 78 weights 15.3 ->
+// 7.8 us against 1024 threads).  Longer ones: 1024 threads, digits of 11, 11 and 10 bits (of 8 bits the first
+// takes 5.2 us for 16383 weights, which crowd in few counters).
+// Bound: latency (barriers between the digits): 16 x 8 rows of 1088 weights 7.6 us (43 with a histogram
+// searched by one thread), 4 x 8 rows of up to 16383 weights 16.6 us.
+template <int K, uint32_t NT>
+__global__ __launch_bounds__(NT) void k_evict_select(Paged g, float* __restrict__ weights, uint32_t keep,
                                                         uint32_t recent, EvictPlan plan, uint32_t* __restrict__ kept) {
-  constexpr uint32_t COPIES = 2, BINS = 2048, PIECE = EV_NT * K;
-  constexpr int V = K < 4 ? K : 4, N = K / V;  // N runs of V positions, EV_NT * V apart
+  constexpr uint32_t COPIES = 2, BITS = NT == 1024 ? 11 : 8, BINS = 1u << BITS, PIECE = NT * K;
+  constexpr uint32_t PER = BINS / NT;          // digits of a thread
+  constexpr int V = K < 4 ? K : 4, N = K / V;  // N runs of V positions, NT * V apart
   typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
   __shared__ uint32_t hist[COPIES][BINS];
-  __shared__ uint32_t wave_sums[N][EV_NT / 64], wave_touched[N][EV_NT / 64];
+  __shared__ uint32_t wave_sums[N][NT / 64], wave_touched[N][NT / 64];
   __shared__ uint32_t s_digit, s_rank, s_bad;
   const uint32_t s = blockIdx.x / g.n_kv, h = blockIdx.x - s * g.n_kv, tid = threadIdx.x, lane = tid & 63u;
   const uint32_t L = g.lens[s], cap = g.stride << g.shift, mask = (1u << g.shift) - 1u;
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
   const bool too_long = (uint64_t)L > ((uint64_t)g.stride << g.shift);
   // the first piece's weights, on their way while the pages are looked through
   float x[N][V];
-  const auto at = [&](uint32_t p0, int i, int e) { return p0 + (i * EV_NT + tid) * V + e; };
+  const auto at = [&](uint32_t p0, int i, int e) { return p0 + (i * NT + tid) * V + e; };
   const auto read = [&](uint32_t p0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
   } else {
     if (L > keep) read(0);
     bool bad = false;
-    for (uint32_t i = tid; i < (L + mask) >> g.shift; i += EV_NT) bad |= tab[i] >= g.n_pages;
+    for (uint32_t i = tid; i < (L + mask) >> g.shift; i += NT) bad |= tab[i] >= g.n_pages;
     if (bad) s_bad = 1;
   }
   __syncthreads();
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
   uint32_t* kp = kept ? kept + (size_t)blockIdx.x * keep : nullptr;
   if (!moves) {
     if (kp && !too_long)
-      for (uint32_t j = tid; j < min(L, keep); j += EV_NT) kp[j] = j;
+      for (uint32_t j = tid; j < min(L, keep); j += NT) kp[j] = j;
     return;
   }
   const size_t row0 = (size_t)blockIdx.x * keep;
@@ -455,10 +455,10 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
   uint32_t rank = keep - recent;  // positions still to be found among the keys equal in the digits so far
   const bool any = rank != 0;
   uint32_t prefix = 0;
-  for (int b = 21; b >= 0 && any; b -= b > 10 ? 11 : 10) {
-    const uint32_t bins = b ? BINS : 1024u;  // digits of key >> b below those found, in `prefix` >> above
-    const int above_bits = b + (b ? 11 : 10);
-    for (uint32_t i = tid; i < COPIES * BINS; i += EV_NT) hist[0][i] = 0;
+  for (int top = 32; top > 0 && any;) {  // the digit in bits b .. top - 1, those above are in `prefix`
+    const int b = max(0, top - (int)BITS);
+    const uint32_t bins = 1u << (top - b);
+    for (uint32_t i = tid; i < COPIES * BINS; i += NT) hist[0][i] = 0;
     __syncthreads();
     for (uint32_t p0 = 0; p0 < cut; p0 += PIECE) {
       if (!one) {
@@ -470,18 +470,19 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const uint32_t k = key[i][e];
-          if (at(p0, i, e) < cut && (b == 21 || k >> (above_bits & 31) == prefix >> (above_bits & 31)))
+          if (at(p0, i, e) < cut && (top == 32 || k >> (top & 31) == prefix >> (top & 31)))
             atomicAdd(&hist[(tid >> 6) % COPIES][(k >> b) & (bins - 1)], 1u);
         }
     }
     __syncthreads();
-    // thread t: digits 2047 - 2 t and 2046 - 2 t
-    const uint32_t hi = BINS - 1 - 2 * tid, c0 = hist[0][hi] + hist[1][hi], c1 = hist[0][hi - 1] + hist[1][hi - 1];
+    // thread t: digit BINS - 1 - PER t and, for PER = 2, the one below it
+    const uint32_t hi = BINS - 1 - PER * tid, c0 = hist[0][hi] + hist[1][hi];
+    const uint32_t c1 = PER == 2 ? hist[0][hi - 1] + hist[1][hi - 1] : 0u;
     const uint32_t incl = ev_wave_scan(c0 + c1);
     if (lane == 63) wave_sums[0][tid >> 6] = incl;
     __syncthreads();
     uint32_t above = incl - c0 - c1;
-    for (uint32_t v = 0; v < EV_NT / 64; ++v) above += v < tid >> 6 ? wave_sums[0][v] : 0u;
+    for (uint32_t v = 0; v < NT / 64; ++v) above += v < tid >> 6 ? wave_sums[0][v] : 0u;
     if (above < rank && above + c0 + c1 >= rank) {
       const bool first = above + c0 >= rank;
       s_digit = first ? hi : hi - 1;
@@ -490,6 +491,7 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
     __syncthreads();
     prefix |= s_digit << b;
     rank = s_rank;
+    top = b;
   }
   // kept: every key above `prefix`, the first `rank` keys equal to it, and the recent positions
   uint32_t eq0 = 0, gt0 = 0, touched0 = 0;  // of the pieces before
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       uint32_t all = 0;
-      for (uint32_t v = 0; v < EV_NT / 64; ++v) {
+      for (uint32_t v = 0; v < NT / 64; ++v) {
         const uint32_t y = wave_sums[i][v];
         if (v < tid >> 6) before[i] += y;
         all += y;
@@ -547,7 +549,7 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       uint32_t t = touched0 + seen[i] - 1;
-      for (uint32_t v = 0; v < EV_NT / 64; ++v) {
+      for (uint32_t v = 0; v < NT / 64; ++v) {
         const uint32_t y = wave_touched[i][v];
         if (v < tid >> 6) t += y;
         touched0 += y;
@@ -570,72 +572,82 @@ __global__ __launch_bounds__(EV_NT) void k_evict_select(Paged g, float* __restri
 }
 
 // The move, in place: output positions in chunks, a chunk's sources read before any of it is
-// written.  A source is never below its output position, so no later chunk misses a row.  Bound:
-// HBM: 16 x 8 x 1024 of 1088 rows of 128 dims, 134 MB, 24 us, 5.6 TB/s; 4 x 8 x 2048 of up to 16383
-// rows 19 us, where rows far apart share their 128-byte lines with rows that are left behind (about 160
+// written.  A source is never below its output position, so no later chunk misses a row.  A workgroup takes
+// as many dims as leave all kept rows one chunk (ks, vs; 95 x 8 x 22 of up to 78 rows: 25 -> 8.4 us against 8
+// dims of K and 16 of V), and where there are few workgroups larger chunks (F; 2 x 8 x 14511 of 20144 rows:
+// 40 -> 36 us).  Bound: HBM: 16 x 8 x 1024 of 1088 rows of 128 dims, 134 MB, 26 us, 5.2 TB/s; 4 x 8 x 2048 of up
+// to 16383 rows 20 us, where rows far apart share their 128-byte lines with rows that are left behind (about 160
 // MB of lines for 67 MB).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// K: one workgroup per (sequence, KV head, 8 dims), whole granules, chunks of R * EM_NT rows in registers.
-constexpr uint32_t EM_NT = 512;
+// K: one workgroup per (sequence, KV head, 8 << ks dims), whole granules, chunks of 2048 F >> ks rows in
+// registers.
+constexpr uint32_t EM_NT = 512, EM_K_LOG2 = 11;
+template <uint32_t F>
 __device__ __forceinline__ void evict_move_k(const Paged& g, uint16_t* __restrict__ kc, uint32_t keep,
-                                             const EvictPlan& plan, uint32_t sh, uint32_t d) {
-  constexpr uint32_t R = 4;
+                                             const EvictPlan& plan, uint32_t sh, uint32_t sl, uint32_t ks) {
+  constexpr uint32_t R = (F << EM_K_LOG2) / EM_NT;
   const uint32_t tid = threadIdx.x, s = sh / g.n_kv, h = sh - s * g.n_kv;
   const uint32_t* tab = g.table + (size_t)s * g.stride;
   const uint32_t* sp = plan.slot + (size_t)sh * keep;
-  const uint32_t mask = (1u << g.shift) - 1u;
-  for (uint32_t j0 = 0; j0 < keep; j0 += R * EM_NT) {
+  const uint32_t mask = (1u << g.shift) - 1u, bits = EM_K_LOG2 + __builtin_ctz(F) - ks, rows = 1u << bits;
+  for (uint32_t j0 = 0; j0 < keep; j0 += rows) {
     u32x4 x[R];
     uint32_t to[R], slot[R];
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
-      const uint32_t j = min(j0 + r * EM_NT + tid, keep - 1);
+      const uint32_t j = min(j0 + ((r * EM_NT + tid) & (rows - 1)), keep - 1);
       slot[r] = sp[j];
       to[r] = (tab[j >> g.shift] << g.shift) + (j & mask);
     }
+    const auto place = [&](uint32_t at, uint32_t r) {
+      return kc + paged_base(g, at >> g.shift, h) + paged_k(g, at & mask, 8 * ((sl << ks) + ((r * EM_NT + tid) >> bits)));
+    };
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r)
-      x[r] = *reinterpret_cast<const u32x4*>(kc + paged_base(g, slot[r] >> g.shift, h) + paged_k(g, slot[r] & mask, d));
+      if (j0 + ((r * EM_NT + tid) & (rows - 1)) < keep) x[r] = *reinterpret_cast<const u32x4*>(place(slot[r], r));
     __syncthreads();
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r)
-      if (j0 + r * EM_NT + tid < keep && slot[r] != to[r])
-        *reinterpret_cast<u32x4*>(kc + paged_base(g, to[r] >> g.shift, h) + paged_k(g, to[r] & mask, d)) = x[r];
+      if (j0 + ((r * EM_NT + tid) & (rows - 1)) < keep && slot[r] != to[r])
+        *reinterpret_cast<u32x4*>(place(to[r], r)) = x[r];
   }
 }
 
-// V: one workgroup per (sequence, KV head, 16 dims).  A granule holds 8 positions, an output granule
-// gathers from up to 8 of them, so a chunk is as many rows as EM_G distinct granules feed; these go to LDS
-// whole (2-byte loads from memory, 16 bytes apart between lanes, took the L1 47 accesses each: 24 us of
+// V: one workgroup per (sequence, KV head, 8 << vs dims).  A granule holds 8 positions, an output granule
+// gathers from up to 8 of them, so a chunk is as many rows as 256 F >> vs distinct granules feed; these go to
+// LDS whole (2-byte loads from memory, 16 bytes apart between lanes, took the L1 47 accesses each: 24 us of
 // the 37 us that the move of 16x1088 -> 1024 rows took) and the output granules are put together from there.
-constexpr uint32_t EM_G = 128, EM_D = 16;
+constexpr uint32_t EM_G = 256;
+constexpr uint32_t em_lds(uint32_t f) { return f * EM_G * 8 * 16; }
+template <uint32_t F>
 __device__ __forceinline__ void evict_move_v(const Paged& g, uint16_t* __restrict__ vc, uint32_t keep,
-                                             const EvictPlan& plan, uint32_t sh, uint32_t sl, u32x4* s_g, uint32_t* s_end) {
+                                             const EvictPlan& plan, uint32_t sh, uint32_t sl, uint32_t vs, u32x4* s_g,
+                                             uint32_t* s_end) {
   const uint32_t tid = threadIdx.x, s = sh / g.n_kv, h = sh - s * g.n_kv;
   const uint32_t* tab = g.table + (size_t)s * g.stride;
   const uint32_t* fp = plan.from + (size_t)sh * keep;
   const uint32_t* gp = plan.granule + (size_t)sh * keep;
-  const uint32_t mask = (1u << g.shift) - 1u, d = sl * EM_D + (tid % EM_D);
+  const uint32_t bits = 3 + vs, dim = tid & ((1u << bits) - 1u), granules = F * EM_G >> vs;
+  const uint32_t mask = (1u << g.shift) - 1u, d = (sl << bits) + dim;
   const uint16_t* elems = reinterpret_cast<const uint16_t*>(s_g);
+  constexpr uint32_t U = F * EM_G * 8 / EM_NT;  // granules of a thread
   for (uint32_t j0 = 0, j1; j0 < keep; j0 = j1) {
-    // the chunk's rows [j0, j1): whole output granules (but for the last) whose sources are granules t0 .. t0 + EM_G - 1
+    // the chunk's rows [j0, j1): whole output granules (but for the last) whose sources are granules t0 and up;
+    // 512 ends of 8 rows are looked at, and granules up to the last that any of them can have; more than
+    // the chunk's are not loaded
     const uint32_t t0 = fp[j0] >> 3;
-    static_assert(EM_G * 8 <= EM_NT * 8, "every end a chunk can have is looked at");
-    const uint32_t end = min(keep, j0 + 8 * (tid + 1));
-    const uint32_t t_end = fp[end - 1] >> 3;
-    constexpr uint32_t U = EM_G * EM_D / EM_NT;  // granules of a thread
-    // granules up to the last that any chunk from here can have: more than this chunk's are not loaded
+    const uint32_t t_end = fp[min(keep, j0 + 8 * (tid + 1)) - 1] >> 3;
     uint32_t slot[U];
 #pragma unroll
-    for (uint32_t k = 0; k < U; ++k) slot[k] = gp[min(t0 + (k * EM_NT + tid) / EM_D, keep - 1)] << 3;
-    const uint64_t fit = __ballot(j0 + 8 * tid < keep && t_end < t0 + EM_G);
+    for (uint32_t k = 0; k < U; ++k) slot[k] = gp[min(t0 + ((k * EM_NT + tid) >> bits), keep - 1)] << 3;
+    const uint64_t fit = __ballot(j0 + 8 * tid < keep && t_end < t0 + granules);
     if ((tid & 63u) == 0) s_end[tid >> 6] = __popcll(fit);
     __syncthreads();
     uint32_t n8 = 0;
     for (uint32_t i = 0; i < EM_NT / 64; ++i) n8 += s_end[i];
     j1 = min(keep, j0 + 8 * n8);
-    const uint32_t n_u = ((fp[j1 - 1] >> 3) - t0 + 1) * EM_D;
+    const uint32_t n_u = ((fp[j1 - 1] >> 3) - t0 + 1) << bits;
     u32x4 x[U];
 #pragma unroll
     for (uint32_t k = 0; k < U; ++k)
@@ -645,12 +657,12 @@ __device__ __forceinline__ void evict_move_v(const Paged& g, uint16_t* __restric
     for (uint32_t k = 0; k < U; ++k)
       if (k * EM_NT + tid < n_u) s_g[k * EM_NT + tid] = x[k];
     __syncthreads();
-    for (uint32_t j = j0 + tid / EM_D * 8; j < j1; j += EM_NT / EM_D * 8) {
+    for (uint32_t j = j0 + ((tid >> bits) << 3); j < j1; j += (EM_NT >> bits) << 3) {
       uint32_t v[8];
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) {
         const uint32_t f = fp[min(j + i, keep - 1)];
-        v[i] = elems[(((f >> 3) - t0) * EM_D + tid % EM_D) * 8 + (f & 7u)];
+        v[i] = elems[(((((f >> 3) - t0) << bits) + dim) << 3) + (f & 7u)];
       }
       uint16_t* dst = vc + paged_base(g, tab[j >> g.shift], h) + paged_v(g, j & mask, d);
       if (j + 8 <= keep) {
@@ -666,18 +678,20 @@ __device__ __forceinline__ void evict_move_v(const Paged& g, uint16_t* __restric
 }
 
 // V's workgroups first: they take longer.
-__global__ __launch_bounds__(EM_NT, 8) void k_evict_move(Paged g, uint16_t* __restrict__ kc, uint16_t* __restrict__ vc,
-                                                         uint32_t keep, EvictPlan plan, uint32_t* __restrict__ lens_out) {
-  __shared__ u32x4 s_g[EM_G * EM_D];  // [granule][dim], 8 positions each
+template <uint32_t F>
+__global__ __launch_bounds__(EM_NT, F == 1 ? 8 : F == 2 ? 4 : 2)
+void k_evict_move(Paged g, uint16_t* __restrict__ kc, uint16_t* __restrict__ vc, uint32_t keep, EvictPlan plan,
+                  uint32_t* __restrict__ lens_out, uint32_t ks, uint32_t vs) {
+  extern __shared__ u32x4 s_g[];  // [granule][dim], 8 positions each
   __shared__ uint32_t s_end[EM_NT / 64];
-  const uint32_t v_slices = g.hd / EM_D, n_v = g.n_seqs * g.n_kv * v_slices;
+  const uint32_t v_slices = g.hd >> (3 + vs), n_v = g.n_seqs * g.n_kv * v_slices;
   const bool is_v = blockIdx.x < n_v;
-  const uint32_t b = is_v ? blockIdx.x : blockIdx.x - n_v, slices = is_v ? v_slices : g.hd / 8;
+  const uint32_t b = is_v ? blockIdx.x : blockIdx.x - n_v, slices = is_v ? v_slices : g.hd >> (3 + ks);
   const uint32_t sh = b / slices, sl = b - sh * slices, s = sh / g.n_kv;
   if (is_v && sl == 0 && sh == s * g.n_kv && threadIdx.x == 0) lens_out[s] = plan.new_lens[s];
   if (!plan.old_lens[s]) return;
-  if (is_v) evict_move_v(g, vc, keep, plan, sh, sl, s_g, s_end);
-  else evict_move_k(g, kc, keep, plan, sh, sl * 8);
+  if (is_v) evict_move_v<F>(g, vc, keep, plan, sh, sl, vs, s_g, s_end);
+  else evict_move_k<F>(g, kc, keep, plan, sh, sl, ks);
 }
 
 }  // namespace cm

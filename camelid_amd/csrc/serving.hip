@@ -288,7 +288,13 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
     return cm::fail_global(me, why);
   if (!keep || keep > (1u << 24)) return cm::fail_global(me, "keep must be in 1..=2^24");
   if (recent > keep) return cm::fail_global(me, "recent must be at most keep");
-  const uint64_t movers = (uint64_t)n_seqs * n_kv * (hd / cm::EM_D + hd / 8);
+  // dims of a workgroup of the move: as many as still let all kept rows be one chunk, else 8, of V 16 where that
+  // leaves two workgroups a CU (4 x 8 rows of V with 8 dims: 31.8 us for the call, with 16: 33.0)
+  uint32_t ks = 0, vs = 0;
+  while (hd >> (4 + ks) && keep <= (1u << cm::EM_K_LOG2) >> (ks + 1)) ++ks;
+  while (hd >> (4 + vs) && keep <= cm::EM_G >> (vs + 1)) ++vs;
+  if (!vs && (uint64_t)n_seqs * n_kv * hd >= 512 * 16) vs = 1;
+  const uint64_t movers = (uint64_t)n_seqs * n_kv * ((hd >> (3 + ks)) + (hd >> (3 + vs)));
   if (!grid_ok(movers, cm::EM_NT)) return cm::fail_global(me, "n_seqs * n_kv * head_dim too large for one call");
   if ((uint64_t)n_pages * page_size > 0xffffffffull)
     return cm::fail_global(me, "n_pages * page_size must be below 2^32");
@@ -306,14 +312,32 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
   plan.slot = reinterpret_cast<uint32_t*>(ws);
   plan.from = reinterpret_cast<uint32_t*>(ws + rows);
   plan.granule = reinterpret_cast<uint32_t*>(ws + 2 * rows);
-  // rows of at most 2048, 8192 and 16384 positions have their weights read once
+  // rows of at most 512, 2048, 8192 and 16384 positions have their weights read once
   const uint32_t cap = page_size * table_stride;
-  const auto select = cap <= 2048 ? cm::k_evict_select<2> : cap <= 8192 ? cm::k_evict_select<8> : cm::k_evict_select<16>;
-  hipLaunchKernelGGL(select, dim3(n_seqs * n_kv), dim3(cm::EV_NT), 0, (hipStream_t)stream, g, weights, keep, recent, plan,
-                     kept);
-  hipLaunchKernelGGL(cm::k_evict_move, dim3((uint32_t)movers), dim3(cm::EM_NT), 0,
-                     (hipStream_t)stream, g, static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc), keep, plan, lens_out);
-  return launched(me);
+  const auto select = [&](auto kernel, uint32_t threads) {
+    hipLaunchKernelGGL(kernel, dim3(n_seqs * n_kv), dim3(threads), 0, (hipStream_t)stream, g, weights, keep, recent, plan,
+                       kept);
+  };
+  if (cap <= 512) select(cm::k_evict_select<2, 256>, 256);
+  else if (cap <= 2048) select(cm::k_evict_select<2, 1024>, 1024);
+  else if (cap <= 8192) select(cm::k_evict_select<8, 1024>, 1024);
+  else select(cm::k_evict_select<16, 1024>, 1024);
+  const auto go = [&](auto kernel, uint32_t f) {
+    const size_t lds = cm::em_lds(f);
+    if (lds >= 64 * 1024) {
+      const hipError_t st = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (st != hipSuccess) return cm::fail_global(me, hipGetErrorString(st));
+    }
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)movers), dim3(cm::EM_NT), lds, (hipStream_t)stream, g,
+                       static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc), keep, plan, lens_out, ks, vs);
+    return launched(me);
+  };
+  // few workgroups (one or two a CU) with many rows take them in larger chunks (2 x 8 x 14511 rows: 73 us for the
+  // call against 78, 1 x 8 x 14027: 56 against 59)
+  if (!ks && !vs && movers <= 256) return go(cm::k_evict_move<4>, 4);
+  if (!ks && !vs && movers <= 512) return go(cm::k_evict_move<2>, 2);
+  return go(cm::k_evict_move<1>, 1);
 }
 
 static uint32_t vd_shares(uint32_t vocab) { return (vocab + cm::VD_SHARE - 1) / cm::VD_SHARE; }

@@ -570,6 +570,11 @@ EVICT_CASES = [
     (2, 64, [20000, 9], 128, 3001, 17, heavy),
     (2, 64, [40], 8, 1000, 10, heavy),
     (8, 128, [1088] * 3, 32, 1024, 256, heavy),
+    (8, 128, [3000, 2500], 32, 2100, 50, strange),
+    (8, 128, [78, 11, 60, 33] * 20, 8, 22, 9, heavy),
+    (4, 64, [400, 512, 1, 0, 257], 64, 130, 0, strange),
+    (8, 256, [300, 512], 128, 256, 255, tied),
+    (2, 256, [40, 17], 8, 3, 1, strange),
 ]
 
 
