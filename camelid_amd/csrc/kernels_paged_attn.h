@@ -582,14 +582,14 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
 }
 
 // Joins the cut segments: workgroups of PER rows of a (sequence, KV head), a row's parts dealt out to
-// PARTS / PER groups of HD / 4 lanes; then, where weights are kept, workgroups of 256 positions.  Bound:
+// PARTS / PER groups of HD / 4 lanes; then, where weights are kept, workgroups of 256 or 64 positions.  Bound:
 // latency (4.4 us for 8 segments of 65 pieces), with weights the scores' bytes too.  A launch of its own:
 // joins by the last workgroup of a segment would need device-wide fences, which write back the L2.
-constexpr uint32_t PJ_SPAN = 256, PJ_ROWS = 64, PJ_AHEAD = 16;
+constexpr uint32_t PJ_ROWS = 64, PJ_AHEAD = 16;
 constexpr uint32_t pj_parts(uint32_t hd) { return PA_NT / (hd / 4); }
 template <int HD, int QT, int NR, uint32_t PER>
 __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, uint32_t row_groups,
-                                                   uint32_t spans) {
+                                                   uint32_t spans, uint32_t span_bits) {
   constexpr uint32_t ROWS = 16 * NR, PARTS = pj_parts(HD), STEP = PARTS / PER;
   __shared__ f32x4 s_o[PARTS][HD / 4];
   __shared__ float s_ml[PARTS][2];
@@ -646,24 +646,26 @@ __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, ui
     }
     return;
   }
-  // weights of 256 positions: the scores, PJ_AHEAD rows' on their way at a time, against each row's
-  // maximum and sum
-  const uint32_t pos = (blockIdx.x - n_out - sh * spans) * PJ_SPAN + tid;
+  // weights of 1 << span_bits positions, the rows dealt out to the 256 >> span_bits groups of threads that are
+  // left: the scores, PJ_AHEAD rows' on their way at a time, against each row's maximum and sum
+  const uint32_t span = 1u << span_bits, teams = PA_NT >> span_bits, team = __builtin_amdgcn_readfirstlane(tid >> span_bits);
+  const uint32_t pos0 = (blockIdx.x - n_out - sh * spans) << span_bits, pos = pos0 + (tid & (span - 1));
   const PaSeq sq = pa_seq<NR>(a, s, false);
-  if (!sq.rows || pos - tid >= sq.len) return;
+  if (!sq.rows || pos0 >= sq.len) return;
   const uint32_t cap = g.stride << g.shift;
   const size_t all = (size_t)a.n_new * a.group, base = (size_t)sh * all;
   const uint32_t at_pos = min(pos, sq.len - 1);
   float* wp = a.weights + (size_t)sh * cap;
-  float acc = at_pos < sq.first ? wp[at_pos] : 0.0f;
+  float acc = team == 0 && at_pos < sq.first ? wp[at_pos] : 0.0f;
   for (uint32_t r0 = 0; r0 < sq.rows; r0 += PJ_ROWS) {
     const uint32_t n = min(PJ_ROWS, sq.rows - r0);
     float sc[PJ_AHEAD];
     const auto fetch = [&](uint32_t k) {
 #pragma unroll
-      for (uint32_t i = 0; i < PJ_AHEAD; ++i) sc[i] = a.scores[(base + min(r0 + k + i, sq.rows - 1)) * cap + at_pos];
+      for (uint32_t i = 0; i < PJ_AHEAD; ++i)
+        if (k + i * teams < n) sc[i] = a.scores[(base + r0 + k + i * teams) * cap + at_pos];
     };
-    fetch(0);
+    fetch(team);
     __syncthreads();
     // a quarter wave per row: 16 lanes over its parts
     for (uint32_t k = tid >> 4; k < n; k += PA_NT / 16) {
@@ -695,14 +697,22 @@ __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, ui
       }
     }
     __syncthreads();
-    for (uint32_t k = 0; k < n; k += PJ_AHEAD) {
-      if (k) fetch(k);
+    for (uint32_t k = team; k < n; k += PJ_AHEAD * teams) {
+      if (k != team) fetch(k);
 #pragma unroll
-      for (uint32_t i = 0; i < PJ_AHEAD; ++i)
-        if (k + i < n) acc += __builtin_amdgcn_exp2f(sc[i] - s_stat[k + i][0]) * s_stat[k + i][1];
+      for (uint32_t i = 0; i < PJ_AHEAD; ++i) {
+        const uint32_t r = k + i * teams;
+        if (r < n) acc += __builtin_amdgcn_exp2f(sc[i] - s_stat[r][0]) * s_stat[r][1];
+      }
     }
   }
-  if (pos < sq.len) wp[pos] = acc;
+  if (teams > 1) {
+    float* s_acc = reinterpret_cast<float*>(s_o);
+    s_acc[tid] = acc;
+    __syncthreads();
+    for (uint32_t t = 1; t < teams; ++t) acc += s_acc[t * span + (tid & (span - 1))];
+  }
+  if (team == 0 && pos < sq.len) wp[pos] = acc;
 }
 
 }  // namespace cm

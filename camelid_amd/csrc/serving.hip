@@ -101,15 +101,20 @@ bool pa_launch(const cm::PaArgs& a, const PaSizes& z, hipStream_t stream) {
   }
   hipLaunchKernelGGL(split, dim3(z.grid), dim3(cm::PA_NT), lds, stream, a);
   if (!z.join) return true;
-  // segments of up to 16 pieces: a row to one group of lanes (16x1100 with 5 drafts: 6.6 us against 7.6
-  // with a workgroup a row); longer ones: a workgroup a row (1x8199: 4.1 us against 6.6)
+  // tables of up to 16 pieces, or many segments (which make larger pieces): a row to one group of lanes (16x1100
+  // with 5 drafts: 6.6 us against 7.6 with a workgroup a row, 83x2152 with 5: 123 us for the call against
+  // 135); few longer ones: a workgroup a row (1x8199: 4.1 us against 6.6)
   const uint32_t rows = a.n_new * a.group, sh = a.g.n_seqs * a.g.n_kv;
-  const uint32_t spans = a.weights ? ((a.g.stride << a.g.shift) + cm::PJ_SPAN - 1) / cm::PJ_SPAN : 0;
+  // weights: positions of a workgroup 256, or 64 with the rows dealt to its four waves where that makes less than
+  // two workgroups a CU (5x940, 64 rows: 19.1 us for the call against 22.7; 1x46046, 56 rows: 65 against 47)
+  const uint32_t cap = a.g.stride << a.g.shift, span_bits = (uint64_t)sh * ((cap + 255) >> 8) >= 512 ? 8 : 6;
+  const uint32_t spans = a.weights ? (cap + (1u << span_bits) - 1) >> span_bits : 0;
   const auto join = [&](auto per, auto kernel) {
     const uint32_t row_groups = (rows + per.value - 1) / per.value;
-    hipLaunchKernelGGL(kernel, dim3(sh * (row_groups + spans)), dim3(cm::PA_NT), 0, stream, a, rows, row_groups, spans);
+    hipLaunchKernelGGL(kernel, dim3(sh * (row_groups + spans)), dim3(cm::PA_NT), 0, stream, a, rows, row_groups, spans,
+                       span_bits);
   };
-  if ((a.g.stride << a.g.shift) <= 16 * 4 * cm::PA_TILE)
+  if (cap <= 16 * 4 * cm::PA_TILE || sh >= 256)
     join(std::integral_constant<uint32_t, cm::pj_parts(HD)>{}, cm::k_pa_join<HD, QT, NR, cm::pj_parts(HD)>);
   else
     join(std::integral_constant<uint32_t, 1>{}, cm::k_pa_join<HD, QT, NR, 1>);
@@ -223,7 +228,7 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   if (q_type != TY_F32 && q_type != kv_type)
     return cm::fail_global(me, "16-bit q rows must have the cache's type");
   if (!std::isfinite(scale)) return cm::fail_global(me, "attention score scale must be finite");
-  const uint64_t groups = (uint64_t)n_seqs * n_kv * (n_new * (n_heads / n_kv) + (weights ? 1 + ((uint64_t)table_stride * page_size >> 8) : 0));
+  const uint64_t groups = (uint64_t)n_seqs * n_kv * (n_new * (n_heads / n_kv) + (weights ? 1 + ((uint64_t)table_stride * page_size >> 6) : 0));
   if (!grid_ok(groups, cm::PA_NT)) return cm::fail_global(me, "too many rows in one call");
   const uint32_t unit = q_type == TY_F32 ? 4 : 8;
   if (q_stride < (uint64_t)n_heads * hd || out_stride < (uint64_t)n_heads * hd || q_stride % unit || out_stride % unit)
