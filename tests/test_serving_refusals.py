@@ -57,7 +57,7 @@ def test_attention_refuses(native, change, match):
 @pytest.mark.parametrize("change,match", GEOMETRY + [
     (dict(keep=0), "keep"), (dict(recent=17), "recent"), (dict(weights=None), "null"), (dict(lens_out=None), "null"),
     (dict(ws_bytes=0), "workspace too small"), (dict(ws=P + 4), "aligned"), (dict(kept=P + 2), "aligned"),
-    (dict(n_seqs=1 << 19, ws_bytes=1 << 60), "too large for one call")])
+    (dict(n_seqs=1 << 19, keep=1 << 12, ws_bytes=1 << 60), "too large for one call")])
 def test_evict_refuses(native, change, match):
     from camelid_amd._native import HipError
     with pytest.raises(HipError, match="paged_evict: .*" + match):
