@@ -155,7 +155,7 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, uint32_t s, bool flag) 
 }
 
 // Tiles of a piece at most, for `total` of the batch.  Small batches: one tile per wave, or as many as
-// bring the pieces below what the chip holds at once (a second round of workgroups costs its
+// bring the pieces below what the chip holds at once (a second generation of workgroups costs its
 // whole latency again), the same for every wave (16x1100 with 5 drafts: 22.9 us at 8 tiles, 24.0 at 5).
 // Large ones: 16, so that workgroups ending early make room for others, and
 // more once that makes over 2048 pieces.
