@@ -29,8 +29,8 @@
 //
 // Numbers.  f32 queries are the sum of two f16 (scaled by a power of two into f16's range; 22 bits) or
 // of three bf16, 16-bit queries are used as they are; the weights exp2(s - max) are the sum of
-// two 16-bit numbers (three bf16 for f32 outputs), so they keep 16 bits at least where the output
-// has 8 or 11.  f16 weights carry a factor 2^14: small ones next to the row's maximum stay normal.
+// two f16 (22 bits) or of three bf16 (all 24 of them).  f16 weights carry a factor 2^14: a term's steps are
+// 2^-39 of the row's largest weight at least.
 #pragma once
 #include <type_traits>
 #include "kernels_paged.h"
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
   typedef typename Op16<KT>::v8 v8;
   typedef typename Op16<KT>::e e16;
   constexpr int NQ = QT != TY_F32 ? 1 : KT == TY_F16 ? 2 : 3;  // 16-bit terms of a query
-  constexpr int NP = QT == TY_F32 && KT == TY_BF16 ? 3 : 2;    // ... of a weight
+  constexpr int NP = KT == TY_F16 ? 2 : 3;                     // ... of a weight
   constexpr int KS = HD / 32, DS = HD / 16;
   constexpr int ROWS = 16 * NR, PITCH = HD + 4;
   extern __shared__ float smem[];  // [4][ROWS][PITCH] rows, [4][ROWS][2] states, [ROWS]

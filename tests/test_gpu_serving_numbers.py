@@ -1,0 +1,47 @@
+"""Batched serving over a paged cache on the GPU: the bits that its numbers keep, and values at the ends of their
+types."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_serving import (BF16, F16, F32, HALF_STEP, U, Pages, attention_reference, from16, run_attention, to16,
+                              typed, value)
+
+pytestmark = pytest.mark.gpu
+
+
+def cancelling(kv, n=64, n_kv=2, g=4, hd=64):
+    """Two positions a sequence whose values are each other's negatives and whose scores are 2^-11 apart: an
+    output is v tanh(2^-12), a difference of weights near 1/2, so that an error of a weight is one of the
+    output 2^12 times as large relative to it.  Every row has a score of its own."""
+    rng = np.random.default_rng(81)
+    pg = Pages(rng, [2] * n, 8, n_kv, hd, kv)
+    v = rng.uniform(0.5, 1, (n, n_kv, hd))
+    k = np.zeros((2, hd))
+    k[:, 0], k[:, 1] = (1.0, 1.0 + 2.0 ** -7), 1.0
+    for s in range(n):
+        pg.set(s, [0, 1], to16(np.broadcast_to(k[:, None], (2, n_kv, hd)), kv), to16(np.stack([-v[s], v[s]]), kv))
+    q = np.zeros((n, n_kv * g, hd))
+    q[..., 0], q[..., 1] = 2.0 ** -4, rng.uniform(-2, 2, (n, n_kv * g))
+    return pg, typed(q.reshape(n, -1), kv)
+
+
+# Weights as sums of 16-bit numbers: three bf16 hold 24 bits (half a step of each term's 8 bits is left to the
+# next), two f16 hold 22.
+WEIGHT_BITS = {BF16: 2.0 ** -24, F16: 2.0 ** -22}
+
+
+@pytest.mark.parametrize("kv", [BF16, F16])
+def test_weights_of_16_bit_rows_keep_their_bits(native, kv):
+    pg, q = cancelling(kv)
+    nh = 8
+    out, _ = run_attention(native, pg, q, kv, 1, [1] * pg.n, nh, 1.0)
+    ref = attention_reference(pg, q, kv, 1, [1] * pg.n, nh, 1.0, None)[0]
+    for r in range(pg.n):
+        want, got = ref[r][0], value(out[r], kv)
+        # |score| < 2.5: its two products and sum are exact, log2(e) rounded and the fma off by 2^-24 of less than 4
+        # each; the exponential by 2^-23; the weight's terms; sums and quotient: 8 roundings at most of a single tile's
+        # two positions.  All relative to the sum of p |v|, which is at most 1
+        tol = 2 * 4 * U + 2.0 ** -23 + WEIGHT_BITS[kv] + 8 * U + HALF_STEP[kv] * np.abs(want)
+        assert (np.abs(got - want) <= tol).all(), (r, np.abs(got - want).max(), tol.max())
