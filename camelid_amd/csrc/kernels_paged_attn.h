@@ -27,8 +27,8 @@
 // K of the next tile is in flight from the moment the scores are done, V of the next from the
 // moment the products are: about 16 KB a wave outstanding.
 //
-// Numbers.  f32 queries are the sum of two f16 (scaled by a power of two into f16's range; 22 bits) or
-// of three bf16, 16-bit queries are used as they are; the weights exp2(s - max) are the sum of
+// Numbers.  f32 queries are the sum of two f16 (22 bits) or of three bf16, a row scaled by a power of two
+// into their range, 16-bit queries are used as they are; the weights exp2(s - max) are the sum of
 // two f16 (22 bits) or of three bf16 (all 24 of them).  f16 weights carry a factor 2^14: a term's steps are
 // 2^-39 of the row's largest weight at least.
 #pragma once
@@ -324,13 +324,17 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
       const uint32_t u = tid + k * PA_NT, row = u / LPR, d8 = u % LPR;
       float factor = a.scale * PA_LOG2E;
       int up = 0;
-      if constexpr (QT == TY_F32 && KT == TY_F16) {  // the row's largest element to [2^13, 2^14)
+      if constexpr (QT == TY_F32) {
+        // f16 terms: the row's largest element to [2^13, 2^14), whatever it is.  bf16 terms have f32's exponents:
+        // rows beyond 2^65 or below 2^-64 to there, so that the first term cannot round to infinity nor the last
+        // be subnormal
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, f2u(raw[k][i]) & 0x7fffffffu);
         const int ex = (int)(pa_group_max<LPR>(top) >> 23) - 127;
-        up = ex == 128 ? 0 : max(-100, min(100, 13 - ex));
-        factor = ldexpf(factor, -up);
+        if (ex < 128) up = KT == TY_F16 ? 13 - ex : max(-64, min(64, ex)) - ex;
+        // (a factor beyond f32: the scores' differences are past exp's range with the largest one as well)
+        factor = fmaxf(PA_LOWEST, fminf(-PA_LOWEST, ldexpf(a.scale, -up) * PA_LOG2E));
       }
       v8 term[NQ];
 #pragma unroll
@@ -338,7 +342,7 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
         if constexpr (QT != TY_F32) {
           term[0][i] = raw[k][i];
         } else {
-          float v = KT == TY_F16 ? ldexpf(raw[k][i], up) : raw[k][i];
+          float v = ldexpf(raw[k][i], up);
           const bool fin = fabsf(v) < INFINITY;
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {

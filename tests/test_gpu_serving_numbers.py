@@ -45,3 +45,29 @@ def test_weights_of_16_bit_rows_keep_their_bits(native, kv):
         # two positions.  All relative to the sum of p |v|, which is at most 1
         tol = 2 * 4 * U + 2.0 ** -23 + WEIGHT_BITS[kv] + 8 * U + HALF_STEP[kv] * np.abs(want)
         assert (np.abs(got - want) <= tol).all(), (r, np.abs(got - want).max(), tol.max())
+
+
+def rows_near(got, ref, qt):
+    for r, want in enumerate(ref):
+        y, tol = want
+        x = value(got[r], qt)
+        assert (np.abs(x - y) <= tol + HALF_STEP[qt] * (np.abs(y) + tol) + 2.0 ** -25).all(), (r, x, y)
+
+
+@pytest.mark.parametrize("kv", [F16, BF16])
+@pytest.mark.parametrize("size,scale,keys", [(1e37, 1e-37, 1.0), (3e38, 1e-37, 0.05), (1.5 * 2.0 ** 117, 2.0 ** -118, 1.0),
+                                             (1.0, 0.125, 1.0), (1e-30, 1e29, 1.0), (1e-37, 1e37, 1.0),
+                                             (1e-40, 3e38, 20.0)])
+def test_f32_queries_of_any_size(native, kv, size, scale, keys):
+    """Queries from subnormal to the largest f32, with a scale that brings their scores near 1."""
+    rng = np.random.default_rng(82)
+    nh, n_kv, hd, lens = 8, 2, 64, [70, 300]
+    pg = Pages(rng, lens, 16, n_kv, hd, kv, rows=lambda *sh: rng.normal(0, keys, sh))
+    q = np.clip(rng.normal(0, 1, (2, nh * hd)), -1.1, 1.1) * size
+    if size == 3e38:
+        q[0, 5], q[1, 100] = np.finfo(np.float32).max, -np.finfo(np.float32).max
+    q = q.astype(np.float32)
+    assert np.isfinite(q).all()
+    scale = float(np.float32(scale))
+    out, _ = run_attention(native, pg, q, F32, 1, [1, 1], nh, scale)
+    rows_near(out, attention_reference(pg, q, F32, 1, [1, 1], nh, scale, None)[0], F32)
