@@ -448,10 +448,18 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
             for (int d = 0; d < DS; ++d) o[r][d] *= alpha;
             m[r] = m_new;
           }
-          const float base = a.p_bits - ref;
+          float cr = c[r], base = a.p_bits - ref;
+          if (__ballot(fabsf(ref) >= 1024.0f)) {
+            // far from zero the product before its rounding may lie well above the reference, which comes from
+            // the rounded ones, and the factor may be lost in the reference
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sc[r][i >> 2][i & 3] = (sc[r][i >> 2][i & 3] * cr - ref) + a.p_bits;
+            cr = 1.0f;
+            base = 0.0f;
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], c[r], base));
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], cr, base));
             if (edge && !(gpos + i <= limit[r] && page_ok)) p = 0.0f;
             l[r] += p;
 #pragma unroll
@@ -696,8 +704,8 @@ __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, ui
         }
       }
       if (lane == 0) {
-        s_stat[k][0] = M == -INFINITY ? 0.0f : M - a.p_bits;
-        s_stat[k][1] = M == -INFINITY ? 0.0f : 1.0f / L;
+        s_stat[k][0] = M == -INFINITY ? 0.0f : M;
+        s_stat[k][1] = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(a.p_bits) / L;
       }
     }
     __syncthreads();

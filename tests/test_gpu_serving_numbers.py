@@ -71,3 +71,42 @@ def test_f32_queries_of_any_size(native, kv, size, scale, keys):
     scale = float(np.float32(scale))
     out, _ = run_attention(native, pg, q, F32, 1, [1, 1], nh, scale)
     rows_near(out, attention_reference(pg, q, F32, 1, [1, 1], nh, scale, None)[0], F32)
+
+
+@pytest.mark.parametrize("kv", [F16, BF16])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** 13, 2.0 ** 40, 2.0 ** 80])
+def test_scores_of_any_size(native, kv, wide, scale):
+    """Scores from 1e4 to 1e32 in size, of either sign: the positions of the largest share the row (three, far
+    apart), the others are e^-64 or less beside them, and a row's weights add up to 1."""
+    rng = np.random.default_rng(83)
+    nh, n_kv, hd = 4, 2, 64
+    lens = [1200, 70, 333]
+    pg = Pages(rng, lens, 16, n_kv, hd, kv)
+    qt = F32 if wide else kv
+    best = {}
+    for s, n in enumerate(lens):
+        kb, vb = pg.get(s, np.arange(n))
+        k = np.zeros((n, n_kv, hd))
+        k[..., 0] = 1024 + 8 * rng.integers(1, 100, (n, n_kv))
+        for h in range(n_kv):
+            at = rng.permutation(n)[:6]
+            k[at[:3], h, 0], k[at[3:], h, 0] = 2040, 1024  # the largest, the smallest
+            best[s, h] = at[:3], at[3:]
+        pg.set(s, np.arange(n), to16(k, kv), vb)
+    q = np.zeros((3, nh, hd))
+    q[..., 0] = np.exp2(rng.integers(3, 15, (3, nh))) * [1, -1, 1, -1]
+    weights = np.zeros((3, n_kv, pg.cap), np.float32)
+    out, got_w = run_attention(native, pg, typed(q.reshape(3, -1), qt), qt, 1, [1] * 3, nh, scale, weights)
+    for s, n in enumerate(lens):
+        v = from16(pg.get(s, np.arange(n))[1], kv)
+        chain = (n / 32 + 64) * U  # with the weights' bits, 2^-22, and the exponentials', 2^-23
+        for h in range(nh):
+            at = best[s, h // 2][h % 2]
+            want = v[at, h // 2].mean(0)
+            tol = (chain + 2.0 ** -21) * np.abs(v[at, h // 2]).mean(0) + HALF_STEP[qt] * np.abs(want)
+            assert (np.abs(value(out[s], qt).reshape(nh, hd)[h] - want) <= tol).all(), (s, h)
+        for h in range(n_kv):
+            want = np.zeros(pg.cap)
+            want[np.r_[best[s, h]]] = 1 / 3
+            assert (np.abs(got_w[s, h] - want) <= chain + 2.0 ** -21).all(), (s, h)
