@@ -30,7 +30,8 @@
 // Numbers.  f32 queries are the sum of two f16 (22 bits) or of three bf16, a row scaled by a power of two
 // into their range, 16-bit queries are used as they are; the weights exp2(s - max) are the sum of
 // two f16 (22 bits) or of three bf16 (all 24 of them).  f16 weights carry a factor 2^14: a term's steps are
-// 2^-39 of the row's largest weight at least.
+// 2^-39 of the row's largest weight at least.  bf16 weights carry 2^-24: the sum over 2^24 positions at most
+// of values near the largest f32 stays below it (products below f32's subnormals vanish: 2^-126 of an output).
 #pragma once
 #include <type_traits>
 #include "kernels_paged.h"

@@ -256,7 +256,7 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   a.scores = weights ? reinterpret_cast<float*>(ws + z.scores) : nullptr;
   a.weights = weights;
   a.scale = scale;
-  a.p_bits = kv_type == TY_F16 ? 14.0f : 0.0f;
+  a.p_bits = kv_type == TY_F16 ? 14.0f : -24.0f;
   a.q_stride = q_stride;
   a.out_stride = out_stride;
   a.n_new = n_new;

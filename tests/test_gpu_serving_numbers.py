@@ -110,3 +110,33 @@ def test_scores_of_any_size(native, kv, wide, scale):
             want = np.zeros(pg.cap)
             want[np.r_[best[s, h]]] = 1 / 3
             assert (np.abs(got_w[s, h] - want) <= chain + 2.0 ** -21).all(), (s, h)
+
+
+@pytest.mark.parametrize("qt", [F32, BF16])
+@pytest.mark.parametrize("lens,new", [([70, 200, 1], [1, 1, 1]), ([3000, 1900, 40], [5, 2, 4])])
+def test_values_near_the_largest(native, qt, lens, new):
+    """Rows that average values of bf16's largest sizes: every one finite, whatever the number of positions."""
+    rng = np.random.default_rng(84)
+    nh, n_kv, hd = 8, 2, 128
+    pg = Pages(rng, lens, 16, n_kv, hd, BF16)
+    for s, n in enumerate(lens):
+        kb, vb = pg.get(s, np.arange(n))
+        pg.set(s, np.arange(n), to16(rng.normal(0, 0.1, (n, n_kv, hd)), BF16),
+               to16(rng.uniform(2.5e38, 3.3e38, (n, n_kv, hd)) * rng.choice([1, 1, -1], (1, n_kv, hd)), BF16))
+    n_new = max(new)
+    q = typed(rng.normal(0, 1, (len(lens) * n_new, nh * hd)), qt)
+    out, _ = run_attention(native, pg, q, qt, n_new, new, nh, 0.125)
+    ref = attention_reference(pg, q, qt, n_new, new, nh, 0.125, None)[0]
+    rows = [r for r in range(len(ref)) if ref[r] is not None]
+    rows_near(out[rows], [ref[r] for r in rows], qt)
+
+
+def test_values_near_the_smallest(native):
+    """bf16 values down to its smallest normal ones: off by f32's smallest normal number at most."""
+    rng = np.random.default_rng(85)
+    nh, n_kv, hd, lens = 8, 2, 64, [70, 1000]
+    pg = Pages(rng, lens, 16, n_kv, hd, BF16, rows=lambda *sh: rng.normal(0, 1, sh) * 2.0 ** -118)
+    q = typed(rng.normal(0, 1, (2, nh * hd)), F32)
+    out, _ = run_attention(native, pg, q, F32, 1, [1, 1], nh, 0.125)
+    for r, (y, tol) in enumerate(attention_reference(pg, q, F32, 1, [1, 1], nh, 0.125, None)[0]):
+        assert (np.abs(value(out[r], F32) - y) <= tol + 2.0 ** -126).all(), r
