@@ -2339,6 +2339,16 @@ int camelid_hip_verify(camelid_hip_engine* e, const float* embs, const float* co
   return 0;
 }
 
+// No NaN or +infinity, and something above -infinity.
+static bool has_distribution(const float* logits, uint32_t n) {
+  bool below = true, any = false;
+  for (uint32_t i = 0; i < n; ++i) {
+    below &= logits[i] < INFINITY;
+    any |= logits[i] > -INFINITY;
+  }
+  return below && any;
+}
+
 int camelid_hip_verify_sampled(camelid_hip_engine* e, const float* embs, const float* cos_all, const float* sin_all,
                                uint32_t base_position, uint32_t k, float scale, const uint32_t* draft_tokens,
                                const float* draft_logits, float temperature, const float* uniforms,
@@ -2379,6 +2389,10 @@ int camelid_hip_verify_sampled(camelid_hip_engine* e, const float* embs, const f
   if (verify_wait(e)) return 1;
   HIP_TRY(e, hipMemcpy(out, e->vs_out, sizeof out, hipMemcpyDeviceToHost));
   if (out[0] >= k || out[1 + out[0]] == 0xffffffffu) {
+    // the draft's row is the caller's: the forward and its K and V are sound
+    if (with_draft && temperature > 0.0f && out[0] < drafts &&
+        !has_distribution(draft_logits + (size_t)out[0] * vocab, vocab))
+      return fail(e, "verify: draft_logits without a distribution (NaN, +infinity or nothing above -infinity)");
     e->filled = 0;
     return fail(e, "verify: logits without a distribution (NaN or infinite)");
   }

@@ -128,7 +128,10 @@ int camelid_hip_verify(camelid_hip_engine* e, const float* embs, const float* co
  * [0, 1).  draft_logits (host, [k - 1][vocab]; NULL: each draft was certain): the drafts' own
  * distributions.  *accepted_out drafts are accepted; tokens_out [k] receives them, the token drawn
  * behind them, then 0xffffffff; logprobs_out (NULL: not told) [k] their log-probabilities.  k = 1
- * samples the next token.  filled is not changed: the caller sets it to base_position + 1 + accepted. */
+ * samples the next token.  filled is not changed: the caller sets it to base_position + 1 + accepted.
+ * A row of draft_logits that is needed (temperature > 0, no draft rejected before it) and holds NaN,
+ * +infinity or nothing above -infinity is an error that leaves filled as it was; logits of the model's
+ * own like that are one that sets it to 0. */
 int camelid_hip_verify_sampled(camelid_hip_engine* e, const float* embs, const float* cos_all, const float* sin_all,
                                uint32_t base_position, uint32_t k, float scale, const uint32_t* draft_tokens,
                                const float* draft_logits, float temperature, const float* uniforms,

@@ -140,3 +140,38 @@ def test_values_near_the_smallest(native):
     out, _ = run_attention(native, pg, q, F32, 1, [1, 1], nh, 0.125)
     for r, (y, tol) in enumerate(attention_reference(pg, q, F32, 1, [1, 1], nh, 0.125, None)[0]):
         assert (np.abs(value(out[r], F32) - y) <= tol + 2.0 ** -126).all(), r
+
+
+def test_bad_draft_logits_leave_the_engine_as_it_was(native):
+    """A draft's row of logits without a distribution is the caller's mistake: refused, nothing of the engine's
+    cache lost.  Rows that are not needed (T = 0, drafts behind a rejected one) may hold anything."""
+    from camelid_amd._native import HipError
+    from camelid_amd.model import ResidentSession, SyntheticModel, prompt_tokens, rope_tables, tiny_config
+    cfg = tiny_config(prompt_len=12)
+    model = SyntheticModel.generate(cfg)
+    sess = ResidentSession(model, 32)
+    prompt = prompt_tokens(cfg)
+    sess.prefill(prompt[:-1])
+    eng, base = sess.engine, len(prompt) - 1
+    step = [int(prompt[-1]), 3, 5]
+    cos, sin = rope_tables(cfg, base, 3)
+
+    def call(draft_logits, temp=1.0, u=(0.4, 0.5, 0.6)):
+        return [x.tolist() for x in eng.verify_sampled(model.embed(step), cos, sin, base, cfg.scale(), step[1:], u, temp,
+                                                       draft_logits)]
+
+    good = np.random.default_rng(86).normal(0, 1, (2, cfg.vocab)).astype(np.float32)
+    want = call(good)
+    for bad in (np.nan, np.inf, -np.inf):
+        rows = good.copy()
+        rows[0, slice(None) if bad == -np.inf else 7] = bad
+        with pytest.raises(HipError, match="draft_logits"):
+            call(rows)
+        assert eng.filled() == base and call(good) == want
+        assert call(rows, temp=0.0) == call(None, temp=0.0)
+    rows = good.copy()
+    rows[0, 3] = 1e4          # the first draft certain of itself: rejected by any number above its probability
+    rows[1, 9] = np.nan
+    assert len(call(rows, u=(0.9999, 0.5, 0.6))[0]) == 1
+    assert eng.filled() == base and call(good) == want
+    sess.close()
