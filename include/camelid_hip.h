@@ -408,13 +408,26 @@ int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new,
 /* Attention of the new tokens (1..=CAMELID_MAX_VERIFY_K per sequence) over the cache, their own
  * positions included: out[row][h] = sum_p softmax_p(scale q[row][h].k_p) v_p over p <= the row's
  * position, query head h reading KV head h / (n_heads / n_kv).  q and out: rows of q_stride and
- * out_stride elements (multiples of 16 bytes) of q_type (CAMELID_F32 or the cache's type).  Scores,
- * softmax and sums are f32.  K and V of masked positions, whatever their bits, do not reach a row.
+ * out_stride elements (multiples of 16 bytes) of q_type (CAMELID_F32 or the cache's type).  Softmax
+ * statistics and all sums are f32.  Both products are on matrix cores, whose operands are 16 bits wide:
+ * 16-bit q, K and V enter as they are; f32 q as two f16 (22 bits) or three bf16 (24), by the cache's
+ * type; softmax weights likewise as two f16 (22 bits, or 2^-39 of the row's largest weight) or three
+ * bf16.  Results take one more rounding to q_type.  K and V of masked positions, whatever their bits,
+ * do not reach a row.
  * weights (NULL: not kept): f32 [n_seqs][n_kv][table_stride * page_size]; every cached position's
  * softmax weights, summed over the sequence's new tokens and the KV head's query heads, are added to
- * it (a new token's own position starts at 0).  n_heads * n_new row sums are taken in a fixed order:
- * the same call gives the same bits.
- * An infinity or NaN in K or V that a row does see makes that row's outputs infinite or NaN.
+ * it (a new token's own position starts at 0).  Drafts count with the rest: attention comes before
+ * anyone knows which are accepted, and the weight that rejected ones gave to earlier positions stays
+ * (their own positions start at 0 again with the next call's tokens).  A caller that wants accepted
+ * tokens alone keeps weights only in calls without drafts.  n_heads * n_new row sums are taken in a
+ * fixed order: the same call gives the same bits.
+ * A NaN in K, and an infinity or NaN in V, that a row does see makes that row's outputs (of V: in that
+ * dim) infinite or NaN.  An infinity in K makes them NaN where its score is +infinity; where it is
+ * -infinity the position weighs nothing with 16-bit q, and with f32 q, whose terms are multiplied one by
+ * one, either that or NaN.
+ * The call reads all lens in every workgroup, and its workspace with weights holds
+ * n_seqs * n_heads * n_new * table_stride * page_size scores of 4 bytes: it goes by the tables' room, not
+ * by the lengths, as a captured graph needs it.
  * _workspace: bytes for calls with this n_heads, n_kv and hd and at most the other sizes (with_weights:
  * weights != NULL). */
 size_t camelid_hip_paged_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
@@ -429,11 +442,12 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
 /* Eviction by accumulated attention weight, in place: a sequence of lens[s] > keep positions keeps,
  * for each KV head on its own, its last `recent` positions (recent <= keep) and the keep - recent of
  * highest weights[s][head][p] among the others (of equal weights the lower position; NaN lowest),
- * in their order, K, V and weights moved to positions [0, keep); lens_out[s] = min(lens[s], keep)
- * (lens_out may be lens).  kept (NULL: not told) [n_seqs][n_kv][keep]: the positions kept, entries
- * from lens_out[s] on untouched.  Cache positions and weights from keep on keep their bits.  Pages of
- * the evicted sequences must belong to one table entry each.  _workspace: bytes for calls of at most
- * these sizes (keep counts, page_size and table_stride do not). */
+ * in their order, K, V and weights moved to positions [0, keep); lens_out[s] = min(lens[s], keep), or
+ * lens[s] for a sequence that a bad page or length keeps as it is (lens_out may be lens).  kept (NULL:
+ * not told) [n_seqs][n_kv][keep]: the positions kept, entries from lens_out[s] on untouched.  Cache
+ * positions and weights from keep on keep their bits.  Pages of the evicted sequences must belong to one
+ * table entry each.  _workspace: bytes for calls of at most these sizes (keep counts, page_size and
+ * table_stride do not). */
 size_t camelid_hip_paged_evict_workspace(uint32_t n_seqs, uint32_t n_kv, uint32_t page_size, uint32_t table_stride,
                                          uint32_t keep);
 int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_size, uint32_t n_kv, uint32_t hd,
@@ -449,7 +463,8 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
  * accepted while u_t q_t(x_t) < p_t(x_t); the token behind the accepted ones is the smallest i with
  * C_i > u_last S, C the prefix sums and S the sum of max(p_t - q_t, 0) at the first rejected draft
  * (of p_t where nothing is left), of p_n behind the last draft.  T = 0 (or below, or NaN): the
- * argmax, lowest index of equals, accepts and replaces.  Exponentials and sums are f64.
+ * argmax, lowest index of equals, accepts and replaces.  Sums are f64, of exponentials that are right
+ * to 1.6e-13 relative: a number closer than that to a border may fall on either side of it.
  * accepted[s]: drafts accepted; tokens_out [n_seqs][n_draft + 1]: these, the drawn token, then
  * 0xffffffff; logprobs_out (NULL: not told) [n_seqs][n_draft + 1]: the natural log of p of each of
  * these tokens (T = 0: of softmax(target)), then 0.  n_draft = 0 samples one token per sequence;

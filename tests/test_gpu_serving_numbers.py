@@ -175,3 +175,31 @@ def test_bad_draft_logits_leave_the_engine_as_it_was(native):
     assert len(call(rows, u=(0.9999, 0.5, 0.6))[0]) == 1
     assert eng.filled() == base and call(good) == want
     sess.close()
+
+
+@pytest.mark.parametrize("kv", [F16, BF16])
+def test_infinite_keys_of_16_bit_rows(native, kv):
+    """An infinity in K that a row sees: a weight of zero where it makes the score -infinity, NaN where
+    +infinity, whichever of its sequence's tiles it is in; not seen by a row: nothing."""
+    rng = np.random.default_rng(87)
+    nh, n_kv, hd, m = 8, 2, 64, 3
+    lens = [45, 45, 700, 700]
+    at = [10, 43, 5, 698]  # the last but one of the new tokens' positions: seen by two of the three rows
+    pg = Pages(rng, lens, 16, n_kv, hd, kv)
+    q = rng.normal(0, 1, (4 * m, nh, hd))
+    q[:, :4, 3], q[:, 4:, 3] = -np.abs(q[:, :4, 3]) - 0.1, np.abs(q[:, 4:, 3]) + 0.1  # KV head 0 below zero, 1 above
+    q = typed(q.reshape(4 * m, -1), kv)
+    for s, p in enumerate(at):
+        kb, vb = pg.get(s, [p])
+        kb[0, :, 3] = 0x7C00 if kv == F16 else 0x7F80
+        pg.set(s, [p], kb, vb)
+    out, _ = run_attention(native, pg, q, kv, m, [m] * 4, nh, 0.125)
+    masked = attention_reference(pg, q, kv, m, [m] * 4, nh, 0.125, None, {(s, p) for s, p in enumerate(at)})[0]
+    for s, p in enumerate(at):
+        for t in range(m):
+            got = value(out[s * m + t], kv).reshape(nh, hd)
+            y, tol = (z.reshape(nh, hd) for z in masked[s * m + t])
+            sees = p <= lens[s] - m + t
+            near = np.abs(got - y) <= tol + HALF_STEP[kv] * (np.abs(y) + tol) + 2.0 ** -25
+            assert near[:4].all(), (s, t)
+            assert np.isnan(got[4:]).all() if sees else near[4:].all(), (s, t)
