@@ -4,11 +4,11 @@
 //
 // Bound: the cache's bytes (4 hd per position and KV head, against 4 hd flop per position and row),
 // so the kernel's work is to keep HBM busy whatever the batch looks like.  Heads of 128:
-//   4 sequences of 65536, 32 + 8 heads: 166 + 5 us (split + join), 6.3 TB/s
-//   64 of up to 4001, 24 + 8 heads: 90 + 5 us, 5.7 TB/s
-//   1 of 8199, 32 + 8 heads: 9.6 + 4.4 us for 34 MB: latency (launch 1, plan 1.2, pages 0.6, K and V and
+//   4 sequences of 65536, 32 + 8 heads: 165 + 5 us (split + join), 6.5 TB/s in the split
+//   64 of up to 4001, 24 + 8 heads: 90 + 5 us, 6.0 TB/s
+//   1 of 8199, 32 + 8 heads: 9.4 + 4.3 us for 34 MB: latency (launch 1, plan 1.2, pages 0.6, K and V and
 //     the query operands 2, products and softmax 1.4, states joined and written 1.3, then the join's launch)
-//   16 of up to 1100, up to 5 new tokens, weights kept: 17.5 + 6.2 us for 39 MB: the same, two tiles a wave
+//   16 of up to 1100, up to 5 new tokens, weights kept: 16.8 + 6.4 us for 39 MB: the same, two tiles a wave
 //
 // Split.  A segment is (sequence, KV head, block of 16 NR query rows); its tiles are 32 positions.
 // The query rows are the new tokens times the KV head's query heads, so K and V are read once for
