@@ -464,7 +464,9 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
  * C_i > u_last S, C the prefix sums and S the sum of max(p_t - q_t, 0) at the first rejected draft
  * (of p_t where nothing is left), of p_n behind the last draft.  T = 0 (or below, or NaN): the
  * argmax, lowest index of equals, accepts and replaces.  Sums are f64, of exponentials that are right
- * to 1.6e-13 relative: a number closer than that to a border may fall on either side of it.
+ * to 1.6e-13 relative: a number closer than that to a border may fall on either side of it, and where p_t
+ * and q_t agree to 1e-12 or so, what is left of their difference behind a rejected draft is rounding (a
+ * draft drawn from q_t is rejected there once in as many draws).
  * accepted[s]: drafts accepted; tokens_out [n_seqs][n_draft + 1]: these, the drawn token, then
  * 0xffffffff; logprobs_out (NULL: not told) [n_seqs][n_draft + 1]: the natural log of p of each of
  * these tokens (T = 0: of softmax(target)), then 0.  n_draft = 0 samples one token per sequence;
