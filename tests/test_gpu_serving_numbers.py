@@ -203,3 +203,17 @@ def test_infinite_keys_of_16_bit_rows(native, kv):
             near = np.abs(got - y) <= tol + HALF_STEP[kv] * (np.abs(y) + tol) + 2.0 ** -25
             assert near[:4].all(), (s, t)
             assert np.isnan(got[4:]).all() if sees else near[4:].all(), (s, t)
+
+
+@pytest.mark.parametrize("qt", [F32, F16])
+def test_subnormal_keys_and_values(native, qt):
+    """f16 K and V below its smallest normal number count with all their bits."""
+    rng = np.random.default_rng(88)
+    nh, n_kv, hd, lens = 8, 2, 64, [70, 1000]
+    pg = Pages(rng, lens, 16, n_kv, hd, F16, rows=lambda *sh: rng.normal(0, 1, sh) * 2.0 ** -17)
+    q = typed(rng.normal(0, 1, (2, nh * hd)) * 256, qt)
+    scale = 2.0 ** 6  # scores near 1
+    out, _ = run_attention(native, pg, q, qt, 1, [1, 1], nh, scale)
+    for r, (y, tol) in enumerate(attention_reference(pg, q, qt, 1, [1, 1], nh, scale, None)[0]):
+        half = np.maximum(HALF_STEP[qt] * np.abs(y), 2.0 ** -25 if qt == F16 else 0.0)  # (f16 results are subnormal)
+        assert (np.abs(value(out[r], qt) - y) <= tol + half).all(), r
