@@ -334,7 +334,10 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
         for (int i = 0; i < 8; ++i) top = max(top, f2u(raw[k][i]) & 0x7fffffffu);
         const int ex = (int)(pa_group_max<LPR>(top) >> 23) - 127;
         if (ex < 128) up = KT == TY_F16 ? 13 - ex : max(-64, min(64, ex)) - ex;
-        // (a factor beyond f32: the scores' differences are past exp's range with the largest one as well)
+        // a scale so large that log2(e) takes it beyond f32: 4 of it go to the row (whose products with keys of
+        // bf16 may be as small as they like)
+        if (KT == TY_BF16 && ex < 128 && fabsf(a.scale) > 0x1p126f) up += 2;
+        // (other factors beyond f32: the scores' differences are past exp's range with the largest one as well)
         factor = fmaxf(PA_LOWEST, fminf(-PA_LOWEST, ldexpf(a.scale, -up) * PA_LOG2E));
       }
       v8 term[NQ];

@@ -228,6 +228,8 @@ int camelid_hip_paged_attention(const void* q, uint32_t q_type, uint32_t q_strid
   if (q_type != TY_F32 && q_type != kv_type)
     return cm::fail_global(me, "16-bit q rows must have the cache's type");
   if (!std::isfinite(scale)) return cm::fail_global(me, "attention score scale must be finite");
+  if (q_type != TY_F32 && !std::isfinite(scale * cm::PA_LOG2E))
+    return cm::fail_global(me, "scale times log2(e) must be finite for 16-bit q rows");
   const uint64_t groups = (uint64_t)n_seqs * n_kv * (n_new * (n_heads / n_kv) + (weights ? 1 + ((uint64_t)table_stride * page_size >> 6) : 0));
   if (!grid_ok(groups, cm::PA_NT)) return cm::fail_global(me, "too many rows in one call");
   const uint32_t unit = q_type == TY_F32 ? 4 : 8;

@@ -412,8 +412,8 @@ int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new,
  * statistics and all sums are f32.  Both products are on matrix cores, whose operands are 16 bits wide:
  * 16-bit q, K and V enter as they are; f32 q as two f16 (22 bits) or three bf16 (24), by the cache's
  * type; softmax weights likewise as two f16 (22 bits, or 2^-39 of the row's largest weight) or three
- * bf16.  Results take one more rounding to q_type.  K and V of masked positions, whatever their bits,
- * do not reach a row.
+ * bf16.  For 16-bit q scale times log2(e) has to be finite, too.  Results take one more rounding to
+ * q_type.  K and V of masked positions, whatever their bits, do not reach a row.
  * weights (NULL: not kept): f32 [n_seqs][n_kv][table_stride * page_size]; every cached position's
  * softmax weights, summed over the sequence's new tokens and the KV head's query heads, are added to
  * it (a new token's own position starts at 0).  Drafts count with the rest: attention comes before

@@ -73,6 +73,24 @@ def test_f32_queries_of_any_size(native, kv, size, scale, keys):
     rows_near(out, attention_reference(pg, q, F32, 1, [1, 1], nh, scale, None)[0], F32)
 
 
+@pytest.mark.parametrize("scale", [1.0, 2.3e38, 3e38, -3.4e38])
+def test_scales_near_the_largest(native, scale):
+    """f32 rows with every finite scale: keys so small that the scores are near 1."""
+    rng = np.random.default_rng(89)
+    nh, n_kv, hd, lens = 4, 2, 64, [70, 300]
+    pg = Pages(rng, lens, 16, n_kv, hd, BF16)
+    for s, n in enumerate(lens):
+        k = np.zeros((n, n_kv, hd))
+        k[..., 0] = (1 + rng.integers(0, 128, (n, n_kv)) / 128) * 2.0 ** -125 * (3e38 if scale == 1.0 else 1.0)
+        pg.set(s, np.arange(n), to16(k, BF16), pg.get(s, np.arange(n))[1])
+    q = np.zeros((2, nh, hd), np.float32)
+    q[..., 0] = rng.choice([0.5, 1.0], (2, nh)) * rng.choice([1, -1], (2, nh))
+    q = q.reshape(2, -1)
+    scale = float(np.float32(scale))
+    out, _ = run_attention(native, pg, q, F32, 1, [1, 1], nh, scale)
+    rows_near(out, attention_reference(pg, q, F32, 1, [1, 1], nh, scale, None)[0], F32)
+
+
 @pytest.mark.parametrize("kv", [F16, BF16])
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("scale", [1.0, 2.0 ** 13, 2.0 ** 40, 2.0 ** 80])

@@ -75,6 +75,16 @@ def test_verify_refuses(native, change, match):
         _check(native.camelid_hip_verify_drafts(*{**VERIFY, **change}.values()))
 
 
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38])
+@pytest.mark.parametrize("kind", [1, 2])
+def test_attention_refuses_scales_beyond_the_exponent_of_16_bit_rows(native, scale, kind):
+    """Scores are taken in powers of two: for 16-bit q scale times log2(e) has to be an f32 too."""
+    from camelid_amd._native import HipError
+    change = {"scale": scale, "q_type": kind, "kv_type": kind}
+    with pytest.raises(HipError, match="paged_attention: .*log2"):
+        _check(native.camelid_hip_paged_attention(*{**ATTN, **change}.values()))
+
+
 def test_empty_calls_do_nothing(native):
     """No sequences, or no new tokens: success without a launch."""
     _check(native.camelid_hip_paged_rope_kv(*{**ROPE, "n_seqs": 0}.values()))
