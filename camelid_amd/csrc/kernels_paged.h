@@ -575,8 +575,8 @@ __global__ __launch_bounds__(NT) void k_evict_select(Paged g, float* __restrict_
 // written.  A source is never below its output position, so no later chunk misses a row.  A workgroup takes
 // as many dims as leave all kept rows one chunk (ks, vs; 95 x 8 x 22 of up to 78 rows: 25 -> 8.4 us against 8
 // dims of K and 16 of V), and where there are few workgroups larger chunks (F; 8 x 14511 of 20144 rows of
-// one of two sequences: 40 -> 36 us).  Bound: HBM: 16 x 8 x 1024 of 1088 rows of 128 dims 26.6 us, 83 MB of lines read and 67 written,
-// 5.6 TB/s; 4 x 8 x 2048 of up to 16383 rows 19 us, where rows far apart share their 128-byte lines with rows that
+// one of two sequences: 40 -> 36 us).  Bound: HBM: 16 x 8 x 1024 of 1088 rows of 128 dims 26.6 us, 83 MB of
+// lines read and 67 written, 5.6 TB/s; 4 x 8 x 2048 of up to 16383 rows 19 us, where rows far apart share their 128-byte lines with rows that
 // are left behind (68 MB of lines read for the 34 MB that are written).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 

@@ -14,9 +14,10 @@
 // Bound: every row's logits read once (k_vd_stats: a wave per 2048 of them, its maximum and its sum of
 // exponentials; no barriers behind the loads).  139 MB of f32 logits (32 sequences with up to 5 drafts of a
 // draft model, 151936 tokens) take 31.6 us, 4.4 TB/s; 20 VALU instructions a logit, 9 of them f64, are
-// active in 78 % of the CUs' busy cycles, and 44 M logits take 35 us in bf16 as in f32 (83 %).  Only sequences that rejected a draft of a draft model read two rows again for max(p - q, 0)
-// (k_vd_rest, spread over the chip like the first pass: 15 us there); otherwise the shares' sums are known.
-// k_vd_pick then needs one share's logits: latency (7 us there and for one sequence without a draft model).
+// active in 78 % of the CUs' busy cycles, and 44 M logits take 35 us in bf16 as in f32 (83 %).  Only
+// sequences that rejected a draft of a draft model read two rows again for max(p - q, 0) (k_vd_rest, spread
+// over the chip like the first pass: 15 us there); otherwise the shares' sums are known.  k_vd_pick then needs
+// one share's logits: latency (7 us there and for one sequence without a draft model).
 // Rest and pick as one launch, the draw by the sequence's last workgroup, took 47 us: its fences write back
 // and invalidate the L2.
 #pragma once

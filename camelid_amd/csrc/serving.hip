@@ -340,8 +340,8 @@ int camelid_hip_paged_evict(void* kc, void* vc, uint32_t n_pages, uint32_t page_
                        static_cast<uint16_t*>(kc), static_cast<uint16_t*>(vc), keep, plan, lens_out, ks, vs);
     return launched(me);
   };
-  // few workgroups (one or two a CU) with many rows take them in larger chunks (8 x 14511 rows of one of two sequences: 73 us
-  // for the call against 78, 1 x 8 x 14027: 56 against 59)
+  // few workgroups (one or two a CU) with many rows take them in larger chunks (8 x 14511 rows of one of two
+  // sequences: 73 us for the call against 78, 1 x 8 x 14027: 56 against 59)
   if (!ks && !vs && movers <= 256) return go(cm::k_evict_move<4>, 4);
   if (!ks && !vs && movers <= 512) return go(cm::k_evict_move<2>, 2);
   return go(cm::k_evict_move<1>, 1);
