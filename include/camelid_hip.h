@@ -425,7 +425,8 @@ int camelid_hip_paged_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new,
  * dim) infinite or NaN.  An infinity in K makes them NaN where its score is +infinity; where it is
  * -infinity the position weighs nothing with 16-bit q, and with f32 q, whose terms are multiplied one by
  * one, either that or NaN.
- * The call reads all lens in every workgroup, and its workspace with weights holds
+ * The call reads all lens in every workgroup (meant for up to a few thousand sequences; more than 65535
+ * are refused), and its workspace with weights holds
  * n_seqs * n_heads * n_new * table_stride * page_size scores of 4 bytes: it goes by the tables' room, not
  * by the lengths, as a captured graph needs it.
  * _workspace: bytes for calls with this n_heads, n_kv and hd and at most the other sizes (with_weights:

@@ -85,6 +85,13 @@ def test_attention_refuses_scales_beyond_the_exponent_of_16_bit_rows(native, sca
         _check(native.camelid_hip_paged_attention(*{**ATTN, **change}.values()))
 
 
+def test_attention_refuses_batches_that_its_plan_cannot_serve(native):
+    """Every workgroup reads all lengths: batches whose plan alone takes seconds are refused."""
+    from camelid_amd._native import HipError
+    with pytest.raises(HipError, match="paged_attention: .*65535 sequences"):
+        _check(native.camelid_hip_paged_attention(*{**ATTN, "n_seqs": 65536}.values()))
+
+
 def test_empty_calls_do_nothing(native):
     """No sequences, or no new tokens: success without a launch."""
     _check(native.camelid_hip_paged_rope_kv(*{**ROPE, "n_seqs": 0}.values()))
