@@ -161,6 +161,30 @@ SIGNATURES: dict[str, tuple] = {
     "camelid_hip_verify_drafts_workspace": (C.c_size_t, [C.c_uint32] * 3),
     "camelid_hip_verify_drafts": (C.c_int, [vp, vp, C.c_uint32, vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, vp, vp,
                                             vp, vp, vp, vp, C.c_size_t, vp]),
+    "camelid_hip_paged8_rope_kv": (C.c_int, [vp, C.c_uint32, C.c_uint32, vp, C.c_uint32, C.c_uint32, C.c_uint32,
+                                             C.c_uint32, C.c_uint32, vp, vp, vp, vp, C.c_float, vp, C.c_uint32, vp,
+                                             vp, vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp, vp,
+                                             vp]),
+    "camelid_hip_paged8_read": (C.c_int, [vp, vp, vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                          vp, C.c_uint32, vp, C.c_uint32, vp, vp, C.c_uint32, C.c_uint32, vp, vp]),
+    "camelid_hip_paged8_attention_workspace": (C.c_size_t, [C.c_uint32] * 7),
+    "camelid_hip_paged8_attention": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, C.c_uint32,
+                                               C.c_uint32, C.c_uint32, vp, vp, vp, vp, C.c_uint32, C.c_uint32,
+                                               C.c_uint32, vp, C.c_uint32, vp, C.c_float, vp, C.c_uint32, vp,
+                                               C.c_size_t, vp, vp]),
+    "camelid_hip_pages_reserve_workspace": (C.c_size_t, [C.c_uint32] * 2),
+    "camelid_hip_pages_reserve": (C.c_int, [vp, C.c_uint32, vp, C.c_uint32, vp, vp, C.c_uint32, vp, C.c_uint32, vp,
+                                            C.c_uint32, vp, vp, vp, C.c_size_t, vp, vp]),
+    "camelid_hip_pages_fork": (C.c_int, [vp, C.c_uint32, vp, C.c_uint32, vp, vp, C.c_uint32, vp, C.c_uint32, vp,
+                                         C.c_uint32, vp, vp]),
+    "camelid_hip_pages_compact_workspace": (C.c_size_t, [C.c_uint32]),
+    "camelid_hip_pages_compact": (C.c_int, [vp, C.c_uint32, vp, C.c_uint32, vp, C.c_uint32, vp, vp, vp, C.c_uint32,
+                                            vp, vp, vp, C.c_size_t, vp, vp]),
+    "camelid_hip_pages_copy": (C.c_int, [C.POINTER(vp), C.POINTER(C.c_size_t), C.c_uint32, C.c_uint32, vp,
+                                         C.c_uint32, vp, vp, vp]),
+    "camelid_hip_adjust_logits": (C.c_int, [vp, C.c_size_t, vp, C.c_size_t, C.c_uint32, C.c_uint32, C.c_uint32,
+                                            C.c_uint32, vp, C.c_size_t, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_uint32,
+                                            vp, vp, C.c_size_t, vp]),
     "camelid_hip_verify_sampled": (C.c_int, [vp, f32p, f32p, f32p, C.c_uint32, C.c_uint32, C.c_float, u32p, f32p,
                                              C.c_float, f32p, u32p, u32p, f32p]),
     "camelid_hip_inorder_sum_rows": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, vp]),

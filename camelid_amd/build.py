@@ -18,7 +18,7 @@ LIB_DIR = PKG / "_lib"
 BUILD_DIR = PKG / "_build"
 LIB = LIB_DIR / "libcamelid_hip.so"
 
-HIP_SOURCES = ["engine.hip", "serving.hip"]
+HIP_SOURCES = ["engine.hip", "serving.hip", "serving8.hip"]
 HOST_SOURCES = ["seam.cpp", "synth.cpp", "gguf.cpp"]
 
 HIPCC_FLAGS = [

@@ -481,6 +481,122 @@ int camelid_hip_verify_drafts(const void* target, const void* draft_logits, uint
                               uint32_t* accepted, uint32_t* tokens_out, float* logprobs_out, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * The same cache held in 8 bits (no reference counterpart).  kc and vc hold n_pages pages of page_size
+ * positions (a power of two, 16..=4096), elements of kv_type (CAMELID_I8 or CAMELID_E4M3, the 4-bit exponent 3-bit
+ * mantissa format without infinities).  K of one page is [n_kv][hd / 16][page_size][16] bytes, V is
+ * [n_kv][page_size / 16][hd][16].  A block is 16 positions (from a multiple of 16 on) of one KV head; k_exp and
+ * v_exp [n_pages][n_kv][page_size / 16] hold a byte b for each block of K and of V: an element is its 8-bit number
+ * times 2^(b - 127), NaN where b is 255.  Everything else (new tokens, lengths, tables, status, streams,
+ * workspaces, alignment of 16 bytes) is as in the 16-bit calls above; the exponents need no alignment. */
+enum { CAMELID_I8 = 3, CAMELID_E4M3 = 4 };
+
+/* camelid_hip_paged_rope_kv for this cache (the same q rows, q_out of any type): the exponent of a block is the smallest
+ * with which the largest of the block's new elements is at most 127 (CAMELID_I8) or 448 (CAMELID_E4M3), -126 at
+ * least, 121 (119) at most, which leaves f32's last binade to saturate; elements are rounded to the nearest, ties
+ * to even.  Where the block begins before the new tokens and its exponent is larger, that one stays; where it is
+ * smaller, the earlier positions are rounded to the new one (CAMELID_E4M3: exactly, but for subnormals).  The exponent of
+ * drafts that are rejected later stays until the block is stored to from its first position again.  A NaN or infinity
+ * among the new elements makes the block's exponent 255: all of its positions read as NaN.  Bytes of positions
+ * outside [0, lens[s]) stay.  No two sequences of a call may store into the same block. */
+int camelid_hip_paged8_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new, const uint32_t* new_lens,
+                               uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t rope_dim, uint32_t split_half,
+                               const float* cos_tab, const float* sin_tab, const float* q_norm, const float* k_norm,
+                               float eps, void* q_out, uint32_t q_type, void* kc, void* vc, uint8_t* k_exp,
+                               uint8_t* v_exp, uint32_t kv_type, uint32_t n_pages, uint32_t page_size,
+                               const uint32_t* table, uint32_t table_stride, const uint32_t* lens, uint32_t* status,
+                               void* stream);
+/* K and V of each sequence as rows: k_out and v_out [n_seqs][n_kv][out_positions][hd] of out_type (CAMELID_F32, _F16 or
+ * _BF16), positions from 0 to min(lens[s], out_positions); later rows are left as they are, and so are 16 rows whose
+ * page is none. */
+int camelid_hip_paged8_read(const void* kc, const void* vc, const uint8_t* k_exp, const uint8_t* v_exp,
+                            uint32_t kv_type, uint32_t n_pages, uint32_t page_size, uint32_t n_kv, uint32_t hd,
+                            const uint32_t* table, uint32_t table_stride, const uint32_t* lens, uint32_t n_seqs,
+                            void* k_out, void* v_out, uint32_t out_type, uint32_t out_positions, uint32_t* status,
+                            void* stream);
+/* camelid_hip_paged_attention for this cache, without weights, for any number of new tokens (whole prompts too) and
+ * q rows of any type. */
+size_t camelid_hip_paged8_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
+                                              uint32_t hd, uint32_t page_size, uint32_t table_stride);
+int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stride, uint32_t n_seqs, uint32_t n_new,
+                                 const uint32_t* new_lens, uint32_t n_heads, uint32_t n_kv, uint32_t hd, const void* kc,
+                                 const void* vc, const uint8_t* k_exp, const uint8_t* v_exp, uint32_t kv_type,
+                                 uint32_t n_pages, uint32_t page_size, const uint32_t* table, uint32_t table_stride,
+                                 const uint32_t* lens, float scale, void* out, uint32_t out_stride, void* workspace,
+                                 size_t workspace_bytes, uint32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Who holds which page (no reference counterpart), for caches of either kind.  Row s of table [n_seqs][table_stride]
+ * names held[s] pages; refs[p] counts the entries that name page p, 0 means free.  A caller starts with held and refs
+ * zero and leaves the three to these calls, which keep them consistent; on inconsistent ones results have no
+ * meaning, but no memory outside the buffers is touched.  All results are whole numbers in a fixed order.
+ * Status bits beside the two above: CAMELID_PAGED_NO_PAGE, CAMELID_PAGED_BAD_FORK.  n_pages < 2^31, n_seqs *
+ * table_stride < 2^31, n_seqs <= 2^20.  Streams, capture and workspaces as above. */
+enum { CAMELID_PAGED_NO_PAGE = 4, CAMELID_PAGED_BAD_FORK = 8 };
+
+/* Rows made as long as they have to be, and their own where they are about to be written.  Sequence s is to hold the
+ * pages of lens[s] positions; positions [first[s], lens[s]) are going to be stored (first NULL: none).  First
+ * every row gives back the entries it has beyond that (lens[s] = 0 frees a sequence).  Then it needs a page for every
+ * entry that it lacks, and for every entry of the positions to be stored whose page other rows hold, too: the k-th page
+ * needed, in the order of sequences and entries, is the k-th free page in ascending order, replaced ones first in
+ * a row.  pairs [max_pairs][2] and *n_pairs (first NULL: may be NULL): (old, new) of the replaced ones in the same
+ * order, for camelid_hip_pages_copy; the old ones lose this holder behind the call's other steps, so
+ * that rows which share a page and all write to it all get copies, and it is free behind the call.
+ * A sequence for which the free pages, counted with all sequences' needs up to its own, or the room in pairs, counted
+ * alike, do not suffice gets no page, keeps the rest, and sets CAMELID_PAGED_NO_PAGE; granted[s] (NULL: not told) is 1 for the
+ * others (also where nothing was needed).  A row with held[s] or the length beyond table_stride or a page >= n_pages
+ * among its entries is left alone, with granted 0 and status as above. */
+size_t camelid_hip_pages_reserve_workspace(uint32_t n_seqs, uint32_t n_pages);
+int camelid_hip_pages_reserve(uint32_t* table, uint32_t table_stride, uint32_t* held, uint32_t n_seqs,
+                              const uint32_t* first, const uint32_t* lens, uint32_t page_size, uint32_t* refs,
+                              uint32_t n_pages, uint32_t* pairs, uint32_t max_pairs, uint32_t* n_pairs,
+                              uint32_t* granted, void* workspace, size_t workspace_bytes, uint32_t* status,
+                              void* stream);
+/* Sequence children[i] (which holds nothing) gets the pages of parents[i], those of lens[parents[i]] positions at most
+ * (lens NULL: all).  A pair with an index >= n_seqs, a child that holds pages, is named in two pairs or is the parent of any
+ * pair, does nothing and sets CAMELID_PAGED_BAD_FORK; one whose parent's row is bad, nothing, with the status above. */
+int camelid_hip_pages_fork(uint32_t* table, uint32_t table_stride, uint32_t* held, uint32_t n_seqs,
+                           const uint32_t* parents, const uint32_t* children, uint32_t n_forks, const uint32_t* lens,
+                           uint32_t page_size, uint32_t* refs, uint32_t n_pages, uint32_t* status, void* stream);
+/* Pages in use moved to the front of the pool: of n_live pages in use the i-th highest that is not below n_live goes to
+ * the i-th lowest free one that is, max_pairs of them at most.  pairs [max_pairs][2] and *n_pairs: (from, to), for
+ * camelid_hip_pages_copy; *extent (NULL: not told): all pages from there on are free now.  table_out
+ * and refs_out (which may be table and refs) get all entries and counts, moved ones changed. */
+size_t camelid_hip_pages_compact_workspace(uint32_t n_pages);
+int camelid_hip_pages_compact(const uint32_t* table, uint32_t table_stride, const uint32_t* held, uint32_t n_seqs,
+                              const uint32_t* refs, uint32_t n_pages, uint32_t* table_out, uint32_t* refs_out,
+                              uint32_t* pairs, uint32_t max_pairs, uint32_t* n_pairs, uint32_t* extent,
+                              void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
+/* Page pairs[i][1] becomes a copy of page pairs[i][0] in each buffer, for i < *n_pairs (a device word; NULL or more: max_pairs).
+ * buffers and page_bytes are host arrays, read before the call returns: device pointers to n_pages pages of
+ * page_bytes[b] bytes (K, V and exponents of every layer).  No page may be written by two pairs, or written by one and read by another.
+ * A pair that names no page is left out, with CAMELID_PAGED_BAD_PAGE. */
+int camelid_hip_pages_copy(void* const* buffers, const size_t* page_bytes, uint32_t n_buffers, uint32_t n_pages,
+                           const uint32_t* pairs, uint32_t max_pairs, const uint32_t* n_pairs, uint32_t* status,
+                           void* stream);
+
+/* Logits before camelid_hip_verify_drafts (no reference counterpart): rows t <= draft_lens[s] (NULL: all; others are
+ * padding) of logits [n_seqs][n_rows][in_stride] to out [n_seqs][n_rows][out_stride] of the same type (f32, f16 or bf16;
+ * out may be logits).  The text of row t is history[s][0 .. history_lens[s]) (NULL: history_stride; larger values
+ * count as that) and draft_tokens [n_seqs][n_rows - 1] before t (NULL: none); its first prompt_lens[s] tokens (NULL: 0)
+ * are the prompt.  For each token i < vocab, with c occurrences in the text behind the prompt:
+ *   x = x / repetition[s] where x > 0, else x * repetition[s], if i is in the text, prompt included;
+ *   x = x - frequency[s] * c, then x - presence[s], if c > 0;
+ *   x = x + bias, if i is in bias_tokens[s][0 .. bias_lens[s]) (of equal ones the last counts);
+ *   x = -infinity, if bit i % 32 of mask[s][t][i / 32] is 0, whatever x was.
+ * Each step is rounded in f32, the result to the logits' type.  NULL leaves a step out.  Tokens >= vocab in a list count
+ * for nothing.  A mask that leaves no token makes a row of -infinity, which verify_drafts answers with 0xffffffff.
+ * repetition, frequency, presence: f32 [n_seqs]; bias_tokens, bias_values (f32): [n_seqs][bias_stride]; mask: rows
+ * of mask_stride words.  n_rows <= 32, vocab <= 2^24, history_stride <= 2^28.  Asynchronous on `stream`, allocates
+ * nothing, may be captured. */
+int camelid_hip_adjust_logits(const void* logits, size_t in_stride, void* out, size_t out_stride, uint32_t logits_type,
+                              uint32_t n_seqs, uint32_t n_rows, uint32_t vocab, const uint32_t* history,
+                              size_t history_stride, const uint32_t* history_lens, const uint32_t* prompt_lens,
+                              const uint32_t* draft_tokens, const uint32_t* draft_lens, const float* repetition,
+                              const float* frequency, const float* presence, const uint32_t* bias_tokens,
+                              const float* bias_values, uint32_t bias_stride, const uint32_t* bias_lens,
+                              const uint32_t* mask, size_t mask_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
