@@ -1,77 +1,457 @@
 // kernels_paged8_attn.h -- attention of a sequence's newest tokens over an 8-bit cache in pages.
 //
 //   s_p = scale 2^ke(p) (q . k_p) for p <= the row's position;  w = softmax(s);  o = sum_p w_p 2^ve(p) v_p
+//
+// The plan (segments of a sequence, KV head and block of query rows, cut into pieces of tiles), the parts and
+// their join are those of kernels_paged_attn.h; tiles are 64 positions here.
+//
+// Operands.  Granules of 16 bytes become two operands of v_mfma_f32_16x16x32_f16 each: int8 as the low byte of the
+// f16 1024 + u, minus 1152, e4m3 by the conversion instruction, both exact.
+//   S^T = K Q^T: the dims of a step are 8 of a K granule for each lane group, the same ones of q.  The rows r of
+//   the four products of a tile are the positions 16 (r / 4) + 4 b + r % 4, so that lane group l / 16
+//   ends up with the 16 consecutive positions of one block: one exponent of K and V a lane.
+//   O^T = V^T P^T: those 16 positions are one V granule, two operands; P never leaves the lane.
+//
+// Numbers.  q: f32 and bf16 rows are scaled by a power of two into f16's range, f32 as the sum of two f16 (22
+// bits), bf16 and f16 as they are.  K's exponent goes to the scores in f32.  V's goes to the weights before
+// they become f16: the matrix cores see w 2^ve / 2^D, D the running maximum of (exponent of the block's largest
+// weight + ve) over the row, so that what is lost is measured against the largest contribution and not against the
+// largest weight.  D is kept relative to the softmax's reference; both are whole numbers and rescaling is exact.
 #pragma once
+#include <type_traits>
 #include "kernels_paged8.h"
+#include "kernels_paged_attn.h"
 
 namespace cm {
 
+constexpr uint32_t P8_TILE = 64;
+
 struct P8Args {
-  Paged8 c;
-  const void* q;
-  const uint32_t* new_lens;
-  void* out;
-  float scale;
-  uint32_t q_stride, out_stride, n_new, n_heads, group;
+  PaArgs a;  // kc and vc: bytes
+  const uint8_t* ke;
+  const uint8_t* ve;
 };
 
-// One wave per (row, head): a lane per position for the scores of 64 positions, a lane per dim for the sum.
-template <int HD, int KT, int QT>
-__global__ __launch_bounds__(64) void k_p8_rows(P8Args a) {
-  __shared__ float s_q[HD], s_w[64];
-  const Paged& g = a.c.g;
-  const uint32_t lane = threadIdx.x, head = blockIdx.x % a.n_heads, row = blockIdx.x / a.n_heads;
-  const uint32_t s = row / a.n_new, t = row - s * a.n_new, h = head / a.group;
-  uint32_t first, len;
-  if (!paged_rows(g, a.new_lens, a.n_new, s, &first, &len)) return;
-  if (first + t >= len) return;
-  const uint32_t seen = first + t + 1, mask = (1u << g.shift) - 1u;
-  for (uint32_t d = lane; d < HD; d += 64) s_q[d] = load_as_f32<QT>(a.q, (size_t)row * a.q_stride + (size_t)head * HD + d);
-  __syncthreads();
-  const uint32_t* tab = g.table + (size_t)s * g.stride;
-  float m = -INFINITY, l = 0.0f, o[HD / 64] = {};
-  for (uint32_t p0 = 0; p0 < seen; p0 += 64) {
-    const uint32_t p = p0 + lane, pg = p < seen ? tab[p >> g.shift] : 0u;
-    const bool here = p < seen && pg < g.n_pages;
-    if (p < seen && !here) paged_flag(g, PG_BAD_PAGE);
-    float x = -INFINITY;
-    if (here) {
-      const uint8_t* k = a.c.kc + p8_base(g, pg, h);
-      float dot = 0.0f;
-      for (uint32_t d = 0; d < HD; d += 4) {
-        float y[4];
-        p8_unpack4<KT>(*reinterpret_cast<const uint32_t*>(k + p8_k(g, p & mask, d)), y);
-        for (int i = 0; i < 4; ++i) dot += y[i] * s_q[d + i];
-      }
-      x = dot * p8_scale(a.c.ke[p8_exp(g, pg, h, p & mask)]) * a.scale;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes of a granule -> 16 f16, in order: two operands.
+template <int KT>
+__device__ __forceinline__ void p8_operands(u32x4 u, f16x8 (&to)[2]) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  union {
+    f16x2 h[8];
+    f16x8 v[2];
+  } r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (KT == TY_I8) {
+      const uint32_t b = u[i] ^ 0x80808080u;
+      r.h[2 * i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - (_Float16)1152.0f;
+      r.h[2 * i + 1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - (_Float16)1152.0f;
+    } else {
+      r.h[2 * i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u[i], 1.0f, false));
+      r.h[2 * i + 1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u[i], 1.0f, true));
     }
-    float top = x;
-    for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
-    const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.0f : now;
-    const float keep = expf(m - ref), w = here ? expf(x - ref) : 0.0f;
-    m = now;
-    float sum = w;
-    for (int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
-    l = l * keep + sum;
-    __syncthreads();
-    s_w[lane] = w;
-    __syncthreads();
-    for (int i = 0; i < HD / 64; ++i) o[i] *= keep;
-    for (uint32_t j = 0; j < 64 && p0 + j < seen; ++j) {
-      const uint32_t at = p0 + j, page = tab[at >> g.shift];
-      if (page >= g.n_pages) continue;
-      const float e = p8_scale(a.c.ve[p8_exp(g, page, h, at & mask)]);
-      const uint8_t* v = a.c.vc + p8_base(g, page, h);
-      for (int i = 0; i < HD / 64; ++i) {
-        float y[4];
-        p8_unpack4<KT>(v[p8_v(g, at & mask, lane + 64 * i)], y);
-        o[i] += s_w[j] * (y[0] * e);
+  }
+  to[0] = r.v[0];
+  to[1] = r.v[1];
+}
+
+// Terms of 8 elements of a query row.  top: bits of the largest |element| of the row.  Returns the power of two
+// that the row was scaled by.
+template <int QT, int NQ, typename R>
+__device__ __forceinline__ int p8_query(const R& raw, uint32_t top, bool negate, f16x8 (&term)[NQ]) {
+  int up = 0;
+  if constexpr (QT != TY_F16) {
+    const int ex = (int)(top >> 23) - 127;
+    if (ex < 128) up = 13 - ex;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v = (float)raw[i];
+    if constexpr (QT != TY_F16) v = ldexpf(v, up);
+    if (negate) v = -v;
+    const bool fin = fabsf(v) < INFINITY;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const _Float16 b = (_Float16)v;
+      term[n][i] = b;
+      v = fin ? v - (float)b : 0.0f;
+    }
+  }
+  return up;
+}
+
+// |scale| log2(e) 2^-up as a mantissa and an exponent, so that K's exponents can neither overflow nor lose it.
+struct P8Factor {
+  float m;
+  int e;
+};
+__device__ __forceinline__ P8Factor p8_factor(float scale, int up) {
+  int e;
+  const float m = frexpf(fabsf(scale), &e);
+  return P8Factor{m * PA_LOG2E, e - up};
+}
+__device__ __forceinline__ float p8_times(const P8Factor& f, uint32_t exp_byte) {
+  const float x = fminf(ldexpf(f.m, f.e + (int)exp_byte - 127), -PA_LOWEST);
+  return exp_byte == P8_NAN ? u2f(0x7fc00000u) : x;
+}
+
+// What a wave keeps of its 16 NR rows (lane: row 16 r + l % 16, outputs of dims 16 d + 4 (l / 16) + i).
+template <int HD, int NR>
+struct P8Rows {
+  f32x4 o[NR][HD / 16];  // in units of 2^(D - 14)
+  float m[NR], D[NR];    // softmax reference, and the reference of o relative to it; whole numbers
+  float l[NR];           // this lane's share of the sum
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      m[r] = D[r] = -INFINITY;
+      l[r] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) o[r][d] = f32x4{0, 0, 0, 0};
+    }
+  }
+};
+
+// One tile's scores sc (positions gpos + 4 b + i of this lane's block) to weights pf (operands of positions gpos
+// + 8 half ...), and the rows' states.  EDGE: some row does not see some position.
+template <int HD, int NR, int NP, bool EDGE>
+__device__ __forceinline__ void p8_softmax(P8Rows<HD, NR>& st, f32x4 (&sc)[NR][4], const P8Factor (&factor)[NR], uint32_t ke,
+                                           uint32_t ve, uint32_t gpos, const uint32_t (&limit)[NR], bool page_ok,
+                                           f16x8 (&pf)[NR][NP][2]) {
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const float fk = p8_times(factor[r], ke);
+    float top = EDGE ? -INFINITY : sc[r][0][0];
+    // positions of this lane's that the row sees
+    const uint32_t n = !EDGE ? 16u : !page_ok || limit[r] < gpos ? 0u : min(16u, limit[r] - gpos + 1);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (EDGE) top = (uint32_t)i < n ? fmaxf(top, sc[r][i >> 2][i & 3]) : top;
+      else top = fmaxf(top, sc[r][i >> 2][i & 3]);
+    }
+    // (the factor is not negative; -infinity and NaN scores count as the lowest number)
+    top = n ? fmaxf(top * fk, PA_LOWEST) : -INFINITY;
+    const float ctop = ceilf(top);
+    // the reference of the exponents is a whole number: rescaling by powers of two is exact
+    const float m_new = fmaxf(st.m[r], pa_max4(ctop)), ref = m_new == -INFINITY ? 0.0f : m_new;
+    const float d_tile = pa_max4(ctop - ref + ((float)ve - 127.0f));
+    if (__ballot(m_new > st.m[r] || d_tile > st.D[r])) {
+      const float down = st.m[r] - ref, d_old = st.D[r] + down;
+      st.l[r] *= __builtin_amdgcn_exp2f(down);
+      st.m[r] = m_new;
+      st.D[r] = fmaxf(d_old, d_tile);
+      const float alpha = __builtin_amdgcn_exp2f(d_old - (st.D[r] == -INFINITY ? 0.0f : st.D[r]));
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) st.o[r][d] *= alpha;
+    }
+    float cr = fk, base = -ref;
+    if (__ballot(fabsf(ref) >= 1024.0f)) {
+      // far from zero the product before its rounding may lie well above the reference, which comes from the
+      // rounded ones, and the shift below may be lost in the reference
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[r][i >> 2][i & 3] = sc[r][i >> 2][i & 3] * fk - ref;
+      cr = 1.0f;
+      base = 0.0f;
+    }
+    // weights times 2^shift are what the matrix cores get: 2^14 at most
+    const float d_ref = st.D[r] == -INFINITY ? 0.0f : st.D[r];
+    const int shift = (int)fmaxf(-512.0f, fminf(512.0f, (float)ve - 127.0f - d_ref + 14.0f));
+    float sum = 0.0f;
+    const auto put = [&](int i, float p) {
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        const _Float16 b = (_Float16)p;
+        pf[r][k][i >> 3][i & 7] = b;
+        p -= (float)b;
+      }
+    };
+    if (__ballot(shift < -60 || ve == P8_NAN)) {
+      // (the shifted weights may be too small to be summed)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], cr, base));
+        if (EDGE) p = (uint32_t)i < n ? p : 0.0f;
+        sum += p;
+        p = ve == P8_NAN && (uint32_t)i < n ? u2f(0x7fc00000u) : ldexpf(p, shift);
+        put(i, p);
+      }
+      st.l[r] += sum;
+    } else {
+      base += (float)shift;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], cr, base));
+        if (EDGE) p = (uint32_t)i < n ? p : 0.0f;
+        sum += p;
+        put(i, p);
+      }
+      st.l[r] += ldexpf(sum, -shift);
+    }
+  }
+}
+
+// NaN bytes (e4m3) of an operand's granule to zero: a zero weight times them would be NaN.  Whether there were any.
+__device__ __forceinline__ uint32_t p8_clear_nan(u32x4& u) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t bits = (((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+    any |= bits;
+    u[i] &= ~(bits * 255u);
+  }
+  return any;
+}
+
+// Workgroups of a CU, by registers and LDS.
+constexpr int p8_per_cu(int hd, int nr) { return hd == 64 ? 5 - nr : hd == 128 ? 4 - nr : 2; }
+
+// One piece per workgroup; its 4 waves take the tiles in turn and join their states through LDS at the end.
+template <int HD, int KT, int QT, int NR, bool STREAM>
+__global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8) {
+  typedef typename std::conditional<QT == TY_F32, float, typename std::conditional<QT == TY_F16, _Float16, __bf16>::type>::type QE;
+  typedef QE q8v __attribute__((ext_vector_type(8)));
+  constexpr int NQ = QT == TY_F32 ? 2 : 1, NP = 2, KS = HD / 32, DS = HD / 16, KG = HD / 64;
+  constexpr int ROWS = 16 * NR, PITCH = HD + 4;
+  const PaArgs& a = p8.a;
+  extern __shared__ float smem[];  // [4][ROWS][PITCH] rows, [4][ROWS][2] states, [ROWS][2] factors
+  float* s_ml = smem + 4 * ROWS * PITCH;
+  float* s_f = s_ml + 4 * ROWS * 2;
+  float* s_q = smem;  // [NR][NQ][KS][64] operands of 16 bytes
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t col = lane & 15u, grp = lane >> 4;
+  const Paged& g = a.g;
+
+  const PaPiece pc = pa_piece<NR, P8_TILE>(a, blockIdx.x, blockIdx.x == 0);
+  if (!pc.any) return;
+  const PaSeq& sq = pc.q;
+  const uint32_t s = pc.s, h = pc.h, rb = pc.rb, t0 = pc.t0, t1 = pc.t1, group = a.group;
+  const uint32_t* tab = g.table + (size_t)s * g.stride;
+  const uint32_t len = sq.len, first = sq.first;
+  const uint8_t *kc = reinterpret_cast<const uint8_t*>(a.kc), *vc = reinterpret_cast<const uint8_t*>(a.vc);
+
+  // ---- tiles t0 + w, t0 + w + 4, ...: the first one's pages, then its K and V, are on their way before
+  // the query rows are made ready
+  const uint32_t ta = t0 + w;
+  const uint32_t kpos = 16 * (col >> 2), ko = kpos + (col & 3u);  // this lane's K rows in a tile: ko + 4 b
+  const size_t head_bytes = (size_t)HD << g.shift;
+  const uint32_t pmask = (1u << g.shift) - 1u;
+  u32x4 kf[4][KG], vf[DS];
+  uint32_t ke = 0, ve = 0, odd_tile = ~0u;
+  const auto load_k = [&](uint32_t pos0, uint32_t page) {
+    if (page >= g.n_pages) page = 0;
+    const uint8_t* p = kc + ((size_t)page * g.n_kv + h) * head_bytes + (((size_t)grp << g.shift) + ((pos0 + ko) & pmask)) * 16;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)  // granules of 64 dims apart
+      pa_load<STREAM, KG>(reinterpret_cast<const u32x4*>(p) + 4 * b, (size_t)4 << g.shift, kf[b]);
+  };
+  const auto load_v = [&](uint32_t pos0, uint32_t page) {
+    if (page >= g.n_pages) page = 0;
+    const uint32_t o = (pos0 + 16 * grp) & pmask;
+    const uint8_t* p = vc + ((size_t)page * g.n_kv + h) * head_bytes + ((size_t)(o >> 4) * HD + col) * 16;
+    pa_load<STREAM, DS>(reinterpret_cast<const u32x4*>(p), 16, vf);
+  };
+  const auto load_e = [&](uint32_t pos0, uint32_t page) {
+    if (page >= g.n_pages) page = 0;
+    const size_t at = p8_exp(g, page, h, (pos0 + 16 * grp) & pmask);
+    ke = p8.ke[at];
+    ve = p8.ve[at];
+  };
+  uint32_t pk = 0, pv = 0, pkn = 0, pvn = 0;
+  if (ta < t1) {
+    pk = pa_page(a, tab, ta * P8_TILE + kpos, len);
+    pv = pa_page(a, tab, ta * P8_TILE + 16 * grp, len);
+    pkn = pa_page(a, tab, (ta + 4) * P8_TILE + kpos, len);
+    pvn = pa_page(a, tab, (ta + 4) * P8_TILE + 16 * grp, len);
+  }
+  // the query rows as operands in LDS: unit (row, 8 dims) of every thread, a row in HD / 8 lanes
+  constexpr int LPR = HD / 8, UNITS = ROWS * LPR, PASSES = (UNITS + PA_NT - 1) / PA_NT;
+  q8v raw[PASSES];
+#pragma unroll
+  for (int k = 0; k < PASSES; ++k) {
+    const uint32_t u = tid + k * PA_NT, row = rb * ROWS + u / LPR;
+    const uint32_t t = pa_token(a, row), qh = h * group + (row - t * group);
+    raw[k] = q8v{};
+    if (u < UNITS && row < sq.rows)
+      raw[k] = *reinterpret_cast<const q8v*>(static_cast<const QE*>(a.q) + ((size_t)s * a.n_new + t) * a.q_stride +
+                                             (size_t)qh * HD + 8 * (u % LPR));
+  }
+  if (ta < t1) {
+    load_k(ta * P8_TILE, pk);
+    load_e(ta * P8_TILE, pv);
+    load_v(ta * P8_TILE, pv);
+  }
+#pragma unroll
+  for (int k = 0; k < PASSES; ++k) {
+    const uint32_t u = tid + k * PA_NT, row = u / LPR, d8 = u % LPR;
+    uint32_t top = 0;
+    if constexpr (QT != TY_F16) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, f2u((float)raw[k][i]) & 0x7fffffffu);
+      top = pa_group_max<LPR>(top);
+    }
+    f16x8 term[NQ];
+    const int up = p8_query<QT, NQ>(raw[k], top, a.scale < 0.0f, term);
+    if (UNITS >= PA_NT || u < UNITS) {
+      // dims 8 d8 are operand (d8 / 8) * 2 + d8 % 2 of lane group (d8 / 2) % 4
+      const uint32_t j = (d8 >> 3) * 2 + (d8 & 1u), to = ((d8 >> 1) & 3u) * 16 + (row & 15u);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+        *reinterpret_cast<f16x8*>(&s_q[((((row >> 4) * NQ + n) * KS + j) * 64 + to) * 4]) = term[n];
+      if (d8 == 0) {
+        const P8Factor f = p8_factor(a.scale, up);
+        s_f[2 * row] = f.m;
+        s_f[2 * row + 1] = u2f((uint32_t)f.e);
       }
     }
   }
-  for (int i = 0; i < HD / 64; ++i)
-    store_from_f32<QT>(a.out, (size_t)row * a.out_stride + (size_t)head * HD + lane + 64 * i,
-                       m == -INFINITY ? 0.0f : o[i] / l);
+  __syncthreads();
+  P8Factor factor[NR];
+  uint32_t limit[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const uint32_t row = rb * ROWS + r * 16 + col;
+    factor[r] = P8Factor{s_f[2 * (r * 16 + col)], (int)f2u(s_f[2 * (r * 16 + col) + 1])};
+    limit[r] = first + (row < sq.rows ? pa_token(a, row) : 0u);
+  }
+  P8Rows<HD, NR> st;
+  st.clear();
+  for (uint32_t t = ta; t < t1; t += 4) {
+    const uint32_t pos0 = t * P8_TILE;
+    const bool next = t + 4 < t1;
+    f32x4 sc[NR][4];
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) sc[r][b] = f32x4{0, 0, 0, 0};
+    asm volatile("" ::: "memory");  // (the query operands stay in LDS: registers)
+#pragma unroll
+    for (int gi = 0; gi < KG; ++gi)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        f16x8 kk[2];
+        p8_operands<KT>(kf[b][gi], kk);
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int n = NQ - 1; n >= 0; --n) {
+              const f16x8 qf = *reinterpret_cast<const f16x8*>(&s_q[(((r * NQ + n) * KS + 2 * gi + j) * 64 + lane) * 4]);
+              sc[r][b] = Op16<TY_F16>::mfma(kk[j], qf, sc[r][b]);
+            }
+      }
+    const bool page_ok = pv < g.n_pages;
+    const uint32_t ke_now = ke, ve_now = ve;
+    uint32_t pv2 = 0;
+    if (next) {
+      const uint32_t pk2 = pa_page(a, tab, (t + 8) * P8_TILE + kpos, len);
+      pv2 = pa_page(a, tab, (t + 8) * P8_TILE + 16 * grp, len);
+      load_k(pos0 + 4 * P8_TILE, pkn);
+      load_e(pos0 + 4 * P8_TILE, pvn);
+      pkn = pk2;
+    }
+    const uint32_t gpos = pos0 + 16 * grp;  // this lane's 16 positions
+    if (!page_ok) paged_flag(g, PG_BAD_PAGE);
+    const bool edge = pos0 + P8_TILE - 1 > first || __ballot(!page_ok) != 0;
+    f16x8 pf[NR][NP][2];
+    if (edge) {
+      p8_softmax<HD, NR, NP, true>(st, sc, factor, ke_now, ve_now, gpos, limit, page_ok, pf);
+      if (KT == TY_E4M3) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int d = 0; d < DS; ++d) odd |= p8_clear_nan(vf[d]);
+        if (__ballot(odd != 0)) odd_tile = t;
+      }
+    } else {
+      p8_softmax<HD, NR, NP, false>(st, sc, factor, ke_now, ve_now, gpos, limit, page_ok, pf);
+    }
+#pragma unroll
+    for (int d = 0; d < DS; ++d) {
+      f16x8 vv[2];
+      p8_operands<KT>(vf[d], vv);
+#pragma unroll
+      for (int n = NP - 1; n >= 0; --n)  // the small terms first
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) st.o[r][d] = Op16<TY_F16>::mfma(vv[k], pf[r][n][k], st.o[r][d]);
+    }
+    if (odd_tile == t) {
+      // NaN in V to the rows that see it; this lane's outputs: dims 16 d + 4 grp + i
+#pragma unroll 1
+      for (uint32_t pos = pos0; pos < min(len, pos0 + P8_TILE); ++pos) {
+        const uint32_t page = tab[pos >> g.shift];
+        if (page >= g.n_pages) continue;
+        const uint8_t* p = vc + ((size_t)page * g.n_kv + h) * head_bytes + ((size_t)((pos & pmask) >> 4) * HD + 4 * grp) * 16 + (pos & 15u);
+#pragma unroll
+        for (int d = 0; d < DS; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float add = (p[(16 * d + i) * 16] & 0x7fu) == 0x7fu ? u2f(0x7fc00000u) : 0.0f;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) st.o[r][d][i] += pos <= limit[r] ? add : 0.0f;
+          }
+      }
+    }
+    if (next) {
+      pv = pvn;
+      pvn = pv2;
+      load_v(pos0 + 4 * P8_TILE, pv);
+    }
+  }
+
+  // ---- the waves' states joined; rows finished, or a part written.  Sums and rows in units of 2^24: over 2^24
+  // positions of values near the largest f32 they stay below it
+  __syncthreads();  // (the query operands lie where the states go)
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const float sum = pa_sum4(st.l[r]);
+    if (grp == 0) {
+      s_ml[(w * ROWS + r * 16 + col) * 2] = st.m[r];
+      s_ml[(w * ROWS + r * 16 + col) * 2 + 1] = ldexpf(sum, -24);
+    }
+    const int unit = st.D[r] == -INFINITY ? 0 : (int)fmaxf(-512.0f, fminf(512.0f, st.D[r])) - 14 - 24;
+#pragma unroll
+    for (int d = 0; d < DS; ++d) {
+      f32x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = ldexpf(st.o[r][d][i], unit);
+      *reinterpret_cast<f32x4*>(&smem[(w * ROWS + r * 16 + col) * PITCH + 16 * d + 4 * grp]) = y;
+    }
+  }
+  __syncthreads();
+  const bool whole = pc.n == 1;
+  if (t0 == 0 && tid == 0) a.cuts[((size_t)s * g.n_kv + h) * a.blocks + rb] = make_uint2(pc.slot, pc.n);
+  const uint32_t here = min((uint32_t)ROWS, sq.rows - rb * ROWS);
+  for (uint32_t i = tid; i < here * (HD / 4); i += PA_NT) {
+    const uint32_t row = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) M = fmaxf(M, s_ml[(v * ROWS + row) * 2]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    f32x4 y = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float f = __builtin_amdgcn_exp2f(s_ml[(v * ROWS + row) * 2] - ref);
+      L += f * s_ml[(v * ROWS + row) * 2 + 1];
+      y += f * *reinterpret_cast<const f32x4*>(&smem[(v * ROWS + row) * PITCH + d]);
+    }
+    const uint32_t full = rb * ROWS + row;
+    if (whole) {
+      const f32x4 z = M == -INFINITY ? f32x4{0, 0, 0, 0} : y / L;  // (no position left: zeros)
+      const uint32_t t = pa_token(a, full);
+      const size_t dst = ((size_t)s * a.n_new + t) * a.out_stride + (size_t)(h * group + (full - t * group)) * HD + d;
+      pa_store4<QT>(a.out, dst, z);
+    } else {
+      *reinterpret_cast<f32x4*>(&a.part_o[((size_t)pc.slot * a.part_rows + row) * HD + d]) = y;
+      if (d == 0) {
+        a.part_ml[((size_t)pc.slot * a.part_rows + row) * 2] = M;
+        a.part_ml[((size_t)pc.slot * a.part_rows + row) * 2 + 1] = L;
+      }
+    }
+  }
 }
 
 }  // namespace cm

@@ -141,7 +141,7 @@ __device__ __forceinline__ uint32_t pa_token(const PaArgs& a, uint32_t row) {
 struct PaSeq {
   uint32_t len, first, rows, tiles, blocks;  // blocks: row blocks of the sequence
 };
-template <int NR>
+template <int NR, uint32_t TILE = PA_TILE>
 __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, uint32_t s, bool flag) {
   PaSeq q;
   const uint32_t L = a.g.lens[s], m = a.new_lens ? a.new_lens[s] : a.n_new;
@@ -150,7 +150,7 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, uint32_t s, bool flag) 
   q.len = L;
   q.first = L - m;
   q.rows = ok ? m * a.group : 0u;
-  q.tiles = q.rows ? (L + PA_TILE - 1) / PA_TILE : 0u;
+  q.tiles = q.rows ? (L + TILE - 1) / TILE : 0u;
   q.blocks = (q.rows + 16 * NR - 1) / (16 * NR);
   return q;
 }
@@ -160,10 +160,12 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, uint32_t s, bool flag) 
 // whole latency again), the same for every wave (16x1100 with 5 drafts: 22.9 us at 8 tiles, 24.0 at 5).
 // Large ones: 16, so that workgroups ending early make room for others, and
 // more once that makes over 2048 pieces.
-__device__ __forceinline__ uint32_t pa_target(const PaArgs& a, uint32_t total) {
-  const uint32_t one = (total + a.at_once - 1) / a.at_once;
-  return one <= 16 ? max(4u, (one + 3) & ~3u) : max(16u, (total + 2047) / 2048);
-}
+struct PaTarget {
+  __device__ __forceinline__ uint32_t operator()(const PaArgs& a, uint32_t total) const {
+    const uint32_t one = (total + a.at_once - 1) / a.at_once;
+    return one <= 16 ? max(4u, (one + 3) & ~3u) : max(16u, (total + 2047) / 2048);
+  }
+};
 
 struct PaPiece {
   uint32_t s, h, rb, t0, t1, n, slot;  // n: the segment's pieces; slot: this piece's (n > 1)
@@ -173,22 +175,22 @@ struct PaPiece {
 
 // Piece `index` of the batch (pieces in the order sequence, KV head, block, tiles).  Each wave works
 // it out by itself: a lane for every 64th part of the sequences.
-template <int NR>
+template <int NR, uint32_t TILE = PA_TILE, typename Target = PaTarget>
 __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, bool flag) {
   const uint32_t lane = threadIdx.x & 63u, n = a.g.n_seqs, per = (n + 63) / 64;
   const uint32_t s0 = min(n, lane * per), s1 = min(n, s0 + per);
   uint32_t total = 0;
   PaSeq q{};
   for (uint32_t s = s0; s < s1; ++s) {
-    q = pa_seq<NR>(a, s, flag);
+    q = pa_seq<NR, TILE>(a, s, flag);
     total += q.tiles * q.blocks * a.g.n_kv;
   }
   total = __builtin_amdgcn_readlane(pa_scan(total), 63);
-  const uint32_t target = pa_target(a, total);
+  const uint32_t target = Target{}(a, total);
   const auto count = [&](const PaSeq& z) { return (z.tiles + target - 1) / target; };
   uint32_t mine = 0, cut = 0;
   for (uint32_t s = s0; s < s1; ++s) {
-    if (per > 1) q = pa_seq<NR>(a, s, false);
+    if (per > 1) q = pa_seq<NR, TILE>(a, s, false);
     const uint32_t c = count(q), k = c * q.blocks * a.g.n_kv;
     mine += k;
     if (c > 1) cut += k;
@@ -202,7 +204,7 @@ __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, boo
   uint32_t before = __builtin_amdgcn_readlane(x - mine, owner), slots = __builtin_amdgcn_readlane(y - cut, owner);
   uint32_t s = owner * per;
   for (;; ++s) {
-    q = pa_seq<NR>(a, s, false);
+    q = pa_seq<NR, TILE>(a, s, false);
     const uint32_t c = count(q), k = c * q.blocks * a.g.n_kv;
     if (index - before < k) break;
     before += k;
@@ -231,6 +233,21 @@ template <bool STREAM, int N, typename V>
 __device__ __forceinline__ void pa_load(const V* p, size_t step, V* to) {
 #pragma unroll
   for (int i = 0; i < N; ++i) to[i] = STREAM ? __builtin_nontemporal_load(p + i * step) : p[i * step];
+}
+
+// Four outputs to elements from dst on.
+template <int QT>
+__device__ __forceinline__ void pa_store4(void* out, size_t dst, f32x4 z) {
+  if constexpr (QT == TY_F32) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(out) + dst) = z;
+  } else {
+    ushort4 b;
+    b.x = to_bits16<QT>(z[0]);
+    b.y = to_bits16<QT>(z[1]);
+    b.z = to_bits16<QT>(z[2]);
+    b.w = to_bits16<QT>(z[3]);
+    *reinterpret_cast<ushort4*>(static_cast<uint16_t*>(out) + dst) = b;
+  }
 }
 
 // Workgroups of a CU, by registers and LDS.
@@ -571,16 +588,7 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
         const f32x4 z = M == -INFINITY ? f32x4{0, 0, 0, 0} : y / L;
         const uint32_t t = pa_token(a, full);
         const size_t dst = ((size_t)s * a.n_new + t) * a.out_stride + (size_t)(h * group + (full - t * group)) * HD + d;
-        if constexpr (QT == TY_F32) {
-          *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + dst) = z;
-        } else {
-          ushort4 b;
-          b.x = to_bits16<QT>(z[0]);
-          b.y = to_bits16<QT>(z[1]);
-          b.z = to_bits16<QT>(z[2]);
-          b.w = to_bits16<QT>(z[3]);
-          *reinterpret_cast<ushort4*>(static_cast<uint16_t*>(a.out) + dst) = b;
-        }
+        pa_store4<QT>(a.out, dst, z);
         if (a.scores && d == 0) {
           float* st = a.stats + (((size_t)s * g.n_kv + h) * ((size_t)a.n_new * group) + full) * 2;
           st[0] = M;
@@ -649,16 +657,7 @@ __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, ui
       const f32x4 z = M == -INFINITY ? f32x4{0, 0, 0, 0} : y / L;
       const uint32_t t = pa_token(a, row);
       const size_t dst = ((size_t)s * a.n_new + t) * a.out_stride + (size_t)(h * a.group + (row - t * a.group)) * HD + 4 * d;
-      if constexpr (QT == TY_F32) {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + dst) = z;
-      } else {
-        ushort4 b;
-        b.x = to_bits16<QT>(z[0]);
-        b.y = to_bits16<QT>(z[1]);
-        b.z = to_bits16<QT>(z[2]);
-        b.w = to_bits16<QT>(z[3]);
-        *reinterpret_cast<ushort4*>(static_cast<uint16_t*>(a.out) + dst) = b;
-      }
+      pa_store4<QT>(a.out, dst, z);
     }
     return;
   }

@@ -43,6 +43,64 @@ uint32_t log2_of(uint32_t power) {
   return n;
 }
 
+// What a call of the attention needs: row blocks of 16 * nr query rows, workgroups, workspace.
+struct P8Sizes {
+  uint32_t nr, blocks, part_rows, at_once, grid;
+  bool join;                   // some segment may be cut
+  bool fits;                   // the plan's 32-bit counts hold
+  size_t part_o, cuts, bytes;  // offsets of the workspace's parts, its size
+};
+
+P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap) {
+  P8Sizes z;
+  const uint64_t rows = n_new * (n_heads / n_kv), cap_tiles = (cap + cm::P8_TILE - 1) / cm::P8_TILE;
+  z.nr = rows > 16 && hd <= 128 ? 2 : 1;
+  z.blocks = (uint32_t)((rows + 16 * z.nr - 1) / (16 * z.nr));
+  z.part_rows = (uint32_t)std::min<uint64_t>(rows, 16 * z.nr);
+  // 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
+  z.at_once = 256 * cm::p8_per_cu((int)hd, (int)z.nr) * 7 / 8;
+  const uint64_t segments = n_seqs * n_kv * z.blocks, most = 2048;
+  // a segment has at most ceil(its tiles / 4) pieces, all of them together at most 2048 and one each
+  const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + 3) / 4));
+  z.fits = segments * cap_tiles < (1ull << 31) && grid_ok(pieces, cm::PA_NT);
+  z.grid = (uint32_t)pieces;
+  z.join = cap_tiles > 4;
+  // cut segments have more tiles than the target: at most 2048 of them, twice as many pieces
+  const size_t slots = z.join ? (size_t)std::min(2 * most, pieces) : 0;
+  z.part_o = up256(slots * z.part_rows * 8);
+  z.cuts = z.part_o + up256(slots * z.part_rows * hd * 4);
+  z.bytes = z.cuts + up256(segments * 8);
+  return z;
+}
+
+template <int HD, int KT, int QT, int NR>
+bool p8_launch(const cm::P8Args& p, const P8Sizes& z, hipStream_t stream) {
+  const cm::PaArgs& a = p.a;
+  // K and V that the batch's tables can hold, against the 256 MB of the memory-side cache (several row blocks read
+  // them several times)
+  const bool passing = z.blocks == 1 && ((uint64_t)a.g.n_seqs * a.g.n_kv * HD * 2 * a.g.stride << a.g.shift) > (256u << 20);
+  const auto split = passing ? cm::k_p8_split<HD, KT, QT, NR, true> : cm::k_p8_split<HD, KT, QT, NR, false>;
+  constexpr size_t lds = (size_t)16 * NR * (4 * (HD + 4 + 2) + 2) * 4;
+  if (lds > 64 * 1024) {
+    const hipError_t st = hipFuncSetAttribute(reinterpret_cast<const void*>(split),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (st != hipSuccess) return cm::fail_global("paged8_attention", hipGetErrorString(st)) == 0;
+  }
+  hipLaunchKernelGGL(split, dim3(z.grid), dim3(cm::PA_NT), lds, stream, p);
+  if (!z.join) return true;
+  const uint32_t rows = a.n_new * a.group, sh = a.g.n_seqs * a.g.n_kv;
+  const uint32_t cap = a.g.stride << a.g.shift;
+  const auto join = [&](auto per, auto kernel) {
+    const uint32_t row_groups = (rows + per.value - 1) / per.value;
+    hipLaunchKernelGGL(kernel, dim3(sh * row_groups), dim3(cm::PA_NT), 0, stream, a, rows, row_groups, 0u, 8u);
+  };
+  if (cap <= 16 * 4 * cm::P8_TILE || sh >= 256)
+    join(std::integral_constant<uint32_t, cm::pj_parts(HD)>{}, cm::k_pa_join<HD, QT, NR, cm::pj_parts(HD)>);
+  else
+    join(std::integral_constant<uint32_t, 1>{}, cm::k_pa_join<HD, QT, NR, 1>);
+  return true;
+}
+
 }  // namespace
 
 extern "C" {
@@ -113,7 +171,8 @@ int camelid_hip_paged8_read(const void* kc, const void* vc, const uint8_t* k_exp
 
 size_t camelid_hip_paged8_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
                                               uint32_t hd, uint32_t page_size, uint32_t table_stride) {
-  return 256;
+  if (!n_kv) return 0;
+  return p8_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride).bytes;
 }
 
 int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stride, uint32_t n_seqs, uint32_t n_new,
@@ -126,9 +185,10 @@ int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stri
   if (!n_seqs || !n_new) return 0;
   if (!q || !kc || !vc || !k_exp || !v_exp || !table || !lens || !out || !workspace)
     return cm::fail_global(me, "null argument");
-  cm::P8Args a{};
+  cm::P8Args p{};
+  cm::PaArgs& a = p.a;
   const char* why;
-  if (!paged_geometry(&a.c.g, n_seqs, n_kv, hd, n_pages, page_size, table, table_stride, lens, status, &why, 16))
+  if (!paged_geometry(&a.g, n_seqs, n_kv, hd, n_pages, page_size, table, table_stride, lens, status, &why, 16))
     return cm::fail_global(me, why);
   if (!heads_ok(n_heads, n_kv)) return cm::fail_global(me, "n_heads must be a nonzero multiple of n_kv, at most 4096");
   if (!type_ok(q_type) || !kv8_ok(kv_type)) return cm::fail_global(me, "unknown type");
@@ -140,25 +200,43 @@ int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stri
     return cm::fail_global(me, "q, out, the cache and the workspace must be 16-byte aligned, the rest 4-byte aligned");
   if (workspace_bytes < camelid_hip_paged8_attention_workspace(n_seqs, n_new, n_heads, n_kv, hd, page_size, table_stride))
     return cm::fail_global(me, "workspace too small (camelid_hip_paged8_attention_workspace)");
-  const uint64_t grid = (uint64_t)n_seqs * n_new * n_heads;
-  if (!grid_ok(grid, 64)) return cm::fail_global(me, "too many rows in one call");
-  a.c.kc = const_cast<uint8_t*>(static_cast<const uint8_t*>(kc));
-  a.c.vc = const_cast<uint8_t*>(static_cast<const uint8_t*>(vc));
-  a.c.ke = const_cast<uint8_t*>(k_exp);
-  a.c.ve = const_cast<uint8_t*>(v_exp);
+  const uint64_t groups = (uint64_t)n_seqs * n_kv * n_new * (n_heads / n_kv);
+  if (!grid_ok(groups, cm::PA_NT)) return cm::fail_global(me, "too many rows in one call");
+  const P8Sizes z = p8_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride);
+  if (!z.fits) return cm::fail_global(me, "n_seqs * n_kv * table_stride * page_size too large for one call");
+  // (every workgroup works the plan out from all lengths)
+  if (n_seqs > 65535) return cm::fail_global(me, "at most 65535 sequences");
+  char* ws = static_cast<char*>(workspace);
+  p.ke = k_exp;
+  p.ve = v_exp;
+  a.kc = static_cast<const uint16_t*>(kc);
+  a.vc = static_cast<const uint16_t*>(vc);
   a.q = q;
   a.new_lens = new_lens;
   a.out = out;
+  a.part_ml = reinterpret_cast<float*>(ws);
+  a.part_o = reinterpret_cast<float*>(ws + z.part_o);
+  a.cuts = reinterpret_cast<uint2*>(ws + z.cuts);
   a.scale = scale;
   a.q_stride = q_stride;
   a.out_stride = out_stride;
   a.n_new = n_new;
   a.n_heads = n_heads;
   a.group = n_heads / n_kv;
+  a.group_magic = a.group == 1 ? 0 : (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
+  a.at_once = z.at_once;
+  a.blocks = z.blocks;
+  a.part_rows = z.part_rows;
+  bool ok = true;
   by_types(hd, kv_type, q_type, [&](auto d, auto k, auto t) {
-    hipLaunchKernelGGL((cm::k_p8_rows<d(), k(), t()>), dim3((uint32_t)grid), dim3(64), 0, (hipStream_t)stream, a);
+    if constexpr (d() <= 128)
+      if (z.nr == 2) {
+        ok = p8_launch<d(), k(), t(), 2>(p, z, (hipStream_t)stream);
+        return;
+      }
+    ok = p8_launch<d(), k(), t(), 1>(p, z, (hipStream_t)stream);
   });
-  return launched(me);
+  return ok ? launched(me) : 1;
 }
 
 // ---- pages
