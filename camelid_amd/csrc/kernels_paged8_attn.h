@@ -205,7 +205,7 @@ __device__ __forceinline__ uint32_t p8_clear_nan(u32x4& u) {
 }
 
 // Workgroups of a CU, by registers and LDS.
-constexpr int p8_per_cu(int hd, int nr) { return hd == 64 ? 5 - nr : hd == 128 ? 4 - nr : 2; }
+constexpr int p8_per_cu(int hd, int nr) { return hd == 64 ? 4 - nr : hd == 128 ? 3 - nr : 1; }
 
 // One piece per workgroup; its 4 waves take the tiles in turn and join their states through LDS at the end.
 template <int HD, int KT, int QT, int NR, bool STREAM>
