@@ -32,8 +32,6 @@ struct P8Args {
   const uint8_t* ve;
 };
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 // 16 bytes of a granule -> 16 f16, in order: two operands.
 template <int KT>
 __device__ __forceinline__ void p8_operands(u32x4 u, f16x8 (&to)[2]) {
@@ -167,8 +165,8 @@ __device__ __forceinline__ void p8_softmax(P8Rows<HD, NR>& st, f32x4 (&sc)[NR][4
         p -= (float)b;
       }
     };
-    if (__ballot(shift < -60 || ve == P8_NAN)) {
-      // (the shifted weights may be too small to be summed)
+    if (__ballot(shift < -16 || ve == P8_NAN)) {
+      // (the shift in the exponent would cost the weights bits)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], cr, base));

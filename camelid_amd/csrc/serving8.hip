@@ -126,16 +126,23 @@ int camelid_hip_paged8_rope_kv(const float* qkv, uint32_t n_seqs, uint32_t n_new
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(kc) || !aligned16(vc) || !aligned4(cos_tab) ||
       !aligned4(sin_tab) || !aligned4(q_norm) || !aligned4(k_norm) || !aligned4(new_lens))
     return cm::fail_global(me, "qkv, q_out and the cache must be 16-byte aligned, the rest 4-byte aligned");
-  const uint64_t grid = (uint64_t)n_seqs * cm::r8_blocks(n_new) * (n_heads + 2 * n_kv);
+  const bool whole = rope_dim == hd;
+  const uint32_t roles = whole ? cm::r8_roles(hd, n_heads, n_kv) : n_heads + 2 * n_kv, blocks = cm::r8_blocks(n_new);
+  const uint64_t grid = (uint64_t)n_seqs * blocks * roles;
   if (!grid_ok(grid, cm::R8_NT)) return cm::fail_global(me, "too many rows in one call");
   c.kc = static_cast<uint8_t*>(kc);
   c.vc = static_cast<uint8_t*>(vc);
   c.ke = k_exp;
   c.ve = v_exp;
-  by_types(hd, kv_type, q_type, [&](auto, auto k, auto q) {
-    hipLaunchKernelGGL((cm::k_paged8_rope_kv<q(), k()>), dim3((uint32_t)grid), dim3(cm::R8_NT), 0, (hipStream_t)stream, c,
-                       qkv, n_new, new_lens, n_heads, rope_dim, split_half, cos_tab, sin_tab, q_norm, k_norm, eps, q_out,
-                       cm::r8_blocks(n_new));
+  by_types(hd, kv_type, q_type, [&](auto d, auto k, auto q) {
+    if (whole)
+      hipLaunchKernelGGL((cm::k_paged8_rope_kv16<d(), q(), k()>), dim3((uint32_t)grid), dim3(cm::R8_NT), 0,
+                         (hipStream_t)stream, c, qkv, n_new, new_lens, n_heads, split_half, cos_tab, sin_tab, q_norm,
+                         k_norm, eps, q_out, roles, blocks);
+    else
+      hipLaunchKernelGGL((cm::k_paged8_rope_kv<q(), k()>), dim3((uint32_t)grid), dim3(cm::R8_NT), 0, (hipStream_t)stream,
+                         c, qkv, n_new, new_lens, n_heads, rope_dim, split_half, cos_tab, sin_tab, q_norm, k_norm, eps,
+                         q_out, blocks);
   });
   return launched(me);
 }
