@@ -95,6 +95,13 @@ __device__ __forceinline__ float p8_times(const P8Factor& f, uint32_t exp_byte) 
   return exp_byte == P8_NAN ? u2f(0x7fc00000u) : x;
 }
 
+// The page of position min(pos, len - 1).
+__device__ __forceinline__ uint32_t p8_page(const PaArgs& a, const uint32_t* tab, uint32_t pos, uint32_t len) {
+  return tab[min(pos, len - 1) >> a.g.shift];
+}
+// page * unit + more, one multiply-add (unit: bytes of a page, at most 2^30).
+__device__ __forceinline__ uint64_t p8_at(uint32_t page, uint32_t unit, uint32_t more) { return (uint64_t)page * unit + more; }
+
 // What a wave keeps of its 16 NR rows (lane: row 16 r + l % 16, outputs of dims 16 d + 4 (l / 16) + i).
 template <int HD, int NR>
 struct P8Rows {
@@ -113,28 +120,29 @@ struct P8Rows {
 };
 
 // One tile's scores sc (positions gpos + 4 b + i of this lane's block) to weights pf (operands of positions gpos
-// + 8 half ...), and the rows' states.  EDGE: some row does not see some position.
-template <int HD, int NR, int NP, bool EDGE>
+// + 8 half ...), and the rows' states.  edge: some row may not see some position.
+template <int HD, int NR, int NP>
 __device__ __forceinline__ void p8_softmax(P8Rows<HD, NR>& st, f32x4 (&sc)[NR][4], const P8Factor (&factor)[NR], uint32_t ke,
-                                           uint32_t ve, uint32_t gpos, const uint32_t (&limit)[NR], bool page_ok,
+                                           uint32_t ve, uint32_t gpos, const uint32_t (&limit)[NR], bool page_ok, bool edge,
                                            f16x8 (&pf)[NR][NP][2]) {
+  const float vexp = (float)((int)ve - 127);
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    const float fk = p8_times(factor[r], ke);
-    float top = EDGE ? -INFINITY : sc[r][0][0];
-    // positions of this lane's that the row sees
-    const uint32_t n = !EDGE ? 16u : !page_ok || limit[r] < gpos ? 0u : min(16u, limit[r] - gpos + 1);
+    float fk = p8_times(factor[r], ke);
+    if (edge) {  // positions that the row does not see: -infinity (their factor a positive number)
+      const uint32_t n = !page_ok || limit[r] < gpos ? 0u : limit[r] - gpos + 1;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (EDGE) top = (uint32_t)i < n ? fmaxf(top, sc[r][i >> 2][i & 3]) : top;
-      else top = fmaxf(top, sc[r][i >> 2][i & 3]);
+      for (int i = 0; i < 16; ++i) sc[r][i >> 2][i & 3] = (uint32_t)i < n ? sc[r][i >> 2][i & 3] : -INFINITY;
+      fk = n ? fmaxf(fk, 0x1p-126f) : 1.0f;
+      if (n && ke == P8_NAN) fk = u2f(0x7fc00000u);
     }
-    // (the factor is not negative; -infinity and NaN scores count as the lowest number)
-    top = n ? fmaxf(top * fk, PA_LOWEST) : -INFINITY;
-    const float ctop = ceilf(top);
+    float top = sc[r][0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[r][i >> 2][i & 3]);
+    const float ctop = ceilf(top * fk);  // (the factor is not negative)
     // the reference of the exponents is a whole number: rescaling by powers of two is exact
     const float m_new = fmaxf(st.m[r], pa_max4(ctop)), ref = m_new == -INFINITY ? 0.0f : m_new;
-    const float d_tile = pa_max4(ctop - ref + ((float)ve - 127.0f));
+    const float d_tile = pa_max4(ctop - ref + vexp);
     if (__ballot(m_new > st.m[r] || d_tile > st.D[r])) {
       const float down = st.m[r] - ref, d_old = st.D[r] + down;
       st.l[r] *= __builtin_amdgcn_exp2f(down);
@@ -144,49 +152,42 @@ __device__ __forceinline__ void p8_softmax(P8Rows<HD, NR>& st, f32x4 (&sc)[NR][4
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) st.o[r][d] *= alpha;
     }
-    float cr = fk, base = -ref;
+    float base = -ref;
     if (__ballot(fabsf(ref) >= 1024.0f)) {
       // far from zero the product before its rounding may lie well above the reference, which comes from the
       // rounded ones, and the shift below may be lost in the reference
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[r][i >> 2][i & 3] = sc[r][i >> 2][i & 3] * fk - ref;
-      cr = 1.0f;
+      fk = 1.0f;
       base = 0.0f;
     }
-    // weights times 2^shift are what the matrix cores get: 2^14 at most
+    // weights times 2^shift are what the matrix cores get: 2^14 at most.  Inside the exponent the shift costs
+    // nothing, and up to 16 of it no bits that matter (half a step of an argument of 16 is 2^-21)
     const float d_ref = st.D[r] == -INFINITY ? 0.0f : st.D[r];
-    const int shift = (int)fmaxf(-512.0f, fminf(512.0f, (float)ve - 127.0f - d_ref + 14.0f));
-    float sum = 0.0f;
-    const auto put = [&](int i, float p) {
+    const int shift = (int)fmaxf(-512.0f, fminf(512.0f, vexp - d_ref + 14.0f)), inside = max(shift, -16);
+    base += (float)inside;
+    float sum = 0.0f, p[16];
 #pragma unroll
-      for (int k = 0; k < NP; ++k) {
-        const _Float16 b = (_Float16)p;
-        pf[r][k][i >> 3][i & 7] = b;
-        p -= (float)b;
-      }
-    };
-    if (__ballot(shift < -16 || ve == P8_NAN)) {
-      // (the shift in the exponent would cost the weights bits)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], cr, base));
-        if (EDGE) p = (uint32_t)i < n ? p : 0.0f;
-        sum += p;
-        p = ve == P8_NAN && (uint32_t)i < n ? u2f(0x7fc00000u) : ldexpf(p, shift);
-        put(i, p);
-      }
-      st.l[r] += sum;
-    } else {
-      base += (float)shift;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], cr, base));
-        if (EDGE) p = (uint32_t)i < n ? p : 0.0f;
-        sum += p;
-        put(i, p);
-      }
-      st.l[r] += ldexpf(sum, -shift);
+    for (int i = 0; i < 16; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], fk, base));
+      sum += p[i];
     }
+    st.l[r] += ldexpf(sum, -inside);
+    if (__ballot(shift < -16 || ve == P8_NAN)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = ldexpf(p[i], shift - inside);
+        if (ve == P8_NAN && sc[r][i >> 2][i & 3] != -INFINITY) p[i] = u2f(0x7fc00000u);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const _Float16 b = (_Float16)p[i];
+        pf[r][k][i >> 3][i & 7] = b;
+        if (k + 1 < NP) p[i] -= (float)b;
+      }
   }
 }
 
@@ -200,6 +201,28 @@ __device__ __forceinline__ uint32_t p8_clear_nan(u32x4& u) {
     u[i] &= ~(bits * 255u);
   }
   return any;
+}
+
+// NaN of tile t's V to the rows that see it (outputs of dims 16 d + 4 (l / 16) + i of this lane).
+template <int HD, int NR>
+__device__ __forceinline__ void p8_add_nan(P8Rows<HD, NR>& st, const uint8_t* vc, uint32_t page_bytes,
+                                           const Paged& g, const uint32_t* tab, uint32_t t, uint32_t len,
+                                           const uint32_t (&limit)[NR]) {
+  const uint32_t grp = (threadIdx.x & 63u) >> 4;
+#pragma unroll 1
+  for (uint32_t pos = t * P8_TILE; pos < min(len, (t + 1) * P8_TILE); ++pos) {
+    const uint32_t page = tab[pos >> g.shift];
+    if (page >= g.n_pages) continue;
+    const uint8_t* p = vc + p8_at(page, page_bytes, p8_v(g, pos & ((1u << g.shift) - 1u), 4 * grp));
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float add = (p[(16 * d + i) * 16] & 0x7fu) == 0x7fu ? u2f(0x7fc00000u) : 0.0f;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) st.o[r][d][i] += pos <= limit[r] ? add : 0.0f;
+      }
+  }
 }
 
 // Workgroups of a CU, by registers and LDS.
@@ -237,9 +260,13 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
   const uint32_t pmask = (1u << g.shift) - 1u;
   u32x4 kf[4][KG], vf[DS];
   uint32_t ke = 0, ve = 0, odd_tile = ~0u;
+  const uint32_t page_bytes = g.n_kv * HD << g.shift, page_exps = g.n_kv << (g.shift - 4);
+  const uint32_t head_exps = h << (g.shift - 4);
+  kc += h * head_bytes;
+  vc += h * head_bytes;
   const auto load_k = [&](uint32_t pos0, uint32_t page) {
     if (page >= g.n_pages) page = 0;
-    const uint8_t* p = kc + ((size_t)page * g.n_kv + h) * head_bytes + (((size_t)grp << g.shift) + ((pos0 + ko) & pmask)) * 16;
+    const uint8_t* p = kc + p8_at(page, page_bytes, ((grp << g.shift) + ((pos0 + ko) & pmask)) * 16);
 #pragma unroll
     for (int b = 0; b < 4; ++b)  // granules of 64 dims apart
       pa_load<STREAM, KG>(reinterpret_cast<const u32x4*>(p) + 4 * b, (size_t)4 << g.shift, kf[b]);
@@ -247,21 +274,21 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
   const auto load_v = [&](uint32_t pos0, uint32_t page) {
     if (page >= g.n_pages) page = 0;
     const uint32_t o = (pos0 + 16 * grp) & pmask;
-    const uint8_t* p = vc + ((size_t)page * g.n_kv + h) * head_bytes + ((size_t)(o >> 4) * HD + col) * 16;
+    const uint8_t* p = vc + p8_at(page, page_bytes, ((o >> 4) * HD + col) * 16);
     pa_load<STREAM, DS>(reinterpret_cast<const u32x4*>(p), 16, vf);
   };
   const auto load_e = [&](uint32_t pos0, uint32_t page) {
     if (page >= g.n_pages) page = 0;
-    const size_t at = p8_exp(g, page, h, (pos0 + 16 * grp) & pmask);
+    const uint64_t at = p8_at(page, page_exps, head_exps + (((pos0 + 16 * grp) & pmask) >> 4));
     ke = p8.ke[at];
     ve = p8.ve[at];
   };
   uint32_t pk = 0, pv = 0, pkn = 0, pvn = 0;
   if (ta < t1) {
-    pk = pa_page(a, tab, ta * P8_TILE + kpos, len);
-    pv = pa_page(a, tab, ta * P8_TILE + 16 * grp, len);
-    pkn = pa_page(a, tab, (ta + 4) * P8_TILE + kpos, len);
-    pvn = pa_page(a, tab, (ta + 4) * P8_TILE + 16 * grp, len);
+    pk = p8_page(a, tab, ta * P8_TILE + kpos, len);
+    pv = p8_page(a, tab, ta * P8_TILE + 16 * grp, len);
+    pkn = p8_page(a, tab, (ta + 4) * P8_TILE + kpos, len);
+    pvn = p8_page(a, tab, (ta + 4) * P8_TILE + 16 * grp, len);
   }
   // the query rows as operands in LDS: unit (row, 8 dims) of every thread, a row in HD / 8 lanes
   constexpr int LPR = HD / 8, UNITS = ROWS * LPR, PASSES = (UNITS + PA_NT - 1) / PA_NT;
@@ -344,8 +371,8 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
     const uint32_t ke_now = ke, ve_now = ve;
     uint32_t pv2 = 0;
     if (next) {
-      const uint32_t pk2 = pa_page(a, tab, (t + 8) * P8_TILE + kpos, len);
-      pv2 = pa_page(a, tab, (t + 8) * P8_TILE + 16 * grp, len);
+      const uint32_t pk2 = p8_page(a, tab, (t + 8) * P8_TILE + kpos, len);
+      pv2 = p8_page(a, tab, (t + 8) * P8_TILE + 16 * grp, len);
       load_k(pos0 + 4 * P8_TILE, pkn);
       load_e(pos0 + 4 * P8_TILE, pvn);
       pkn = pk2;
@@ -354,16 +381,12 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
     if (!page_ok) paged_flag(g, PG_BAD_PAGE);
     const bool edge = pos0 + P8_TILE - 1 > first || __ballot(!page_ok) != 0;
     f16x8 pf[NR][NP][2];
-    if (edge) {
-      p8_softmax<HD, NR, NP, true>(st, sc, factor, ke_now, ve_now, gpos, limit, page_ok, pf);
-      if (KT == TY_E4M3) {
-        uint32_t odd = 0;
+    p8_softmax<HD, NR, NP>(st, sc, factor, ke_now, ve_now, gpos, limit, page_ok, edge, pf);
+    if (KT == TY_E4M3 && edge) {
+      uint32_t odd = 0;
 #pragma unroll
-        for (int d = 0; d < DS; ++d) odd |= p8_clear_nan(vf[d]);
-        if (__ballot(odd != 0)) odd_tile = t;
-      }
-    } else {
-      p8_softmax<HD, NR, NP, false>(st, sc, factor, ke_now, ve_now, gpos, limit, page_ok, pf);
+      for (int d = 0; d < DS; ++d) odd |= p8_clear_nan(vf[d]);
+      if (__ballot(odd != 0)) odd_tile = t;
     }
 #pragma unroll
     for (int d = 0; d < DS; ++d) {
@@ -376,23 +399,7 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
 #pragma unroll
           for (int k = 0; k < 2; ++k) st.o[r][d] = Op16<TY_F16>::mfma(vv[k], pf[r][n][k], st.o[r][d]);
     }
-    if (odd_tile == t) {
-      // NaN in V to the rows that see it; this lane's outputs: dims 16 d + 4 grp + i
-#pragma unroll 1
-      for (uint32_t pos = pos0; pos < min(len, pos0 + P8_TILE); ++pos) {
-        const uint32_t page = tab[pos >> g.shift];
-        if (page >= g.n_pages) continue;
-        const uint8_t* p = vc + ((size_t)page * g.n_kv + h) * head_bytes + ((size_t)((pos & pmask) >> 4) * HD + 4 * grp) * 16 + (pos & 15u);
-#pragma unroll
-        for (int d = 0; d < DS; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float add = (p[(16 * d + i) * 16] & 0x7fu) == 0x7fu ? u2f(0x7fc00000u) : 0.0f;
-#pragma unroll
-            for (int r = 0; r < NR; ++r) st.o[r][d][i] += pos <= limit[r] ? add : 0.0f;
-          }
-      }
-    }
+    if (odd_tile == t) p8_add_nan<HD, NR>(st, vc, page_bytes, g, tab, t, len, limit);
     if (next) {
       pv = pvn;
       pvn = pv2;
@@ -448,6 +455,251 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
         a.part_ml[((size_t)pc.slot * a.part_rows + row) * 2] = M;
         a.part_ml[((size_t)pc.slot * a.part_rows + row) * 2 + 1] = L;
       }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Prompts: blocks of 128 query rows (64 for heads of 256), 32 (16) a wave, so that a tile's K and V are turned into
+// operands once for all of them, in LDS, while the tile before is multiplied.  The plan is the split's; tiles behind
+// a block's last row are left out.
+constexpr int p8p_nr(int hd) { return hd == 256 ? 1 : 2; }          // 16-row groups of a wave
+constexpr int p8p_rows(int hd) { return 4 * 16 * p8p_nr(hd); }      // rows of a block
+constexpr int p8p_lds(int hd) { return 2 * (2 * 64 * hd * 2 + 192) + 16; }
+// Tiles of a piece at most: enough for whole segments where there are many, pieces for all CUs where not.
+struct P8PromptTarget {
+  __device__ __forceinline__ uint32_t operator()(const PaArgs&, uint32_t total) const {
+    return max(16u, (total + 511) / 512);
+  }
+};
+
+template <int HD, int KT, int QT>
+__global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p8) {
+  typedef typename std::conditional<QT == TY_F32, float, typename std::conditional<QT == TY_F16, _Float16, __bf16>::type>::type QE;
+  typedef QE q8v __attribute__((ext_vector_type(8)));
+  constexpr int NQ = QT == TY_F32 ? 2 : 1, NP = QT == TY_F32 ? 2 : 1, KS = HD / 32, DS = HD / 16, KG = HD / 64;
+  constexpr int NR = p8p_nr(HD), ROWS = p8p_rows(HD);
+  constexpr uint32_t K_BYTES = 64 * HD * 2 + 192, BUF = K_BYTES + 64 * HD * 2;  // (64 bytes between the products' rows of K)
+  const PaArgs& a = p8.a;
+  extern __shared__ char lds[];  // [2] K operands [4][KS][64], V operands [DS][2][64]; [2] flags
+  uint32_t* s_odd = reinterpret_cast<uint32_t*>(lds + 2 * BUF);
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t col = lane & 15u, grp = lane >> 4;
+  const Paged& g = a.g;
+  PaPiece pc = pa_piece<ROWS / 16, P8_TILE, P8PromptTarget>(a, blockIdx.x, blockIdx.x == 0);
+  if (!pc.any) return;
+  const PaSeq& sq = pc.q;
+  // KV heads next to each other, so that with 8 of them each XCD's cache sees one; the rows with the most
+  // positions first
+  {
+    const uint32_t rest = pc.at / g.n_kv, block = rest / pc.n;
+    pc.h = pc.at - rest * g.n_kv;
+    pc.rb = sq.blocks - 1 - block;
+    pc.place(rest - block * pc.n);
+  }
+  const uint32_t s = pc.s, h = pc.h, rb = pc.rb, group = a.group;
+  const uint32_t* tab = g.table + (size_t)s * g.stride;
+  const uint32_t len = sq.len, first = sq.first;
+  const uint32_t last = first + pa_token(a, min(sq.rows, (rb + 1) * ROWS) - 1);  // position of the block's last row
+  const uint32_t t0 = pc.t0, t1 = min(pc.t1, last / P8_TILE + 1);
+  const uint8_t *kc = reinterpret_cast<const uint8_t*>(a.kc), *vc = reinterpret_cast<const uint8_t*>(a.vc);
+  const size_t head_bytes = (size_t)HD << g.shift;
+  const uint32_t pmask = (1u << g.shift) - 1u;
+  const uint32_t page_bytes = g.n_kv * HD << g.shift, page_exps = g.n_kv << (g.shift - 4);
+  const uint32_t head_exps = h << (g.shift - 4);
+  kc += h * head_bytes;
+  vc += h * head_bytes;
+
+  // ---- query rows of this wave: operands in registers
+  f16x8 qf[NR][NQ][KS];
+  P8Factor factor[NR];
+  uint32_t limit[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const uint32_t row = rb * ROWS + (w * NR + r) * 16 + col, t = pa_token(a, row), qh = h * group + (row - t * group);
+    q8v raw[KS];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      raw[j] = q8v{};
+      // dims of operand j: 8 of granule grp + 4 (j / 2)
+      if (row < sq.rows)
+        raw[j] = *reinterpret_cast<const q8v*>(static_cast<const QE*>(a.q) + ((size_t)s * a.n_new + t) * a.q_stride +
+                                               (size_t)qh * HD + 16 * (grp + 4 * (j >> 1)) + 8 * (j & 1));
+    }
+    if constexpr (QT != TY_F16) {
+#pragma unroll
+      for (int j = 0; j < KS; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, f2u((float)raw[j][i]) & 0x7fffffffu);
+      // (over the 4 lanes of a row)
+      auto x = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+      top = max((uint32_t)x[0], (uint32_t)x[1]);
+      auto y = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+      top = max((uint32_t)y[0], (uint32_t)y[1]);
+    }
+    int up = 0;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      f16x8 term[NQ];
+      up = p8_query<QT, NQ>(raw[j], top, a.scale < 0.0f, term);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) qf[r][n][j] = term[n];
+    }
+    factor[r] = p8_factor(a.scale, up);
+    limit[r] = first + (row < sq.rows ? t : 0u);
+  }
+
+  // ---- this thread's granules of a tile: K of position tid % 64, V of dims vd
+  u32x4 kraw[KG], vraw[KG];
+  uint32_t k_page = 0, v_page[KG], e_page = 0, ke = 0, ve = 0, ke_next = 0, ve_next = 0;
+  bool ok_now = true, ok_next = true;
+  const auto v_grp = [&](int i) { return (tid + PA_NT * i) / HD; };
+  const auto pages = [&](uint32_t t) {
+    const uint32_t pos0 = t * P8_TILE;
+    k_page = p8_page(a, tab, pos0 + lane, len);
+    e_page = p8_page(a, tab, pos0 + 16 * grp, len);
+#pragma unroll
+    for (int i = 0; i < KG; ++i) v_page[i] = p8_page(a, tab, pos0 + 16 * v_grp(i), len);
+  };
+  bool k_bad = false, v_bad[KG];
+  const auto fetch = [&](uint32_t t) {
+    const uint32_t pos0 = t * P8_TILE;
+    k_bad = k_page >= g.n_pages;
+    ok_next = e_page < g.n_pages;
+    const uint8_t* p = kc + p8_at(k_bad ? 0u : k_page, page_bytes, ((w << g.shift) + ((pos0 + lane) & pmask)) * 16);
+#pragma unroll
+    for (int i = 0; i < KG; ++i) kraw[i] = *reinterpret_cast<const u32x4*>(p + (((size_t)4 * i) << g.shift) * 16);
+#pragma unroll
+    for (int i = 0; i < KG; ++i) {
+      v_bad[i] = v_page[i] >= g.n_pages;
+      const uint32_t block = ((pos0 + 16 * v_grp(i)) & pmask) >> 4;
+      vraw[i] = *reinterpret_cast<const u32x4*>(
+          vc + p8_at(v_bad[i] ? 0u : v_page[i], page_bytes, (block * HD + (tid + PA_NT * i) % HD) * 16));
+    }
+    const uint64_t at = p8_at(ok_next ? e_page : 0u, page_exps, head_exps + (((pos0 + 16 * grp) & pmask) >> 4));
+    ke_next = p8.ke[at];
+    ve_next = p8.ve[at];
+  };
+  // the granules as operands into buffer b
+  const auto stage = [&](uint32_t t, uint32_t b) {
+    char* kd = lds + b * BUF;
+    char* vd = kd + K_BYTES;
+    // position p: row 4 (p / 16) + p % 4 of product (p / 4) % 4
+    const uint32_t prod = (lane >> 2) & 3u, pr = 4 * (lane >> 4) + (lane & 3u);
+#pragma unroll
+    for (int i = 0; i < KG; ++i) {
+      f16x8 x[2];
+      p8_operands<KT>(kraw[i], x);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<f16x8*>(kd + ((prod * KS + 2 * i + j) * 64 + 16 * w + pr) * 16 + 64 * prod) = x[j];
+    }
+    const bool edge = t * P8_TILE + P8_TILE - 1 > first;
+#pragma unroll
+    for (int i = 0; i < KG; ++i) {
+      const uint32_t dim = (tid + PA_NT * i) % HD;
+      if (KT == TY_E4M3 && (edge || v_bad[i])) {
+        const uint32_t odd = p8_clear_nan(vraw[i]);
+        if (odd && !v_bad[i]) s_odd[b] = 1;
+      }
+      f16x8 x[2];
+      p8_operands<KT>(vraw[i], x);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<f16x8*>(vd + (((dim >> 4) * 2 + j) * 64 + 16 * v_grp(i) + (dim & 15u)) * 16) = x[j];
+    }
+  };
+
+  P8Rows<HD, NR> st;
+  st.clear();
+  if (t0 < t1) {
+    if (tid < 2) s_odd[tid] = 0;
+    pages(t0);
+    fetch(t0);
+    pages(t0 + 1);
+    __syncthreads();
+    stage(t0, 0);
+    ke = ke_next;
+    ve = ve_next;
+    ok_now = ok_next;
+    if (t0 + 1 < t1) {
+      fetch(t0 + 1);
+      pages(t0 + 2);
+    }
+    __syncthreads();
+    for (uint32_t t = t0, b = 0; t < t1; ++t, b ^= 1) {
+      const char* kd = lds + b * BUF;
+      const char* vd = kd + K_BYTES;
+      f32x4 sc[NR][4];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sc[r][k] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < KS; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const f16x8 kk = *reinterpret_cast<const f16x8*>(kd + ((k * KS + j) * 64 + lane) * 16 + 64 * k);
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int n = NQ - 1; n >= 0; --n) sc[r][k] = Op16<TY_F16>::mfma(kk, qf[r][n][j], sc[r][k]);
+        }
+      const uint32_t gpos = t * P8_TILE + 16 * grp;  // this lane's 16 positions
+      if (!ok_now) paged_flag(g, PG_BAD_PAGE);
+      f16x8 pf[NR][NP][2];
+      p8_softmax<HD, NR, NP>(st, sc, factor, ke, ve, gpos, limit, ok_now,
+                             t * P8_TILE + P8_TILE - 1 > first || __ballot(!ok_now) != 0, pf);
+      const bool odd = KT == TY_E4M3 && s_odd[b];
+      if (t + 1 < t1) {
+        stage(t + 1, b ^ 1);
+        ke = ke_next;
+        ve = ve_next;
+        ok_now = ok_next;
+        if (t + 2 < t1) {
+          fetch(t + 2);
+          pages(t + 3);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DS; ++d)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const f16x8 vv = *reinterpret_cast<const f16x8*>(vd + ((d * 2 + k) * 64 + lane) * 16);
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int n = NP - 1; n >= 0; --n) st.o[r][d] = Op16<TY_F16>::mfma(vv, pf[r][n][k], st.o[r][d]);
+        }
+      if (odd) p8_add_nan<HD, NR>(st, vc, page_bytes, g, tab, t, len, limit);
+      __syncthreads();
+    }
+  }
+
+  // ---- rows finished, or a part written
+  if (pc.t0 == 0 && tid == 0) a.cuts[((size_t)s * g.n_kv + h) * a.blocks + rb] = make_uint2(pc.slot, pc.n);
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const uint32_t in = (w * NR + r) * 16 + col, full = rb * ROWS + in;
+    const float L = ldexpf(pa_sum4(st.l[r]), -24);
+    const int unit = st.D[r] == -INFINITY ? 0 : (int)fmaxf(-512.0f, fminf(512.0f, st.D[r])) - 14 - 24;
+    if (full >= sq.rows) continue;
+    const uint32_t t = pa_token(a, full);
+    const size_t dst = ((size_t)s * a.n_new + t) * a.out_stride + (size_t)(h * group + (full - t * group)) * HD + 4 * grp;
+#pragma unroll
+    for (int d = 0; d < DS; ++d) {
+      f32x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = ldexpf(st.o[r][d][i], unit);
+      if (pc.n == 1)
+        pa_store4<QT>(a.out, dst + 16 * d, st.m[r] == -INFINITY ? f32x4{0, 0, 0, 0} : y / L);  // (no position left: zeros)
+      else
+        *reinterpret_cast<f32x4*>(&a.part_o[((size_t)pc.slot * a.part_rows + in) * HD + 16 * d + 4 * grp]) = y;
+    }
+    if (pc.n > 1 && grp == 0) {
+      a.part_ml[((size_t)pc.slot * a.part_rows + in) * 2] = st.m[r];
+      a.part_ml[((size_t)pc.slot * a.part_rows + in) * 2 + 1] = L;
     }
   }
 }

@@ -169,8 +169,16 @@ struct PaTarget {
 
 struct PaPiece {
   uint32_t s, h, rb, t0, t1, n, slot;  // n: the segment's pieces; slot: this piece's (n > 1)
+  uint32_t at, slots;                  // index among the sequence's pieces, the sequence's first slot
   PaSeq q;
   bool any;
+  // Piece `piece` of segment (h, rb).
+  __device__ __forceinline__ void place(uint32_t piece) {
+    const uint32_t even = q.tiles / n, more = q.tiles - even * n;  // the first `more` pieces take one tile more
+    t0 = piece * even + min(piece, more);
+    t1 = t0 + even + (piece < more ? 1u : 0u);
+    slot = slots + (h * q.blocks + rb) * n + piece;
+  }
 };
 
 // Piece `index` of the batch (pieces in the order sequence, KV head, block, tiles).  Each wave works
@@ -213,13 +221,12 @@ __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, boo
   p.s = s;
   p.q = q;
   p.n = count(q);
-  const uint32_t at = index - before, seg = at / p.n, piece = at - seg * p.n;
+  p.slots = slots;
+  p.at = index - before;
+  const uint32_t seg = p.at / p.n;
   p.h = q.blocks == 1 ? seg : seg / q.blocks;
   p.rb = seg - p.h * q.blocks;
-  const uint32_t even = q.tiles / p.n, more = q.tiles - even * p.n;  // the first `more` pieces take one tile more
-  p.t0 = piece * even + min(piece, more);
-  p.t1 = p.t0 + even + (piece < more ? 1u : 0u);
-  p.slot = slots + seg * p.n + piece;
+  p.place(p.at - seg * p.n);
   return p;
 }
 

@@ -46,6 +46,7 @@ uint32_t log2_of(uint32_t power) {
 // What a call of the attention needs: row blocks of 16 * nr query rows, workgroups, workspace.
 struct P8Sizes {
   uint32_t nr, blocks, part_rows, at_once, grid;
+  bool prompt;                 // the prompts' kernel
   bool join;                   // some segment may be cut
   bool fits;                   // the plan's 32-bit counts hold
   size_t part_o, cuts, bytes;  // offsets of the workspace's parts, its size
@@ -54,18 +55,19 @@ struct P8Sizes {
 P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap) {
   P8Sizes z;
   const uint64_t rows = n_new * (n_heads / n_kv), cap_tiles = (cap + cm::P8_TILE - 1) / cm::P8_TILE;
-  z.nr = rows > 16 && hd <= 128 ? 2 : 1;
+  z.prompt = n_new > CAMELID_MAX_VERIFY_K && rows >= 128;
+  z.nr = z.prompt ? cm::p8p_rows((int)hd) / 16 : rows > 16 && hd <= 128 ? 2 : 1;
   z.blocks = (uint32_t)((rows + 16 * z.nr - 1) / (16 * z.nr));
   z.part_rows = (uint32_t)std::min<uint64_t>(rows, 16 * z.nr);
   // 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
-  z.at_once = 256 * cm::p8_per_cu((int)hd, (int)z.nr) * 7 / 8;
-  const uint64_t segments = n_seqs * n_kv * z.blocks, most = 2048;
-  // a segment has at most ceil(its tiles / 4) pieces, all of them together at most 2048 and one each
-  const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + 3) / 4));
+  z.at_once = z.prompt ? 0 : 256 * cm::p8_per_cu((int)hd, (int)z.nr) * 7 / 8;
+  // a piece has at least `least` tiles, or all; pieces altogether are at most `most` and one for each segment
+  const uint64_t segments = n_seqs * n_kv * z.blocks, least = z.prompt ? 16 : 4, most = z.prompt ? 512 : 2048;
+  const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + least - 1) / least));
   z.fits = segments * cap_tiles < (1ull << 31) && grid_ok(pieces, cm::PA_NT);
   z.grid = (uint32_t)pieces;
-  z.join = cap_tiles > 4;
-  // cut segments have more tiles than the target: at most 2048 of them, twice as many pieces
+  z.join = cap_tiles > least;
+  // cut segments have more tiles than the target: at most `most` of them, twice as many pieces
   const size_t slots = z.join ? (size_t)std::min(2 * most, pieces) : 0;
   z.part_o = up256(slots * z.part_rows * 8);
   z.cuts = z.part_o + up256(slots * z.part_rows * hd * 4);
@@ -73,32 +75,52 @@ P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_k
   return z;
 }
 
-template <int HD, int KT, int QT, int NR>
-bool p8_launch(const cm::P8Args& p, const P8Sizes& z, hipStream_t stream) {
-  const cm::PaArgs& a = p.a;
-  // K and V that the batch's tables can hold, against the 256 MB of the memory-side cache (several row blocks read
-  // them several times)
-  const bool passing = z.blocks == 1 && ((uint64_t)a.g.n_seqs * a.g.n_kv * HD * 2 * a.g.stride << a.g.shift) > (256u << 20);
-  const auto split = passing ? cm::k_p8_split<HD, KT, QT, NR, true> : cm::k_p8_split<HD, KT, QT, NR, false>;
-  constexpr size_t lds = (size_t)16 * NR * (4 * (HD + 4 + 2) + 2) * 4;
-  if (lds > 64 * 1024) {
-    const hipError_t st = hipFuncSetAttribute(reinterpret_cast<const void*>(split),
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (st != hipSuccess) return cm::fail_global("paged8_attention", hipGetErrorString(st)) == 0;
-  }
-  hipLaunchKernelGGL(split, dim3(z.grid), dim3(cm::PA_NT), lds, stream, p);
-  if (!z.join) return true;
-  const uint32_t rows = a.n_new * a.group, sh = a.g.n_seqs * a.g.n_kv;
-  const uint32_t cap = a.g.stride << a.g.shift;
+template <int HD, int QT, int NR>
+void p8_join(const cm::PaArgs& a, hipStream_t stream) {
+  const uint32_t rows = a.n_new * a.group, sh = a.g.n_seqs * a.g.n_kv, cap = a.g.stride << a.g.shift;
   const auto join = [&](auto per, auto kernel) {
     const uint32_t row_groups = (rows + per.value - 1) / per.value;
     hipLaunchKernelGGL(kernel, dim3(sh * row_groups), dim3(cm::PA_NT), 0, stream, a, rows, row_groups, 0u, 8u);
   };
-  if (cap <= 16 * 4 * cm::P8_TILE || sh >= 256)
+  if (NR > 2 || cap <= 16 * 4 * cm::P8_TILE || sh >= 256)
     join(std::integral_constant<uint32_t, cm::pj_parts(HD)>{}, cm::k_pa_join<HD, QT, NR, cm::pj_parts(HD)>);
   else
     join(std::integral_constant<uint32_t, 1>{}, cm::k_pa_join<HD, QT, NR, 1>);
+}
+
+bool p8_start(void (*kernel)(cm::P8Args), const cm::P8Args& p, const P8Sizes& z, size_t lds, hipStream_t stream) {
+  if (lds > 64 * 1024) {
+    const hipError_t st = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (st != hipSuccess) return cm::fail_global("paged8_attention", hipGetErrorString(st)) == 0;
+  }
+  hipLaunchKernelGGL(kernel, dim3(z.grid), dim3(cm::PA_NT), lds, stream, p);
   return true;
+}
+
+template <int HD, int KT, int QT, int NR>
+bool p8_split(const cm::P8Args& p, const P8Sizes& z, hipStream_t stream) {
+  const cm::PaArgs& a = p.a;
+  // K and V that the batch's tables can hold, against the 256 MB of the memory-side cache (several row blocks read
+  // them several times)
+  const bool passing = z.blocks == 1 && ((uint64_t)a.g.n_seqs * a.g.n_kv * HD * 2 * a.g.stride << a.g.shift) > (256u << 20);
+  constexpr size_t lds = (size_t)16 * NR * (4 * (HD + 4 + 2) + 2) * 4;
+  if (!p8_start(passing ? cm::k_p8_split<HD, KT, QT, NR, true> : cm::k_p8_split<HD, KT, QT, NR, false>, p, z, lds, stream))
+    return false;
+  if (z.join) p8_join<HD, QT, NR>(a, stream);
+  return true;
+}
+
+template <int HD, int KT, int QT>
+bool p8_launch(const cm::P8Args& p, const P8Sizes& z, hipStream_t stream) {
+  if (z.prompt) {
+    if (!p8_start(cm::k_p8_prompt<HD, KT, QT>, p, z, cm::p8p_lds(HD), stream)) return false;
+    if (z.join) p8_join<HD, QT, cm::p8p_rows(HD) / 16>(p.a, stream);
+    return true;
+  }
+  if constexpr (HD <= 128)
+    if (z.nr == 2) return p8_split<HD, KT, QT, 2>(p, z, stream);
+  return p8_split<HD, KT, QT, 1>(p, z, stream);
 }
 
 }  // namespace
@@ -236,12 +258,7 @@ int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stri
   a.part_rows = z.part_rows;
   bool ok = true;
   by_types(hd, kv_type, q_type, [&](auto d, auto k, auto t) {
-    if constexpr (d() <= 128)
-      if (z.nr == 2) {
-        ok = p8_launch<d(), k(), t(), 2>(p, z, (hipStream_t)stream);
-        return;
-      }
-    ok = p8_launch<d(), k(), t(), 1>(p, z, (hipStream_t)stream);
+    ok = p8_launch<d(), k(), t()>(p, z, (hipStream_t)stream);
   });
   return ok ? launched(me) : 1;
 }
