@@ -102,16 +102,19 @@ __device__ __forceinline__ uint32_t p8_page(const PaArgs& a, const uint32_t* tab
 // page * unit + more, one multiply-add (unit: bytes of a page, at most 2^30).
 __device__ __forceinline__ uint64_t p8_at(uint32_t page, uint32_t unit, uint32_t more) { return (uint64_t)page * unit + more; }
 
+constexpr float P8_NONE = -1e30f;  // no reference of o yet
+
 // What a wave keeps of its 16 NR rows (lane: row 16 r + l % 16, outputs of dims 16 d + 4 (l / 16) + i).
 template <int HD, int NR>
 struct P8Rows {
   f32x4 o[NR][HD / 16];  // in units of 2^(D - 14)
-  float m[NR], D[NR];    // softmax reference, and the reference of o relative to it; whole numbers
+  float m[NR], D[NR];    // softmax reference, and the reference of o relative to it; whole numbers (none: the lowest)
   float l[NR];           // this lane's share of the sum
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      m[r] = D[r] = -INFINITY;
+      m[r] = PA_LOWEST;
+      D[r] = P8_NONE;
       l[r] = 0.0f;
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) o[r][d] = f32x4{0, 0, 0, 0};
@@ -141,42 +144,44 @@ __device__ __forceinline__ void p8_softmax(P8Rows<HD, NR>& st, f32x4 (&sc)[NR][4
     for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[r][i >> 2][i & 3]);
     const float ctop = ceilf(top * fk);  // (the factor is not negative)
     // the reference of the exponents is a whole number: rescaling by powers of two is exact
-    const float m_new = fmaxf(st.m[r], pa_max4(ctop)), ref = m_new == -INFINITY ? 0.0f : m_new;
-    const float d_tile = pa_max4(ctop - ref + vexp);
+    const float m_new = fmaxf(st.m[r], pa_max4(ctop));
+    const float d_tile = pa_max4(ctop - m_new + vexp);
     if (__ballot(m_new > st.m[r] || d_tile > st.D[r])) {
-      const float down = st.m[r] - ref, d_old = st.D[r] + down;
+      const float down = st.m[r] - m_new, d_old = st.D[r] + down;
       st.l[r] *= __builtin_amdgcn_exp2f(down);
       st.m[r] = m_new;
-      st.D[r] = fmaxf(d_old, d_tile);
-      const float alpha = __builtin_amdgcn_exp2f(d_old - (st.D[r] == -INFINITY ? 0.0f : st.D[r]));
+      st.D[r] = fmaxf(fmaxf(d_old, d_tile), P8_NONE);
+      const float alpha = __builtin_amdgcn_exp2f(d_old - st.D[r]);
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) st.o[r][d] *= alpha;
     }
-    float base = -ref;
-    if (__ballot(fabsf(ref) >= 1024.0f)) {
+    float base = -m_new;
+    if (__ballot(fabsf(m_new) >= 1024.0f)) {
       // far from zero the product before its rounding may lie well above the reference, which comes from the
       // rounded ones, and the shift below may be lost in the reference
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[r][i >> 2][i & 3] = sc[r][i >> 2][i & 3] * fk - ref;
+      for (int i = 0; i < 16; ++i) sc[r][i >> 2][i & 3] = sc[r][i >> 2][i & 3] * fk - m_new;
       fk = 1.0f;
       base = 0.0f;
     }
     // weights times 2^shift are what the matrix cores get: 2^14 at most.  Inside the exponent the shift costs
     // nothing, and up to 16 of it no bits that matter (half a step of an argument of 16 is 2^-21)
-    const float d_ref = st.D[r] == -INFINITY ? 0.0f : st.D[r];
-    const int shift = (int)fmaxf(-512.0f, fminf(512.0f, vexp - d_ref + 14.0f)), inside = max(shift, -16);
-    base += (float)inside;
+    const float shift = vexp - st.D[r] + 14.0f, inside = fmaxf(shift, -16.0f);
+    base += inside;
     float sum = 0.0f, p[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], fk, base));
       sum += p[i];
     }
-    st.l[r] += ldexpf(sum, -inside);
-    if (__ballot(shift < -16 || ve == P8_NAN)) {
+    sum = ldexpf(sum, (int)-inside);
+    asm volatile("" : "+v"(sum));  // (summed here: later it would keep copies of the weights)
+    st.l[r] += sum;
+    if (__ballot(shift < -16.0f || ve == P8_NAN)) {
+      const int more = (int)(shift - inside);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        p[i] = ldexpf(p[i], shift - inside);
+        p[i] = ldexpf(p[i], more);
         if (ve == P8_NAN && sc[r][i >> 2][i & 3] != -INFINITY) p[i] = u2f(0x7fc00000u);
       }
     }
@@ -414,10 +419,10 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
   for (int r = 0; r < NR; ++r) {
     const float sum = pa_sum4(st.l[r]);
     if (grp == 0) {
-      s_ml[(w * ROWS + r * 16 + col) * 2] = st.m[r];
+      s_ml[(w * ROWS + r * 16 + col) * 2] = sum == 0.0f ? -INFINITY : st.m[r];  // (no position: no weight)
       s_ml[(w * ROWS + r * 16 + col) * 2 + 1] = ldexpf(sum, -24);
     }
-    const int unit = st.D[r] == -INFINITY ? 0 : (int)fmaxf(-512.0f, fminf(512.0f, st.D[r])) - 14 - 24;
+    const int unit = (int)fmaxf(-512.0f, fminf(512.0f, st.D[r])) - 14 - 24;
 #pragma unroll
     for (int d = 0; d < DS; ++d) {
       f32x4 y;
@@ -663,14 +668,18 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
         }
       }
 #pragma unroll
-      for (int d = 0; d < DS; ++d)
+      for (int d0 = 0; d0 < DS; d0 += 2)  // (two dims' chains in turn)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const f16x8 vv = *reinterpret_cast<const f16x8*>(vd + ((d * 2 + k) * 64 + lane) * 16);
+          f16x8 vv[2];
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
+          for (int d = 0; d < 2; ++d) vv[d] = *reinterpret_cast<const f16x8*>(vd + (((d0 + d) * 2 + k) * 64 + lane) * 16);
 #pragma unroll
-            for (int n = NP - 1; n >= 0; --n) st.o[r][d] = Op16<TY_F16>::mfma(vv, pf[r][n][k], st.o[r][d]);
+          for (int n = NP - 1; n >= 0; --n)
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+#pragma unroll
+              for (int r = 0; r < NR; ++r) st.o[r][d0 + d] = Op16<TY_F16>::mfma(vv[d], pf[r][n][k], st.o[r][d0 + d]);
         }
       if (odd) p8_add_nan<HD, NR>(st, vc, page_bytes, g, tab, t, len, limit);
       __syncthreads();
@@ -683,7 +692,7 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
   for (int r = 0; r < NR; ++r) {
     const uint32_t in = (w * NR + r) * 16 + col, full = rb * ROWS + in;
     const float L = ldexpf(pa_sum4(st.l[r]), -24);
-    const int unit = st.D[r] == -INFINITY ? 0 : (int)fmaxf(-512.0f, fminf(512.0f, st.D[r])) - 14 - 24;
+    const int unit = (int)fmaxf(-512.0f, fminf(512.0f, st.D[r])) - 14 - 24;
     if (full >= sq.rows) continue;
     const uint32_t t = pa_token(a, full);
     const size_t dst = ((size_t)s * a.n_new + t) * a.out_stride + (size_t)(h * group + (full - t * group)) * HD + 4 * grp;
@@ -693,12 +702,12 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = ldexpf(st.o[r][d][i], unit);
       if (pc.n == 1)
-        pa_store4<QT>(a.out, dst + 16 * d, st.m[r] == -INFINITY ? f32x4{0, 0, 0, 0} : y / L);  // (no position left: zeros)
+        pa_store4<QT>(a.out, dst + 16 * d, L == 0.0f ? f32x4{0, 0, 0, 0} : y / L);  // (no position left: zeros)
       else
         *reinterpret_cast<f32x4*>(&a.part_o[((size_t)pc.slot * a.part_rows + in) * HD + 16 * d + 4 * grp]) = y;
     }
     if (pc.n > 1 && grp == 0) {
-      a.part_ml[((size_t)pc.slot * a.part_rows + in) * 2] = st.m[r];
+      a.part_ml[((size_t)pc.slot * a.part_rows + in) * 2] = L == 0.0f ? -INFINITY : st.m[r];
       a.part_ml[((size_t)pc.slot * a.part_rows + in) * 2 + 1] = L;
     }
   }
