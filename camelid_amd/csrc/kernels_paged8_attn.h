@@ -129,71 +129,98 @@ __device__ __forceinline__ void p8_softmax(P8Rows<HD, NR>& st, f32x4 (&sc)[NR][4
                                            uint32_t ve, uint32_t gpos, const uint32_t (&limit)[NR], bool page_ok, bool edge,
                                            f16x8 (&pf)[NR][NP][2]) {
   const float vexp = (float)((int)ve - 127);
+  // (each step for all rows: their chains run side by side)
+  float fk[NR], m_new[NR], d_tile[NR], base[NR], shift[NR], inside[NR], p[NR][16];
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    float fk = p8_times(factor[r], ke);
-    if (edge) {  // positions that the row does not see: -infinity (their factor a positive number)
+  for (int r = 0; r < NR; ++r) fk[r] = p8_times(factor[r], ke);
+  if (edge) {  // positions that the row does not see: -infinity (their factor a positive number)
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
       const uint32_t n = !page_ok || limit[r] < gpos ? 0u : limit[r] - gpos + 1;
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[r][i >> 2][i & 3] = (uint32_t)i < n ? sc[r][i >> 2][i & 3] : -INFINITY;
-      fk = n ? fmaxf(fk, 0x1p-126f) : 1.0f;
-      if (n && ke == P8_NAN) fk = u2f(0x7fc00000u);
+      fk[r] = n ? fmaxf(fk[r], 0x1p-126f) : 1.0f;
+      if (n && ke == P8_NAN) fk[r] = u2f(0x7fc00000u);
     }
+  }
+  bool rises = false, far = false, fine = false;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
     float top = sc[r][0][0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[r][i >> 2][i & 3]);
-    const float ctop = ceilf(top * fk);  // (the factor is not negative)
+    const float ctop = ceilf(top * fk[r]);  // (the factor is not negative)
     // the reference of the exponents is a whole number: rescaling by powers of two is exact
-    const float m_new = fmaxf(st.m[r], pa_max4(ctop));
-    const float d_tile = pa_max4(ctop - m_new + vexp);
-    if (__ballot(m_new > st.m[r] || d_tile > st.D[r])) {
-      const float down = st.m[r] - m_new, d_old = st.D[r] + down;
+    m_new[r] = fmaxf(st.m[r], pa_max4(ctop));
+    d_tile[r] = pa_max4(ctop - m_new[r] + vexp);
+    rises |= m_new[r] > st.m[r] || d_tile[r] > st.D[r];
+    far |= fabsf(m_new[r]) >= 1024.0f;
+  }
+  if (__ballot(rises)) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float down = st.m[r] - m_new[r], d_old = st.D[r] + down;
       st.l[r] *= __builtin_amdgcn_exp2f(down);
-      st.m[r] = m_new;
-      st.D[r] = fmaxf(fmaxf(d_old, d_tile), P8_NONE);
+      st.m[r] = m_new[r];
+      st.D[r] = fmaxf(fmaxf(d_old, d_tile[r]), P8_NONE);
       const float alpha = __builtin_amdgcn_exp2f(d_old - st.D[r]);
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) st.o[r][d] *= alpha;
     }
-    float base = -m_new;
-    if (__ballot(fabsf(m_new) >= 1024.0f)) {
-      // far from zero the product before its rounding may lie well above the reference, which comes from the
-      // rounded ones, and the shift below may be lost in the reference
+  }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[r][i >> 2][i & 3] = sc[r][i >> 2][i & 3] * fk - m_new;
-      fk = 1.0f;
-      base = 0.0f;
+  for (int r = 0; r < NR; ++r) base[r] = -m_new[r];
+  if (__ballot(far)) {
+    // far from zero the product before its rounding may lie well above the reference, which comes from the
+    // rounded ones, and the shift below may be lost in the reference
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[r][i >> 2][i & 3] = sc[r][i >> 2][i & 3] * fk[r] - m_new[r];
+      fk[r] = 1.0f;
+      base[r] = 0.0f;
     }
-    // weights times 2^shift are what the matrix cores get: 2^14 at most.  Inside the exponent the shift costs
-    // nothing, and up to 16 of it no bits that matter (half a step of an argument of 16 is 2^-21)
-    const float shift = vexp - st.D[r] + 14.0f, inside = fmaxf(shift, -16.0f);
-    base += inside;
-    float sum = 0.0f, p[16];
+  }
+  // weights times 2^shift are what the matrix cores get: 2^14 at most.  Inside the exponent the shift costs
+  // nothing, and up to 16 of it no bits that matter (half a step of an argument of 16 is 2^-21)
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    shift[r] = vexp - st.D[r] + 14.0f;
+    inside[r] = fmaxf(shift[r], -16.0f);
+    base[r] += inside[r];
+    fine |= shift[r] < -16.0f || ve == P8_NAN;
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], fk, base));
-      sum += p[i];
+      p[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i >> 2][i & 3], fk[r], base[r]));
+      sum += p[r][i];
     }
-    sum = ldexpf(sum, (int)-inside);
+    sum = ldexpf(sum, (int)-inside[r]);
     asm volatile("" : "+v"(sum));  // (summed here: later it would keep copies of the weights)
     st.l[r] += sum;
-    if (__ballot(shift < -16.0f || ve == P8_NAN)) {
-      const int more = (int)(shift - inside);
+  }
+  if (__ballot(fine)) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int more = (int)(shift[r] - inside[r]);
+      const uint32_t n = !edge ? 16u : !page_ok || limit[r] < gpos ? 0u : limit[r] - gpos + 1;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        p[i] = ldexpf(p[i], more);
-        if (ve == P8_NAN && sc[r][i >> 2][i & 3] != -INFINITY) p[i] = u2f(0x7fc00000u);
+        p[r][i] = ldexpf(p[r][i], more);
+        if (ve == P8_NAN && (uint32_t)i < n) p[r][i] = u2f(0x7fc00000u);
       }
     }
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
 #pragma unroll
     for (int k = 0; k < NP; ++k)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const _Float16 b = (_Float16)p[i];
+        const _Float16 b = (_Float16)p[r][i];
         pf[r][k][i >> 3][i & 7] = b;
-        if (k + 1 < NP) p[i] -= (float)b;
+        if (k + 1 < NP) p[r][i] -= (float)b;
       }
-  }
 }
 
 // NaN bytes (e4m3) of an operand's granule to zero: a zero weight times them would be NaN.  Whether there were any.
@@ -468,22 +495,24 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
 // Prompts: blocks of 128 query rows (64 for heads of 256), 32 (16) a wave, so that a tile's K and V are turned into
 // operands once for all of them, in LDS, while the tile before is multiplied.  The plan is the split's; tiles behind
 // a block's last row are left out.
-constexpr int p8p_nr(int hd) { return hd == 256 ? 1 : 2; }          // 16-row groups of a wave
-constexpr int p8p_rows(int hd) { return 4 * 16 * p8p_nr(hd); }      // rows of a block
+constexpr int p8p_rows(int hd) { return hd == 256 ? 64 : 128; }  // rows of a block
 constexpr int p8p_lds(int hd) { return 2 * (2 * 64 * hd * 2 + 192) + 16; }
-// Tiles of a piece at most: enough for whole segments where there are many, pieces for all CUs where not.
+// Tiles of a piece at most: `at_once` (4 where the batch is small, else 16: a piece's part is written and read again,
+// 64 KB), and more once that makes over 512 pieces, two for each CU.
 struct P8PromptTarget {
-  __device__ __forceinline__ uint32_t operator()(const PaArgs&, uint32_t total) const {
-    return max(16u, (total + 511) / 512);
+  __device__ __forceinline__ uint32_t operator()(const PaArgs& a, uint32_t total) const {
+    return max(a.at_once, (total + 511) / 512);
   }
 };
 
-template <int HD, int KT, int QT>
-__global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p8) {
+template <int HD, int KT, int QT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p8) {
   typedef typename std::conditional<QT == TY_F32, float, typename std::conditional<QT == TY_F16, _Float16, __bf16>::type>::type QE;
   typedef QE q8v __attribute__((ext_vector_type(8)));
-  constexpr int NQ = QT == TY_F32 ? 2 : 1, NP = QT == TY_F32 ? 2 : 1, KS = HD / 32, DS = HD / 16, KG = HD / 64;
-  constexpr int NR = p8p_nr(HD), ROWS = p8p_rows(HD);
+  constexpr int NQ = QT == TY_F32 ? 2 : 1, NP = QT == TY_F32 ? 2 : 1, KS = HD / 32, DS = HD / 16;
+  constexpr int ROWS = p8p_rows(HD), NR = ROWS / 16 / WAVES, NT = 64 * WAVES;
+  constexpr int KG = (HD / 16 + WAVES - 1) / WAVES;  // granules of K (and of V) of a thread
+  constexpr bool ALL = HD / 16 >= WAVES;             // else of the first HD / 16 waves
   constexpr uint32_t K_BYTES = 64 * HD * 2 + 192, BUF = K_BYTES + 64 * HD * 2;  // (64 bytes between the products' rows of K)
   const PaArgs& a = p8.a;
   extern __shared__ char lds[];  // [2] K operands [4][KS][64], V operands [DS][2][64]; [2] flags
@@ -522,21 +551,21 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     const uint32_t row = rb * ROWS + (w * NR + r) * 16 + col, t = pa_token(a, row), qh = h * group + (row - t * group);
-    q8v raw[KS];
+    q8v qr[KS];
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
-      raw[j] = q8v{};
+      qr[j] = q8v{};
       // dims of operand j: 8 of granule grp + 4 (j / 2)
       if (row < sq.rows)
-        raw[j] = *reinterpret_cast<const q8v*>(static_cast<const QE*>(a.q) + ((size_t)s * a.n_new + t) * a.q_stride +
+        qr[j] = *reinterpret_cast<const q8v*>(static_cast<const QE*>(a.q) + ((size_t)s * a.n_new + t) * a.q_stride +
                                                (size_t)qh * HD + 16 * (grp + 4 * (j >> 1)) + 8 * (j & 1));
     }
     if constexpr (QT != TY_F16) {
 #pragma unroll
       for (int j = 0; j < KS; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, f2u((float)raw[j][i]) & 0x7fffffffu);
+        for (int i = 0; i < 8; ++i) top = max(top, f2u((float)qr[j][i]) & 0x7fffffffu);
       // (over the 4 lanes of a row)
       auto x = __builtin_amdgcn_permlane32_swap(top, top, false, false);
       top = max((uint32_t)x[0], (uint32_t)x[1]);
@@ -547,7 +576,7 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
       f16x8 term[NQ];
-      up = p8_query<QT, NQ>(raw[j], top, a.scale < 0.0f, term);
+      up = p8_query<QT, NQ>(qr[j], top, a.scale < 0.0f, term);
 #pragma unroll
       for (int n = 0; n < NQ; ++n) qf[r][n][j] = term[n];
     }
@@ -555,11 +584,16 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
     limit[r] = first + (row < sq.rows ? t : 0u);
   }
 
-  // ---- this thread's granules of a tile: K of position tid % 64, V of dims vd
-  u32x4 kraw[KG], vraw[KG];
-  uint32_t k_page = 0, v_page[KG], e_page = 0, ke = 0, ve = 0, ke_next = 0, ve_next = 0;
-  bool ok_now = true, ok_next = true;
-  const auto v_grp = [&](int i) { return (tid + PA_NT * i) / HD; };
+  // ---- this thread's granules of a tile: K of position tid % 64, V of dims (tid + NT i) % HD.  The next
+  // tile's are on their way while one is multiplied (two tiles ahead: no gain)
+  struct Raw {
+    u32x4 k[KG], v[KG];
+    uint32_t ke, ve;
+    bool ok, v_bad[KG];
+  };
+  Raw raw;
+  uint32_t k_page = 0, v_page[KG], e_page = 0;
+  const auto v_grp = [&](int i) { return min(3u, (tid + NT * i) / HD); };
   const auto pages = [&](uint32_t t) {
     const uint32_t pos0 = t * P8_TILE;
     k_page = p8_page(a, tab, pos0 + lane, len);
@@ -567,27 +601,32 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
 #pragma unroll
     for (int i = 0; i < KG; ++i) v_page[i] = p8_page(a, tab, pos0 + 16 * v_grp(i), len);
   };
-  bool k_bad = false, v_bad[KG];
-  const auto fetch = [&](uint32_t t) {
+  // tile t's granules, then the pages of the tile behind it (those first in the queue: loads come back in order)
+  const auto fetch = [&](uint32_t t, Raw& to) {
     const uint32_t pos0 = t * P8_TILE;
-    k_bad = k_page >= g.n_pages;
-    ok_next = e_page < g.n_pages;
-    const uint8_t* p = kc + p8_at(k_bad ? 0u : k_page, page_bytes, ((w << g.shift) + ((pos0 + lane) & pmask)) * 16);
-#pragma unroll
-    for (int i = 0; i < KG; ++i) kraw[i] = *reinterpret_cast<const u32x4*>(p + (((size_t)4 * i) << g.shift) * 16);
+    const uint8_t* kp = kc + p8_at(k_page < g.n_pages ? k_page : 0u, page_bytes, ((w << g.shift) + ((pos0 + lane) & pmask)) * 16);
+    const uint8_t* vp[KG];
 #pragma unroll
     for (int i = 0; i < KG; ++i) {
-      v_bad[i] = v_page[i] >= g.n_pages;
+      to.v_bad[i] = v_page[i] >= g.n_pages;
       const uint32_t block = ((pos0 + 16 * v_grp(i)) & pmask) >> 4;
-      vraw[i] = *reinterpret_cast<const u32x4*>(
-          vc + p8_at(v_bad[i] ? 0u : v_page[i], page_bytes, (block * HD + (tid + PA_NT * i) % HD) * 16));
+      vp[i] = vc + p8_at(to.v_bad[i] ? 0u : v_page[i], page_bytes, (block * HD + (tid + NT * i) % HD) * 16);
     }
-    const uint64_t at = p8_at(ok_next ? e_page : 0u, page_exps, head_exps + (((pos0 + 16 * grp) & pmask) >> 4));
-    ke_next = p8.ke[at];
-    ve_next = p8.ve[at];
+    to.ok = e_page < g.n_pages;
+    const uint64_t at = p8_at(to.ok ? e_page : 0u, page_exps, head_exps + (((pos0 + 16 * grp) & pmask) >> 4));
+    pages(t + 1);
+    to.ke = p8.ke[at];
+    to.ve = p8.ve[at];
+#pragma unroll
+    for (int i = 0; i < KG; ++i)
+      if (ALL || w < HD / 16) to.k[i] = *reinterpret_cast<const u32x4*>(kp + (((size_t)WAVES * i) << g.shift) * 16);
+#pragma unroll
+    for (int i = 0; i < KG; ++i)
+      if (ALL || w < HD / 16) to.v[i] = *reinterpret_cast<const u32x4*>(vp[i]);
   };
   // the granules as operands into buffer b
-  const auto stage = [&](uint32_t t, uint32_t b) {
+  const auto stage = [&](uint32_t t, uint32_t b, Raw& from) {
+    if (!ALL && w >= HD / 16) return;
     char* kd = lds + b * BUF;
     char* vd = kd + K_BYTES;
     // position p: row 4 (p / 16) + p % 4 of product (p / 4) % 4
@@ -595,21 +634,22 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
 #pragma unroll
     for (int i = 0; i < KG; ++i) {
       f16x8 x[2];
-      p8_operands<KT>(kraw[i], x);
+      p8_operands<KT>(from.k[i], x);
+      const uint32_t gi = w + WAVES * i;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        *reinterpret_cast<f16x8*>(kd + ((prod * KS + 2 * i + j) * 64 + 16 * w + pr) * 16 + 64 * prod) = x[j];
+        *reinterpret_cast<f16x8*>(kd + ((prod * KS + 2 * (gi >> 2) + j) * 64 + 16 * (gi & 3u) + pr) * 16 + 64 * prod) = x[j];
     }
     const bool edge = t * P8_TILE + P8_TILE - 1 > first;
 #pragma unroll
     for (int i = 0; i < KG; ++i) {
-      const uint32_t dim = (tid + PA_NT * i) % HD;
-      if (KT == TY_E4M3 && (edge || v_bad[i])) {
-        const uint32_t odd = p8_clear_nan(vraw[i]);
-        if (odd && !v_bad[i]) s_odd[b] = 1;
+      const uint32_t dim = (tid + NT * i) % HD;
+      if (KT == TY_E4M3 && (edge || from.v_bad[i])) {
+        const uint32_t odd = p8_clear_nan(from.v[i]);
+        if (odd && !from.v_bad[i]) s_odd[b] = 1;
       }
       f16x8 x[2];
-      p8_operands<KT>(vraw[i], x);
+      p8_operands<KT>(from.v[i], x);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         *reinterpret_cast<f16x8*>(vd + (((dim >> 4) * 2 + j) * 64 + 16 * v_grp(i) + (dim & 15u)) * 16) = x[j];
@@ -618,71 +658,74 @@ __global__ __launch_bounds__(PA_NT, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p
 
   P8Rows<HD, NR> st;
   st.clear();
+  uint32_t ke = 0, ve = 0;
+  bool ok = true;
+  // tile t, in buffer B
+  const auto tile = [&](uint32_t t, auto which) {
+    constexpr uint32_t B = which.value;
+    const char* kd = lds + B * BUF;
+    const char* vd = kd + K_BYTES;
+    f32x4 sc[NR][4];
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sc[r][k] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < KS; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f16x8 kk = *reinterpret_cast<const f16x8*>(kd + ((k * KS + j) * 64 + lane) * 16 + 64 * k);
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int n = NQ - 1; n >= 0; --n) sc[r][k] = Op16<TY_F16>::mfma(kk, qf[r][n][j], sc[r][k]);
+      }
+    const uint32_t gpos = t * P8_TILE + 16 * grp;  // this lane's 16 positions
+    if (!ok) paged_flag(g, PG_BAD_PAGE);
+    f16x8 pf[NR][NP][2];
+    p8_softmax<HD, NR, NP>(st, sc, factor, ke, ve, gpos, limit, ok,
+                           t * P8_TILE + P8_TILE - 1 > first || __ballot(!ok) != 0, pf);
+    const bool odd = KT == TY_E4M3 && s_odd[B];
+    if (t + 1 < t1) {
+      stage(t + 1, B ^ 1, raw);
+      ke = raw.ke;
+      ve = raw.ve;
+      ok = raw.ok;
+      if (t + 2 < t1) fetch(t + 2, raw);
+    }
+#pragma unroll
+    for (int d0 = 0; d0 < DS; d0 += 2)  // (two dims' chains in turn)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        f16x8 vv[2];
+#pragma unroll
+        for (int d = 0; d < 2; ++d) vv[d] = *reinterpret_cast<const f16x8*>(vd + (((d0 + d) * 2 + k) * 64 + lane) * 16);
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n)
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int r = 0; r < NR; ++r) st.o[r][d0 + d] = Op16<TY_F16>::mfma(vv[d], pf[r][n][k], st.o[r][d0 + d]);
+      }
+    if (odd) p8_add_nan<HD, NR>(st, vc, page_bytes, g, tab, t, len, limit);
+    __syncthreads();
+  };
   if (t0 < t1) {
     if (tid < 2) s_odd[tid] = 0;
     pages(t0);
-    fetch(t0);
-    pages(t0 + 1);
+    fetch(t0, raw);
     __syncthreads();
-    stage(t0, 0);
-    ke = ke_next;
-    ve = ve_next;
-    ok_now = ok_next;
-    if (t0 + 1 < t1) {
-      fetch(t0 + 1);
-      pages(t0 + 2);
-    }
+    stage(t0, 0, raw);
+    ke = raw.ke;
+    ve = raw.ve;
+    ok = raw.ok;
+    if (t0 + 1 < t1) fetch(t0 + 1, raw);
     __syncthreads();
-    for (uint32_t t = t0, b = 0; t < t1; ++t, b ^= 1) {
-      const char* kd = lds + b * BUF;
-      const char* vd = kd + K_BYTES;
-      f32x4 sc[NR][4];
-#pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sc[r][k] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < KS; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const f16x8 kk = *reinterpret_cast<const f16x8*>(kd + ((k * KS + j) * 64 + lane) * 16 + 64 * k);
-#pragma unroll
-          for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int n = NQ - 1; n >= 0; --n) sc[r][k] = Op16<TY_F16>::mfma(kk, qf[r][n][j], sc[r][k]);
-        }
-      const uint32_t gpos = t * P8_TILE + 16 * grp;  // this lane's 16 positions
-      if (!ok_now) paged_flag(g, PG_BAD_PAGE);
-      f16x8 pf[NR][NP][2];
-      p8_softmax<HD, NR, NP>(st, sc, factor, ke, ve, gpos, limit, ok_now,
-                             t * P8_TILE + P8_TILE - 1 > first || __ballot(!ok_now) != 0, pf);
-      const bool odd = KT == TY_E4M3 && s_odd[b];
-      if (t + 1 < t1) {
-        stage(t + 1, b ^ 1);
-        ke = ke_next;
-        ve = ve_next;
-        ok_now = ok_next;
-        if (t + 2 < t1) {
-          fetch(t + 2);
-          pages(t + 3);
-        }
-      }
-#pragma unroll
-      for (int d0 = 0; d0 < DS; d0 += 2)  // (two dims' chains in turn)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          f16x8 vv[2];
-#pragma unroll
-          for (int d = 0; d < 2; ++d) vv[d] = *reinterpret_cast<const f16x8*>(vd + (((d0 + d) * 2 + k) * 64 + lane) * 16);
-#pragma unroll
-          for (int n = NP - 1; n >= 0; --n)
-#pragma unroll
-            for (int d = 0; d < 2; ++d)
-#pragma unroll
-              for (int r = 0; r < NR; ++r) st.o[r][d0 + d] = Op16<TY_F16>::mfma(vv[d], pf[r][n][k], st.o[r][d0 + d]);
-        }
-      if (odd) p8_add_nan<HD, NR>(st, vc, page_bytes, g, tab, t, len, limit);
-      __syncthreads();
+    for (uint32_t t = t0;;) {
+      tile(t, std::integral_constant<uint32_t, 0>{});
+      if (++t >= t1) break;
+      tile(t, std::integral_constant<uint32_t, 1>{});
+      if (++t >= t1) break;
     }
   }
 

@@ -47,6 +47,7 @@ uint32_t log2_of(uint32_t power) {
 struct P8Sizes {
   uint32_t nr, blocks, part_rows, at_once, grid;
   bool prompt;                 // the prompts' kernel
+  uint64_t tiles;              // of all row blocks, as the tables have room
   bool join;                   // some segment may be cut
   bool fits;                   // the plan's 32-bit counts hold
   size_t part_o, cuts, bytes;  // offsets of the workspace's parts, its size
@@ -59,12 +60,14 @@ P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_k
   z.nr = z.prompt ? cm::p8p_rows((int)hd) / 16 : rows > 16 && hd <= 128 ? 2 : 1;
   z.blocks = (uint32_t)((rows + 16 * z.nr - 1) / (16 * z.nr));
   z.part_rows = (uint32_t)std::min<uint64_t>(rows, 16 * z.nr);
-  // 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
-  z.at_once = z.prompt ? 0 : 256 * cm::p8_per_cu((int)hd, (int)z.nr) * 7 / 8;
   // a piece has at least `least` tiles, or all; pieces altogether are at most `most` and one for each segment
-  const uint64_t segments = n_seqs * n_kv * z.blocks, least = z.prompt ? 16 : 4, most = z.prompt ? 512 : 2048;
+  const uint64_t segments = n_seqs * n_kv * z.blocks;
+  z.tiles = segments * cap_tiles;
+  const uint64_t least = z.prompt && z.tiles > 2048 ? 16 : 4, most = z.prompt ? 512 : 2048;
+  // the split's: 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
+  z.at_once = z.prompt ? (uint32_t)least : 256 * cm::p8_per_cu((int)hd, (int)z.nr) * 7 / 8;
   const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + least - 1) / least));
-  z.fits = segments * cap_tiles < (1ull << 31) && grid_ok(pieces, cm::PA_NT);
+  z.fits = z.tiles < (1ull << 31) && grid_ok(pieces, 512);
   z.grid = (uint32_t)pieces;
   z.join = cap_tiles > least;
   // cut segments have more tiles than the target: at most `most` of them, twice as many pieces
@@ -73,6 +76,22 @@ P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_k
   z.cuts = z.part_o + up256(slots * z.part_rows * hd * 4);
   z.bytes = z.cuts + up256(segments * 8);
   return z;
+}
+
+// Workspace of calls of at most these sizes: parts of at most `slots` pieces, and a word pair for each segment; the
+// most that either kernel takes up to n_new.
+size_t p8_workspace(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap) {
+  const uint64_t group = std::max<uint64_t>(n_heads / n_kv, 1), cap_tiles = (cap + cm::P8_TILE - 1) / cm::P8_TILE;
+  const auto most = [&](uint64_t rows, uint64_t block, uint64_t slots) {
+    const uint64_t segments = n_seqs * n_kv * ((rows + block - 1) / block), part_rows = std::min(rows, block);
+    slots = cap_tiles > 4 ? std::min(slots, segments * ((cap_tiles + 3) / 4)) : 0;
+    return up256(slots * part_rows * 8) + up256(slots * part_rows * hd * 4) + up256(segments * 8);
+  };
+  const uint64_t few = std::min(n_new, std::max<uint64_t>(CAMELID_MAX_VERIFY_K, 127 / group)) * group;
+  size_t bytes = std::max(most(std::min<uint64_t>(few, 16), 16, 4096), most(few, few > 16 && hd <= 128 ? 32 : 16, 4096));
+  if (n_new > CAMELID_MAX_VERIFY_K && n_new * group >= 128)
+    bytes = std::max(bytes, most(n_new * group, cm::p8p_rows((int)hd), 1024));
+  return bytes;
 }
 
 template <int HD, int QT, int NR>
@@ -88,13 +107,14 @@ void p8_join(const cm::PaArgs& a, hipStream_t stream) {
     join(std::integral_constant<uint32_t, 1>{}, cm::k_pa_join<HD, QT, NR, 1>);
 }
 
-bool p8_start(void (*kernel)(cm::P8Args), const cm::P8Args& p, const P8Sizes& z, size_t lds, hipStream_t stream) {
+bool p8_start(void (*kernel)(cm::P8Args), const cm::P8Args& p, const P8Sizes& z, uint32_t threads, size_t lds,
+              hipStream_t stream) {
   if (lds > 64 * 1024) {
     const hipError_t st = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (st != hipSuccess) return cm::fail_global("paged8_attention", hipGetErrorString(st)) == 0;
   }
-  hipLaunchKernelGGL(kernel, dim3(z.grid), dim3(cm::PA_NT), lds, stream, p);
+  hipLaunchKernelGGL(kernel, dim3(z.grid), dim3(threads), lds, stream, p);
   return true;
 }
 
@@ -105,7 +125,8 @@ bool p8_split(const cm::P8Args& p, const P8Sizes& z, hipStream_t stream) {
   // them several times)
   const bool passing = z.blocks == 1 && ((uint64_t)a.g.n_seqs * a.g.n_kv * HD * 2 * a.g.stride << a.g.shift) > (256u << 20);
   constexpr size_t lds = (size_t)16 * NR * (4 * (HD + 4 + 2) + 2) * 4;
-  if (!p8_start(passing ? cm::k_p8_split<HD, KT, QT, NR, true> : cm::k_p8_split<HD, KT, QT, NR, false>, p, z, lds, stream))
+  if (!p8_start(passing ? cm::k_p8_split<HD, KT, QT, NR, true> : cm::k_p8_split<HD, KT, QT, NR, false>, p, z, cm::PA_NT, lds,
+                stream))
     return false;
   if (z.join) p8_join<HD, QT, NR>(a, stream);
   return true;
@@ -114,7 +135,20 @@ bool p8_split(const cm::P8Args& p, const P8Sizes& z, hipStream_t stream) {
 template <int HD, int KT, int QT>
 bool p8_launch(const cm::P8Args& p, const P8Sizes& z, hipStream_t stream) {
   if (z.prompt) {
-    if (!p8_start(cm::k_p8_prompt<HD, KT, QT>, p, z, cm::p8p_lds(HD), stream)) return false;
+    // 8 waves of 16 rows a workgroup hide each other's latency; f32 rows, which take twice the products, have enough
+    // of those from some size on, and 4 waves of 32 rows read LDS half as often.  Heads of 128, f32: 3 prompts of up to
+    // 1023 49.5 us with 8 waves and 62.6 with 4, 1024 tokens at 7168 287 and 265, 4096 at 12288 1870 and 1653; bf16:
+    // 38.8 and 44.6, 189 and 190, 1159 and 1159
+    const auto go = [&](auto waves) {
+      return p8_start(cm::k_p8_prompt<HD, KT, QT, waves()>, p, z, 64 * waves(), cm::p8p_lds(HD), stream);
+    };
+    typedef std::integral_constant<int, 4> Four;
+    typedef std::integral_constant<int, 8> Eight;
+    bool ok;
+    if constexpr (HD == 256) ok = go(Four{});
+    else if constexpr (HD == 128 && QT == TY_F32) ok = z.tiles >= 16384 ? go(Four{}) : go(Eight{});
+    else ok = go(Eight{});
+    if (!ok) return false;
     if (z.join) p8_join<HD, QT, cm::p8p_rows(HD) / 16>(p.a, stream);
     return true;
   }
@@ -201,7 +235,7 @@ int camelid_hip_paged8_read(const void* kc, const void* vc, const uint8_t* k_exp
 size_t camelid_hip_paged8_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
                                               uint32_t hd, uint32_t page_size, uint32_t table_stride) {
   if (!n_kv) return 0;
-  return p8_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride).bytes;
+  return p8_workspace(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride);
 }
 
 int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stride, uint32_t n_seqs, uint32_t n_new,
@@ -229,8 +263,9 @@ int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stri
     return cm::fail_global(me, "q, out, the cache and the workspace must be 16-byte aligned, the rest 4-byte aligned");
   if (workspace_bytes < camelid_hip_paged8_attention_workspace(n_seqs, n_new, n_heads, n_kv, hd, page_size, table_stride))
     return cm::fail_global(me, "workspace too small (camelid_hip_paged8_attention_workspace)");
-  const uint64_t groups = (uint64_t)n_seqs * n_kv * n_new * (n_heads / n_kv);
-  if (!grid_ok(groups, cm::PA_NT)) return cm::fail_global(me, "too many rows in one call");
+  const uint64_t group = n_heads / n_kv;
+  if (!grid_ok((uint64_t)n_seqs * n_kv * n_new * group, cm::PA_NT) || n_new * group * group >= (1ull << 32))
+    return cm::fail_global(me, "too many rows in one call");
   const P8Sizes z = p8_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride);
   if (!z.fits) return cm::fail_global(me, "n_seqs * n_kv * table_stride * page_size too large for one call");
   // (every workgroup works the plan out from all lengths)
