@@ -174,7 +174,7 @@ __device__ __forceinline__ void r8_turn(F (&a)[8], F (&b)[8], const float (&c)[8
 }
 
 template <int HD, int QT, int KT>
-__global__ __launch_bounds__(R8_NT) void k_paged8_rope_kv16(Paged8 c, const float* __restrict__ qkv, uint32_t n_new,
+__global__ __launch_bounds__(R8_NT, 3) void k_paged8_rope_kv16(Paged8 c, const float* __restrict__ qkv, uint32_t n_new,
                                                             const uint32_t* __restrict__ new_lens, uint32_t n_heads,
                                                             uint32_t split_half, const float* __restrict__ cosv,
                                                             const float* __restrict__ sinv,
@@ -281,11 +281,6 @@ __global__ __launch_bounds__(R8_NT) void k_paged8_rope_kv16(Paged8 c, const floa
     for (int i = 0; i < 8; ++i) a[i] = b[i] = ca[i] = sa[i] = 0.0f;
   }
   const float* nw = isq ? q_norm : k_norm;
-  float wa[8], wb[8];
-  if (nw && live) {
-    rk_load8(nw + 8 * j, wa);
-    rk_load8(nw + HALF + 8 * j, wb);
-  }
   if (isq) {
     if (nw) {
       if (live) {
@@ -298,16 +293,22 @@ __global__ __launch_bounds__(R8_NT) void k_paged8_rope_kv16(Paged8 c, const floa
       __syncthreads();
       if (tid < PAIRS) {  // (padding rows sum what lies there)
         float acc = 0.0f;
-#pragma unroll 8
-        for (uint32_t d = 0; d < HD; ++d) {
-          const float x = s_x[tid][d];
-          acc = acc + x * x;
+#pragma unroll 2
+        for (uint32_t d = 0; d < HD; d += 4) {
+          const f32x4v x = *reinterpret_cast<const f32x4v*>(&s_x[tid][d]);
+          acc = acc + x[0] * x[0];
+          acc = acc + x[1] * x[1];
+          acc = acc + x[2] * x[2];
+          acc = acc + x[3] * x[3];
         }
         s_scale[tid] = 1.0f / sqrtf(acc / (float)HD + eps);
       }
       __syncthreads();
       if (live) {
         const float sc = s_scale[pair];
+        float wa[8], wb[8];
+        rk_load8(nw + 8 * j, wa);
+        rk_load8(nw + HALF + 8 * j, wb);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           a[i] = (a[i] * sc) * wa[i];
@@ -357,6 +358,9 @@ __global__ __launch_bounds__(R8_NT) void k_paged8_rope_kv16(Paged8 c, const floa
     for (uint32_t i = 1; i < LPR; i <<= 1) acc += __shfl_xor(acc, i);
     const double sc = 1.0 / sqrt(acc / (double)HD + (double)eps);
     if (live) {
+      float wa[8], wb[8];
+      rk_load8(nw + 8 * j, wa);
+      rk_load8(nw + HALF + 8 * j, wb);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         x[i] = (x[i] * sc) * wa[i];
@@ -487,16 +491,19 @@ __global__ __launch_bounds__(R8_NT) void k_paged8_rope_kv(Paged8 c, const float*
 }
 
 // ---------------------------------------------------------------------------
-// K and V of each sequence's positions [0, min(lens, n_out)) as rows [n_kv][n_out][hd] of type T.  One
-// workgroup per (sequence, KV head, 16 positions, K or V); V's granules are turned in LDS.  Bound: HBM.
+// K and V of each sequence's positions [0, min(lens, n_out)) as rows [n_kv][n_out][hd] of type T.  One workgroup per
+// (sequence, KV head, 4096 bytes of K or V: a granule a thread), which go through LDS so that rows are written
+// whole.  Bound: HBM.
 constexpr uint32_t RD_NT = 256;
+constexpr uint32_t rd_span(uint32_t hd) { return RD_NT * 16 / hd; }  // positions of a workgroup
 template <int HD, int KT, int T>
 __global__ __launch_bounds__(RD_NT) void k_paged8_read(Paged8 c, void* __restrict__ k_out, void* __restrict__ v_out,
-                                                       uint32_t n_out, uint32_t blocks) {
+                                                       uint32_t n_out, uint32_t spans) {
+  constexpr uint32_t SPAN = rd_span(HD), PITCH = HD + 4;
   const Paged& g = c.g;
-  __shared__ float s_v[P8_BLOCK][HD + 1];
+  __shared__ float s_x[SPAN * PITCH];
   const uint32_t tid = threadIdx.x, which = blockIdx.x & 1u, rest = blockIdx.x >> 1;
-  const uint32_t sh = rest / blocks, p0 = (rest - sh * blocks) * P8_BLOCK, s = sh / g.n_kv, h = sh - s * g.n_kv;
+  const uint32_t sh = rest / spans, p0 = (rest - sh * spans) * SPAN, s = sh / g.n_kv, h = sh - s * g.n_kv;
   const uint32_t len = g.lens[s];
   if ((uint64_t)len > ((uint64_t)g.stride << g.shift)) {
     if (tid == 0) paged_flag(g, PG_BAD_LENGTH);
@@ -504,34 +511,41 @@ __global__ __launch_bounds__(RD_NT) void k_paged8_read(Paged8 c, void* __restric
   }
   const uint32_t end = min(len, n_out);
   if (p0 >= end) return;
-  const uint32_t page = g.table[(size_t)s * g.stride + (p0 >> g.shift)], o0 = p0 & ((1u << g.shift) - 1u);
-  if (page >= g.n_pages) {
-    if (tid == 0) paged_flag(g, PG_BAD_PAGE);
-    return;
-  }
-  const uint8_t* src = (which ? c.vc : c.kc) + p8_base(g, page, h);
-  const float scale = p8_scale((which ? c.ve : c.ke)[p8_exp(g, page, h, o0)]);
-  const size_t dst = ((size_t)sh * n_out + p0) * HD;
-  const uint32_t rows = min(P8_BLOCK, end - p0);
-  for (uint32_t i = tid; i < P8_BLOCK * HD / 16; i += RD_NT) {
-    const uint32_t t = i % P8_BLOCK, d = which ? i : i / P8_BLOCK;  // K: granule d of position t; V: dim d
-    if (!which && t >= rows) continue;
-    const uint4 u = *reinterpret_cast<const uint4*>(src + (which ? p8_v(g, o0, d) : p8_k(g, o0 + t, 16 * d)));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  // K: granule tid / SPAN of position tid % SPAN; V: dim tid % HD of block tid / HD
+  const uint32_t t = which ? 16 * (tid / HD) : tid % SPAN, d = which ? tid % HD : tid / SPAN;
+  const uint32_t pos = min(p0 + t, end - 1), page = g.table[(size_t)s * g.stride + (pos >> g.shift)];
+  const uint32_t o = pos & ((1u << g.shift) - 1u);
+  const bool good = page < g.n_pages;
+  if (!good) paged_flag(g, PG_BAD_PAGE);
+  if (good) {
+    const uint8_t* src = (which ? c.vc : c.kc) + p8_base(g, page, h) + (which ? p8_v(g, o & ~15u, d) : p8_k(g, o, 16 * d));
+    const float scale = p8_scale((which ? c.ve : c.ke)[p8_exp(g, page, h, o)]);
+    const u32x4 u = *reinterpret_cast<const u32x4*>(src);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float x[4];
-      p8_unpack4<KT>(w[j], x);
+      p8_unpack4<KT>(u[j], x);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        if (which) s_v[4 * j + n][d] = x[n] * scale;
-        else store_from_f32<T>(k_out, dst + (size_t)t * HD + 16 * d + 4 * j + n, x[n] * scale);
-      }
+      for (int n = 0; n < 4; ++n)
+        s_x[which ? (t + 4 * j + n) * PITCH + d : t * PITCH + 16 * d + 4 * j + n] = x[n] * scale;
     }
   }
-  if (!which) return;
   __syncthreads();
-  for (uint32_t i = tid; i < rows * HD; i += RD_NT) store_from_f32<T>(v_out, dst + i, s_v[i / HD][i % HD]);
+  constexpr uint32_t V = T == TY_F32 ? 4 : 8;  // elements of a store
+  const uint32_t rows = min(SPAN, end - p0);
+  char* out = static_cast<char*>(which ? v_out : k_out) + ((size_t)sh * n_out + p0) * HD * (T == TY_F32 ? 4 : 2);
+  for (uint32_t i = tid; i < rows * (HD / V); i += RD_NT) {
+    const uint32_t row = i / (HD / V), at = (i % (HD / V)) * V;
+    if (g.table[(size_t)s * g.stride + ((p0 + row) >> g.shift)] >= g.n_pages) continue;
+    const f32x4v a = *reinterpret_cast<const f32x4v*>(&s_x[row * PITCH + at]);
+    if constexpr (T == TY_F32) {
+      reinterpret_cast<f32x4v*>(out)[i] = a;
+    } else {
+      const f32x4v b = *reinterpret_cast<const f32x4v*>(&s_x[row * PITCH + at + 4]);
+      const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      reinterpret_cast<rk_u32x4*>(out)[i] = rk_pack8<T>(x);
+    }
+  }
 }
 
 }  // namespace cm

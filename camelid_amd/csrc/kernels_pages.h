@@ -10,7 +10,7 @@
 namespace cm {
 
 constexpr uint32_t PG_NT = 256;
-constexpr uint32_t PG_CHUNK = 4096;  // pages of a workgroup that counts or lists them
+constexpr uint32_t PG_CHUNK = 1024;  // pages of a workgroup that counts or lists them
 constexpr uint32_t PG_COW = 0x80000000u;  // mark of an entry to be replaced, between two launches
 enum { PG_NO_PAGE = 4, PG_BAD_FORK = 8 };  // CAMELID_PAGED_NO_PAGE, CAMELID_PAGED_BAD_FORK
 
@@ -207,6 +207,103 @@ __global__ __launch_bounds__(PG_NT) void k_pages_grant(PagesArgs a) {
   if (tid == 0 && want > held) a.held[s] = want;
 }
 
+// The four steps by one workgroup with barriers in the place of launches, for small batches and pools: a thread per
+// entry.  What other waves changed is waited for and read past the L1.
+constexpr uint32_t PG_ONE_SEQS = 1024, PG_ONE_PAGES = 8192, PG_ONE_ENTRIES = 16384;
+__device__ __forceinline__ uint32_t pg_read(const uint32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__global__ __launch_bounds__(PG_PLAN_NT) void k_pages_reserve(PagesArgs a) {
+  constexpr uint32_t NT = PG_PLAN_NT, PER = PG_ONE_PAGES / NT;
+  __shared__ uint32_t s_wave[NT / 64], s_held[PG_ONE_SEQS], s_want[PG_ONE_SEQS], s_write[PG_ONE_SEQS], s_bad[PG_ONE_SEQS];
+  __shared__ uint32_t s_cows[PG_ONE_SEQS], s_before[PG_ONE_SEQS], s_cows_before[PG_ONE_SEQS];
+  __shared__ uint32_t s_mark[PG_ONE_ENTRIES / 32], s_free[PG_ONE_PAGES], s_told;
+  const uint32_t tid = threadIdx.x, entries = a.n_seqs * a.stride;
+  for (uint32_t i = tid; i < PG_ONE_ENTRIES / 32; i += NT) s_mark[i] = 0;
+  if (tid == 0) s_told = 0;
+  if (tid < a.n_seqs) {
+    const uint32_t held = a.held[tid], want = pages_wanted(a, tid);
+    s_held[tid] = held;
+    s_want[tid] = want;
+    s_write[tid] = a.first && a.first[tid] < a.lens[tid] ? a.first[tid] >> a.shift : ~0u;  // first entry to be written
+    s_bad[tid] = held > a.stride || want > a.stride ? PG_BAD_LENGTH : 0u;
+    s_cows[tid] = 0;
+  }
+  __syncthreads();
+  // 1: entries that a row no longer needs
+  for (uint32_t i = tid; i < entries; i += NT) {
+    const uint32_t s = i / a.stride, j = i - s * a.stride;
+    if (j < s_held[s] && a.table[i] >= a.n_pages && s_bad[s] == 0) s_bad[s] = PG_BAD_PAGE;
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < entries; i += NT) {
+    const uint32_t s = i / a.stride, j = i - s * a.stride;
+    if (!s_bad[s] && j >= s_want[s] && j < s_held[s]) atomicSub(&a.refs[a.table[i]], 1u);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  // 2: entries to be replaced marked; the free pages in ascending order (thread i: PER pages side by side)
+  for (uint32_t i = tid; i < entries; i += NT) {
+    const uint32_t s = i / a.stride, j = i - s * a.stride;
+    if (!s_bad[s] && j >= s_write[s] && j < min(s_held[s], s_want[s]) && pg_read(&a.refs[a.table[i]]) > 1) {
+      atomicOr(&s_mark[i >> 5], 1u << (i & 31u));
+      atomicAdd(&s_cows[s], 1u);
+    }
+  }
+  uint32_t mine = 0, mask = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) {
+    const uint32_t p = tid * PER + i;
+    if (p < a.n_pages && pg_read(&a.refs[p]) == 0) {
+      mask |= 1u << i;
+      ++mine;
+    }
+  }
+  const PgScan free = pg_scan<NT>(mine, s_wave);
+  for (uint32_t i = 0, k = free.before; i < PER; ++i)
+    if (mask >> i & 1u) s_free[k++] = tid * PER + i;
+  __syncthreads();
+  // 3: the sequences' shares
+  const bool here = tid < a.n_seqs, live = here && !s_bad[tid];
+  const uint32_t held = live ? min(s_held[tid], s_want[tid]) : 0u, cow = live ? s_cows[tid] : 0u;
+  const uint32_t need = live ? cow + s_want[tid] - held : 0u;
+  const PgScan n = pg_scan<NT>(need, s_wave), c = pg_scan<NT>(cow, s_wave);
+  const bool ok = live && (need == 0 || (n.before + need <= free.total && (cow == 0 || c.before + cow <= a.max_pairs)));
+  if (here) {
+    s_before[tid] = ok ? n.before : ~0u;
+    s_cows_before[tid] = c.before;
+    if (live) a.held[tid] = ok ? s_want[tid] : held;
+    if (a.granted) a.granted[tid] = ok;
+    if (!ok) pages_flag(a.status, live ? PG_NO_PAGE : s_bad[tid]);
+    if (ok && cow) atomicMax(&s_told, c.before + cow);
+  }
+  __syncthreads();
+  if (a.n_pairs && tid == 0) *a.n_pairs = s_told;
+  // 4: the rows' new entries
+  for (uint32_t i = tid; i < entries; i += NT) {
+    const uint32_t s = i / a.stride, j = i - s * a.stride, before = s_before[s];
+    if (before == ~0u) continue;
+    if (s_mark[i >> 5] >> (i & 31u) & 1u) {
+      uint32_t rank = 0;  // marked entries of the row before this one
+      for (uint32_t k = s * a.stride; k < i;) {
+        const uint32_t bits = s_mark[k >> 5] >> (k & 31u), most = min(32 - (k & 31u), i - k);
+        rank += __popc(most < 32 ? bits & ((1u << most) - 1u) : bits);
+        k += most;
+      }
+      const uint32_t old = a.table[i], page = s_free[before + rank], at = s_cows_before[s] + rank;
+      a.pairs[2 * at] = old;
+      a.pairs[2 * at + 1] = page;
+      a.table[i] = page;
+      a.refs[page] = 1;
+      atomicSub(&a.refs[old], 1u);
+    } else if (j >= s_held[s] && j < s_want[s]) {
+      const uint32_t page = s_free[before + s_cows[s] + (j - s_held[s])];
+      a.table[i] = page;
+      a.refs[page] = 1;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Children get their parents' pages.  A workgroup per (parent, child) pair; a pair whose child holds pages or is
 // named twice, or whose parent is a child itself, does nothing but flag: what the others do does not depend on
@@ -395,6 +492,7 @@ struct PageCopyArgs {
   uint32_t* status;
   uint32_t max_pairs, n_pages, n_buffers;
 };
+template <bool STREAM>
 __global__ __launch_bounds__(PC_NT) void k_pages_copy(PageCopyArgs a) {
   const uint32_t n = a.n_pairs ? min(*a.n_pairs, a.max_pairs) : a.max_pairs;
   const uint32_t b = blockIdx.x % a.n_buffers;
@@ -407,8 +505,21 @@ __global__ __launch_bounds__(PC_NT) void k_pages_copy(PageCopyArgs a) {
     const uint8_t* src = a.buffer[b] + from * a.bytes[b];
     uint8_t* dst = a.buffer[b] + to * a.bytes[b];
     if (((reinterpret_cast<uintptr_t>(a.buffer[b]) | a.bytes[b]) & 15u) == 0) {
-      for (uint64_t i = threadIdx.x; i < a.bytes[b] / 16; i += PC_NT)
-        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+      const uint64_t units = a.bytes[b] / 16;
+      const rk_u32x4* from16 = reinterpret_cast<const rk_u32x4*>(src);
+      rk_u32x4* to16 = reinterpret_cast<rk_u32x4*>(dst);
+      for (uint64_t i = threadIdx.x; i < units; i += 4 * PC_NT) {  // 4 a thread on their way
+        rk_u32x4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i + j * PC_NT < units) x[j] = STREAM ? __builtin_nontemporal_load(from16 + i + j * PC_NT) : from16[i + j * PC_NT];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i + j * PC_NT < units) {
+            if (STREAM) __builtin_nontemporal_store(x[j], to16 + i + j * PC_NT);
+            else to16[i + j * PC_NT] = x[j];
+          }
+      }
     } else {
       for (uint64_t i = threadIdx.x; i < a.bytes[b]; i += PC_NT) dst[i] = src[i];
     }
