@@ -10,6 +10,7 @@
 namespace cm {
 
 constexpr uint32_t LG_NT = 512;
+constexpr uint32_t LG_BIASES = 32 * LG_NT;  // of a sequence at most
 constexpr uint32_t LG_SLICE = 4096;  // tokens of a workgroup
 constexpr uint32_t LG_SEEN = 1u << 31, LG_DRAFT = 1u << 30, LG_BIAS = 1u << 29, LG_COUNT = LG_BIAS - 1;
 
@@ -29,7 +30,7 @@ struct LogitsArgs {
   const uint32_t* bias_lens;
   const uint32_t* mask;
   uint64_t in_stride, out_stride, history_stride, mask_stride;
-  uint32_t n_rows, vocab, slices, bias_stride;
+  uint32_t n_rows, vocab, slices, bias_stride, per, groups;  // per: rows of a workgroup
 };
 
 // What the lists say of a token (its word w, not 0) applied to its logit.
@@ -37,21 +38,14 @@ struct LogitsRow {
   float r, f, p;
   const uint32_t* drafts;
   uint32_t n_drafts;  // before the row
-  const float* biases;
 };
 __device__ __forceinline__ float lg_adjusted(float x, uint32_t w, uint32_t token, uint32_t bias, const LogitsRow& a) {
   uint32_t count = w & LG_COUNT;
-  bool seen = w & LG_SEEN;
-  if (w & LG_DRAFT) {
-    for (uint32_t j = 0; j < a.n_drafts; ++j) {
-      const bool same = a.drafts[j] == token;
-      count += same;
-      seen |= same;
-    }
-  }
-  if (seen) x = x > 0.0f ? x / a.r : x * a.r;
+  if (w & LG_DRAFT)
+    for (uint32_t j = 0; j < a.n_drafts; ++j) count += a.drafts[j] == token;
+  if (count || (w & LG_SEEN)) x = x > 0.0f ? x / a.r : x * a.r;
   if (count) x = (x - a.f * (float)count) - a.p;
-  if (w & LG_BIAS) x = x + a.biases[bias - 1];
+  if (w & LG_BIAS) x = x + u2f(bias);
   return x;
 }
 
@@ -62,17 +56,18 @@ __device__ __forceinline__ float lg_adjusted(float x, uint32_t w, uint32_t token
 template <int T, bool SPARSE>
 __global__ __launch_bounds__(LG_NT) void k_adjust_logits(LogitsArgs a) {
   __shared__ uint32_t s_word[LG_SLICE];  // LG_COUNT: occurrences behind the prompt
-  __shared__ uint32_t s_bias[LG_SLICE];  // index of the last bias + 1 (where LG_BIAS is set)
-  const uint32_t tid = threadIdx.x, s = blockIdx.x / a.slices, v0 = (blockIdx.x - s * a.slices) * LG_SLICE;
+  __shared__ uint32_t s_bias[LG_SLICE];  // where LG_BIAS is set: first the index of the last bias + 1, then its bits
+  const uint32_t tid = threadIdx.x, unit = blockIdx.x / a.slices, v0 = (blockIdx.x - unit * a.slices) * LG_SLICE;
+  const uint32_t s = unit / a.groups, t0 = (unit - s * a.groups) * a.per;  // first row
   const uint32_t n = min(LG_SLICE, a.vocab - v0);
   const uint32_t known = a.history ? (uint32_t)min((uint64_t)(a.history_lens ? a.history_lens[s] : ~0u), a.history_stride) : 0u;
   const uint32_t prompt = a.prompt_lens ? a.prompt_lens[s] : 0u;
   const uint32_t last = a.draft_lens ? min(a.draft_lens[s], a.n_rows - 1) : a.n_rows - 1;
-  const uint32_t n_drafts = a.drafts ? last : 0u, rows = last + 1;
+  const uint32_t rows = min(last + 1, t0 + a.per), n_drafts = a.drafts && rows ? rows - 1 : 0u;
+  if (t0 >= rows) return;
   const uint32_t biases = a.bias_tokens ? (a.bias_lens ? min(a.bias_lens[s], a.bias_stride) : a.bias_stride) : 0u;
   LogitsRow row{a.repetition ? a.repetition[s] : 1.0f, a.frequency ? a.frequency[s] : 0.0f,
-                a.presence ? a.presence[s] : 0.0f, a.drafts + (size_t)s * (a.n_rows - 1), 0,
-                a.bias_values + (size_t)s * a.bias_stride};
+                a.presence ? a.presence[s] : 0.0f, a.drafts + (size_t)s * (a.n_rows - 1), 0};
   // this thread's 8 logits of a row, as they lie, and their mask bits; a row's are on their way while the lists are
   // read or the two rows before are worked on
   constexpr uint32_t E = T == TY_F32 ? 4 : 2, W = 2 * E;
@@ -107,45 +102,63 @@ __global__ __launch_bounds__(LG_NT) void k_adjust_logits(LogitsArgs a) {
     to.bits = !a.mask ? 0xffu : mine ? reinterpret_cast<const uint8_t*>(a.mask + at * a.mask_stride)[(v0 + i0) >> 3] : 0u;
   };
   if (!SPARSE) {
-    load(0, sets[0]);
-    if (rows > 1) load(1, sets[1]);
+    load(t0, sets[0]);
+    if (t0 + 1 < rows) load(t0 + 1, sets[1]);
   }
+  // the first of the lists' tokens come before anything waits
+  const uint32_t* history = a.history + s * a.history_stride;
+  const uint32_t* bias_tokens = a.bias_tokens + (size_t)s * a.bias_stride;
+  constexpr uint32_t H = 4;
+  uint32_t v[H], draft = ~0u, bias = ~0u;
+  const auto fetch = [&](uint32_t from) {
+#pragma unroll
+    for (uint32_t j = 0; j < H; ++j) v[j] = from + j * LG_NT < known ? history[from + j * LG_NT] - v0 : ~0u;
+  };
+  fetch(tid);
+  if (tid < n_drafts) draft = row.drafts[tid] - v0;
+  if (tid < biases) bias = bias_tokens[tid] - v0;
   for (uint32_t i = tid; i < LG_SLICE; i += LG_NT) {
     s_word[i] = 0;
     if (biases) s_bias[i] = 0;
   }
   __syncthreads();
-  const uint32_t* history = a.history + s * a.history_stride;
-  for (uint32_t i0 = tid; i0 < known; i0 += 4 * LG_NT) {
-    uint32_t v[4];
+  for (uint32_t from = tid; from < known; from += H * LG_NT) {
+    if (from != tid) fetch(from);
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) v[j] = i0 + j * LG_NT < known ? history[i0 + j * LG_NT] - v0 : ~0u;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
+    for (uint32_t j = 0; j < H; ++j) {
       if (v[j] >= n) continue;
-      atomicOr(&s_word[v[j]], LG_SEEN);
-      if (i0 + j * LG_NT >= prompt) atomicAdd(&s_word[v[j]], 1u);
+      if (from + j * LG_NT < prompt) atomicOr(&s_word[v[j]], LG_SEEN);
+      else atomicAdd(&s_word[v[j]], 1u);
     }
   }
-  if (tid < n_drafts) {
-    const uint32_t v = row.drafts[tid] - v0;
-    if (v < n) atomicOr(&s_word[v], LG_DRAFT);
-  }
+  if (draft < n) atomicOr(&s_word[draft], LG_DRAFT);
   for (uint32_t i = tid; i < biases; i += LG_NT) {
-    const uint32_t v = a.bias_tokens[(size_t)s * a.bias_stride + i] - v0;
-    if (v < n) {
-      atomicOr(&s_word[v], LG_BIAS);
-      atomicMax(&s_bias[v], i + 1);
-    }
+    const uint32_t b = i == tid ? bias : bias_tokens[i] - v0;
+    if (b >= n) continue;
+    atomicOr(&s_word[b], LG_BIAS);
+    atomicMax(&s_bias[b], i + 1);
   }
   __syncthreads();
+  if (biases) {
+    uint32_t wins = 0;  // entries i = tid + k LG_NT that are their token's last
+    for (uint32_t k = 0; tid + k * LG_NT < biases; ++k) {
+      if (k) bias = bias_tokens[tid + k * LG_NT] - v0;
+      if (bias < n && s_bias[bias] == tid + k * LG_NT + 1) wins |= 1u << k;
+    }
+    __syncthreads();
+    for (; wins; wins &= wins - 1) {
+      const uint32_t i = tid + (__ffs(wins) - 1) * LG_NT;
+      s_bias[bias_tokens[i] - v0] = f2u(a.bias_values[(size_t)s * a.bias_stride + i]);
+    }
+    __syncthreads();
+  }
   if (!mine) return;
   uint32_t word[8], named = 0;
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i) named |= word[i] = s_word[i0 + i];
   if (SPARSE && !named) return;
   if (SPARSE) {
-    for (uint32_t t = 0; t < rows; ++t) {
+    for (uint32_t t = t0; t < rows; ++t) {
       const uint64_t in = ((uint64_t)s * a.n_rows + t) * a.in_stride + v0 + i0;
       row.n_drafts = min(t, n_drafts);
 #pragma unroll 1
@@ -188,7 +201,7 @@ __global__ __launch_bounds__(LG_NT) void k_adjust_logits(LogitsArgs a) {
         if (i < mine) store_from_f32<T>(a.out, out + i, x[i]);
     }
   };
-  for (uint32_t t = 0; t < rows; t += 2) {
+  for (uint32_t t = t0; t < rows; t += 2) {
     finish(t, sets[0]);
     if (t + 1 < rows) finish(t + 1, sets[1]);
   }

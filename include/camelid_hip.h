@@ -587,7 +587,7 @@ int camelid_hip_pages_copy(void* const* buffers, const size_t* page_bytes, uint3
  * Each step is rounded in f32, the result to the logits' type.  NULL leaves a step out.  Tokens >= vocab in a list count
  * for nothing.  A mask that leaves no token makes a row of -infinity, which verify_drafts answers with 0xffffffff.
  * repetition, frequency, presence: f32 [n_seqs]; bias_tokens, bias_values (f32): [n_seqs][bias_stride]; mask: rows
- * of mask_stride words.  n_rows <= 32, vocab <= 2^24, history_stride <= 2^28.  Asynchronous on `stream`, allocates
+ * of mask_stride words.  n_rows <= 32, vocab <= 2^24, history_stride <= 2^28, bias_stride <= 16384.  Asynchronous on `stream`, allocates
  * nothing, may be captured. */
 int camelid_hip_adjust_logits(const void* logits, size_t in_stride, void* out, size_t out_stride, uint32_t logits_type,
                               uint32_t n_seqs, uint32_t n_rows, uint32_t vocab, const uint32_t* history,
