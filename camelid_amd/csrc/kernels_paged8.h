@@ -286,20 +286,17 @@ __global__ __launch_bounds__(R8_NT, 3) void k_paged8_rope_kv16(Paged8 c, const f
       if (live) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          s_x[pair][8 * j + i] = a[i];
-          s_x[pair][HALF + 8 * j + i] = b[i];
+          s_x[pair][8 * j + i] = a[i] * a[i];  // (the squares, rounded: the sum in order is left to one lane)
+          s_x[pair][HALF + 8 * j + i] = b[i] * b[i];
         }
       }
       __syncthreads();
       if (tid < PAIRS) {  // (padding rows sum what lies there)
         float acc = 0.0f;
-#pragma unroll 2
+#pragma unroll 8
         for (uint32_t d = 0; d < HD; d += 4) {
           const f32x4v x = *reinterpret_cast<const f32x4v*>(&s_x[tid][d]);
-          acc = acc + x[0] * x[0];
-          acc = acc + x[1] * x[1];
-          acc = acc + x[2] * x[2];
-          acc = acc + x[3] * x[3];
+          acc = (((acc + x[0]) + x[1]) + x[2]) + x[3];
         }
         s_scale[tid] = 1.0f / sqrtf(acc / (float)HD + eps);
       }
