@@ -3,7 +3,20 @@
 //   s_p = scale 2^ke(p) (q . k_p) for p <= the row's position;  w = softmax(s);  o = sum_p w_p 2^ve(p) v_p
 //
 // The plan (segments of a sequence, KV head and block of query rows, cut into pieces of tiles), the parts and
-// their join are those of kernels_paged_attn.h; tiles are 64 positions here.
+// their join are those of kernels_paged_attn.h; tiles are 64 positions here.  k_p8_split: a few rows a sequence,
+// k_p8_prompt: many.
+//
+// Bound, split: the cache's bytes (2 hd per position and KV head, 4 hd flop per position and row).  Heads of 128:
+//   64 sequences of up to 4001, 24 + 8 heads: 58 + 4.6 us (split + join) for 270 MB, 4.7 TB/s in the split; all of
+//     them 4001 long: 94 us for 525 MB, 5.6 TB/s; 4 of 65536: 93 us, 5.8 TB/s
+//   1 of 32775, 32 + 8 heads: 17.8 + 3.9 us for 67 MB, 16 of up to 1100 with up to 5 new tokens: 13.6 + 3.9 us for
+//     20 MB: chains of latencies (launch, plan, pages, K and V, products, states joined)
+// The conversion costs about 320 vector instructions a wave and tile of 16 KB, under the time that its bytes take.
+// Bound, prompts: vector instructions.  A wave's 16 rows of a tile take about 200 (operands 40, addresses 40, softmax
+// 100 of which 16 exponentials at a quarter of the rate) and 32 matrix instructions (64 and more for f32
+// rows).  4096 tokens at 12288, 32 + 8 heads of 128, bf16 rows: 1.18 ms, 815 TFLOP/s, vector units busy 70 % of the
+// cycles by instructions alone, matrix units 36 %; e4m3, whose conversion is shorter, 1.11 ms; f32 rows 1.68 ms.
+//   3 prompts of up to 1023, f32: 45 us: a workgroup's tiles follow each other, 2 us each.
 //
 // Operands.  Granules of 16 bytes become two operands of v_mfma_f32_16x16x32_f16 each: int8 as the low byte of the
 // f16 1024 + u, minus 1152, e4m3 by the conversion instruction, both exact.
@@ -492,9 +505,11 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
 }
 
 // ---------------------------------------------------------------------------
-// Prompts: blocks of 128 query rows (64 for heads of 256), 32 (16) a wave, so that a tile's K and V are turned into
-// operands once for all of them, in LDS, while the tile before is multiplied.  The plan is the split's; tiles behind
-// a block's last row are left out.
+// Prompts: blocks of 128 query rows (64 for heads of 256), so that a tile's K and V are turned into operands once for
+// all of them, in LDS, while the tile before is worked on.  The plan is the split's; tiles behind a block's last row
+// are left out.  8 waves of 16 rows within 128 registers, two workgroups a CU (over 128: 8 sequences of 43 tokens at
+// 4000 77 us and not 60); the host's rule says where 4 waves of 32 rows do better.  16-bit rows take weights as one
+// f16 (11 bits of each, rounded to the nearest: their outputs keep 11 or 8), f32 rows as two.
 constexpr int p8p_rows(int hd) { return hd == 256 ? 64 : 128; }  // rows of a block
 constexpr int p8p_lds(int hd) { return 2 * (2 * 64 * hd * 2 + 192) + 16; }
 // Tiles of a piece at most: `at_once` (4 where the batch is small, else 16: a piece's part is written and read again,
@@ -506,7 +521,7 @@ struct P8PromptTarget {
 };
 
 template <int HD, int KT, int QT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void k_p8_prompt(P8Args p8) {
+__global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : WAVES == 8 && QT != TY_F32 ? 4 : 2) void k_p8_prompt(P8Args p8) {
   typedef typename std::conditional<QT == TY_F32, float, typename std::conditional<QT == TY_F16, _Float16, __bf16>::type>::type QE;
   typedef QE q8v __attribute__((ext_vector_type(8)));
   constexpr int NQ = QT == TY_F32 ? 2 : 1, NP = QT == TY_F32 ? 2 : 1, KS = HD / 32, DS = HD / 16;

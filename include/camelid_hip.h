@@ -494,7 +494,7 @@ enum { CAMELID_I8 = 3, CAMELID_E4M3 = 4 };
 /* camelid_hip_paged_rope_kv for this cache (the same q rows, q_out of any type): the exponent of a block is the smallest
  * with which the largest of the block's new elements is at most 127 (CAMELID_I8) or 448 (CAMELID_E4M3), -126 at
  * least, 121 (119) at most, which leaves f32's last binade to saturate; elements are rounded to the nearest, ties
- * to even.  Where the block begins before the new tokens and its exponent is larger, that one stays; where it is
+ * to even; K's norm and rotation are f64 up to there.  Where the block begins before the new tokens and its exponent is larger, that one stays; where it is
  * smaller, the earlier positions are rounded to the new one (CAMELID_E4M3: exactly, but for subnormals).  The exponent of
  * drafts that are rejected later stays until the block is stored to from its first position again.  A NaN or infinity
  * among the new elements makes the block's exponent 255: all of its positions read as NaN.  Bytes of positions
@@ -515,7 +515,17 @@ int camelid_hip_paged8_read(const void* kc, const void* vc, const uint8_t* k_exp
                             void* k_out, void* v_out, uint32_t out_type, uint32_t out_positions, uint32_t* status,
                             void* stream);
 /* camelid_hip_paged_attention for this cache, without weights, for any number of new tokens (whole prompts too) and
- * q rows of any type. */
+ * q rows of any type: out[row][h] = sum_p softmax_p(scale q[row][h].k_p) v_p over p <= the row's position.  8-bit elements
+ * enter the matrix cores as f16, exactly; f32 q as two f16 of a row scaled into their range (22 bits, or 2^-38 of
+ * the row's largest element), bf16 q as one, scaled alike (its 8 bits, or 2^-38), f16 q as it is; softmax weights as two f16
+ * (22 bits, or 2^-39 of the row's largest weight times its block's scale), and as one (11 bits) for 16-bit q in
+ * calls with n_new > CAMELID_MAX_VERIFY_K.  Statistics and sums are f32, results take one rounding to q_type.  Scores
+ * have to stay below f32's largest number; results below 2^-100 may lose bits.  Elements of masked positions,
+ * whatever their bits, do not reach a row; NaN that it sees (a block's exponent of 255 from the block's first position
+ * on, an e4m3 byte's from its own) makes its outputs NaN (of V: in that dim).  The order of sums goes by n_new, the sizes and the lengths:
+ * the same call gives the same bits.  scale must be finite; n_new (n_heads / n_kv)^2 < 2^32; at most 65535 sequences.
+ * _workspace: bytes for calls with this n_heads, n_kv and hd and at most the other sizes: up to 1024 parts of 128 rows for
+ * prompts (68 MB for heads of 128). */
 size_t camelid_hip_paged8_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
                                               uint32_t hd, uint32_t page_size, uint32_t table_stride);
 int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stride, uint32_t n_seqs, uint32_t n_new,

@@ -160,6 +160,9 @@ LONG = [
     (8, 2, 64, [1500, 900], [500, 700], 64, F32, I8, None),
     (2, 1, 256, [1200], [300], 16, BF16, I8, None),
     (3, 1, 128, [1400], [300], 4096, F32, E4M3, 1 << 18),               # large f32 prompts, by the table's room
+    (3, 1, 128, [1400], [300], 4096, F16, E4M3, 1 << 18),               # and 16-bit ones
+    (4, 2, 128, [900, 1, 2000, 0, 130], [128, 1, 257, 0, 130], 64, BF16, I8, 1 << 18),
+    (1, 1, 128, [70000], [130], 16, F16, I8, 1 << 20),
     (2, 2, 128, [64 * i % 700 + 1 for i in range(90)], [min(64 * i % 700 + 1, i % 70) for i in range(90)], 16, BF16, I8, None),
 ]
 
