@@ -555,7 +555,8 @@ enum { CAMELID_PAGED_NO_PAGE = 4, CAMELID_PAGED_BAD_FORK = 8 };
  * A sequence for which the free pages, counted with all sequences' needs up to its own, or the room in pairs, counted
  * alike, do not suffice gets no page, keeps the rest, and sets CAMELID_PAGED_NO_PAGE; granted[s] (NULL: not told) is 1 for the
  * others (also where nothing was needed).  A row with held[s] or the length beyond table_stride or a page >= n_pages
- * among its entries is left alone, with granted 0 and status as above. */
+ * among its entries is left alone, with granted 0 and status as above.  A call for no sequences does nothing: *n_pairs
+ * stays as it is. */
 size_t camelid_hip_pages_reserve_workspace(uint32_t n_seqs, uint32_t n_pages);
 int camelid_hip_pages_reserve(uint32_t* table, uint32_t table_stride, uint32_t* held, uint32_t n_seqs,
                               const uint32_t* first, const uint32_t* lens, uint32_t page_size, uint32_t* refs,
@@ -563,8 +564,9 @@ int camelid_hip_pages_reserve(uint32_t* table, uint32_t table_stride, uint32_t* 
                               uint32_t* granted, void* workspace, size_t workspace_bytes, uint32_t* status,
                               void* stream);
 /* Sequence children[i] (which holds nothing) gets the pages of parents[i], those of lens[parents[i]] positions at most
- * (lens NULL: all).  A pair with an index >= n_seqs, a child that holds pages, is named in two pairs or is the parent of any
- * pair, does nothing and sets CAMELID_PAGED_BAD_FORK; one whose parent's row is bad, nothing, with the status above. */
+ * (lens NULL: all).  A pair with an index >= n_seqs, with a child that holds pages or is named in two pairs, or with a
+ * parent that is the child of some pair, does nothing and sets CAMELID_PAGED_BAD_FORK; one whose parent's row is
+ * bad, nothing, with the status above. */
 int camelid_hip_pages_fork(uint32_t* table, uint32_t table_stride, uint32_t* held, uint32_t n_seqs,
                            const uint32_t* parents, const uint32_t* children, uint32_t n_forks, const uint32_t* lens,
                            uint32_t page_size, uint32_t* refs, uint32_t n_pages, uint32_t* status, void* stream);
