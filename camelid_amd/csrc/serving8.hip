@@ -420,8 +420,12 @@ int camelid_hip_pages_compact(const uint32_t* table, uint32_t table_stride, cons
   a.n_seqs = n_seqs;
   a.n_pages = n_pages;
   a.max_pairs = max_pairs;
-  hipLaunchKernelGGL(cm::k_compact_count, dim3(a.chunks), dim3(cm::PG_NT), 0, (hipStream_t)stream, a);
-  hipLaunchKernelGGL(cm::k_compact_list, dim3(a.chunks), dim3(cm::PG_PLAN_NT), 0, (hipStream_t)stream, a);
+  if (n_pages <= cm::PG_COUNT_PAGES) {
+    hipLaunchKernelGGL(cm::k_compact_list<true>, dim3(a.chunks), dim3(cm::PG_PLAN_NT), 0, (hipStream_t)stream, a);
+  } else {
+    hipLaunchKernelGGL(cm::k_compact_count, dim3(a.chunks), dim3(cm::PG_NT), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(cm::k_compact_list<false>, dim3(a.chunks), dim3(cm::PG_PLAN_NT), 0, (hipStream_t)stream, a);
+  }
   hipLaunchKernelGGL(cm::k_compact_move, dim3(a.chunks + n_seqs), dim3(cm::PG_PLAN_NT), 0, (hipStream_t)stream, a);
   return launched(me);
 }
