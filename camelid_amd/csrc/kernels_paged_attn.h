@@ -161,7 +161,8 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, uint32_t s, bool flag) 
 // Large ones: 16, so that workgroups ending early make room for others, and
 // more once that makes over 2048 pieces.
 struct PaTarget {
-  __device__ __forceinline__ uint32_t operator()(const PaArgs& a, uint32_t total) const {
+  template <typename F>
+  __device__ __forceinline__ uint32_t operator()(const PaArgs& a, uint32_t total, F) const {
     const uint32_t one = (total + a.at_once - 1) / a.at_once;
     return one <= 16 ? max(4u, (one + 3) & ~3u) : max(16u, (total + 2047) / 2048);
   }
@@ -194,7 +195,14 @@ __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, boo
     total += q.tiles * q.blocks * a.g.n_kv;
   }
   total = __builtin_amdgcn_readlane(pa_scan(total), 63);
-  const uint32_t target = Target{}(a, total);
+  const uint32_t target = Target{}(a, total, [&](uint32_t most) {  // pieces of `most` tiles at most
+    uint32_t k = 0;
+    for (uint32_t s = s0; s < s1; ++s) {
+      if (per > 1) q = pa_seq<NR, TILE>(a, s, false);
+      k += (q.tiles + most - 1) / most * q.blocks * a.g.n_kv;
+    }
+    return (uint32_t)__builtin_amdgcn_readlane(pa_scan(k), 63);
+  });
   const auto count = [&](const PaSeq& z) { return (z.tiles + target - 1) / target; };
   uint32_t mine = 0, cut = 0;
   for (uint32_t s = s0; s < s1; ++s) {
