@@ -53,7 +53,8 @@ struct P8Sizes {
   size_t part_o, cuts, bytes;  // offsets of the workspace's parts, its size
 };
 
-P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap) {
+P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap,
+                 uint32_t q_type) {
   P8Sizes z;
   const uint64_t rows = n_new * (n_heads / n_kv), cap_tiles = (cap + cm::P8_TILE - 1) / cm::P8_TILE;
   z.prompt = n_new > CAMELID_MAX_VERIFY_K && rows >= 128;
@@ -63,7 +64,12 @@ P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_k
   // a piece has at least `least` tiles, or all; pieces altogether are at most `most` and one for each segment
   const uint64_t segments = n_seqs * n_kv * z.blocks;
   z.tiles = segments * cap_tiles;
-  const uint64_t least = z.prompt && z.tiles > 2048 ? 16 : 4, most = z.prompt ? 512 : 2048;
+  uint64_t least = !z.prompt || z.tiles <= 2048 ? 4 : 16;
+  const uint64_t most = z.prompt ? 512 : 2048;
+  // prompts whose pieces of 16 would be one for each CU at most, where two fit (not f32's 8 waves), and most of whose
+  // pieces do not end at the diagonal: 512 tokens at 1536 38 us against 43, 256 at 3840 40 against 44; f32 57 against 50
+  if (least == 16 && q_type != TY_F32 && segments < 256 && segments * ((cap_tiles + 15) / 16) <= 256 && cap >= 2 * n_new)
+    least = 8;
   // the split's: 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
   z.at_once = z.prompt ? (uint32_t)least : 256 * cm::p8_per_cu((int)hd, (int)z.nr) * 7 / 8;
   const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + least - 1) / least));
@@ -267,7 +273,7 @@ int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stri
   const uint64_t group = n_heads / n_kv;
   if (!grid_ok((uint64_t)n_seqs * n_kv * n_new * group, cm::PA_NT) || n_new * group * group >= (1ull << 32))
     return cm::fail_global(me, "too many rows in one call");
-  const P8Sizes z = p8_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride);
+  const P8Sizes z = p8_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride, q_type);
   if (!z.fits) return cm::fail_global(me, "n_seqs * n_kv * table_stride * page_size too large for one call");
   // (every workgroup works the plan out from all lengths)
   if (n_seqs > 65535) return cm::fail_global(me, "at most 65535 sequences");
