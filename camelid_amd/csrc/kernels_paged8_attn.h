@@ -516,12 +516,20 @@ constexpr int p8p_lds(int hd) { return 2 * (2 * 64 * hd * 2 + 192) + 16; }
 // 64 KB), and more once that makes over 512 pieces, two for each CU.  Segments cut evenly may make some more than 512 all
 // the same, which wait for all the others: an eighth more tiles then, if that brings them to 512 (512 tokens at 32256,
 // 24 + 8 heads, bf16: 576 pieces 356 us, 480 286; an eighth more always: 43 at 39957 70 and 76 us).
+// Where more than half of the tiles lie behind the first new position, pieces would end at the diagonal, many of them
+// empty, so segments stay whole up to P8P_WHOLE tiles if there is one for each CU (2048 tokens at 0, 24 + 8 heads,
+// f32: 129 us cut at 16, 83 whole).
+constexpr uint32_t P8P_WHOLE = 64;
 struct P8PromptTarget {
   template <typename F>
-  __device__ __forceinline__ uint32_t operator()(const PaArgs& a, uint32_t total, F pieces) const {
+  __device__ __forceinline__ uint32_t operator()(const PaArgs& a, uint32_t total, F all) const {
+    const auto pieces = [&](uint32_t most) { return all([=](const PaSeq& q) { return (q.tiles + most - 1) / most; }); };
+    uint32_t least = a.at_once;
+    if (least > 4 && all([](const PaSeq& q) { return q.first / P8_TILE; }) < total / 2)
+      least = max(least, all([](const PaSeq&) { return 1u; }) >= 256 ? P8P_WHOLE : 16u);
     const uint32_t even = (total + 511) / 512, fewer = (total + 447) / 448;
-    if (even <= a.at_once) return a.at_once;
-    return pieces(even) > 512 && pieces(fewer) <= 512 ? fewer : even;
+    if (even <= least) return least;
+    return pieces(even) > 512 && pieces(fewer) <= 512 ? max(fewer, least) : even;
   }
 };
 

@@ -195,11 +195,11 @@ __device__ __forceinline__ PaPiece pa_piece(const PaArgs& a, uint32_t index, boo
     total += q.tiles * q.blocks * a.g.n_kv;
   }
   total = __builtin_amdgcn_readlane(pa_scan(total), 63);
-  const uint32_t target = Target{}(a, total, [&](uint32_t most) {  // pieces of `most` tiles at most
+  const uint32_t target = Target{}(a, total, [&](auto of) {  // the sum over all segments of what `of` says of theirs
     uint32_t k = 0;
     for (uint32_t s = s0; s < s1; ++s) {
       if (per > 1) q = pa_seq<NR, TILE>(a, s, false);
-      k += (q.tiles + most - 1) / most * q.blocks * a.g.n_kv;
+      k += of(q) * q.blocks * a.g.n_kv;
     }
     return (uint32_t)__builtin_amdgcn_readlane(pa_scan(k), 63);
   });

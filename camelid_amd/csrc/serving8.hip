@@ -70,6 +70,8 @@ P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_k
   // pieces do not end at the diagonal: 512 tokens at 1536 38 us against 43, 256 at 3840 40 against 44; f32 57 against 50
   if (least == 16 && q_type != TY_F32 && segments < 256 && segments * ((cap_tiles + 15) / 16) <= 256 && cap >= 2 * n_new)
     least = 8;
+  // prompts without much before them (the tables have no room for it; the kernel looks at the lengths, too): not cut
+  if (least == 16 && cap < 2 * n_new && segments >= 256) least = cm::P8P_WHOLE;
   // the split's: 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
   z.at_once = z.prompt ? (uint32_t)least : 256 * cm::p8_per_cu((int)hd, (int)z.nr) * 7 / 8;
   const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + least - 1) / least));
