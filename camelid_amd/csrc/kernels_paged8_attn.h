@@ -14,8 +14,8 @@
 // The conversion costs about 320 vector instructions a wave and tile of 16 KB, under the time that its bytes take.
 // Bound, prompts: vector instructions.  A wave's 16 rows of a tile take about 200 (operands 40, addresses 40, softmax
 // 100 of which 16 exponentials at a quarter of the rate) and 32 matrix instructions (64 and more for f32
-// rows).  4096 tokens at 12288, 32 + 8 heads of 128, bf16 rows: 1.18 ms, 815 TFLOP/s, vector units busy 70 % of the
-// cycles by instructions alone, matrix units 36 %; e4m3, whose conversion is shorter, 1.11 ms; f32 rows 1.68 ms.
+// rows).  4096 tokens at 12288, 32 + 8 heads of 128, bf16 rows: 1.12 ms, 860 TFLOP/s, vector units busy 75 % of the
+// cycles by instructions alone, matrix units 38 %; e4m3, whose conversion is shorter, 1.08 ms; f32 rows 1.66 ms.
 //   3 prompts of up to 1023, f32: 45 us: a workgroup's tiles follow each other, 2 us each.
 //
 // Operands.  Granules of 16 bytes become two operands of v_mfma_f32_16x16x32_f16 each: int8 as the low byte of the
