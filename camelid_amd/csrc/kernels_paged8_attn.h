@@ -12,10 +12,10 @@
 //   1 of 32775, 32 + 8 heads: 17.8 + 3.9 us for 67 MB, 16 of up to 1100 with up to 5 new tokens: 13.6 + 3.9 us for
 //     20 MB: chains of latencies (launch, plan, pages, K and V, products, states joined)
 // The conversion costs about 320 vector instructions a wave and tile of 16 KB, under the time that its bytes take.
-// Bound, prompts: vector instructions.  A wave's 16 rows of a tile take about 200 (operands 40, addresses 40, softmax
-// 100 of which 16 exponentials at a quarter of the rate) and 32 matrix instructions (64 and more for f32
-// rows).  4096 tokens at 12288, 32 + 8 heads of 128, bf16 rows: 1.12 ms, 860 TFLOP/s, vector units busy 75 % of the
-// cycles by instructions alone, matrix units 38 %; e4m3, whose conversion is shorter, 1.08 ms; f32 rows 1.66 ms.
+// Bound, prompts: vector instructions, then matrix ones.  A wave's 16 rows of a tile take about 230 (operands 40,
+// addresses 40, softmax 130 of which 16 exponentials at a quarter of the rate) and 48 matrix instructions (64 for
+// f32 rows).  4096 tokens at 12288, 32 + 8 heads of 128, the whole call: bf16 rows 1.36 ms, 705 TFLOP/s; e4m3, whose
+// conversion is shorter, 1.34 ms; f32 rows 1.58 ms.
 //   3 prompts of up to 1023, f32: 45 us: a workgroup's tiles follow each other, 2 us each.
 //
 // Operands.  Granules of 16 bytes become two operands of v_mfma_f32_16x16x32_f16 each: int8 as the low byte of the
@@ -29,7 +29,8 @@
 // bits), bf16 and f16 as they are.  K's exponent goes to the scores in f32.  V's goes to the weights before
 // they become f16: the matrix cores see w 2^ve / 2^D, D the running maximum of (exponent of the block's largest
 // weight + ve) over the row, so that what is lost is measured against the largest contribution and not against the
-// largest weight.  D is kept relative to the softmax's reference; both are whole numbers and rescaling is exact.
+// largest weight.  D is kept relative to the softmax's reference; both are whole numbers and rescaling is exact.  A weight
+// is the sum of two f16: 22 bits.
 #pragma once
 #include <type_traits>
 #include "kernels_paged8.h"
@@ -38,6 +39,10 @@
 namespace cm {
 
 constexpr uint32_t P8_TILE = 64;
+constexpr int P8_TERMS = 2;  // f16 that a softmax weight is the sum of
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 struct P8Args {
   PaArgs a;  // kc and vc: bytes
@@ -48,7 +53,6 @@ struct P8Args {
 // 16 bytes of a granule -> 16 f16, in order: two operands.
 template <int KT>
 __device__ __forceinline__ void p8_operands(u32x4 u, f16x8 (&to)[2]) {
-  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
   union {
     f16x2 h[8];
     f16x8 v[2];
@@ -137,10 +141,10 @@ struct P8Rows {
 
 // One tile's scores sc (positions gpos + 4 b + i of this lane's block) to weights pf (operands of positions gpos
 // + 8 half ...), and the rows' states.  edge: some row may not see some position.
-template <int HD, int NR, int NP>
+template <int HD, int NR>
 __device__ __forceinline__ void p8_softmax(P8Rows<HD, NR>& st, f32x4 (&sc)[NR][4], const P8Factor (&factor)[NR], uint32_t ke,
                                            uint32_t ve, uint32_t gpos, const uint32_t (&limit)[NR], bool page_ok, bool edge,
-                                           f16x8 (&pf)[NR][NP][2]) {
+                                           f16x8 (&pf)[NR][P8_TERMS][2]) {
   const float vexp = (float)((int)ve - 127);
   // (each step for all rows: their chains run side by side)
   float fk[NR], m_new[NR], d_tile[NR], base[NR], shift[NR], inside[NR], p[NR][16];
@@ -224,16 +228,25 @@ __device__ __forceinline__ void p8_softmax(P8Rows<HD, NR>& st, f32x4 (&sc)[NR][4
       }
     }
   }
+  // two weights' terms in one instruction, what is left of each in one (exact; a known factor would be a conversion and
+  // a subtraction)
+  float minus = -1.0f;
+  asm("" : "+s"(minus));
 #pragma unroll
   for (int r = 0; r < NR; ++r)
 #pragma unroll
-    for (int k = 0; k < NP; ++k)
+    for (int i = 0; i < 16; i += 2) {
+      float a = p[r][i], b = p[r][i + 1];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const _Float16 b = (_Float16)p[r][i];
-        pf[r][k][i >> 3][i & 7] = b;
-        if (k + 1 < NP) p[r][i] -= (float)b;
+      for (int k = 0; k < P8_TERMS; ++k) {
+        const f16x2 h = __builtin_convertvector((f32x2{a, b}), f16x2);
+        pf[r][k][i >> 3][i & 7] = h[0];
+        pf[r][k][i >> 3][(i & 7) + 1] = h[1];
+        if (k + 1 == P8_TERMS) break;
+        a = __builtin_fmaf((float)h[0], minus, a);
+        b = __builtin_fmaf((float)h[1], minus, b);
       }
+    }
 }
 
 // NaN bytes (e4m3) of an operand's granule to zero: a zero weight times them would be NaN.  Whether there were any.
@@ -278,7 +291,7 @@ template <int HD, int KT, int QT, int NR, bool STREAM>
 __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8) {
   typedef typename std::conditional<QT == TY_F32, float, typename std::conditional<QT == TY_F16, _Float16, __bf16>::type>::type QE;
   typedef QE q8v __attribute__((ext_vector_type(8)));
-  constexpr int NQ = QT == TY_F32 ? 2 : 1, NP = 2, KS = HD / 32, DS = HD / 16, KG = HD / 64;
+  constexpr int NQ = QT == TY_F32 ? 2 : 1, KS = HD / 32, DS = HD / 16, KG = HD / 64;
   constexpr int ROWS = 16 * NR, PITCH = HD + 4;
   const PaArgs& a = p8.a;
   extern __shared__ float smem[];  // [4][ROWS][PITCH] rows, [4][ROWS][2] states, [ROWS][2] factors
@@ -425,8 +438,8 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
     const uint32_t gpos = pos0 + 16 * grp;  // this lane's 16 positions
     if (!page_ok) paged_flag(g, PG_BAD_PAGE);
     const bool edge = pos0 + P8_TILE - 1 > first || __ballot(!page_ok) != 0;
-    f16x8 pf[NR][NP][2];
-    p8_softmax<HD, NR, NP>(st, sc, factor, ke_now, ve_now, gpos, limit, page_ok, edge, pf);
+    f16x8 pf[NR][P8_TERMS][2];
+    p8_softmax<HD, NR>(st, sc, factor, ke_now, ve_now, gpos, limit, page_ok, edge, pf);
     if (KT == TY_E4M3 && edge) {
       uint32_t odd = 0;
 #pragma unroll
@@ -438,7 +451,7 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
       f16x8 vv[2];
       p8_operands<KT>(vf[d], vv);
 #pragma unroll
-      for (int n = NP - 1; n >= 0; --n)  // the small terms first
+      for (int n = P8_TERMS - 1; n >= 0; --n)  // the small terms first
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -508,8 +521,9 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
 // Prompts: blocks of 128 query rows (64 for heads of 256), so that a tile's K and V are turned into operands once for
 // all of them, in LDS, while the tile before is worked on.  The plan is the split's; tiles behind a block's last row
 // are left out.  8 waves of 16 rows within 128 registers, two workgroups a CU (over 128: 8 sequences of 43 tokens at
-// 4000 77 us and not 60); the host's rule says where 4 waves of 32 rows do better.  16-bit rows take weights as one
-// f16 (11 bits of each, rounded to the nearest: their outputs keep 11 or 8), f32 rows as two.
+// 4000 77 us and not 60); the host's rule says where 4 waves of 32 rows do better.  Weights are two f16 for
+// all rows: one is 14 to 22 % faster for 16-bit ones (4096 tokens at 12288, bf16, 1114 us against 1363), but its 11 bits
+// are not enough where values cancel, as up to 8 new tokens would show that do have 22.
 constexpr int p8p_rows(int hd) { return hd == 256 ? 64 : 128; }  // rows of a block
 constexpr int p8p_lds(int hd) { return 2 * (2 * 64 * hd * 2 + 192) + 16; }
 // Tiles of a piece at most: `at_once` (4 where the batch is small, else 16: a piece's part is written and read again,
@@ -537,7 +551,7 @@ template <int HD, int KT, int QT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : WAVES == 8 && QT != TY_F32 ? 4 : 2) void k_p8_prompt(P8Args p8) {
   typedef typename std::conditional<QT == TY_F32, float, typename std::conditional<QT == TY_F16, _Float16, __bf16>::type>::type QE;
   typedef QE q8v __attribute__((ext_vector_type(8)));
-  constexpr int NQ = QT == TY_F32 ? 2 : 1, NP = QT == TY_F32 ? 2 : 1, KS = HD / 32, DS = HD / 16;
+  constexpr int NQ = QT == TY_F32 ? 2 : 1, KS = HD / 32, DS = HD / 16;
   constexpr int ROWS = p8p_rows(HD), NR = ROWS / 16 / WAVES, NT = 64 * WAVES;
   constexpr int KG = (HD / 16 + WAVES - 1) / WAVES;  // granules of K (and of V) of a thread
   constexpr bool ALL = HD / 16 >= WAVES;             // else of the first HD / 16 waves
@@ -710,8 +724,8 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : WAVES == 8 && QT != TY_
       }
     const uint32_t gpos = t * P8_TILE + 16 * grp;  // this lane's 16 positions
     if (!ok) paged_flag(g, PG_BAD_PAGE);
-    f16x8 pf[NR][NP][2];
-    p8_softmax<HD, NR, NP>(st, sc, factor, ke, ve, gpos, limit, ok,
+    f16x8 pf[NR][P8_TERMS][2];
+    p8_softmax<HD, NR>(st, sc, factor, ke, ve, gpos, limit, ok,
                            t * P8_TILE + P8_TILE - 1 > first || __ballot(!ok) != 0, pf);
     const bool odd = KT == TY_E4M3 && s_odd[B];
     if (t + 1 < t1) {
@@ -729,7 +743,7 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : WAVES == 8 && QT != TY_
 #pragma unroll
         for (int d = 0; d < 2; ++d) vv[d] = *reinterpret_cast<const f16x8*>(vd + (((d0 + d) * 2 + k) * 64 + lane) * 16);
 #pragma unroll
-        for (int n = NP - 1; n >= 0; --n)
+        for (int n = P8_TERMS - 1; n >= 0; --n)
 #pragma unroll
           for (int d = 0; d < 2; ++d)
 #pragma unroll

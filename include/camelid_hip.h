@@ -518,9 +518,8 @@ int camelid_hip_paged8_read(const void* kc, const void* vc, const uint8_t* k_exp
  * q rows of any type: out[row][h] = sum_p softmax_p(scale q[row][h].k_p) v_p over p <= the row's position.  8-bit elements
  * enter the matrix cores as f16, exactly; f32 q as two f16 of a row scaled into their range (22 bits, or 2^-38 of
  * the row's largest element), bf16 q as one, scaled alike (its 8 bits, or 2^-38), f16 q as it is; softmax weights as two f16
- * (22 bits, or 2^-39 of the row's largest weight times its block's scale), and as one (11 bits) for 16-bit q in
- * calls with n_new > CAMELID_MAX_VERIFY_K.  Statistics and sums are f32, results take one rounding to q_type.  Scores
- * have to stay below f32's largest number; results below 2^-100 may lose bits.  Elements of masked positions,
+ * (22 bits, or 2^-39 of the row's largest weight times its block's scale).  Statistics and sums are f32, results
+ * take one rounding to q_type.  Scores have to stay below f32's largest number; results below 2^-100 may lose bits.  Elements of masked positions,
  * whatever their bits, do not reach a row; NaN that it sees (a block's exponent of 255 from the block's first position
  * on, an e4m3 byte's from its own) makes its outputs NaN (of V: in that dim).  The order of sums goes by n_new, the sizes and the lengths:
  * the same call gives the same bits.  scale must be finite; n_new (n_heads / n_kv)^2 < 2^32; at most 65535 sequences.
