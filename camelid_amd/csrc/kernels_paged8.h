@@ -102,6 +102,10 @@ __device__ __forceinline__ void p8_unpack4(uint32_t u, float (&x)[4]) {
     x[3] = hi[1];
   }
 }
+// The bytes of a word that are NaN in e4m3, as 255.
+__device__ __forceinline__ uint32_t p8_nan_bytes(uint32_t u) {
+  return ((((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 255u;
+}
 // 2^(b - 127) of an exponent byte.
 __device__ __forceinline__ float p8_scale(uint32_t b) {
   return b == P8_NAN ? u2f(0x7fc00000u) : b ? u2f(b << 23) : 0x1p-127f;
@@ -139,18 +143,19 @@ __device__ __forceinline__ uint32_t r8_wave_max(uint32_t x) {
   return x;
 }
 
-// 8 bytes from a block's exponent `was` to `now`.
+// 4 bytes from a block's exponent `was` to `now`; NaN stays NaN.
+template <int KT>
+__device__ __forceinline__ uint32_t p8_requantised(uint32_t u, uint32_t was, uint32_t now) {
+  float x[4];
+  p8_unpack4<KT>(u, x);
+  const uint32_t w = p8_pack4<KT>(p8_shift(x[0], was, now), p8_shift(x[1], was, now), p8_shift(x[2], was, now),
+                                  p8_shift(x[3], was, now));
+  const uint32_t nan = KT == TY_E4M3 ? p8_nan_bytes(u) : 0u;
+  return (w & ~nan) | (u & nan);
+}
 template <int KT>
 __device__ __forceinline__ uint2 p8_requantised(uint2 u, uint32_t was, uint32_t now) {
-  uint32_t w[2] = {u.x, u.y};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float x[4];
-    p8_unpack4<KT>(w[i], x);
-    w[i] = p8_pack4<KT>(p8_shift(x[0], was, now), p8_shift(x[1], was, now), p8_shift(x[2], was, now),
-                        p8_shift(x[3], was, now));
-  }
-  return make_uint2(w[0], w[1]);
+  return make_uint2(p8_requantised<KT>(u.x, was, now), p8_requantised<KT>(u.y, was, now));
 }
 
 // Pairs (a, b) rotated: a and b hold dims 8 j .. and HALF + 8 j .., pairs across them or inside each.
@@ -238,9 +243,8 @@ __global__ __launch_bounds__(R8_NT, 3) void k_paged8_rope_kv16(Paged8 c, const f
     if (hi - lo < 16) {
       u32x4 kept = old;
       if (lo && now != was) {
-        const uint2 a = p8_requantised<KT>(make_uint2(old[0], old[1]), was, now);
-        const uint2 b = p8_requantised<KT>(make_uint2(old[2], old[3]), was, now);
-        kept = u32x4{a.x, a.y, b.x, b.y};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kept[i] = p8_requantised<KT>(old[i], was, now);
       }
 #pragma unroll
       for (uint32_t i = 0; i < 16; ++i) {
@@ -482,9 +486,7 @@ __global__ __launch_bounds__(R8_NT) void k_paged8_rope_kv(Paged8 c, const float*
     if (t >= lo) {
       *p = (uint8_t)p8_pack4<KT>(p8_round<KT>(ldexp(s_x[t][d], 127 - (int)now)), 0.0f, 0.0f, 0.0f);
     } else if (now != was) {
-      float old[4];
-      p8_unpack4<KT>(*p, old);
-      *p = (uint8_t)p8_pack4<KT>(p8_shift(old[0], was, now), 0.0f, 0.0f, 0.0f);
+      *p = (uint8_t)p8_requantised<KT>((uint32_t)*p, was, now);
     }
   }
 }

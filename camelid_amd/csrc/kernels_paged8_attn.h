@@ -254,9 +254,9 @@ __device__ __forceinline__ uint32_t p8_clear_nan(u32x4& u) {
   uint32_t any = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t bits = (((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-    any |= bits;
-    u[i] &= ~(bits * 255u);
+    const uint32_t nan = p8_nan_bytes(u[i]);
+    any |= nan;
+    u[i] &= ~nan;
   }
   return any;
 }

@@ -495,7 +495,7 @@ enum { CAMELID_I8 = 3, CAMELID_E4M3 = 4 };
  * with which the largest of the block's new elements is at most 127 (CAMELID_I8) or 448 (CAMELID_E4M3), -126 at
  * least, 121 (119) at most, which leaves f32's last binade to saturate; elements are rounded to the nearest, ties
  * to even; K's norm and rotation are f64 up to there.  Where the block begins before the new tokens and its exponent is larger, that one stays; where it is
- * smaller, the earlier positions are rounded to the new one (CAMELID_E4M3: exactly, but for subnormals).  The exponent of
+ * smaller, the earlier positions are rounded to the new one (CAMELID_E4M3: exactly, but for subnormals; NaN stays).  The exponent of
  * drafts that are rejected later stays until the block is stored to from its first position again.  A NaN or infinity
  * among the new elements makes the block's exponent 255: all of its positions read as NaN.  Bytes of positions
  * outside [0, lens[s]) stay.  No two sequences of a call may store into the same block. */
