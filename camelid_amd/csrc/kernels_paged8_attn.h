@@ -35,10 +35,10 @@
 #include <type_traits>
 #include "kernels_paged8.h"
 #include "kernels_paged_attn.h"
+#include "paged8_plan.h"
 
 namespace cm {
 
-constexpr uint32_t P8_TILE = 64;
 constexpr int P8_TERMS = 2;  // f16 that a softmax weight is the sum of
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -283,9 +283,6 @@ __device__ __forceinline__ void p8_add_nan(P8Rows<HD, NR>& st, const uint8_t* vc
   }
 }
 
-// Workgroups of a CU, by registers and LDS.
-constexpr int p8_per_cu(int hd, int nr) { return hd == 64 ? 4 - nr : hd == 128 ? 3 - nr : 1; }
-
 // One piece per workgroup; its 4 waves take the tiles in turn and join their states through LDS at the end.
 template <int HD, int KT, int QT, int NR, bool STREAM>
 __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8) {
@@ -524,7 +521,6 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
 // 4000 77 us and not 60); the host's rule says where 4 waves of 32 rows do better.  Weights are two f16 for
 // all rows: one is 14 to 22 % faster for 16-bit ones (4096 tokens at 12288, bf16, 1114 us against 1363), but its 11 bits
 // are not enough where values cancel, as up to 8 new tokens would show that do have 22.
-constexpr int p8p_rows(int hd) { return hd == 256 ? 64 : 128; }  // rows of a block
 constexpr int p8p_lds(int hd) { return 2 * (2 * 64 * hd * 2 + 192) + 16; }
 // Tiles of a piece at most: `at_once` (4 where the batch is small, else 16: a piece's part is written and read again,
 // 64 KB), and more once that makes over 512 pieces, two for each CU.  Segments cut evenly may make some more than 512 all
@@ -533,7 +529,6 @@ constexpr int p8p_lds(int hd) { return 2 * (2 * 64 * hd * 2 + 192) + 16; }
 // Where more than half of the tiles lie behind the first new position, pieces would end at the diagonal, many of them
 // empty, so segments stay whole up to P8P_WHOLE tiles if there is one for each CU (2048 tokens at 0, 24 + 8 heads,
 // f32: 129 us cut at 16, 83 whole).
-constexpr uint32_t P8P_WHOLE = 64;
 struct P8PromptTarget {
   template <typename F>
   __device__ __forceinline__ uint32_t operator()(const PaArgs& a, uint32_t total, F all) const {

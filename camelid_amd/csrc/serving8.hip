@@ -15,6 +15,7 @@
 
 namespace {
 
+using cm::P8Sizes;
 using cm::TY_E4M3;
 using cm::TY_I8;
 
@@ -41,65 +42,6 @@ uint32_t log2_of(uint32_t power) {
   uint32_t n = 0;
   while ((1u << n) < power) ++n;
   return n;
-}
-
-// What a call of the attention needs: row blocks of 16 * nr query rows, workgroups, workspace.
-struct P8Sizes {
-  uint32_t nr, blocks, part_rows, at_once, grid;
-  bool prompt;                 // the prompts' kernel
-  uint64_t tiles;              // of all row blocks, as the tables have room
-  bool join;                   // some segment may be cut
-  bool fits;                   // the plan's 32-bit counts hold
-  size_t part_o, cuts, bytes;  // offsets of the workspace's parts, its size
-};
-
-P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap,
-                 uint32_t q_type) {
-  P8Sizes z;
-  const uint64_t rows = n_new * (n_heads / n_kv), cap_tiles = (cap + cm::P8_TILE - 1) / cm::P8_TILE;
-  z.prompt = n_new > CAMELID_MAX_VERIFY_K && rows >= 128;
-  z.nr = z.prompt ? cm::p8p_rows((int)hd) / 16 : rows > 16 && hd <= 128 ? 2 : 1;
-  z.blocks = (uint32_t)((rows + 16 * z.nr - 1) / (16 * z.nr));
-  z.part_rows = (uint32_t)std::min<uint64_t>(rows, 16 * z.nr);
-  // a piece has at least `least` tiles, or all; pieces altogether are at most `most` and one for each segment
-  const uint64_t segments = n_seqs * n_kv * z.blocks;
-  z.tiles = segments * cap_tiles;
-  uint64_t least = !z.prompt || z.tiles <= 2048 ? 4 : 16;
-  const uint64_t most = z.prompt ? 512 : 2048;
-  // prompts whose pieces of 16 would be one for each CU at most, where two fit (not f32's 8 waves), and most of whose
-  // pieces do not end at the diagonal: 512 tokens at 1536 38 us against 43, 256 at 3840 40 against 44; f32 57 against 50
-  if (least == 16 && q_type != TY_F32 && segments < 256 && segments * ((cap_tiles + 15) / 16) <= 256 && cap >= 2 * n_new)
-    least = 8;
-  // prompts without much before them (the tables have no room for it; the kernel looks at the lengths, too): not cut
-  if (least == 16 && cap < 2 * n_new && segments >= 256) least = cm::P8P_WHOLE;
-  // the split's: 256 CUs; a seventh less, since cutting every segment evenly makes some more pieces
-  z.at_once = z.prompt ? (uint32_t)least : 256 * cm::p8_per_cu((int)hd, (int)z.nr) * 7 / 8;
-  const uint64_t pieces = std::min(most + segments, segments * ((cap_tiles + least - 1) / least));
-  z.fits = z.tiles < (1ull << 31) && grid_ok(pieces, 512);
-  z.grid = (uint32_t)pieces;
-  z.join = cap_tiles > least;
-  // cut segments have more tiles than the target: at most `most` of them, twice as many pieces
-  const size_t slots = z.join ? (size_t)std::min(2 * most, pieces) : 0;
-  z.part_o = up256(slots * z.part_rows * 8);
-  z.cuts = z.part_o + up256(slots * z.part_rows * hd * 4);
-  z.bytes = z.cuts + up256(segments * 8);
-  return z;
-}
-
-// Workspace of calls of at most these sizes: parts of at most `slots` pieces, and a word pair for each segment; the
-// most that either kernel takes up to n_new.
-size_t p8_workspace(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint64_t n_kv, uint32_t hd, uint64_t cap) {
-  const uint64_t group = std::max<uint64_t>(n_heads / n_kv, 1), cap_tiles = (cap + cm::P8_TILE - 1) / cm::P8_TILE;
-  const auto most = [&](uint64_t rows, uint64_t block, uint64_t slots) {
-    const uint64_t segments = n_seqs * n_kv * ((rows + block - 1) / block), part_rows = std::min(rows, block);
-    slots = cap_tiles > 4 ? std::min(slots, segments * ((cap_tiles + 3) / 4)) : 0;
-    return up256(slots * part_rows * 8) + up256(slots * part_rows * hd * 4) + up256(segments * 8);
-  };
-  const uint64_t few = std::min(n_new, std::max<uint64_t>(CAMELID_MAX_VERIFY_K, 127 / group)) * group;
-  size_t bytes = std::max(most(std::min<uint64_t>(few, 16), 16, 4096), most(few, few > 16 && hd <= 128 ? 32 : 16, 4096));
-  if (n_new > CAMELID_MAX_VERIFY_K && n_new * group >= 128)
-    bytes = std::max(bytes, most(n_new * group, cm::p8p_rows((int)hd), 1024));
-  return bytes;
 }
 
 template <int HD, int QT, int NR>
@@ -244,7 +186,7 @@ int camelid_hip_paged8_read(const void* kc, const void* vc, const uint8_t* k_exp
 size_t camelid_hip_paged8_attention_workspace(uint32_t n_seqs, uint32_t n_new, uint32_t n_heads, uint32_t n_kv,
                                               uint32_t hd, uint32_t page_size, uint32_t table_stride) {
   if (!n_kv) return 0;
-  return p8_workspace(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride);
+  return cm::p8_workspace(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride);
 }
 
 int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stride, uint32_t n_seqs, uint32_t n_new,
@@ -275,8 +217,10 @@ int camelid_hip_paged8_attention(const void* q, uint32_t q_type, uint32_t q_stri
   const uint64_t group = n_heads / n_kv;
   if (!grid_ok((uint64_t)n_seqs * n_kv * n_new * group, cm::PA_NT) || n_new * group * group >= (1ull << 32))
     return cm::fail_global(me, "too many rows in one call");
-  const P8Sizes z = p8_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride, q_type);
+  const P8Sizes z = cm::p8_sizes(n_seqs, n_new, n_heads, n_kv, hd, (uint64_t)page_size * table_stride, q_type == TY_F32);
   if (!z.fits) return cm::fail_global(me, "n_seqs * n_kv * table_stride * page_size too large for one call");
+  // (what the buffer is laid out by, apart from the formula that a caller is told)
+  if (z.bytes > workspace_bytes) return cm::fail_global(me, "workspace too small for its own layout");
   // (every workgroup works the plan out from all lengths)
   if (n_seqs > 65535) return cm::fail_global(me, "at most 65535 sequences");
   char* ws = static_cast<char*>(workspace);

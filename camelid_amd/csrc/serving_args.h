@@ -5,12 +5,15 @@
 
 #include "errors.h"
 #include "kernels_paged.h"
+#include "launch_sizes.h"
 
 namespace {
 
 using cm::TY_BF16;
 using cm::TY_F16;
 using cm::TY_F32;
+using cm::grid_ok;
+using cm::up256;
 
 inline int launched(const char* what) {
   const hipError_t st = hipGetLastError();
@@ -19,9 +22,6 @@ inline int launched(const char* what) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
-// A launch holds at most 2^32 - 1 threads.
-inline bool grid_ok(uint64_t groups, uint32_t threads) { return groups * threads <= 0xffffffffull; }
-inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Cache geometry, pages of `least` positions or more; false: the reason why it is refused in *why.
 inline bool paged_geometry(cm::Paged* g, uint32_t n_seqs, uint32_t n_kv, uint32_t hd, uint32_t n_pages, uint32_t page_size,
