@@ -624,11 +624,13 @@ __global__ __launch_bounds__(PA_NT, pa_per_cu(HD, NR)) void k_pa_split(PaArgs a)
 // PARTS / PER groups of HD / 4 lanes; then, where weights are kept, workgroups of 256 or 64 positions.  Bound:
 // latency (4.4 us for 8 segments of 65 pieces), with weights the scores' bytes too.  A launch of its own:
 // joins by the last workgroup of a segment would need device-wide fences, which write back the L2.
+// static: several objects of the library instantiate it, and with shared names the linker keeps one object's launch
+// stub for both, which another object's kernel may not fit.
 constexpr uint32_t PJ_ROWS = 64, PJ_AHEAD = 16;
 constexpr uint32_t pj_parts(uint32_t hd) { return PA_NT / (hd / 4); }
 template <int HD, int QT, int NR, uint32_t PER>
-__global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, uint32_t row_groups,
-                                                   uint32_t spans, uint32_t span_bits) {
+static __global__ __launch_bounds__(PA_NT) void k_pa_join(PaArgs a, uint32_t n_rows, uint32_t row_groups,
+                                                          uint32_t spans, uint32_t span_bits) {
   constexpr uint32_t ROWS = 16 * NR, PARTS = pj_parts(HD), STEP = PARTS / PER;
   __shared__ f32x4 s_o[PARTS][HD / 4];
   __shared__ float s_ml[PARTS][2];
