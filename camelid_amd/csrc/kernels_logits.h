@@ -1,7 +1,7 @@
 // kernels_logits.h -- logits before a token is drawn from them: penalties for repeated tokens, biases, masks.
 //
 //   x' = x / r where x > 0, else x r, for tokens that the row's text has (history and drafts before the row)
-//   x' -= f count, x' -= p where count > 0, of the text's tokens behind the prompt
+//   x' -= f count, x' -= p where count > 0, of the text's tokens behind the prompt (drafts are, always)
 //   x' += bias of the token (the last one listed);  -infinity where the mask's bit is 0
 // each step rounded in f32, the result once to the logits' type.
 #pragma once

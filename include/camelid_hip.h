@@ -589,8 +589,9 @@ int camelid_hip_pages_copy(void* const* buffers, const size_t* page_bytes, uint3
 /* Logits before camelid_hip_verify_drafts (no reference counterpart): rows t <= draft_lens[s] (NULL: all; others are
  * padding) of logits [n_seqs][n_rows][in_stride] to out [n_seqs][n_rows][out_stride] of the same type (f32, f16 or bf16;
  * out may be logits).  The text of row t is history[s][0 .. history_lens[s]) (NULL: history_stride; larger values
- * count as that) and draft_tokens [n_seqs][n_rows - 1] before t (NULL: none); its first prompt_lens[s] tokens (NULL: 0)
- * are the prompt.  For each token i < vocab, with c occurrences in the text behind the prompt:
+ * count as that) and draft_tokens [n_seqs][n_rows - 1] before t (NULL: none); the history's first prompt_lens[s] tokens
+ * (NULL: 0; larger values: all) are the prompt, drafts never are.  For each token i < vocab, with c occurrences in the text
+ * behind the prompt:
  *   x = x / repetition[s] where x > 0, else x * repetition[s], if i is in the text, prompt included;
  *   x = x - frequency[s] * c, then x - presence[s], if c > 0;
  *   x = x + bias, if i is in bias_tokens[s][0 .. bias_lens[s]) (of equal ones the last counts);
