@@ -552,7 +552,7 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : WAVES == 8 && QT != TY_
   constexpr bool ALL = HD / 16 >= WAVES;             // else of the first HD / 16 waves
   constexpr uint32_t K_BYTES = 64 * HD * 2 + 192, BUF = K_BYTES + 64 * HD * 2;  // (64 bytes between the products' rows of K)
   const PaArgs& a = p8.a;
-  extern __shared__ char lds[];  // [2] K operands [4][KS][64], V operands [DS][2][64]; [2] flags
+  extern __shared__ char lds[];  // [2] K operands [4][KS][64], V operands [DS][2][64]; [2] tiles with NaN, + 1
   uint32_t* s_odd = reinterpret_cast<uint32_t*>(lds + 2 * BUF);
   const uint32_t tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t col = lane & 15u, grp = lane >> 4;
@@ -683,7 +683,7 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : WAVES == 8 && QT != TY_
       const uint32_t dim = (tid + NT * i) % HD;
       if (KT == TY_E4M3 && (edge || from.v_bad[i])) {
         const uint32_t odd = p8_clear_nan(from.v[i]);
-        if (odd && !from.v_bad[i]) s_odd[b] = 1;
+        if (odd && !from.v_bad[i]) s_odd[b] = t + 1;
       }
       f16x8 x[2];
       p8_operands<KT>(from.v[i], x);
@@ -722,7 +722,7 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : WAVES == 8 && QT != TY_
     f16x8 pf[NR][P8_TERMS][2];
     p8_softmax<HD, NR>(st, sc, factor, ke, ve, gpos, limit, ok,
                            t * P8_TILE + P8_TILE - 1 > first || __ballot(!ok) != 0, pf);
-    const bool odd = KT == TY_E4M3 && s_odd[B];
+    const bool odd = KT == TY_E4M3 && s_odd[B] == t + 1;
     if (t + 1 < t1) {
       stage(t + 1, B ^ 1, raw);
       ke = raw.ke;
