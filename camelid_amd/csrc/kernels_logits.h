@@ -53,7 +53,7 @@ __device__ __forceinline__ float lg_adjusted(float x, uint32_t w, uint32_t token
 // to LDS once, then the rows, 8 logits a thread.  In place without a mask only the tokens that the lists name are read
 // and written.  Bound: HBM where every logit is written, and the lists, which every slice reads from the L2.  32
 // sequences of up to 6 rows of 151936 bf16 logits, 2000 tokens of history, 40 biases, masks: 28 us for 72 MB (20 us
-// without the lists; f32 39 us for 143 MB); one row of 32000 in place: 4.4 us, a launch and three loads on each other.
+// without the lists; f32 39 us for 143 MB); one row of 32000 in place: 4.8 us, a launch and three loads on each other.
 template <int T, bool SPARSE>
 __global__ __launch_bounds__(LG_NT) void k_adjust_logits(LogitsArgs a) {
   __shared__ uint32_t s_word[LG_SLICE];  // LG_COUNT: occurrences behind the prompt

@@ -121,8 +121,9 @@ __device__ __forceinline__ float p8_shift(float x, uint32_t from, uint32_t to) {
 // for some heads of q, K or V (a role).
 //   q, K: HD / 16 lanes per (token, head), each 8 dims of either half, which hold the pairs of both pairings.
 //   V:    a lane per dim, its granule in registers.
-// Bound: HBM and, with 3 workgroups a CU (the f64 registers of K), its latency: 56 us for 196 MB (4 prompts of up to 2047
-// tokens, 32 + 8 + 8 heads of 128, QK norm; 46 us without the norm), 3.5 us for one token of 32 + 4 + 4 heads of 64.
+// Bound: HBM and, with 3 workgroups a CU (the f64 registers of K), its latency: 55 us for 196 MB (4 prompts of up to 2047
+// tokens, 32 + 8 + 8 heads of 128, QK norm; 46 us without the norm), 9.0 us for a token of each of 64 sequences of those
+// heads, 3.9 us for one token of 32 + 4 + 4 heads of 64.
 constexpr uint32_t R8_NT = 256;
 constexpr uint32_t r8_heads(uint32_t hd) { return R8_NT / (hd / 16) / P8_BLOCK; }  // q or K heads of a workgroup
 constexpr uint32_t r8_v_heads(uint32_t hd) { return R8_NT / hd; }
@@ -400,7 +401,8 @@ __global__ __launch_bounds__(R8_NT, 3) void k_paged8_rope_kv16(Paged8 c, const f
 }
 
 // The same with part of a head rotated, or none (rope_dim < head_dim): pairs fall anywhere.  One workgroup per
-// (sequence, block, head of q, K or V), rows in LDS.
+// (sequence, block, head of q, K or V), rows in LDS.  Bound: LDS and bytes stored one by one; right, not made fast:
+// the prompts above with half of a head rotated take 247 us, 164 without the norm (sums by one lane a row).
 template <int QT, int KT>
 __global__ __launch_bounds__(R8_NT) void k_paged8_rope_kv(Paged8 c, const float* __restrict__ qkv, uint32_t n_new,
                                                           const uint32_t* __restrict__ new_lens, uint32_t n_heads,

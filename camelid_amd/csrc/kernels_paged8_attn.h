@@ -7,16 +7,16 @@
 // k_p8_prompt: many.
 //
 // Bound, split: the cache's bytes (2 hd per position and KV head, 4 hd flop per position and row).  Heads of 128:
-//   64 sequences of up to 4001, 24 + 8 heads: 58 + 4.6 us (split + join) for 270 MB, 4.7 TB/s in the split; all of
-//     them 4001 long: 94 us for 525 MB, 5.6 TB/s; 4 of 65536: 93 us, 5.8 TB/s
-//   1 of 32775, 32 + 8 heads: 17.8 + 3.9 us for 67 MB, 16 of up to 1100 with up to 5 new tokens: 13.6 + 3.9 us for
+//   64 sequences of up to 4001, 24 + 8 heads: 57 + 4.7 us (split + join) for 270 MB, 4.7 TB/s in the split; calls: all
+//     of them 4001 long 96 us for 525 MB, 5.5 TB/s; 4 of 65536 94 us, 5.7 TB/s
+//   1 of 32775, 32 + 8 heads: 17 + 4.0 us for 67 MB, 16 of up to 1100 with up to 5 new tokens: 13.4 + 4.0 us for
 //     20 MB: chains of latencies (launch, plan, pages, K and V, products, states joined)
 // The conversion costs about 320 vector instructions a wave and tile of 16 KB, under the time that its bytes take.
-// Bound, prompts: vector instructions, then matrix ones.  A wave's 16 rows of a tile take about 230 (operands 40,
-// addresses 40, softmax 130 of which 16 exponentials at a quarter of the rate) and 48 matrix instructions (64 for
-// f32 rows).  4096 tokens at 12288, 32 + 8 heads of 128, the whole call: bf16 rows 1.36 ms, 705 TFLOP/s; e4m3, whose
-// conversion is shorter, 1.34 ms; f32 rows 1.58 ms.
-//   3 prompts of up to 1023, f32: 45 us: a workgroup's tiles follow each other, 2 us each.
+// Bound, prompts: vector instructions, then matrix ones.  A wave's 16 rows of a tile take about 240 (operands 40,
+// addresses 40, softmax 140 of which 16 exponentials at a quarter of the rate) and 48 matrix instructions (64 for
+// f32 rows).  4096 tokens at 12288, 32 + 8 heads of 128, calls among others: bf16 rows 1.36 to 1.40 ms, 690 to 705
+// TFLOP/s, vector units busy 74 % of the cycles with the exponentials' extra, matrix units 49 %; f32 rows 1.58 to 1.63 ms.
+//   3 prompts of up to 1023, f32: 44 us: a workgroup's tiles follow each other, 2 us each.
 //
 // Operands.  Granules of 16 bytes become two operands of v_mfma_f32_16x16x32_f16 each: int8 as the low byte of the
 // f16 1024 + u, minus 1152, e4m3 by the conversion instruction, both exact.
@@ -517,18 +517,18 @@ __global__ __launch_bounds__(PA_NT, p8_per_cu(HD, NR)) void k_p8_split(P8Args p8
 // ---------------------------------------------------------------------------
 // Prompts: blocks of 128 query rows (64 for heads of 256), so that a tile's K and V are turned into operands once for
 // all of them, in LDS, while the tile before is worked on.  The plan is the split's; tiles behind a block's last row
-// are left out.  8 waves of 16 rows within 128 registers, two workgroups a CU (over 128: 8 sequences of 43 tokens at
-// 4000 77 us and not 60); the host's rule says where 4 waves of 32 rows do better.  Weights are two f16 for
-// all rows: one is 14 to 22 % faster for 16-bit ones (4096 tokens at 12288, bf16, 1114 us against 1363), but its 11 bits
-// are not enough where values cancel, as up to 8 new tokens would show that do have 22.
+// are left out.  8 waves of 16 rows within 128 registers, two workgroups a CU (with 130: 4096 tokens at 12288
+// 1716 us and not 1380, 8 sequences of 43 at 4000 87 and not 74; 2048 at 0 74 and not 82); the host's rule says where 4 waves of 32 rows do better.  Weights are two f16 for
+// all rows, as for up to 8 new tokens: one takes 11 to 18 % less for 16-bit rows (4096 tokens at 12288, bf16, 1114 us
+// against 1363), but with its 11 bits sums whose values cancel are 2^-12 of the values' size off.
 constexpr int p8p_lds(int hd) { return 2 * (2 * 64 * hd * 2 + 192) + 16; }
 // Tiles of a piece at most: `at_once` (4 where the batch is small, else 16: a piece's part is written and read again,
 // 64 KB), and more once that makes over 512 pieces, two for each CU.  Segments cut evenly may make some more than 512 all
 // the same, which wait for all the others: an eighth more tiles then, if that brings them to 512 (512 tokens at 32256,
-// 24 + 8 heads, bf16: 576 pieces 356 us, 480 286; an eighth more always: 43 at 39957 70 and 76 us).
+// 24 + 8 heads, bf16: 576 pieces 438 us, 480 324; an eighth more always: 43 at 39957 78 and 82 us).
 // Where more than half of the tiles lie behind the first new position, pieces would end at the diagonal, many of them
 // empty, so segments stay whole up to P8P_WHOLE tiles if there is one for each CU (2048 tokens at 0, 24 + 8 heads,
-// f32: 129 us cut at 16, 83 whole).
+// f32: 127 us cut at 16, 77 whole; bf16 97 and 78).
 struct P8PromptTarget {
   template <typename F>
   __device__ __forceinline__ uint32_t operator()(const PaArgs& a, uint32_t total, F all) const {
@@ -747,9 +747,11 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : WAVES == 8 && QT != TY_
     if (odd) p8_add_nan<HD, NR>(st, vc, page_bytes, g, tab, t, len, limit);
     __syncthreads();
   };
-  // half of the waves first: they are at their softmax while the others multiply.  Not where few workgroups of unequal
-  // lengths leave CUs to one of them: 1024 tokens at 7168 178 us against 191, 512 at 32256 264 against 286, 4096 at
-  // 12288 1129 against 1175; 2048 at 0 94 against 87
+  // half of the waves first: they are at their softmax while the others multiply.  Where half of the positions lie before
+  // the new ones, or where there are workgroups for two rounds of all CUs; not where few workgroups of unequal lengths
+  // leave CUs to one of them.  With and without: 512 tokens at 32256 324 and 344 us, 4096 at 12288 1408 and 1443, 1024
+  // at 7168 223 and 224, 8 of up to 1023 at 0 67 and 70, 4 of up to 1000 at 2000 165 and 169, but 6 of those 198 and
+  // 184; left out, 2048 at 0 84 and 78, 3 of up to 1023 48 and 45, but 4096 at 0 187 and 195
   if (HD == 128 && QT != TY_F32 && w < WAVES / 2 && ((pc.n > 1 && first >= len - first) || gridDim.x >= 1024))
     __builtin_amdgcn_s_setprio(1);
   if (t0 < t1) {

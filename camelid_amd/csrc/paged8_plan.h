@@ -11,7 +11,8 @@
 namespace cm {
 
 constexpr uint32_t P8_TILE = 64;  // positions
-// Workgroups of a CU that the split's plan counts on.
+// Workgroups of a CU that the split's plan counts on and that the compiler is held to.  (Registers and LDS take one more,
+// but for f32 rows over heads of 256.)
 constexpr int p8_per_cu(int hd, int nr) { return hd == 64 ? 4 - nr : hd == 128 ? 3 - nr : 1; }
 // Prompts: rows of a block, and tiles up to which segments stay whole.
 constexpr int p8p_rows(int hd) { return hd == 256 ? 64 : 128; }
@@ -31,6 +32,13 @@ inline P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint6
                         bool f32_rows) {
   P8Sizes z;
   const uint64_t rows = n_new * (n_heads / n_kv), cap_tiles = (cap + P8_TILE - 1) / P8_TILE;
+  // The prompts' kernel converts K and V once for a block of rows and keeps its operands in LDS; the split reads and
+  // converts them once for each 32 rows (16 for heads of 256), but cuts finer and waits at no barrier.  From a whole
+  // block on (two for heads of 256): 16 sequences of 4096 positions, 8 KV heads of 64 / 128 / 256, prompts' kernel and split:
+  // 64 rows 49 and 39 / 68 and 64 / 111 and 133 us, 96 rows 50 and 49 / 73 and 85 / 187 and 239, 128 rows 51 and
+  // 59 / 80 and 104 / 190 and 215, 256 rows 88 and 98 / 132 and 170 / 343 and 370 (groups of 1 and 8 alike; with
+  // one row more than a block the split wins again: 43 tokens of groups of 3 81 and 71 / 119 and 120 / 274 and 232).
+  // One sequence: the split by 1 to 3 us from 64 to 512 rows (128: 18 and 15 / 22 and 22 / 27 and 26).
   z.prompt = n_new > CAMELID_MAX_VERIFY_K && rows >= 128;
   z.nr = z.prompt ? p8p_rows((int)hd) / 16 : rows > 16 && hd <= 128 ? 2 : 1;
   z.blocks = (uint32_t)((rows + 16 * z.nr - 1) / (16 * z.nr));
@@ -41,7 +49,7 @@ inline P8Sizes p8_sizes(uint64_t n_seqs, uint64_t n_new, uint64_t n_heads, uint6
   uint64_t least = !z.prompt || z.tiles <= 2048 ? 4 : 16;
   const uint64_t most = z.prompt ? 512 : 2048;
   // prompts whose pieces of 16 would be one for each CU at most, where two fit (not f32's 8 waves), and most of whose
-  // pieces do not end at the diagonal: 512 tokens at 1536 38 us against 43, 256 at 3840 40 against 44; f32 57 against 50
+  // pieces do not end at the diagonal: 512 tokens at 1536 46 us against 49, 256 at 3840 45 against 47; f32 57 against 50
   if (least == 16 && !f32_rows && segments < 256 && segments * ((cap_tiles + 15) / 16) <= 256 && cap >= 2 * n_new)
     least = 8;
   // prompts without much before them (the tables have no room for it; the kernel looks at the lengths, too): not cut

@@ -87,8 +87,9 @@ bool p8_launch(const cm::P8Args& p, const P8Sizes& z, hipStream_t stream) {
   if (z.prompt) {
     // 8 waves of 16 rows a workgroup hide each other's latency; f32 rows, which take twice the products, have enough
     // of those from some size on, and 4 waves of 32 rows read LDS half as often.  Heads of 128, f32: 3 prompts of up to
-    // 1023 49.5 us with 8 waves and 62.6 with 4, 1024 tokens at 7168 287 and 265, 4096 at 12288 1870 and 1653; bf16
-    // (all waves at one priority): 38.8 and 44.6, 189 and 190, 1159 and 1159
+    // 1023 44.7 us with 8 waves and 56.1 with 4, 512 tokens at 1536 49 and 58, 2048 at 0 77 and 99, 1024 at 7168 267 and
+    // 265, 512 at 32256 427 and 386, 4096 at 12288 1814 and 1628; bf16: 45 and 49, 46 and 48, 78 and 88, 223 and 232, 324
+    // and 334, 1408 and 1407 (e4m3 1400 and 1347)
     const auto go = [&](auto waves) {
       return p8_start(cm::k_p8_prompt<HD, KT, QT, waves()>, p, z, 64 * waves(), cm::p8p_lds(HD), stream);
     };
